@@ -1,0 +1,353 @@
+// Attention of single tokens in parts that are joined afterwards: behind prefixes that rows share (prefix_attention), and
+// with the sum of the weights that every cached entry receives (weighed_attention).  attention_parts.cuh says how parts
+// are cut and joined.
+#include "attention_parts.cuh"
+
+#define PG_THREADS 128
+#define PG_Q 16                // queries of a block
+#define PG_K 64                // entries of a tile
+#define PG_LD (PG_K + 4)
+
+// ---------------------------------------------------------------------------------------------------
+// Any head size up to 256, any page size, 32-bit or bfloat16 storage, all arithmetic in 32-bit.
+// Per tile of 64 entries: 2 queries x 4 entries of scores a thread, then a column of the output for all 16 queries a thread;
+// DP = 32 or 64: as many threads share the columns, and PG_THREADS / DP groups of them share the tile's entries.
+// ---------------------------------------------------------------------------------------------------
+template <typename A> struct Quad;                                  // four numbers of a row at once
+template <> struct Quad<float> {
+    __device__ static float4 load(const float* p) { return *reinterpret_cast<const float4*>(p); }
+};
+template <> struct Quad<bf16> {
+    __device__ static float4 load(const bf16* p) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16),
+                           __uint_as_float(v.y & 0xffff0000u));
+    }
+};
+
+__host__ __device__ inline int pg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
+
+template <typename A, int DP, bool VEC>
+__global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArgs a) {
+    extern __shared__ __align__(16) float smem[];
+    constexpr int GROUPS = PG_THREADS / DP, COLS = DP == 128 ? 2 : 1;
+    PartShare s;
+    pdl_wait();
+    pdl_trigger();
+    if (!part_share(a, PG_Q, blockIdx.x, s)) return;
+    const int d = a.d, ld = pg_row(d), group = a.nh / a.nkv, tid = threadIdx.x;
+    float* qs = smem;                                               // [16][ld]
+    float* ks = qs + PG_Q * ld;                                     // [64][ld]
+    float* vs = ks + PG_K * ld;                                     // [64][ld]
+    float* ps = vs + PG_K * ld;                                     // [16][PG_LD]
+    float* al = ps + PG_Q * PG_LD;                                  // [16]
+    for (int i = tid; i < PG_Q * ld; i += PG_THREADS) {
+        const int row = i / ld, c = i - row * ld, qi = s.q0 + row;
+        float v = 0.f;
+        if (row < s.nq && c < d)
+            v = to_f32(((const A*)a.q)[(size_t)(s.row0 + qi / group) * a.q_stride + (s.kvh * group + qi % group) * d + c]) * a.scale_log2;
+        qs[i] = v;
+    }
+    const size_t page_elems = (size_t)2 * a.nkv * a.page_size * d, to_values = (size_t)a.nkv * a.page_size * d;
+    const int qa = tid >> 4, ka = tid & 15;                         // scores: queries 2 qa, 2 qa + 1; entries ka + 16 j
+    const int col = tid % DP, part = tid / DP;                      // output: column(s) col (+ 128), entries part + GROUPS j
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float acc[COLS][PG_Q];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+        for (int i = 0; i < PG_Q; ++i) acc[c][i] = 0.f;
+    for (int e0 = s.e0; e0 < s.e1; e0 += PG_K) {
+        const int n = min(PG_K, s.e1 - e0);
+        __syncthreads();                                            // the last tile's values are read
+        constexpr int W = VEC ? 4 : 1;
+        const int pieces = VEC ? d / 4 : d;
+        for (int i = tid; i < PG_K * pieces; i += PG_THREADS) {     // rows beyond the part are zeros
+            const int row = i / pieces, c = (i - row * pieces) * W;
+            float4 k4 = {0.f, 0.f, 0.f, 0.f}, v4 = k4;
+            if (row < n) {
+                const int e = e0 + row;
+                const A* src = (const A*)a.kv + (size_t)s.table[e / a.page_size] * page_elems +
+                               ((size_t)s.kvh * a.page_size + e % a.page_size) * d + c;
+                if constexpr (VEC) { k4 = Quad<A>::load(src); v4 = Quad<A>::load(src + to_values); }
+                else { k4.x = to_f32(src[0]); v4.x = to_f32(src[to_values]); }
+            }
+            if constexpr (VEC) {
+                *reinterpret_cast<float4*>(ks + row * ld + c) = k4;
+                *reinterpret_cast<float4*>(vs + row * ld + c) = v4;
+            } else { ks[row * ld + c] = k4.x; vs[row * ld + c] = v4.x; }
+        }
+        if (!VEC)                                                   // the scores read four columns at a time
+            for (int i = tid; i < PG_K * (ld - d); i += PG_THREADS) ks[i / (ld - d) * ld + d + i % (ld - d)] = 0.f;
+        __syncthreads();
+        float sc[2][4] = {};
+        for (int c = 0; c < d; c += 4) {
+            float4 q4[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (2 * qa + i) * ld + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 k4 = *reinterpret_cast<const float4*>(ks + (ka + 16 * j) * ld + c);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    sc[i][j] += q4[i].x * k4.x; sc[i][j] += q4[i].y * k4.y;
+                    sc[i][j] += q4[i].z * k4.z; sc[i][j] += q4[i].w * k4.w;
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int qi = s.q0 + 2 * qa + i;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int e = ka + 16 * j;
+                if (e >= n) sc[i][j] = -INFINITY;
+                else if (a.scores && 2 * qa + i < s.nq)
+                    a.scores[((size_t)(s.row0 + qi / group) * a.nh + s.kvh * group + qi % group) * a.score_ld + e0 + e] = sc[i][j];
+                mx = fmaxf(mx, sc[i][j]);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float mn = fmaxf(m[i], mx), ms = mn == -INFINITY ? 0.f : mn, f = exp2f(m[i] - ms);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(sc[i][j] - ms);
+                ps[(2 * qa + i) * PG_LD + ka + 16 * j] = p;
+                sum += p;
+            }
+            l[i] = l[i] * f + sum;                                  // this thread's entries; added up at the end
+            m[i] = mn;
+            if (ka == 0) al[2 * qa + i] = f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PG_Q; ++i) {
+            const float f = al[i];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) acc[c][i] *= f;
+        }
+        const int some = (n + 4 * GROUPS - 1) / (4 * GROUPS) * (4 * GROUPS);   // the tile's rows up to 64 are zeros behind n
+        for (int e = 4 * part; e < some; e += 4 * GROUPS) {
+            float v[COLS][4];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[c][j] = col + DP * c < d ? vs[(e + j) * ld + col + DP * c] : 0.f;
+#pragma unroll
+            for (int i = 0; i < PG_Q; ++i) {
+                const float4 p4 = *reinterpret_cast<const float4*>(ps + i * PG_LD + e);
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) {
+                    acc[c][i] += p4.x * v[c][0]; acc[c][i] += p4.y * v[c][1];
+                    acc[c][i] += p4.z * v[c][2]; acc[c][i] += p4.w * v[c][3];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    }
+    if constexpr (GROUPS > 1) {                                     // the groups' sums, added in their order
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PG_Q; ++i) ks[i * PG_THREADS + tid] = acc[0][i];
+        __syncthreads();
+        if (part == 0) {
+#pragma unroll
+            for (int i = 0; i < PG_Q; ++i)
+                for (int g = 1; g < GROUPS; ++g) acc[0][i] += ks[i * PG_THREADS + g * DP + col];
+        }
+    }
+    const int slots = a.prefix_parts + a.own_parts;
+    auto place = [&](int row) -> size_t {
+        const int qi = s.q0 + row;
+        return ((size_t)(s.row0 + qi / group) * a.nh + s.kvh * group + qi % group) * slots + s.slot;
+    };
+    if (part == 0) {
+#pragma unroll
+        for (int i = 0; i < PG_Q; ++i)
+            if (i < s.nq)
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                    if (col + DP * c < d) a.part_o[place(i) * d + col + DP * c] = acc[c][i];
+    }
+    if (ka == 0)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (2 * qa + i < s.nq) {
+                a.part_ml[place(2 * qa + i) * 2] = m[i];
+                a.part_ml[place(2 * qa + i) * 2 + 1] = l[i];
+            }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Joining the parts of a row and head, and adding up the weights of a row's entries over the heads of a kv head.
+// ---------------------------------------------------------------------------------------------------
+#define JOIN_THREADS 128
+
+// What this row's softmax came to, from its parts: M and L of head h, by a whole warp (same result in every lane).
+__device__ __forceinline__ void join_ml(const PartArgs& a, int t, int h, int n_prefix, int n_own, float& M, float& L) {
+    const int slots = a.prefix_parts + a.own_parts, lane = threadIdx.x & 31, n = n_prefix + n_own;
+    const float* ml = a.part_ml + ((size_t)t * a.nh + h) * slots * 2;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 32) {
+        const int slot = i < n_prefix ? i : a.prefix_parts + i - n_prefix;
+        const float mi = ml[slot * 2], mn = fmaxf(m, mi), ms = mn == -INFINITY ? 0.f : mn;
+        l = l * exp2f(m - ms) + ml[slot * 2 + 1] * exp2f(mi - ms);
+        m = mn;
+    }
+    M = warp_max(m);
+    const float ms = M == -INFINITY ? 0.f : M;
+    L = warp_sum(l * exp2f(m - ms));
+    M = ms;
+}
+
+template <typename A>
+__device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __restrict__ out, int out_ld) {
+    const int slots = a.prefix_parts + a.own_parts, d = a.d;
+    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n_own = own_parts_of(a, t), n = n_prefix + n_own;
+    float M, L;
+    join_ml(a, t, h, n_prefix, n_own, M, L);
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const size_t base = ((size_t)t * a.nh + h) * slots;
+    for (int c = threadIdx.x; c < d; c += JOIN_THREADS) {
+        float acc = 0.f;
+        for (int i = 0; i < n; ++i) {
+            const size_t slot = base + (i < n_prefix ? i : a.prefix_parts + i - n_prefix);
+            acc += exp2f(a.part_ml[slot * 2] - M) * a.part_o[slot * d + c];
+        }
+        out[(size_t)t * out_ld + h * d + c] = from_f32<A>(acc * inv);
+    }
+}
+
+template <typename A>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const PartArgs a, A* __restrict__ out, int out_ld) {
+    pdl_wait();
+    pdl_trigger();
+    join_row(a, blockIdx.x / a.nh, blockIdx.x % a.nh, out, out_ld);
+}
+
+// Blocks 0 .. T nh - 1 join a row and head; the others add up the weights of 512 entries of a row and kv head:
+//   w[e] = decay w[e] + sum_h 2^(s_h(e) - M_h) / L_h,   the newest entry's w not read
+#define WEIGH_CHUNK 512
+template <typename A>
+__global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A* __restrict__ out, int out_ld,
+                                                             float* __restrict__ weights, long long weights_ld, int n_slots,
+                                                             const int* __restrict__ slots, int chunks, float decay) {
+    pdl_wait();
+    pdl_trigger();
+    int b = blockIdx.x;
+    if (b < a.T * a.nh) { join_row(a, b / a.nh, b % a.nh, out, out_ld); return; }
+    b -= a.T * a.nh;
+    const int chunk = b % chunks, kvh = b / chunks % a.nkv, t = b / chunks / a.nkv, group = a.nh / a.nkv;
+    const int n = own_entries(a, t), e0 = chunk * WEIGH_CHUNK, slot = slots[t];
+    if (e0 >= n || slot < 0 || slot >= n_slots) return;
+    __shared__ float sM[256], sI[256];
+    const int n_own = own_parts_of(a, t), warp = threadIdx.x >> 5;
+    for (int g0 = 0; g0 < group; g0 += 256) {                        // heads of a kv head, up to 256 at a time
+        __syncthreads();
+        for (int g = g0 + warp; g < min(group, g0 + 256); g += JOIN_THREADS / 32) {
+            float M, L;
+            join_ml(a, t, kvh * group + g, 0, n_own, M, L);
+            if ((threadIdx.x & 31) == 0) { sM[g - g0] = M; sI[g - g0] = 1.f / L; }
+        }
+        __syncthreads();
+        float* w = weights + ((size_t)slot * a.nkv + kvh) * weights_ld;
+        for (int e = e0 + threadIdx.x; e < min(n, e0 + WEIGH_CHUNK); e += JOIN_THREADS) {
+            const float* sc = a.scores + ((size_t)t * a.nh + kvh * group) * a.score_ld + e;
+            float sum = 0.f;
+            for (int g = g0; g < min(group, g0 + 256); ++g) sum += exp2f(sc[(size_t)g * a.score_ld] - sM[g - g0]) * sI[g - g0];
+            w[e] = (g0 > 0 ? w[e] : (e == n - 1 ? 0.f : decay * w[e])) + sum;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------
+static int launch_parts_general(const PartArgs& a, int dtype, cudaStream_t s) {
+    const long long blocks = part_blocks(a);
+    if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    if (blocks == 0) return 0;
+    const size_t smem = (size_t)((PG_Q + 2 * PG_K) * pg_row(a.d) + PG_Q * PG_LD + PG_Q) * sizeof(float);
+    const bool vec = a.d % 4 == 0 && (((uintptr_t)a.kv) & (dtype == RG_DTYPE_F32 ? 15 : 7)) == 0;
+#define RG_PG(A, DP, VEC) { cudaError_t e = cudaFuncSetAttribute(parts_general_kernel<A, DP, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
+    if (e != cudaSuccess) return (int)e; \
+    return rg_launch(parts_general_kernel<A, DP, VEC>, dim3((unsigned)blocks), dim3(PG_THREADS), smem, s, 1, a); }
+#define RG_PG_WIDTH(A, VEC) { if (a.d <= 32) RG_PG(A, 32, VEC) if (a.d <= 64) RG_PG(A, 64, VEC) RG_PG(A, 128, VEC) }
+    if (dtype == RG_DTYPE_F32) { if (vec) RG_PG_WIDTH(float, true) RG_PG_WIDTH(float, false) }
+    if (vec) RG_PG_WIDTH(bf16, true)
+    RG_PG_WIDTH(bf16, false)
+#undef RG_PG_WIDTH
+#undef RG_PG
+}
+
+static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void* kv, const int* block_table, int max_blocks,
+                           const int* positions, int T, int nh, int nkv, int d, int page_size, float scale, float* part_o,
+                           float* part_ml, int own_parts, int own_per) {
+    if (T < 0 || d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || own_parts < 0 || own_per < 1) return false;
+    a = PartArgs{};
+    a.q = q; a.q_stride = q_stride; a.kv = kv; a.block_table = block_table; a.max_blocks = max_blocks; a.positions = positions;
+    a.T = T; a.nh = nh; a.nkv = nkv; a.d = d; a.page_size = page_size; a.scale_log2 = scale * 1.4426950408889634f;
+    a.part_o = part_o; a.part_ml = part_ml; a.own_parts = own_parts; a.own_per = own_per; a.prefix_per = 1;
+    a.page_shift = -1;
+    for (int b = 0; b < 31; ++b) if (page_size == (1 << b)) a.page_shift = b;
+    const long long room = (long long)max_blocks * page_size, cut = (long long)own_parts * own_per;
+    a.own_limit = (int)min(0x7fffffffll, min(room, cut));
+    return true;
+}
+
+// Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
+// [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].
+extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int dtype,
+                                   const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
+                                   int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,
+                                   int own_parts, int own_per, int T, int nh, int nkv, int d, int page_size, float scale,
+                                   float* part_o, float* part_ml, void* stream) {
+    if (T <= 0) return 0;
+    PartArgs a;
+    if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
+                        own_parts, own_per) || n_groups < 0 || prefix_parts < 0 || prefix_per < 1 || out_ld < nh * d)
+        return RG_ERR_UNSUPPORTED;
+    const int group = nh / nkv;
+    a.prefix_table = prefix_table; a.prefix_blocks = prefix_blocks; a.groups = groups; a.n_groups = n_groups;
+    a.prefix_parts = prefix_parts; a.prefix_per = prefix_per;
+    a.prefix_limit = (int)min(0x7fffffffll, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
+    if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    a.prefix_tiles = (max_rows * group + PG_Q - 1) / PG_Q;
+    a.own_tiles = (group + PG_Q - 1) / PG_Q;
+    int e = launch_parts_general(a, dtype, (cudaStream_t)stream);
+    if (e) return e;
+    if (dtype == RG_DTYPE_F32)
+        return rg_launch(join_kernel<float>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
+    return rg_launch(join_kernel<bf16>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);
+}
+
+// Single tokens with the weights of their entries.  weights [n_slots, nkv, weights_ld]; scores [T, nh, score_ld] is scratch.
+extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int dtype,
+                                    const int* block_table, int max_blocks, const int* positions, int own_parts, int own_per,
+                                    int T, int nh, int nkv, int d, int page_size, float scale, float* part_o, float* part_ml,
+                                    float* scores, int score_ld, float* weights, int weights_ld, int n_slots, const int* slots,
+                                    int max_context, float decay, void* stream) {
+    if (T <= 0) return 0;
+    PartArgs a;
+    if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
+                        own_parts, own_per) || max_context > score_ld || max_context > weights_ld || out_ld < nh * d)
+        return RG_ERR_UNSUPPORTED;
+    a.scores = scores; a.score_ld = score_ld;
+    a.own_limit = min(a.own_limit, max_context);
+    const int group = nh / nkv;
+    a.own_tiles = (group + PG_Q - 1) / PG_Q;
+    int e = launch_parts_general(a, dtype, (cudaStream_t)stream);
+    if (e) return e;
+    const int chunks = (max_context + WEIGH_CHUNK - 1) / WEIGH_CHUNK;
+    const long long blocks = (long long)T * nh + (long long)T * nkv * chunks;
+    if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    if (dtype == RG_DTYPE_F32)
+        return rg_launch(weigh_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out,
+                         out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
+    return rg_launch(weigh_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out,
+                     out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
+}

@@ -2171,6 +2171,176 @@ def decode_attention(q, q_stride: int, out, kv_cache, block_table, rows, n_token
         _stream()), "decode_attention")
 
 
+def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> int:
+    """What the operators over rows of single tokens and portions ask of queries and cache; returns the page size."""
+    _dtype_code(q)
+    _check_rows(q, "q")
+    _check(kv_cache, "kv_cache", q.dtype)
+    if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
+        raise KernelError(f"{what}: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
+    if kv_cache.dim() != 5 or tuple(kv_cache.shape[1:3]) != (2, nkv) or kv_cache.shape[4] != d or kv_cache.shape[3] < 1:
+        raise KernelError(f"kv cache shape {tuple(kv_cache.shape)} does not match heads {nkv} x {d}")
+    if q.shape[1] < nh * d:
+        raise KernelError(f"{what}: q has {q.shape[1]} columns, {nh} heads of {d} need {nh * d}")
+    return kv_cache.shape[3]
+
+
+def _check_ints(t: torch.Tensor, name: str, shape: tuple) -> None:
+    _check(t, name, torch.int32)
+    if t.dim() != len(shape) or any(n is not None and t.shape[i] != n for i, n in enumerate(shape)):
+        raise KernelError(f"{name} is {tuple(t.shape)}, expected {tuple('any' if n is None else n for n in shape)}")
+
+
+def _check_entry_weights(weights: torch.Tensor, name: str, nkv: int, max_context: int, dtype=torch.float32) -> None:
+    _check(weights, name, dtype)
+    if weights.dim() != 3 or weights.shape[1] != nkv or weights.shape[2] < max_context:
+        raise KernelError(f"{name} is {tuple(weights.shape)}, expected [slots, {nkv}, at least {max_context}]")
+
+
+def attention_parts(blocks: int, longest: int, room: int = 444, least: int = 128) -> tuple:
+    """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would
+    read a list in one part each: as many parts as fill the GPU once (``room`` blocks, three an SM), of whole tiles of 64
+    entries and at least ``least``."""
+    if longest <= 0:
+        return 0, 64
+    parts = max(1, min(-(-longest // least), room // max(1, blocks)))
+    per = -(--(-longest // parts) // 64) * 64
+    return -(-longest // per), per
+
+
+def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positions, nh: int, nkv: int, d: int, scale: float,
+                     max_rows: int, max_prefix: int, max_own: int) -> None:
+    """Attention of single tokens whose requests share prefixes: ``out`` [T, nh * d], row t of ``q`` [T, at least nh * d] (head h
+    at column h * d) over the entries of its group's prefix, which is read once for the group's rows together, and over
+    entries of its own.  ``groups`` [n, 3] = (first row, rows, entries of the prefix), in order of rows; entry e of group g's
+    prefix is row e % page_size of page ``prefix_table[g, e // page_size]``.  Row t sees its own entries 0 ..
+    ``positions[t]`` (-1: none) through ``block_table[t]``.  Rows of no group see their own entries alone; where there is no
+    entry at all the output is 0.  ``max_rows``, ``max_prefix``, ``max_own``: the most rows and prefix entries that a group, and
+    own entries that a row, may have (``groups`` and ``positions`` stay on the device); what lies beyond is not seen.  All
+    sums are 32-bit and have one order."""
+    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prefix_attention")
+    T = q.shape[0]
+    _check_ints(groups, "groups", (None, 3))
+    _check_ints(prefix_table, "prefix_table", (groups.shape[0], None))
+    _check_ints(block_table, "block_table", (T, None))
+    _check_ints(positions, "positions", (T,))
+    _check_out_view(out, T, nh * d, q.dtype, "prefix_attention")
+    if min(max_rows, max_prefix, max_own) < 0:
+        raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
+    n_groups, G = groups.shape[0], nh // nkv
+    p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), max_prefix if n_groups and max_rows else 0)
+    o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own)
+    slots = T * nh * (p_parts + o_parts)
+    parts = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
+    _COUNTER.value += 1                          # the parts, and the kernel that joins them
+    _ok(_fn("attention_parts", "rg_prefix_attention")(
+        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(prefix_table),
+        c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
+        c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
+        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d), _stream()), "prefix_attention")
+
+
+def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, nh: int, nkv: int, d: int, scale: float,
+                      max_context: int, decay: float = 1.0) -> None:
+    """Attention of single tokens, one a request, that adds up the weights its entries receive.  Row r of ``q`` sees entries 0 ..
+    ``positions[r]`` (-1: none, its output is 0) through ``block_table[r]``; ``out`` [R, nh * d].  ``weights`` [slots, nkv, at least
+    max_context] float32, request r's at ``slots[r]`` (negative: a row whose weights nobody keeps): entry e's becomes
+    decay * weight + the sum, over the query heads of each kv head, of the softmax weight that e got from them.  The entry
+    ``positions[r]`` is new: its earlier weight is not read.  ``max_context``: the most entries a row may see; entries beyond
+    are not seen.  All sums are 32-bit and have one order."""
+    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
+    R = q.shape[0]
+    _check_ints(block_table, "block_table", (R, None))
+    _check_ints(positions, "positions", (R,))
+    _check_ints(slots, "slots", (R,))
+    _check_out_view(out, R, nh * d, q.dtype, "weighed_attention")
+    if max_context < 0:
+        raise KernelError("weighed_attention: max_context is a count")
+    _check_entry_weights(weights, "weights", nkv, max_context)
+    n_parts, per = attention_parts(R * nkv * -(-(nh // nkv) // 16), max_context)
+    rows, score_ld = R * nh, -(-max_context // 64) * 64
+    scratch = torch.empty(rows * (n_parts * (d + 2) + score_ld), dtype=torch.float32, device=q.device)
+    part_ml = scratch.data_ptr() + 4 * rows * n_parts * d
+    _COUNTER.value += 1                          # the parts, and the kernel that joins them
+    _ok(_fn("attention_parts", "rg_weighed_attention")(
+        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(block_table),
+        c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
+        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_void_p(part_ml + 8 * rows * n_parts), c_int(score_ld),
+        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), _stream()),
+        "weighed_attention")
+
+
+def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts, fresh, nh: int, nkv: int, d: int, scale: float,
+                       max_rows: int, max_context: int) -> None:
+    """The weights that entries receive from portions of prompts, or from the last rows of prompts: request r's rows of ``q``
+    are ``cu_rows[r]`` .. ``cu_rows[r + 1]`` - 1, at positions ``starts[r]``, + 1, ...; the row at position p gives the entries 0 .. p
+    (already in the cache) its softmax weights.  To ``weights`` [slots, nkv, at least max_context] float32, at ``slots[r]`` (negative: rows
+    whose weights nobody keeps), entry e's sum over the rows and the query heads of each kv head is added; entries from
+    ``fresh[r]`` on are new, their earlier weight is not read.  Entries that no row sees, and requests without rows, keep
+    theirs.  ``max_rows``, ``max_context``: the most rows of a request and the most entries a row may see.  All sums are 32-bit and
+    have one order."""
+    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prompt_key_weights")
+    _check_ints(slots, "slots", (None,))
+    R = slots.shape[0]
+    _check_ints(block_table, "block_table", (R, None))
+    _check_ints(cu_rows, "cu_rows", (R + 1,))
+    _check_ints(starts, "starts", (R,))
+    _check_ints(fresh, "fresh", (R,))
+    if min(max_rows, max_context) < 0:
+        raise KernelError("prompt_key_weights: max_rows and max_context are counts")
+    _check_entry_weights(weights, "weights", nkv, max_context)
+    z = torch.empty(q.shape[0] * nh, dtype=torch.float32, device=q.device)
+    _COUNTER.value += 1                          # the rows' sums, then the entries'
+    _ok(_fn("key_weights", "rg_prompt_key_weights")(
+        _ptr(q), c_int(q.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
+        _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(q.shape[0]),
+        c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z), _stream()),
+        "prompt_key_weights")
+
+
+def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, block_table, lens, keep, positions, nkv: int, d: int,
+                  protect_first: int, protect_last: int, max_context: int) -> torch.Tensor:
+    """Of the ``lens[r]`` entries of request r, ``keep[r]`` stay in every kv head: those of greatest weight, ties to the lowest
+    entry.  ``places`` [slots, nkv, at least max_context] int32 holds every entry's position in the text; entries at a place below
+    ``protect_first`` or above ``positions[r]`` - ``protect_last`` (``positions``: the newest token's place), or whose weight is no number, count as
+    infinitely heavy.  K and V rows behind the new length move, in place, into entries before it that got free, the i-th into
+    the i-th, so what stays is entries 0 .. new length - 1 and no more rows move than have to; the pages behind may be
+    given back.  Weights and places of the entries that stay go to ``weights_out`` and ``places_out`` (other buffers of these shapes;
+    what lies behind the new length there is left alone).  Returns the new lengths [R] int32, min(lens, keep).  Requests with a
+    negative slot are left alone."""
+    _dtype_code(kv_cache)
+    _check(kv_cache, "kv_cache")
+    _check_ints(slots, "slots", (None,))
+    R = slots.shape[0]
+    if kv_cache.dim() != 5 or tuple(kv_cache.shape[1:3]) != (2, nkv) or kv_cache.shape[4] != d or kv_cache.shape[3] < 1:
+        raise KernelError(f"kv cache shape {tuple(kv_cache.shape)} does not match heads {nkv} x {d}")
+    _check_ints(block_table, "block_table", (R, None))
+    for t, name in ((lens, "lens"), (keep, "keep"), (positions, "positions")):
+        _check_ints(t, name, (R,))
+    if max_context < 0 or protect_first < 0 or protect_last < 0:
+        raise KernelError("evict_entries: max_context, protect_first and protect_last are counts")
+    for t, name, dtype in ((weights, "weights", torch.float32), (places, "places", torch.int32),
+                           (weights_out, "weights_out", torch.float32), (places_out, "places_out", torch.int32)):
+        _check_entry_weights(t, name, nkv, max_context, dtype)
+        if t.shape != weights.shape:
+            raise KernelError(f"{name} is {tuple(t.shape)}, weights {tuple(weights.shape)}")
+    if weights_out.data_ptr() == weights.data_ptr() or places_out.data_ptr() == places.data_ptr():
+        raise KernelError("evict_entries: weights and places go to other buffers than their own")
+    new_lens = torch.empty(R, dtype=torch.int32, device=kv_cache.device)
+    if max_context == 0:
+        return new_lens.copy_(torch.minimum(lens, keep))
+    cluster = 1
+    while cluster < 8 and R * nkv * cluster * 2 <= num_sms(kv_cache.device) and max_context > 1024 * cluster:
+        cluster *= 2
+    moves = torch.empty(R * nkv * 2 * (max_context // 2 + 1), dtype=torch.int32, device=kv_cache.device)
+    _ok(_fn("evict", "rg_evict_entries")(
+        _ptr(kv_cache), c_int(kv_cache.element_size()), _ptr(weights), _ptr(places), _ptr(weights_out), _ptr(places_out),
+        c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(lens), _ptr(keep),
+        _ptr(positions), _ptr(new_lens), c_int(R), c_int(nkv), c_int(d), c_int(kv_cache.shape[3]), c_int(protect_first),
+        c_int(protect_last), c_int(max_context), _ptr(moves), c_int(cluster), _stream()), "evict_entries")
+    return new_lens
+
+
 _tc_err: dict = {}
 TC_GEMM_MIN_ROWS = 1024        # from here the fused tcgen05 gate|up product beats cuBLAS + SiLU-mul (measured)
 
