@@ -2,6 +2,11 @@
 // with the sum of the weights that every cached entry receives (weighed_attention).  attention_parts.cuh says how parts
 // are cut and joined.
 #include "attention_parts.cuh"
+#include "mma.cuh"
+#include "tcgen05.cuh"
+using rgmma::ex2;
+using rgmma::mma_bf16;
+using rgmma::pack_bf16;
 
 #define PG_THREADS 128
 #define PG_Q 16                // queries of a block
@@ -185,6 +190,211 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 }
 
 // ---------------------------------------------------------------------------------------------------
+// bfloat16, head sizes 64, 128, 192 and 256, pages of 8 tokens or a larger power of two: mma.sync m16n8k16 on tiles that TMA
+// brings.  What bounds it is memory: every entry's K and V are read once for up to 16 queries.
+//
+// A block is four warps that share nothing until they join at the end.  A warp takes every fourth run of 16 entries: one TMA
+// box of K and V together (a four-dimensional map: 64 columns, rows, 64-column pieces of the head, K and V; pages of 8 take
+// two boxes) into a ring of its own, refilled by the warp itself as soon as it has read a stage: no barrier between warps,
+// no copy instructions beside one a run.  The 128-byte swizzle keeps ldmatrix free of conflicts.
+// ---------------------------------------------------------------------------------------------------
+#define PM_THREADS 128
+#define PM_Q 16
+__host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 6 : (pieces == 3 ? 2 : 3); }
+__host__ __device__ constexpr int pm_stage_bytes(int pieces) { return 16 * 64 * 2 * 2 * pieces; }
+static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1) * pm_stage_bytes(1), "the warps' results fit where the stages were");
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int y) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %3}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_at(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans_at(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+
+template <int PIECES>          // the head size in pieces of 64
+__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
+parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, int* err) {
+    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES), KD = D / 16, ND = D / 8;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t bars[4 * STAGES];
+    __shared__ float ml[4][PM_Q][2];
+    __shared__ int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    const uint32_t base = ((smem_addr(smem_raw) + 1023u) & ~1023u) + (uint32_t)(warp * STAGES * STAGE);
+    const uint32_t bar0 = smem_addr(bars) + (uint32_t)(8 * STAGES * warp);
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0)
+        for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
+    if (lane == 0) fence_barrier_init();
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    PartShare sh;
+    if (!part_share(a, PM_Q, blockIdx.x, sh)) return;
+    const int group = a.nh / a.nkv;
+    const int n_runs = (sh.e1 - sh.e0 + 15) >> 4, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
+    // Page ids of this warp's next 32 runs, one a lane (of both halves of a run where pages hold 8).
+    const int box_shift = a.page_shift < 4 ? 3 : 4, box_rows = 1 << box_shift;
+    int page_a = 0, page_b = 0;
+    auto entry_of = [&](int i) -> int { return sh.e0 + (warp + 4 * i) * 16; };
+    auto fetch_pages = [&](int i0) {
+        const int e = entry_of(i0 + lane);
+        page_a = e < sh.e1 ? sh.table[e >> a.page_shift] : 0;
+        if (box_shift == 3) page_b = e + 8 < sh.e1 ? sh.table[(e + 8) >> a.page_shift] : page_a;   // no such entry: any page
+    };
+    auto issue = [&](int i) {                                         // the whole warp: run i of this warp
+        if ((i & 31) == 0) fetch_pages(i);
+        const int pa = __shfl_sync(0xffffffffu, page_a, i & 31), pb = __shfl_sync(0xffffffffu, page_b, i & 31);
+        if (lane == 0) {
+            const int s = i % STAGES, in_page = entry_of(i) & (a.page_size - 1);
+            const uint32_t bar = bar0 + 8 * s, dst = base + s * STAGE;
+            mbar_expect_tx(bar, STAGE);
+            tma_load_4d(dst, &kv_map, bar, (pa * 2 * a.nkv + sh.kvh) * a.page_size + in_page);
+            if (box_shift == 3) tma_load_4d(dst + STAGE / 2, &kv_map, bar, (pb * 2 * a.nkv + sh.kvh) * a.page_size);
+        }
+        __syncwarp();
+    };
+    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
+
+    // queries: rows g and g + 8 of the tile
+    uint32_t qf[KD][4];
+    const int qa = sh.q0 + g, qb = qa + 8;
+    const bool has_a = g < sh.nq, has_b = g + 8 < sh.nq;
+    auto head_of = [&](int qi) -> int { return sh.kvh * group + qi % group; };
+    auto row_of = [&](int qi) -> int { return sh.row0 + qi / group; };
+    {
+        const bf16* ra = has_a ? (const bf16*)a.q + (size_t)row_of(qa) * a.q_stride + head_of(qa) * D + 2 * tq : nullptr;
+        const bf16* rb = has_b ? (const bf16*)a.q + (size_t)row_of(qb) * a.q_stride + head_of(qb) * D + 2 * tq : nullptr;
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {
+            qf[k][0] = has_a ? *reinterpret_cast<const uint32_t*>(ra + k * 16) : 0u;
+            qf[k][1] = has_b ? *reinterpret_cast<const uint32_t*>(rb + k * 16) : 0u;
+            qf[k][2] = has_a ? *reinterpret_cast<const uint32_t*>(ra + k * 16 + 8) : 0u;
+            qf[k][3] = has_b ? *reinterpret_cast<const uint32_t*>(rb + k * 16 + 8) : 0u;
+        }
+    }
+    float *score_a = nullptr, *score_b = nullptr;
+    if (a.scores) {
+        if (has_a) score_a = a.scores + ((size_t)row_of(qa) * a.nh + head_of(qa)) * a.score_ld + 2 * tq;
+        if (has_b) score_b = a.scores + ((size_t)row_of(qb) * a.nh + head_of(qb)) * a.score_ld + 2 * tq;
+    }
+    float o[ND][4];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    // where this lane's ldmatrix rows are in a stage: K rows as the B operand, V rows transposed
+    auto line = [&](int r) -> uint32_t { return (uint32_t)((((r >> box_shift) * 2 * PIECES) << box_shift) + (r & (box_rows - 1))) * 128u; };
+    const int kr = (lane & 7) + (lane >> 4) * 8, vr = (lane & 7) + ((lane >> 3) & 1) * 8;
+    const uint32_t k_line = line(kr), v_line = line(vr) + (uint32_t)(PIECES << box_shift) * 128u, sw = (uint32_t)(lane & 7);
+    const uint32_t k_c = (lane >> 3) & 1, v_c = lane >> 4, piece = (uint32_t)(128 << box_shift);
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+        const int s = i % STAGES, e = entry_of(i);
+        const uint32_t st = base + s * STAGE;
+        ok = mbar_wait_all(bar0 + 8 * s, (i / STAGES) & 1, err, 61, &abort_flag);
+        if (!ok) break;
+        const int n = sh.e1 - e;                                      // entries of this run, if below 16
+        if (n < 16) {
+            // rows of V behind the last entry are what an earlier request left: 0 times an infinity is no number
+            for (int j = lane; j < (16 - n) * 8 * PIECES; j += 32) {
+                const int r = n + j / (8 * PIECES), c = j % (8 * PIECES);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                             ::"r"(st + line(r) + (uint32_t)(PIECES << box_shift) * 128u + (c >> 3) * piece + (c & 7) * 16), "r"(0) : "memory");
+            }
+            __syncwarp();
+        }
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {
+            uint32_t b[4];
+            ldmatrix_x4_at(b, st + k_line + (k >> 2) * piece + ((((k & 3) * 2 + k_c) ^ sw) << 4));
+            mma_bf16(s0, qf[k], b[0], b[1]);
+            mma_bf16(s1, qf[k], b[2], b[3]);
+        }
+        // rows g (first two of four) and g + 8, entries e + 2 tq + {0, 1} and + 8
+        float v[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] *= a.scale_log2;
+            if (n < 16 && 2 * tq + (j & 1) + ((j & 2) << 2) >= n) v[j] = -INFINITY;
+        }
+        if (score_a) {
+            *reinterpret_cast<float2*>(score_a + e) = make_float2(v[0], v[1]);
+            *reinterpret_cast<float2*>(score_a + e + 8) = make_float2(v[2], v[3]);
+        }
+        if (score_b) {
+            *reinterpret_cast<float2*>(score_b + e) = make_float2(v[4], v[5]);
+            *reinterpret_cast<float2*>(score_b + e + 8) = make_float2(v[6], v[7]);
+        }
+        float x0 = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), x1 = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        const float r0 = n0 == -INFINITY ? 0.f : n0, r1 = n1 == -INFINITY ? 0.f : n1;
+        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {          // some row's maximum moved
+            const float f0 = ex2(m0 - r0), f1 = ex2(m1 - r1);
+            l0 *= f0; l1 *= f1;
+#pragma unroll
+            for (int j = 0; j < ND; ++j) { o[j][0] *= f0; o[j][1] *= f0; o[j][2] *= f1; o[j][3] *= f1; }
+            m0 = n0; m1 = n1;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { v[j] = ex2(v[j] - r0); v[j + 4] = ex2(v[j + 4] - r1); }
+        l0 += (v[0] + v[1]) + (v[2] + v[3]);                          // this thread's entries; added up at the end
+        l1 += (v[4] + v[5]) + (v[6] + v[7]);
+        // weights to bfloat16 for the second product (the sums above are of the weights before that rounding)
+        const uint32_t p[4] = {pack_bf16(v[0], v[1]), pack_bf16(v[4], v[5]), pack_bf16(v[2], v[3]), pack_bf16(v[6], v[7])};
+#pragma unroll
+        for (int k = 0; k < KD; ++k) {                                // 16 columns at a time
+            uint32_t b[4];
+            ldmatrix_x4_trans_at(b, st + v_line + (k >> 2) * piece + ((((k & 3) * 2 + v_c) ^ sw) << 4));
+            mma_bf16(o[2 * k], p, b[0], b[1]);
+            mma_bf16(o[2 * k + 1], p, b[2], b[3]);
+        }
+        __syncwarp();                                                 // every lane has read the stage
+        if (i + STAGES < mine) issue(i + STAGES);
+    }
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (!ok || abort_flag)                                            // give copies in flight time to land
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    // the four warps' results, through the stages' memory (every copy has landed and been read)
+    __syncthreads();
+    float* all = reinterpret_cast<float*>(smem_raw + (((smem_addr(smem_raw) + 1023u) & ~1023u) - smem_addr(smem_raw)));   // [4][16][D]
+    float* co = all + warp * PM_Q * D;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+        *reinterpret_cast<float2*>(co + g * D + j * 8 + 2 * tq) = make_float2(o[j][0], o[j][1]);
+        *reinterpret_cast<float2*>(co + (g + 8) * D + j * 8 + 2 * tq) = make_float2(o[j][2], o[j][3]);
+    }
+    if (tq == 0) { ml[warp][g][0] = m0; ml[warp][g][1] = l0; ml[warp][g + 8][0] = m1; ml[warp][g + 8][1] = l1; }
+    __syncthreads();
+    const int slots = a.prefix_parts + a.own_parts;
+    for (int idx = threadIdx.x; idx < sh.nq * (D / 4); idx += PM_THREADS) {
+        const int r = idx / (D / 4), c = idx % (D / 4) * 4, qi = sh.q0 + r;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][r][0]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = ex2(ml[w][r][0] - ref);
+            const float4 x = *reinterpret_cast<const float4*>(all + (w * PM_Q + r) * D + c);
+            L += f * ml[w][r][1];
+            sum.x += f * x.x; sum.y += f * x.y; sum.z += f * x.z; sum.w += f * x.w;
+        }
+        const size_t place = ((size_t)row_of(qi) * a.nh + head_of(qi)) * slots + sh.slot;
+        *reinterpret_cast<float4*>(a.part_o + place * D + c) = sum;
+        if (c == 0) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(M, L);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------
 // Joining the parts of a row and head, and adding up the weights of a row's entries over the heads of a kv head.
 // ---------------------------------------------------------------------------------------------------
 #define JOIN_THREADS 128
@@ -284,6 +494,48 @@ static int launch_parts_general(const PartArgs& a, int dtype, cudaStream_t s) {
 #undef RG_PG
 }
 
+// The cache as the mma kernel reads it: 64 columns, rows, pieces of 64 columns, K and V; a box of `rows` rows.
+static int make_kv_map(CUtensorMap* map, const void* kv, int num_pages, int nkv, int page_size, int d, int rows) {
+    RgEncodeTiledFn fn = rg_encode_fn();
+    if (!fn) return RG_ERR_UNSUPPORTED;
+    cuuint64_t dims[4] = {64, (cuuint64_t)num_pages * 2 * nkv * page_size, (cuuint64_t)(d / 64), 2};
+    cuuint64_t strides[3] = {(cuuint64_t)d * 2, 128, (cuuint64_t)nkv * page_size * d * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)rows, (cuuint32_t)(d / 64), 2}, estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(kv), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
+}
+
+// bfloat16, head sizes in pieces of 64, pages of a power of two from 8 on, rows on 4-byte boundaries, and addresses that fit
+// the map's coordinates.
+static bool parts_mma_ok(const PartArgs& a, int dtype, int num_pages) {
+    return dtype == RG_DTYPE_BF16 && a.d % 64 == 0 && a.page_shift >= 3 && a.q_stride % 2 == 0 && ((uintptr_t)a.q & 3) == 0 &&
+           ((uintptr_t)a.kv & 15) == 0 && (long long)num_pages * 2 * a.nkv * a.page_size < 0x7fffffffll && a.score_ld % 2 == 0;
+}
+
+static int launch_parts_mma(const PartArgs& a, int num_pages, int* err, cudaStream_t s) {
+    const long long blocks = part_blocks(a);
+    if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    if (blocks == 0) return 0;
+    CUtensorMap map;
+    int e = make_kv_map(&map, a.kv, num_pages, a.nkv, a.page_size, a.d, a.page_size < 16 ? a.page_size : 16);
+    if (e) return e;
+#define RG_PM(P) { constexpr int smem = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
+    cudaError_t ce = cudaFuncSetAttribute(parts_mma_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
+    if (ce != cudaSuccess) return (int)ce; \
+    return rg_launch(parts_mma_kernel<P>, dim3((unsigned)blocks), dim3(PM_THREADS), smem, s, 1, map, a, err); }
+    if (a.d == 64) RG_PM(1)
+    if (a.d == 128) RG_PM(2)
+    if (a.d == 192) RG_PM(3)
+    RG_PM(4)
+#undef RG_PM
+}
+
+static int launch_parts(const PartArgs& a, int dtype, int num_pages, int* err, cudaStream_t s) {
+    return parts_mma_ok(a, dtype, num_pages) ? launch_parts_mma(a, num_pages, err, s) : launch_parts_general(a, dtype, s);
+}
+
 static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void* kv, const int* block_table, int max_blocks,
                            const int* positions, int T, int nh, int nkv, int d, int page_size, float scale, float* part_o,
                            float* part_ml, int own_parts, int own_per) {
@@ -301,11 +553,11 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
 // [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].
-extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int dtype,
+extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                    const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
                                    int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,
                                    int own_parts, int own_per, int T, int nh, int nkv, int d, int page_size, float scale,
-                                   float* part_o, float* part_ml, void* stream) {
+                                   float* part_o, float* part_ml, int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
@@ -318,7 +570,7 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
     if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     a.prefix_tiles = (max_rows * group + PG_Q - 1) / PG_Q;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
-    int e = launch_parts_general(a, dtype, (cudaStream_t)stream);
+    int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
     if (e) return e;
     if (dtype == RG_DTYPE_F32)
         return rg_launch(join_kernel<float>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
@@ -326,11 +578,11 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
 }
 
 // Single tokens with the weights of their entries.  weights [n_slots, nkv, weights_ld]; scores [T, nh, score_ld] is scratch.
-extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int dtype,
+extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                     const int* block_table, int max_blocks, const int* positions, int own_parts, int own_per,
                                     int T, int nh, int nkv, int d, int page_size, float scale, float* part_o, float* part_ml,
                                     float* scores, int score_ld, float* weights, int weights_ld, int n_slots, const int* slots,
-                                    int max_context, float decay, void* stream) {
+                                    int max_context, float decay, int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
@@ -340,7 +592,7 @@ extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int 
     a.own_limit = min(a.own_limit, max_context);
     const int group = nh / nkv;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
-    int e = launch_parts_general(a, dtype, (cudaStream_t)stream);
+    int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
     if (e) return e;
     const int chunks = (max_context + WEIGH_CHUNK - 1) / WEIGH_CHUNK;
     const long long blocks = (long long)T * nh + (long long)T * nkv * chunks;

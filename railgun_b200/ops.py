@@ -2197,6 +2197,16 @@ def _check_entry_weights(weights: torch.Tensor, name: str, nkv: int, max_context
         raise KernelError(f"{name} is {tuple(weights.shape)}, expected [slots, {nkv}, at least {max_context}]")
 
 
+def _tc_error_flag(device) -> torch.Tensor:
+    """The device's error flag of kernels with bounded waits, which ``tc_gemm_check()`` looks at."""
+    global _tc_unchecked
+    _tc_unchecked = True
+    err = _tc_err.get(device)
+    if err is None:
+        err = _tc_err[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return err
+
+
 def attention_parts(blocks: int, longest: int, room: int = 444, least: int = 128) -> tuple:
     """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would
     read a list in one part each: as many parts as fill the GPU once (``room`` blocks, three an SM), of whole tiles of 64
@@ -2234,10 +2244,10 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     parts = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
     _COUNTER.value += 1                          # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_prefix_attention")(
-        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(prefix_table),
+        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(prefix_table),
         c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d), _stream()), "prefix_attention")
+        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
 
 
 def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, nh: int, nkv: int, d: int, scale: float,
@@ -2263,10 +2273,10 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     part_ml = scratch.data_ptr() + 4 * rows * n_parts * d
     _COUNTER.value += 1                          # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_weighed_attention")(
-        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(block_table),
-        c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
+        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)),
+        _ptr(block_table), c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
         c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_void_p(part_ml + 8 * rows * n_parts), c_int(score_ld),
-        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), _stream()),
+        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), _ptr(_tc_error_flag(q.device)), _stream()),
         "weighed_attention")
 
 
