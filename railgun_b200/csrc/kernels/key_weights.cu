@@ -3,7 +3,9 @@
 //   s = scale log2(e) q.k,   z_th = log2 sum_e 2^(s_th(e))
 // in two passes over the scores: z first, then the sums.  A block of the second pass owns its entries and goes over all
 // rows that see them, so sums have one order and need no atomics.
-#include "common.cuh"
+#include "packed_f32.cuh"
+#include "tcgen05.cuh"
+#include <type_traits>
 
 struct WeightArgs {
     const void* q;               // [T, q_stride]: head h of row t at q[t * q_stride + h * d]
@@ -182,11 +184,417 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const We
     }
 }
 
-// z [T, nh] is scratch; max_rows: the most rows of a request; max_context: the most entries a row sees.
-extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv, int dtype, float* weights, int weights_ld,
+// ---------------------------------------------------------------------------------------------------
+// bfloat16, head sizes 64 and 128, up to 128 heads a kv head, pages of 8 tokens or a larger power of two: the 5th-generation
+// tensor cores.  Both passes have one structure and differ in what stays and what streams:
+//   row sums:    128 lanes = queries (rows x heads of a kv head), keys stream by;   m, l of a row run in its thread
+//   entry sums:  128 lanes = entries, queries stream by;   w[e] is a sum over columns, again inside a thread: no exchange
+// A block has two such tiles of 128 (a "side" each: its own accumulator and four warps), which share the streamed tiles,
+// so a streamed tile is fetched once for 256 lanes.  Per streamed tile of 128 and side: S = A B^T in 128 columns of tensor
+// memory, two buffers a side, then one pass of exponentials over it while the tensor core works on the next.  Blocks are
+// persistent: items (kv head, 256 lanes, part of what streams) are dealt out in turn, the heaviest first, and loads and products
+// run on across items.
+//
+// What bounds it: one 2^x an element and pass.  128 x 128 of them take 1,024 cycles of a scheduler's MUFU, the products of a
+// tile 520 of the tensor core (head size 128).
+// ---------------------------------------------------------------------------------------------------
+#define KT_THREADS 320             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9: MMA issue, tensor memory
+#define KT_TILE 128
+__host__ __device__ constexpr int kt_b_stages(int pieces) { return pieces == 1 ? 4 : 2; }
+
+struct KtArgs {
+    WeightArgs w;
+    float* part_ml;              // [T, nh, parts of the first pass, 2]
+    float* part_w;               // [parts of the second pass, R, nkv, limit]; null: the weights themselves are written
+    int* err;
+    int blocks, parts, n_items;  // 256 lanes each, of the longest request; parts of what streams
+    int row_parts;               // parts of the first pass
+    int tile_rows;               // rows of a query tile: 128 / group
+    int page_shift;
+};
+
+struct KtItem {
+    int r, kvh, part, row0, rows, start, entries;
+    int m0, n_m;                 // first lane tile, how many of the two there are
+    int b0, n_b;                 // streamed tiles b0, b0 + parts, ..
+};
+
+template <bool ENTRIES>
+__device__ __forceinline__ bool kt_item(const KtArgs& a, int i, KtItem& t) {
+    const int per_block = a.w.R * a.w.nkv * a.parts, blk = i / per_block, rest = i % per_block;
+    t.part = rest % a.parts;
+    t.kvh = rest / a.parts % a.w.nkv;
+    t.r = rest / a.parts / a.w.nkv;
+    rows_of(a.w, t.r, t.row0, t.rows, t.start, t.entries);
+    if (t.entries <= 0) return false;
+    const int q_tiles = (t.rows + a.tile_rows - 1) / a.tile_rows;
+    if (ENTRIES) {
+        t.m0 = 2 * blk;                                             // the first entries are seen by the most rows
+        t.n_m = min(2, (t.entries + KT_TILE - 1) / KT_TILE - t.m0);
+        t.b0 = max(0, t.m0 * KT_TILE - t.start) / a.tile_rows;
+        t.n_b = q_tiles - t.b0;
+    } else {
+        t.m0 = 2 * (a.blocks - 1 - blk);                            // the last rows see the most entries
+        t.n_m = min(2, q_tiles - t.m0);
+        const int last_row = min(t.rows, (t.m0 + 2) * a.tile_rows) - 1;
+        t.b0 = 0;
+        t.n_b = (min(t.entries, t.start + last_row + 1) + KT_TILE - 1) / KT_TILE;
+    }
+    t.n_b = t.n_b > t.part ? (t.n_b - t.part + a.parts - 1) / a.parts : 0;
+    t.b0 += t.part;
+    return t.n_m > 0;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
+// q_map: 64 columns x heads x rows, a box of 64 x group x tile_rows; kv_map: the cache as rows of the head size, a box of
+// min(page, 128) rows x 64 columns.
+template <int PIECES, bool ENTRIES>
+__global__ void __launch_bounds__(KT_THREADS, 1)
+key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const KtArgs a) {
+    extern __shared__ unsigned char smem_raw[];
+    constexpr int NB = kt_b_stages(PIECES);
+    constexpr uint32_t PIECE = KT_TILE * 128, TILE = PIECE * PIECES;
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, sA = base, sB = sA + 4 * TILE;   // two stages of two tiles; NB tiles
+    __shared__ __align__(8) uint64_t bars[4 + 2 * NB + 8];
+    // -z of a streamed tile's columns and their positions: a copy for every warp, so that warps wait for nothing but tiles
+    __shared__ __align__(16) float col_z[ENTRIES ? 8 : 1][2][KT_TILE];
+    __shared__ __align__(16) int col_p[ENTRIES ? 8 : 1][2][KT_TILE];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const uint32_t a_full = smem_addr(bars), a_empty = a_full + 16, b_full = a_empty + 16, b_empty = b_full + 8 * NB,
+                   s_full = b_empty + 8 * NB, s_empty = s_full + 32;   // s_full, s_empty: side 0's two buffers, side 1's
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.w.nh / a.w.nkv;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; ++i) { mbar_init(a_full + 8 * i, 1); mbar_init(a_empty + 8 * i, 1); }
+        for (int i = 0; i < NB; ++i) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_empty + 8 * i, KT_TILE); }
+        fence_barrier_init();
+    }
+    if (warp == 9) tmem_alloc(&tmem_slot, 512u);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;                                 // side g, buffer b: columns 256 g + 128 b
+    pdl_wait();
+    pdl_trigger();
+    bool ok = true;
+    KtItem t = {};
+    if (warp == 8) {
+        // ---- loads
+        const int box_rows = min(a.w.page_size, KT_TILE), boxes = KT_TILE / box_rows, box = lane % boxes, piece = lane / boxes;
+        const bool mine = piece < PIECES;                            // a box of a piece of the head each
+        auto load_keys = [&](uint32_t dst, uint32_t bar, int tile) {
+            const int e = tile * KT_TILE + box * box_rows;
+            const int page = a.w.block_table[(size_t)t.r * a.w.max_blocks + (e < t.entries ? e >> a.page_shift : 0)];   // behind: any page
+            if (mine)
+                tma_load_2d(dst + piece * PIECE + box * box_rows * 128, &kv_map, bar, 64 * piece,
+                            (page * 2 * a.w.nkv + t.kvh) * a.w.page_size + (e & (a.w.page_size - 1)));
+        };
+        auto load_queries = [&](uint32_t dst, uint32_t bar, int tile) {
+            if (lane < PIECES) tma_load_3d(dst + lane * PIECE, &q_map, bar, 64 * lane, t.kvh * group, t.row0 + tile * a.tile_rows);
+        };
+        const uint32_t q_bytes = (uint32_t)(PIECES * 128 * group * a.tile_rows);
+        const uint32_t a_bytes = ENTRIES ? TILE : q_bytes, b_bytes = ENTRIES ? q_bytes : TILE;
+        int ai = 0, bi = 0;
+        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
+            if (!kt_item<ENTRIES>(a, i, t) || t.n_b == 0) continue;
+            const int sa = ai & 1;
+            if (ai > 1) ok = mbar_wait_all(a_empty + 8 * sa, ((ai >> 1) & 1) ^ 1, a.err, 71, &abort_flag);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(a_full + 8 * sa, (uint32_t)t.n_m * a_bytes);
+            __syncwarp();
+            for (int g = 0; g < t.n_m; ++g) {
+                if (ENTRIES) load_keys(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g);
+                else load_queries(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g);
+            }
+            ++ai;
+            for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
+                const int sb = bi % NB;
+                if (bi >= NB) ok = mbar_wait_all(b_empty + 8 * sb, ((bi / NB) & 1) ^ 1, a.err, 72, &abort_flag);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(b_full + 8 * sb, b_bytes);
+                __syncwarp();
+                if (ENTRIES) load_queries(sB + sb * TILE, b_full + 8 * sb, t.b0 + b * a.parts);
+                else load_keys(sB + sb * TILE, b_full + 8 * sb, t.b0 + b * a.parts);
+            }
+        }
+    } else if (warp == 9) {
+        // ---- products: the whole warp walks and waits, one elected lane issues
+        constexpr uint32_t idesc = make_idesc(KT_TILE, KT_TILE, false);
+        const bool issuer = elect_one();
+        int ai = 0, bi = 0;
+        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
+            if (!kt_item<ENTRIES>(a, i, t) || t.n_b == 0) continue;
+            const int sa = ai & 1;
+            ok = mbar_wait_all(a_full + 8 * sa, (ai >> 1) & 1, a.err, 73, &abort_flag);
+            for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
+                const int sb = bi % NB, buf = bi & 1;
+                ok = mbar_wait_all(b_full + 8 * sb, (bi / NB) & 1, a.err, 74, &abort_flag);
+                for (int g = 0; g < 2 && ok; ++g) {
+                    if (bi > 1) ok = mbar_wait_all(s_empty + 16 * g + 8 * buf, ((bi >> 1) & 1) ^ 1, a.err, 75, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (issuer) {
+                        if (g < t.n_m) {
+#pragma unroll
+                            for (int x = 0; x < PIECES; ++x) {
+                                const uint64_t ad = desc_k_major(sA + (2 * sa + g) * TILE + x * PIECE), bd = desc_k_major(sB + sb * TILE + x * PIECE);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    tc_mma(tmem + 256u * g + 128u * buf, ad + 2u * k, bd + 2u * k, idesc, x + k > 0 ? 1u : 0u);
+                            }
+                        }
+                        tc_commit(s_full + 16 * g + 8 * buf);
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                if (issuer) {
+                    tc_commit(b_empty + 8 * sb);
+                    if (b == t.n_b - 1) tc_commit(a_empty + 8 * sa);
+                }
+                __syncwarp();
+            }
+            ++ai;
+        }
+    } else {
+        // ---- exponentials: thread = lane of the accumulator
+        const int g = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t tmem_row = tmem + 256u * g + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint64_t scale2 = pack2(a.w.scale_log2, a.w.scale_log2);
+        int bi = 0;
+        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
+            if (!kt_item<ENTRIES>(a, i, t)) continue;
+            const bool there = g < t.n_m;
+            if (ENTRIES) {
+                const int e = (t.m0 + g) * KT_TILE + row;
+                // columns lane + 32 j of a streamed tile: their queries' z and positions (-1: no query)
+                float z_next[4];
+                int p_next[4];
+                auto columns = [&](int b) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = lane + 32 * j, r = (t.b0 + b * a.parts) * a.tile_rows + c / group;
+                        p_next[j] = there && c < a.tile_rows * group && r < t.rows && b < t.n_b ? t.start + r : -1;
+                        z_next[j] = p_next[j] >= 0 ? a.w.z[(size_t)(t.row0 + r) * a.w.nh + t.kvh * group + c % group] : 0.f;
+                    }
+                };
+                columns(0);
+                uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+                for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
+                    const int buf = bi & 1;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        col_z[warp][buf][lane + 32 * j] = -z_next[j];
+                        col_p[warp][buf][lane + 32 * j] = p_next[j];
+                    }
+                    __syncwarp();                                    // they are there (and every lane is done with those before)
+                    columns(b + 1);
+                    ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (bi >> 1) & 1, a.err, 76, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float4* z4 = reinterpret_cast<const float4*>(col_z[warp][buf]);
+                    const int4* p4 = reinterpret_cast<const int4*>(col_p[warp][buf]);
+                    const int r0 = (t.b0 + b * a.parts) * a.tile_rows, cols = min(a.tile_rows, t.rows - r0) * group;
+                    // every column a query that sees every entry of this tile?
+                    const bool edge = cols < KT_TILE || t.start + r0 < (t.m0 + g + 1) * KT_TILE - 1;
+                    auto chunk = [&](auto edge_c, int c) {
+                        constexpr bool EDGE = decltype(edge_c)::value;
+                        uint32_t v[32];
+                        tc_ld32(tmem_row + 128u * buf + 32u * c, v);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 z = z4[(32 * c + j) >> 2];
+                            float x[4];
+                            unpack2(fma2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, pack2(z.x, z.y)), x[0], x[1]);
+                            unpack2(fma2(pack2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), scale2, pack2(z.z, z.w)), x[2], x[3]);
+                            if (EDGE) {
+                                const int4 p = p4[(32 * c + j) >> 2];
+                                if (p.x < e) x[0] = -INFINITY;
+                                if (p.y < e) x[1] = -INFINITY;
+                                if (p.z < e) x[2] = -INFINITY;
+                                if (p.w < e) x[3] = -INFINITY;
+                            }
+                            sum2[j / 4 % 2 * 2] = add2(sum2[j / 4 % 2 * 2], pack2(ex2(x[0]), ex2(x[1])));
+                            sum2[j / 4 % 2 * 2 + 1] = add2(sum2[j / 4 % 2 * 2 + 1], pack2(ex2(x[2]), ex2(x[3])));
+                        }
+                    };
+                    if (there) {
+                        if (edge) { for (int c = 0; c < (cols + 31) / 32; ++c) chunk(std::true_type{}, c); }
+                        else {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) chunk(std::false_type{}, c);
+                        }
+                    }
+                    tc_fence_before();
+                    mbar_arrive(s_empty + 16 * g + 8 * buf);
+                }
+                if (there && e < t.entries && ok) {
+                    float x, y;
+                    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
+                    if (a.part_w) {
+                        a.part_w[(((size_t)t.part * a.w.R + t.r) * a.w.nkv + t.kvh) * a.w.limit + e] = x + y;
+                    } else {
+                        const int slot = a.w.slots[t.r];
+                        if (slot >= 0 && slot < a.w.n_slots) {
+                            float* w = a.w.weights + ((size_t)slot * a.w.nkv + t.kvh) * a.w.weights_ld + e;
+                            *w = (e < a.w.fresh[t.r] ? *w : 0.f) + (x + y);
+                        }
+                    }
+                }
+            } else {
+                const int r = (t.m0 + g) * a.tile_rows + row / group;
+                const bool query = there && row < a.tile_rows * group && r < t.rows;
+                const int sees = min(t.entries, t.start + r + 1);                       // entries that this lane's row sees
+                const int first = min(t.entries, t.start + (t.m0 + g) * a.tile_rows + 1);  // .. and the tile's first row
+                float ref = -INFINITY, l = 0.f;
+                for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
+                    const int buf = bi & 1, k0 = (t.b0 + b * a.parts) * KT_TILE;
+                    ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (bi >> 1) & 1, a.err, 77, &abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    // 64 scores at a time under a reference that the first ones seen set: below 2^100 a sum is as good under
+                    // any reference, above it the reference is raised.
+                    if (__any_sync(0xffffffffu, query && k0 < sees)) {
+                        const bool edge = k0 + KT_TILE > first;
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t v[2][32];
+                            tc_ld32_nowait(tmem_row + 128u * buf + 64u * c, v[0]);
+                            tc_ld32_nowait(tmem_row + 128u * buf + 64u * c + 32u, v[1]);
+                            tc_ld_wait();
+                            if (edge) {
+#pragma unroll
+                                for (int j = 0; j < 64; ++j)
+                                    if (k0 + 64 * c + j >= sees) v[j >> 5][j & 31] = 0xff800000u;
+                            }
+                            auto pass = [&](float m) -> float {
+                                uint64_t s2[4] = {0ull, 0ull, 0ull, 0ull};
+                                const uint64_t nm2 = pack2(-m, -m);
+#pragma unroll
+                                for (int j = 0; j < 64; j += 2) {
+                                    float x, y;
+                                    unpack2(fma2(pack2(__uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1])), scale2, nm2), x, y);
+                                    s2[j / 2 % 4] = add2(s2[j / 2 % 4], pack2(ex2(x), ex2(y)));
+                                }
+                                float x, y;
+                                unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), x, y);
+                                return x + y;
+                            };
+                            float sum = pass(ref == -INFINITY ? 0.f : ref);
+                            if (__any_sync(0xffffffffu, query && (ref == -INFINITY || !(sum < 0x1p100f)))) {
+                                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                                for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j >> 5][j & 31]));
+                                const float m = fmaxf(ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.w.scale_log2);
+                                if (m > ref) { l *= ex2(ref - m); ref = m; }            // ref -inf: l is 0
+                                sum = pass(ref == -INFINITY ? 0.f : ref);
+                            }
+                            l += sum;
+                        }
+                    }
+                    tc_fence_before();
+                    mbar_arrive(s_empty + 16 * g + 8 * buf);
+                }
+                if (query && ok) {
+                    const size_t at = (size_t)(t.row0 + r) * a.w.nh + t.kvh * group + row % group;
+                    if (a.parts == 1) a.w.z[at] = l > 0.f ? ref + log2f(l) : INFINITY;
+                    else *reinterpret_cast<float2*>(a.part_ml + (at * a.parts + t.part) * 2) = make_float2(ref, l);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (abort_flag) {                                                // give copies in flight time to land
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_free(tmem, 512u);
+    }
+}
+
+// z of every query of every request from its parts.
+__global__ void __launch_bounds__(256) join_row_sums_kernel(const KtArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)a.w.T * a.w.nh) return;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + i * a.row_parts;
+    float m = -INFINITY, l = 0.f;
+    for (int p = 0; p < a.row_parts; ++p) {
+        const float2 x = ml[p];
+        const float n = fmaxf(m, x.x), ref = n == -INFINITY ? 0.f : n;
+        l = l * ex2(m - ref) + x.y * ex2(x.x - ref);
+        m = n;
+    }
+    a.w.z[i] = l > 0.f ? m + log2f(l) : INFINITY;
+}
+
+// The weights from the second pass's parts, in the parts' order.  grid (entries / 256, nkv, R)
+__global__ void __launch_bounds__(256) join_entry_sums_kernel(const KtArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const int r = blockIdx.z, kvh = blockIdx.y, e = blockIdx.x * 256 + threadIdx.x, slot = a.w.slots[r];
+    int row0, rows, start, entries;
+    rows_of(a.w, r, row0, rows, start, entries);
+    if (e >= entries || slot < 0 || slot >= a.w.n_slots) return;
+    float* w = a.w.weights + ((size_t)slot * a.w.nkv + kvh) * a.w.weights_ld + e;
+    float sum = 0.f;
+    for (int p = 0; p < a.parts; ++p) sum += a.part_w[(((size_t)p * a.w.R + r) * a.w.nkv + kvh) * a.w.limit + e];
+    *w = (e < a.w.fresh[r] ? *w : 0.f) + sum;
+}
+
+// The queries as the tensor cores' kernel reads them: 64 columns of a head, heads, rows; a box of one kv head's and `rows` rows.
+static int make_q_map(CUtensorMap* map, const void* q, int T, int q_stride, int nh, int d, int heads, int rows) {
+    RgEncodeTiledFn fn = rg_encode_fn();
+    if (!fn) return RG_ERR_UNSUPPORTED;
+    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)nh, (cuuint64_t)T}, strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)q_stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)heads, (cuuint32_t)rows}, estr[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
+}
+
+template <int PIECES>
+static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int max_context, cudaStream_t s) {
+    constexpr int smem = (4 + kt_b_stages(PIECES)) * KT_TILE * 128 * PIECES + 1024;
+    const WeightArgs& w = rows.w;
+    CUtensorMap qm, km;
+    int e = make_q_map(&qm, w.q, w.T, w.q_stride, w.nh, w.d, w.nh / w.nkv, rows.tile_rows);
+    if (e) return e;
+    e = rg_make_map(&km, w.kv, (unsigned long long)num_pages * 2 * w.nkv * w.page_size, w.d, w.d, min(w.page_size, KT_TILE));
+    if (e) return e;
+    int dev = 0, sms = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (ce == cudaSuccess)
+        ce = cudaFuncSetAttribute(key_weights_tc_kernel<PIECES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (ce == cudaSuccess) ce = cudaFuncSetAttribute(key_weights_tc_kernel<PIECES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (ce != cudaSuccess) return (int)ce;
+    e = rg_launch(key_weights_tc_kernel<PIECES, false>, dim3(min(sms, rows.n_items)), dim3(KT_THREADS), smem, s, 1, qm, km, rows);
+    if (!e && rows.parts > 1)
+        e = rg_launch(join_row_sums_kernel, dim3((unsigned)(((long long)w.T * w.nh + 255) / 256)), dim3(256), 0, s, 1, rows);
+    if (!e) e = rg_launch(key_weights_tc_kernel<PIECES, true>, dim3(min(sms, entries.n_items)), dim3(KT_THREADS), smem, s, 1, qm, km, entries);
+    if (!e && entries.parts > 1)
+        e = rg_launch(join_entry_sums_kernel, dim3((max_context + 255) / 256, w.nkv, w.R), dim3(256), 0, s, 1, entries);
+    return e;
+}
+
+// max_rows: the most rows of a request; max_context: the most entries a row sees.  Scratch: z [T, nh]; for the tensor cores'
+// kernels (row_parts > 0; the caller has seen to what they take) part_ml [T, nh, row_parts, 2] where row_parts > 1 and part_w
+// [entry_parts, R, nkv, max_context] where entry_parts > 1.
+extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv, int num_pages, int dtype, float* weights, int weights_ld,
                                      int n_slots, const int* slots, const int* block_table, int max_blocks, const int* cu_rows,
                                      const int* starts, const int* fresh, int R, int T, int nh, int nkv, int d, int page_size,
-                                     float scale, int max_rows, int max_context, float* z, void* stream) {
+                                     float scale, int max_rows, int max_context, float* z, int row_parts, float* part_ml,
+                                     int entry_parts, float* part_w, int* err, void* stream) {
     if (R <= 0 || T <= 0 || max_rows <= 0 || max_context <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_context > weights_ld || R > 65535 || nkv > 65535 ||
         (long long)max_rows * (nh / nkv) > 0x7fffffffll)
@@ -195,8 +603,28 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
                           nh, nkv, d, page_size, (int)min((long long)max_context, (long long)max_blocks * page_size),
                           scale * 1.4426950408889634f};
     const cudaStream_t s = (cudaStream_t)stream;
+    const int group = nh / nkv;
+    if (row_parts > 0) {
+        int shift = -1;
+        for (int b = 3; b < 31; ++b) if (page_size == (1 << b)) shift = b;
+        if (dtype != RG_DTYPE_BF16 || (d != 64 && d != 128) || group > KT_TILE || shift < 0 || q_stride % 8 || ((uintptr_t)q & 15) ||
+            ((uintptr_t)kv & 15) || scale <= 0.f || entry_parts < 1 || (long long)num_pages * 2 * nkv * page_size > 0x7fffffffll)
+            return RG_ERR_UNSUPPORTED;
+        KtArgs rows = {a, part_ml, nullptr, err, 0, row_parts, 0, row_parts, KT_TILE / group, shift}, entries = rows;
+        const long long q_tiles = (max_rows + rows.tile_rows - 1) / rows.tile_rows, e_tiles = (max_context + KT_TILE - 1) / KT_TILE;
+        rows.blocks = (int)((q_tiles + 1) / 2);
+        entries.blocks = (int)((e_tiles + 1) / 2);
+        entries.parts = entry_parts;
+        entries.part_w = entry_parts > 1 ? part_w : nullptr;
+        const long long n_rows = (long long)rows.blocks * R * nkv * row_parts, n_entries = (long long)entries.blocks * R * nkv * entry_parts;
+        if (n_rows > 0x3fffffffll || n_entries > 0x3fffffffll) return RG_ERR_UNSUPPORTED;
+        rows.n_items = (int)n_rows;
+        entries.n_items = (int)n_entries;
+        return d == 64 ? launch_key_weights_tc<1>(rows, entries, num_pages, max_context, s)
+                       : launch_key_weights_tc<2>(rows, entries, num_pages, max_context, s);
+    }
     const size_t smem = (size_t)((KW_Q + KW_K) * kw_row(d) + 8 * KW_K) * sizeof(float);
-    const dim3 by_query((max_rows * (nh / nkv) + KW_Q - 1) / KW_Q, nkv, R), by_entry((max_context + KW_K - 1) / KW_K, nkv, R);
+    const dim3 by_query((max_rows * group + KW_Q - 1) / KW_Q, nkv, R), by_entry((max_context + KW_K - 1) / KW_K, nkv, R);
 #define RG_KW(A) { cudaError_t ce = cudaFuncSetAttribute(row_sums_general_kernel<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
     if (ce == cudaSuccess) ce = cudaFuncSetAttribute(entry_sums_general_kernel<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
     if (ce != cudaSuccess) return (int)ce; \

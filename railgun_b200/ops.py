@@ -2280,6 +2280,12 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         "weighed_attention")
 
 
+def key_weight_parts(items: int, tiles: int, room: int = 592) -> int:
+    """Parts that the streamed side of ``prompt_key_weights`` is cut into: until there are four items an SM, of four tiles at
+    least."""
+    return max(1, min(-(-room // max(1, items)), -(-tiles // 4), 32))
+
+
 def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts, fresh, nh: int, nkv: int, d: int, scale: float,
                        max_rows: int, max_context: int) -> None:
     """The weights that entries receive from portions of prompts, or from the last rows of prompts: request r's rows of ``q``
@@ -2299,12 +2305,25 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     if min(max_rows, max_context) < 0:
         raise KernelError("prompt_key_weights: max_rows and max_context are counts")
     _check_entry_weights(weights, "weights", nkv, max_context)
-    z = torch.empty(q.shape[0] * nh, dtype=torch.float32, device=q.device)
-    _COUNTER.value += 1                          # the rows' sums, then the entries'
+    T, G, row_parts, entry_parts = q.shape[0], nh // nkv, 0, 0
+    floats = n_z = -(-T * nh // 4) * 4
+    if (q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and page_size >= 8 and page_size & (page_size - 1) == 0
+            and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and kv_cache.data_ptr() % 16 == 0 and scale > 0
+            and kv_cache.numel() // d < 1 << 31):
+        # tiles of 128 queries and of 128 entries: one kind stays, two at a time, and the other streams by in parts
+        q_tiles, e_tiles = -(-max_rows // (128 // G)), -(-max_context // 128)
+        row_parts = key_weight_parts(R * nkv * -(-q_tiles // 2), e_tiles)
+        entry_parts = key_weight_parts(R * nkv * -(-e_tiles // 2), q_tiles)
+        floats += (T * nh * row_parts * 2 if row_parts > 1 else 0) + (R * nkv * max_context * entry_parts if entry_parts > 1 else 0)
+    z = torch.empty(floats, dtype=torch.float32, device=q.device)
+    part_ml = z.data_ptr() + 4 * n_z
+    part_w = part_ml + (8 * T * nh * row_parts if row_parts > 1 else 0)
+    _COUNTER.value += 1 + (row_parts > 1) + (entry_parts > 1)      # the rows' sums, then the entries', and what joins their parts
     _ok(_fn("key_weights", "rg_prompt_key_weights")(
-        _ptr(q), c_int(q.stride(0)), _ptr(kv_cache), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
+        _ptr(q), c_int(q.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
         _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(q.shape[0]),
-        c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z), _stream()),
+        c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z),
+        c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), _ptr(_tc_error_flag(q.device)), _stream()),
         "prompt_key_weights")
 
 

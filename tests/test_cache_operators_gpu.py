@@ -14,6 +14,13 @@ DEV = "cuda:0"
 U = 2.0 ** -24                                   # half a unit in the last place of a 32-bit number at 1
 
 
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    from railgun_b200 import ops
+    ops.tc_gemm_check()
+
+
 def i32(v):
     return torch.tensor(v, dtype=torch.int32, device=DEV)
 
