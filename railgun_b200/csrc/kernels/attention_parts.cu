@@ -3,8 +3,7 @@
 // are cut and joined.
 #include "attention_parts.cuh"
 #include "mma.cuh"
-#include "tcgen05.cuh"
-using rgmma::ex2;
+#include "attention_prefix_tcgen05.cuh"
 using rgmma::mma_bf16;
 using rgmma::pack_bf16;
 
@@ -204,10 +203,6 @@ __host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 6
 __host__ __device__ constexpr int pm_stage_bytes(int pieces) { return 16 * 64 * 2 * 2 * pieces; }
 static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1) * pm_stage_bytes(1), "the warps' results fit where the stages were");
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int y) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %3}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(y) : "memory");
-}
 __device__ __forceinline__ void ldmatrix_x4_at(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -231,10 +226,16 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
         for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
     if (lane == 0) fence_barrier_init();
     __syncthreads();
-    pdl_wait();
+    // beside: the launch before this one is prefix_tc_kernel for the same rows, whose blocks have all waited for what came
+    // before them; it leaves its own parts.  What comes behind this kernel waits for both: the last block waits at its end.
+    if (!a.beside) pdl_wait();
     pdl_trigger();
     PartShare sh;
-    if (!part_share(a, PM_Q, blockIdx.x, sh)) return;
+    const bool closes = a.beside && blockIdx.x == gridDim.x - 1;
+    if (!part_share(a, PM_Q, blockIdx.x, sh)) {
+        if (closes) pdl_wait();
+        return;
+    }
     const int group = a.nh / a.nkv;
     const int n_runs = (sh.e1 - sh.e0 + 15) >> 4, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
     // Page ids of this warp's next 32 runs, one a lane (of both halves of a run where pages hold 8).
@@ -253,8 +254,8 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
             const int s = i % STAGES, in_page = entry_of(i) & (a.page_size - 1);
             const uint32_t bar = bar0 + 8 * s, dst = base + s * STAGE;
             mbar_expect_tx(bar, STAGE);
-            tma_load_4d(dst, &kv_map, bar, (pa * 2 * a.nkv + sh.kvh) * a.page_size + in_page);
-            if (box_shift == 3) tma_load_4d(dst + STAGE / 2, &kv_map, bar, (pb * 2 * a.nkv + sh.kvh) * a.page_size);
+            tma_load_4d_row(dst, &kv_map, bar, (pa * 2 * a.nkv + sh.kvh) * a.page_size + in_page);
+            if (box_shift == 3) tma_load_4d_row(dst + STAGE / 2, &kv_map, bar, (pb * 2 * a.nkv + sh.kvh) * a.page_size);
         }
         __syncwarp();
     };
@@ -392,6 +393,7 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
         *reinterpret_cast<float4*>(a.part_o + place * D + c) = sum;
         if (c == 0) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(M, L);
     }
+    if (closes) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -552,12 +554,13 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 }
 
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
-// [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].
+// [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].  tensor_cores: 1 the prefixes by prefix_tc_kernel, 2 the same with two
+// parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.
 extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                    const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
                                    int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,
                                    int own_parts, int own_per, int T, int nh, int nkv, int d, int page_size, float scale,
-                                   float* part_o, float* part_ml, int* err, void* stream) {
+                                   float* part_o, float* part_ml, int tensor_cores, int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
@@ -568,10 +571,23 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
     a.prefix_parts = prefix_parts; a.prefix_per = prefix_per;
     a.prefix_limit = (int)min(0x7fffffffll, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
     if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
-    a.prefix_tiles = (max_rows * group + PG_Q - 1) / PG_Q;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
-    int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
-    if (e) return e;
+    if (tensor_cores) {
+        if (!prefix_tc_ok(a, dtype, num_pages)) return RG_ERR_UNSUPPORTED;
+        const int tile_rows = (tensor_cores == 2 ? 1 : 2) * (PT_SIDE / group);
+        a.prefix_tiles = (max_rows + tile_rows - 1) / tile_rows;
+        int e = launch_prefix_tc(a, num_pages, tensor_cores == 2, err, (cudaStream_t)stream);
+        if (e) return e;
+        PartArgs own = a;                                            // their own entries, beside the prefixes
+        own.n_groups = 0;
+        own.beside = a.n_groups > 0 && rg_pdl_enabled;
+        e = launch_parts(own, dtype, num_pages, err, (cudaStream_t)stream);
+        if (e) return e;
+    } else {
+        a.prefix_tiles = (max_rows * group + PG_Q - 1) / PG_Q;
+        int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
+        if (e) return e;
+    }
     if (dtype == RG_DTYPE_F32)
         return rg_launch(join_kernel<float>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
     return rg_launch(join_kernel<bf16>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);

@@ -27,6 +27,7 @@ struct PartArgs {
     int prefix_limit, own_limit;                        // the most entries that tables, parts and scratch have room for
     int T, nh, nkv, d, page_size, page_shift;           // page_shift: log2 of the page size, or -1
     float scale_log2;
+    int beside;                  // the kernel before this one writes nothing that this one reads, and the other way round
 };
 
 // One block's share: the queries [q0, q0 + nq) of (first row, kv head), query i being row row0 + i / group, head

@@ -245,11 +245,6 @@ __device__ __forceinline__ bool kt_item(const KtArgs& a, int i, KtItem& t) {
     return t.n_m > 0;
 }
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
-}
-
 // q_map: 64 columns x heads x rows, a box of 64 x group x tile_rows; kv_map: the cache as rows of the head size, a box of
 // min(page, 128) rows x 64 columns.
 template <int PIECES, bool ENTRIES>

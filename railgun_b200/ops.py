@@ -2207,6 +2207,21 @@ def _tc_error_flag(device) -> torch.Tensor:
     return err
 
 
+def _row_maps_ok(q, kv_cache, scale: float) -> bool:
+    """Can TMA read these rows of queries, and pages of this size, in tiles?"""
+    page_size = kv_cache.shape[3]
+    return (page_size >= 8 and page_size & (page_size - 1) == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
+            and kv_cache.data_ptr() % 16 == 0 and scale > 0 and kv_cache.numel() // kv_cache.shape[4] < (1 << 31) - 1)
+
+
+def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int) -> tuple:
+    """(parts, entries a part) of prefixes of up to ``longest`` entries, of which ``blocks`` thread blocks, one an SM, read a
+    part each (two each where ``tensor_cores`` is 2): whole tiles of 128 entries, as many parts as fill the GPU once."""
+    parts = max(1, sms // max(1, blocks)) * tensor_cores
+    per = -(--(-longest // parts) // 128) * 128
+    return -(-longest // per), per
+
+
 def attention_parts(blocks: int, longest: int, room: int = 444, least: int = 128) -> tuple:
     """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would
     read a list in one part each: as many parts as fill the GPU once (``room`` blocks, three an SM), of whole tiles of 64
@@ -2238,16 +2253,24 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     if min(max_rows, max_prefix, max_own) < 0:
         raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
     n_groups, G = groups.shape[0], nh // nkv
-    p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), max_prefix if n_groups and max_rows else 0)
+    longest, tensor_cores = max_prefix if n_groups and max_rows else 0, 0
+    if (q.dtype == torch.bfloat16 and d in (64, 128) and 16 < max_rows * G and G <= 128 and longest >= 256 and _row_maps_ok(q, kv_cache, scale)):
+        # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
+        side = 128 // G
+        tensor_cores = 1 if max_rows > side else 2
+        p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, num_sms(q.device), tensor_cores)
+    else:
+        p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest)
     o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own)
     slots = T * nh * (p_parts + o_parts)
     parts = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
-    _COUNTER.value += 1                          # the parts, and the kernel that joins them
+    _COUNTER.value += 2 if tensor_cores and o_parts else 1         # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_prefix_attention")(
         _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(prefix_table),
         c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
+        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d),
+        c_int(tensor_cores), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
 
 
 def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, nh: int, nkv: int, d: int, scale: float,
@@ -2307,9 +2330,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     _check_entry_weights(weights, "weights", nkv, max_context)
     T, G, row_parts, entry_parts = q.shape[0], nh // nkv, 0, 0
     floats = n_z = -(-T * nh // 4) * 4
-    if (q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and page_size >= 8 and page_size & (page_size - 1) == 0
-            and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and kv_cache.data_ptr() % 16 == 0 and scale > 0
-            and kv_cache.numel() // d < 1 << 31):
+    if q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, kv_cache, scale):
         # tiles of 128 queries and of 128 entries: one kind stays, two at a time, and the other streams by in parts
         q_tiles, e_tiles = -(-max_rows // (128 // G)), -(-max_context // 128)
         row_parts = key_weight_parts(R * nkv * -(-q_tiles // 2), e_tiles)
