@@ -6,18 +6,15 @@
 // length move: the i-th of them goes into the i-th entry before it that got free.  Sources lie at k and beyond, destinations
 // before k: the moves of K and V rows are independent of one another, and of the fewest bytes there can be.
 //
-// One cluster per (request, kv head).  The k-th greatest key is found by three passes over its bits (11, 11 and 10, from
-// the top): a histogram in shared memory, added up over the cluster, and a sum from the top bin down.  Then every warp walks
-// consecutive entries, 32 at a time, and numbers ties, free entries and late ones by ballots, with the counts of the warps and
-// blocks before it.  Lists of destinations and sources go through global scratch (they stay in L2); the cluster's warps then
-// move a row each.
+// One block per (request, kv head), or a cluster of them.  A warp holds consecutive entries' keys, a key of each run of 32 a
+// lane, in registers.  The k-th greatest key is found by cutting the interval that holds it into four: three counts a step,
+// added up over the block (and the cluster); a step whose count is k ends the search, since the keys above it are the k
+// that stay (without ties about as many steps as n has digits to the base 4, and a few).  Then ties, free entries and late
+// ones are numbered by ballots, with the counts of the warps and blocks before.  A warp takes up to 32 moves at a time: their
+// addresses a lane each, then their rows in 16-byte pieces, several a lane under way.
 #include "common.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;
-
-#define EV_THREADS 512
-#define EV_WARPS (EV_THREADS / 32)
-#define EV_BINS 2048
 
 struct EvictArgs {
     void* kv;                    // [pages, 2, nkv, page_size, d], `row_bytes` a row
@@ -43,178 +40,219 @@ __device__ __forceinline__ uint32_t weight_key(const EvictArgs& a, float w, int 
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Exclusive sum over the block's threads, by thread; total: of all.  scratch: EV_WARPS + 1 ints.
-__device__ __forceinline__ int block_scan(int v, int* scratch, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int s = v;
+// Sums over warps: what every warp's lane 0 gives, for all warps of the block (cluster).
+template <int WARPS, int N, bool CLUSTERED>
+struct Sums {
+    int (*all)[WARPS][N];        // shared memory, two of them in turn: one barrier a sum
+    int turn;
+    // total: over all; before: over the warps before this one, of blocks before this one as well
+    __device__ __forceinline__ void of(const int (&mine)[N], int (&total)[N], int (&before)[N]) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        int (*now)[N] = all[turn];
+        turn ^= 1;
+        if (lane < N) {
+            int v = mine[0];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += u;
-    }
-    __syncthreads();
-    if (lane == 31) scratch[warp] = s;
-    __syncthreads();
-    int before = 0;
-    total = 0;
+            for (int i = 1; i < N; ++i) v = lane == i ? mine[i] : v;
+            now[warp][lane] = v;
+        }
 #pragma unroll
-    for (int w = 0; w < EV_WARPS; ++w) {
-        const int c = scratch[w];
-        if (w < warp) before += c;
-        total += c;
+        for (int i = 0; i < N; ++i) total[i] = before[i] = 0;
+        auto add = [&](const int (*from)[N], bool earlier) {         // a warp's numbers a lane, then over the lanes
+            const int w = lane < WARPS ? lane : 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int v = lane < WARPS ? from[w][i] : 0;
+                total[i] += __reduce_add_sync(0xffffffffu, v);
+                before[i] += __reduce_add_sync(0xffffffffu, earlier || (from == now && lane < warp) ? v : 0);
+            }
+        };
+        if constexpr (CLUSTERED) {
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();
+            for (int q = 0; q < (int)cluster.num_blocks(); ++q) {
+                if (q == (int)cluster.block_rank()) add(now, false);
+                else add(cluster.map_shared_rank(now, q), q < (int)cluster.block_rank());
+            }
+        } else {
+            __syncthreads();
+            add(now, false);
+        }
     }
-    return before + s - v;
-}
+};
 
-template <bool CACHED>          // the block's keys fit its shared memory
-__global__ void __launch_bounds__(EV_THREADS) evict_kernel(const EvictArgs a) {
-    extern __shared__ uint32_t keys[];
-    __shared__ int hist[EV_BINS], scan[EV_WARPS + 1], found[3], counts[4];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int C = cluster.num_blocks(), rank = cluster.block_rank();
+template <int THREADS, int PER, bool CLUSTERED>       // PER: keys a thread holds; 0: they are made anew whenever one is asked for
+__global__ void __launch_bounds__(THREADS) evict_kernel(const EvictArgs a) {
+    constexpr int WARPS = THREADS / 32, DEEP = THREADS > 512 ? 4 : 8;    // pieces a lane under way: 64 KB a block or less
+    extern __shared__ int lists[];                                   // destinations and sources, without a cluster
+    __shared__ int sums_of[2][WARPS][3];
+    const int C = CLUSTERED ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTERED ? (int)cg::this_cluster().block_rank() : 0;
     // No early start for the kernel behind this one: attention kernels ask for cached keys ahead of their own wait.
     pdl_wait();
     const int row = blockIdx.x / C, r = row / a.nkv, h = row % a.nkv;
     const int slot = a.slots[r], n = min(a.lens[r], a.limit), k = min(n, max(0, a.keep[r])), newest = a.positions[r];
-    if (slot < 0 || slot >= a.n_slots || n <= 0) {                  // the same for the whole cluster
-        if (h == 0 && rank == 0 && threadIdx.x == 0) a.new_lens[r] = a.lens[r];
-        return;
-    }
-    if (h == 0 && rank == 0 && threadIdx.x == 0) a.new_lens[r] = k;
+    const bool alone = slot < 0 || slot >= a.n_slots || n <= 0;      // the same for the whole cluster
+    if (h == 0 && rank == 0 && threadIdx.x == 0) a.new_lens[r] = alone ? a.lens[r] : k;
+    if (alone) return;
     const size_t base = ((size_t)slot * a.nkv + h) * a.ld;
     const float* w = a.weights + base;
     const int* places = a.places + base;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // this block's entries, in runs of whole warps: [c0, c1), a warp's share `run` of them
-    const int run = ((n + C * EV_WARPS - 1) / (C * EV_WARPS) + 31) & ~31;
-    const int c0 = min(n, rank * run * EV_WARPS), c1 = min(n, c0 + run * EV_WARPS);
-    auto key_of = [&](int e) -> uint32_t { return CACHED ? keys[e - c0] : weight_key(a, w[e], places[e], newest); };
-    int *dst = a.moves + (size_t)row * 2 * (a.limit / 2 + 1), *src = dst + a.limit / 2 + 1;
-    int n_moves = 0;
+    // this warp's entries: `run` runs of 32 from w0 on
+    const int run = (n + C * THREADS - 1) / (C * THREADS), w0 = (rank * WARPS + warp) * run * 32;
+    uint32_t held[PER ? PER : 1];
+    if constexpr (PER > 0) {
+        float wv[PER];
+        int pv[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int e = w0 + j * 32 + lane;
+            const bool there = j < run && e < n;
+            wv[j] = there ? w[e] : 0.f;
+            pv[j] = there ? places[e] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) held[j] = weight_key(a, wv[j], pv[j], newest);
+    }
+    // f(run, entry, its key, is there such an entry): for every run of the warp, all lanes together
+    auto each = [&](auto f) {
+        if constexpr (PER > 0) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (j < run) { const int e = w0 + j * 32 + lane; f(j, e, held[j], e < n); }
+        } else {
+            for (int j = 0; j < run; ++j) {
+                const int e = w0 + j * 32 + lane;
+                f(j, e, e < n ? weight_key(a, w[e], places[e], newest) : 0u, e < n);
+            }
+        }
+    };
+    Sums<WARPS, 3, CLUSTERED> sums = {sums_of, 0};
+    int n_moves = 0, total[3], before[3];
+    int *dst = CLUSTERED ? a.moves + (size_t)row * 2 * (a.limit / 2 + 1) : lists, *src = dst + a.limit / 2 + 1;
     if (k < n) {
-        if (CACHED) {
-            for (int e = c0 + tid; e < c1; e += EV_THREADS) keys[e - c0] = weight_key(a, w[e], places[e], newest);
-        }
-        // the k-th greatest key: `high` its bits so far, `left` how many of the entries with these bits stay
-        uint32_t high = 0;
-        int left = k;
-#pragma unroll 1
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-            __syncthreads();
-            for (int e = c0 + tid; e < c1; e += EV_THREADS) {
-                const uint32_t key = key_of(e);
-                if (pass == 0 || key >> (shift + bits) == high >> (shift + bits)) atomicAdd(&hist[key >> shift & ((1 << bits) - 1)], 1);
-            }
-            cluster.sync();
-            // bins from the top down, 4 a thread; only counts that are whole numbers are added: any order gives the same
-            int c[EV_BINS / EV_THREADS], mine = 0, total;
+        // The k-th greatest key lies in [lo, hi): at least k keys are lo or above, `above` < k are hi or above.
+        unsigned long long lo = 0, hi = 1ull << 32;
+        int above = 0;
+        bool exact = k == 0;                                         // the keys from hi on are just those that stay
+        while (hi - lo > 1 && !exact) {
+            const unsigned long long step = hi - lo > 4 ? (hi - lo) / 4 : 1;
+            const uint32_t t1 = (uint32_t)(lo + step), t2 = (uint32_t)min(lo + 2 * step, hi - 1), t3 = (uint32_t)min(lo + 3 * step, hi - 1);
+            int c[3] = {0, 0, 0};
+            each([&](int, int, uint32_t key, bool there) {
+                c[0] += there && key >= t1;
+                c[1] += there && key >= t2;
+                c[2] += there && key >= t3;
+            });
 #pragma unroll
-            for (int j = 0; j < EV_BINS / EV_THREADS; ++j) {
-                const int bin = EV_BINS - 1 - (tid * (EV_BINS / EV_THREADS) + j);
-                c[j] = 0;
-                for (int q = 0; q < C; ++q) c[j] += cluster.map_shared_rank(hist, q)[bin];
-                mine += c[j];
-            }
-            int above = block_scan(mine, scan, total);
-#pragma unroll
-            for (int j = 0; j < EV_BINS / EV_THREADS; ++j) {
-                if (above < left && left <= above + c[j]) {
-                    found[0] = EV_BINS - 1 - (tid * (EV_BINS / EV_THREADS) + j);
-                    found[1] = left - above;
-                }
-                above += c[j];
-            }
-            cluster.sync();                                         // histograms are read, `found` is there
-            if (k > 0) { high |= (uint32_t)found[0] << shift; left = found[1]; }
+            for (int i = 0; i < 3; ++i) c[i] = __reduce_add_sync(0xffffffffu, c[i]);
+            sums.of(c, total, before);
+            if (total[2] == k || total[1] == k || total[0] == k) {
+                hi = total[2] == k ? t3 : (total[1] == k ? t2 : t1);
+                exact = true;
+            } else if (total[2] > k) { lo = t3; }
+            else if (total[1] > k) { lo = t2; hi = t3; above = total[2]; }
+            else if (total[0] > k) { lo = t1; hi = t2; above = total[1]; }
+            else { hi = t1; above = total[0]; }
         }
-        // k = 0: nothing stays, and no bin is found
-        const uint32_t kth = k > 0 ? high : 0xffffffffu;
-        // Ties before each entry: counts of the blocks and warps before, then ballots.
-        const int w0 = min(c1, c0 + warp * run), w1 = min(c1, w0 + run);
-        auto before_me = [&](int mine, int which) -> int {          // the sum of `mine` (a warp's) over all warps before this one
-            int total;
-            const int in_block = block_scan(lane == 0 ? mine : 0, scan, total);
-            if (tid == 0) counts[which] = total;
-            cluster.sync();
-            int sum = __shfl_sync(0xffffffffu, in_block, 0);
-            for (int q = 0; q < rank; ++q) sum += cluster.map_shared_rank(counts, q)[which];
-            return sum;
-        };
-        int ties = 0;
-        for (int e = w0 + lane; e - lane < w1; e += 32) ties += __popc(__ballot_sync(0xffffffffu, e < w1 && key_of(e) == kth));
-        int tie = before_me(ties, 0);
-        // which entries stay; how many of this warp's get free or come late
-        int free_n = 0, late_n = 0, t2 = tie;
-        auto stays = [&](int e, int& t) -> bool {
-            const uint32_t key = e < w1 ? key_of(e) : 0u;
-            const bool eq = e < w1 && key == kth;
-            const uint32_t all = __ballot_sync(0xffffffffu, eq);
-            const bool in = e < w1 && (key > kth || (eq && t + __popc(all & ((1u << lane) - 1)) < left)) && k > 0;
-            t += __popc(all);
+        // what stays: keys from hi on, and of those that are lo the first `left`
+        const int left = exact ? 0 : k - above;
+        const uint32_t from = (uint32_t)hi, kth = (uint32_t)lo;
+        const bool none_above = hi >> 32 || k == 0;                  // hi is above every key
+        int tie = 0;
+        if (!exact) {
+            int c[3] = {0, 0, 0};
+            each([&](int, int, uint32_t key, bool there) { c[0] += __popc(__ballot_sync(0xffffffffu, there && key == kth)); });
+            sums.of(c, total, before);
+            tie = before[0];
+        }
+        const uint32_t below = (1u << lane) - 1;
+        auto stays = [&](uint32_t key, bool there, int& t) -> bool {
+            bool in = there && !none_above && key >= from;
+            if (!exact) {
+                const uint32_t all = __ballot_sync(0xffffffffu, there && key == kth);
+                in = in || (there && key == kth && t + __popc(all & below) < left);
+                t += __popc(all);
+            }
             return in;
         };
-        for (int e = w0 + lane; e - lane < w1; e += 32) {
-            const bool in = stays(e, t2);
-            free_n += __popc(__ballot_sync(0xffffffffu, e < w1 && e < k && !in));
-            late_n += __popc(__ballot_sync(0xffffffffu, e < w1 && e >= k && in));
-        }
-        int free_at = before_me(free_n, 1), late_at = before_me(late_n, 2);
-        for (int e = w0 + lane; e - lane < w1; e += 32) {
-            const bool in = stays(e, tie), gone = e < w1 && e < k && !in, late = e < w1 && e >= k && in;
+        int c[3] = {0, 0, 0}, t2 = tie;
+        each([&](int, int e, uint32_t key, bool there) {
+            const bool in = stays(key, there, t2);
+            c[0] += __popc(__ballot_sync(0xffffffffu, there && e < k && !in));
+            c[1] += __popc(__ballot_sync(0xffffffffu, there && e >= k && in));
+        });
+        sums.of(c, total, before);
+        n_moves = total[1];
+        each([&](int, int e, uint32_t key, bool there) {
+            const bool in = stays(key, there, tie), gone = there && e < k && !in, late = there && e >= k && in;
             const uint32_t f = __ballot_sync(0xffffffffu, gone), l = __ballot_sync(0xffffffffu, late);
-            if (gone) dst[free_at + __popc(f & ((1u << lane) - 1))] = e;
-            if (late) src[late_at + __popc(l & ((1u << lane) - 1))] = e;
-            free_at += __popc(f);
-            late_at += __popc(l);
+            if (gone) dst[before[0] + __popc(f & below)] = e;
+            if (late) src[before[1] + __popc(l & below)] = e;
+            before[0] += __popc(f);
+            before[1] += __popc(l);
             if (in && e < k) {
                 a.weights_out[base + e] = w[e];
                 a.places_out[base + e] = places[e];
             }
-        }
-        __threadfence();
-        cluster.sync();                                             // the lists are whole
-        for (int q = 0; q < C; ++q) n_moves += cluster.map_shared_rank(counts, q)[2];
-        cluster.sync();                                             // nobody leaves while its counts are read
+        });
+        if constexpr (CLUSTERED) { __threadfence(); cg::this_cluster().sync(); }
+        else __syncthreads();                                        // the lists are whole, and nobody reads another block's sums any more
     } else {
-        for (int e = c0 + tid; e < c1; e += EV_THREADS) {
-            a.weights_out[base + e] = w[e];
-            a.places_out[base + e] = places[e];
-        }
+        each([&](int, int e, uint32_t, bool there) {
+            if (there) {
+                a.weights_out[base + e] = w[e];
+                a.places_out[base + e] = places[e];
+            }
+        });
     }
-    // The moves, a warp each.
+    // The moves.  Rows are `pieces` pieces of 16 bytes, K and V one after the other; or, where rows are not made of those, bytes.
     const int* table = a.block_table + (size_t)r * a.max_blocks;
-    const size_t half = (size_t)a.nkv * a.page_size * a.row_bytes;  // bytes of a page's keys, or values
-    auto at = [&](int e) -> unsigned char* {
-        return (unsigned char*)a.kv + (size_t)table[e / a.page_size] * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
+    const size_t half = (size_t)a.nkv * a.page_size * a.row_bytes;   // bytes of a page's keys, or values
+    const bool wide = a.row_bytes % 16 == 0 && ((uintptr_t)a.kv & 15) == 0;
+    auto at = [&](int e) -> size_t {
+        return (size_t)table[e / a.page_size] * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
     };
-    for (int i = rank * EV_WARPS + warp; i < n_moves; i += C * EV_WARPS) {
-        const int to = __ldcg(dst + i), from = __ldcg(src + i);
-        unsigned char *pt = at(to), *pf = at(from);
-        if (a.row_bytes % 16 == 0 && ((uintptr_t)a.kv & 15) == 0) {
-            const int n16 = a.row_bytes / 16;
-            for (int j = lane; j < 2 * n16; j += 32) {
-                const size_t off = j < n16 ? (size_t)j * 16 : half + (size_t)(j - n16) * 16;
-                *reinterpret_cast<uint4*>(pt + off) = *reinterpret_cast<const uint4*>(pf + off);
-            }
-        } else {
-            for (int j = lane; j < a.row_bytes; j += 32) {           // rows of 2 or 4 bytes an element
-                pt[j] = pf[j];
-                pt[half + j] = pf[half + j];
-            }
+    const int movers = C * WARPS, batch = min(32, (n_moves + movers - 1) / movers);
+    unsigned char* kv = (unsigned char*)a.kv;
+    for (int i0 = (rank * WARPS + warp) * batch; i0 < n_moves; i0 += movers * batch) {
+        const int m = min(batch, n_moves - i0);
+        long long to = 0, from = 0;
+        if (lane < m) {
+            const int e = dst[i0 + lane], f = src[i0 + lane];
+            to = (long long)at(e);
+            from = (long long)at(f);
+            a.weights_out[base + e] = w[f];
+            a.places_out[base + e] = places[f];
         }
-        if (lane == 0) {
-            a.weights_out[base + to] = w[from];
-            a.places_out[base + to] = places[from];
+        const int row_pieces = wide ? a.row_bytes / 16 : a.row_bytes, pieces = 2 * row_pieces, all = m * pieces;
+        for (int p0 = 0; p0 < all; p0 += 32 * DEEP) {
+            uint4 v[DEEP];
+            long long put[DEEP];
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j) {
+                const int p = p0 + 32 * j + lane, i = min(p / pieces, m - 1), c = p % pieces;
+                const size_t off = (c < row_pieces ? 0 : half) + (size_t)(c < row_pieces ? c : c - row_pieces) * (wide ? 16 : 1);
+                const long long get = __shfl_sync(0xffffffffu, from, i);
+                put[j] = __shfl_sync(0xffffffffu, to, i);
+                if (p < all) {
+                    if (wide) v[j] = *reinterpret_cast<const uint4*>(kv + get + off);
+                    else v[j].x = kv[get + off];
+                }
+                put[j] = p < all ? put[j] + (long long)off : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < DEEP; ++j)
+                if (put[j] >= 0) {
+                    if (wide) *reinterpret_cast<uint4*>(kv + put[j]) = v[j];
+                    else kv[put[j]] = (unsigned char)v[j].x;
+                }
         }
     }
     __threadfence();
 }
 
-#define EV_MOST_KEYS 48000      // that fit a block's shared memory beside the rest
-
-// moves: scratch of R * nkv * 2 * (max_context / 2 + 1) ints.  cluster: blocks a (request, kv head), 1, 2, 4 or 8.
+// moves: scratch of R * nkv * 2 * (max_context / 2 + 1) ints, used with clusters.  cluster: blocks a (request, kv head), 1, 2, 4 or 8.
 extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, const int* places, float* weights_out, int* places_out,
                                 int ld, int n_slots, const int* slots, const int* block_table, int max_blocks, const int* lens,
                                 const int* keep, const int* positions, int* new_lens, int R, int nkv, int d, int page_size,
@@ -223,16 +261,21 @@ extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, 
     if (nkv < 1 || d < 1 || page_size < 1 || max_context < 1 || max_context > ld || cluster < 1 || cluster > 8 || (cluster & (cluster - 1)) ||
         (long long)R * nkv * cluster > 0x7fffffffll)
         return RG_ERR_UNSUPPORTED;
-    const int limit = max_context;
+    const int limit = (int)min((long long)max_context, (long long)max_blocks * page_size);
     const EvictArgs a = {kv, weights, places, weights_out, places_out, slots, block_table, lens, keep, positions, new_lens, moves, ld, n_slots,
-                         max_blocks, R, nkv, page_size, d * elem_bytes, protect_first, protect_last,
-                         (int)min((long long)limit, (long long)max_blocks * page_size)};
-    const long long a_warp = ((((long long)limit + cluster * EV_WARPS - 1) / (cluster * EV_WARPS)) + 31) / 32 * 32;
-    const long long most = a_warp * EV_WARPS;
-    const bool cached = most <= EV_MOST_KEYS;
-    const size_t smem = cached ? (size_t)most * 4 : 0;
-    void (*kernel)(EvictArgs) = cached ? evict_kernel<true> : evict_kernel<false>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    return rg_launch(kernel, dim3((unsigned)(R * nkv * cluster)), dim3(EV_THREADS), smem, (cudaStream_t)stream, cluster, a);
+                         max_blocks, R, nkv, page_size, d * elem_bytes, protect_first, protect_last, limit};
+    // Up to 2,048 entries 256 threads hold them, up to 16,384 a thousand, a cluster up to eight times as many; lists of moves are in
+    // shared memory but for clusters.
+    const dim3 grid((unsigned)(R * nkv * cluster));
+    const int lists = 2 * (limit / 2 + 1) * (int)sizeof(int);
+#define RG_EV(T, P, CL, SMEM) { if (SMEM > 48 * 1024) { \
+        cudaError_t ce = cudaFuncSetAttribute(evict_kernel<T, P, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); \
+        if (ce != cudaSuccess) return (int)ce; } \
+    return rg_launch(evict_kernel<T, P, CL>, grid, dim3(T), SMEM, (cudaStream_t)stream, cluster, a); }
+    if (cluster == 1 && limit <= 256 * 8) RG_EV(256, 8, false, lists)
+    if (cluster == 1 && limit <= 1024 * 16) RG_EV(1024, 16, false, lists)
+    if (cluster == 1) return RG_ERR_UNSUPPORTED;
+    if (limit <= cluster * 1024 * 16) RG_EV(1024, 16, true, 0)
+    RG_EV(1024, 0, true, 0)
+#undef RG_EV
 }
