@@ -7,10 +7,11 @@
 // before k: the moves of K and V rows are independent of one another, and of the fewest bytes there can be.
 //
 // One block per (request, kv head), or a cluster of them.  A warp holds consecutive entries' keys, a key of each run of 32 a
-// lane, in registers.  The k-th greatest key is found by cutting the interval that holds it into four: three counts a step,
-// added up over the block (and the cluster); a step whose count is k ends the search, since the keys above it are the k
-// that stay (without ties about as many steps as n has digits to the base 4, and a few).  Then ties, free entries and late
-// ones are numbered by ballots, with the counts of the warps and blocks before.  A warp takes up to 32 moves at a time: their
+// lane, in registers.  The k-th greatest key is found digit by digit from the top (10 bits a digit, or 12 where a block holds
+// many keys): a histogram of the keys that agree so far, in shared memory, added up over the cluster, and a sum from the top
+// bin down; once at most 128 keys agree they are compared with one another.  (Cutting the interval in four with three counts
+// a step needs 7 to 8 steps to get there: 14 us of 53 for clusters of two on 16,384 keys.)  Then free entries and late ones
+// are numbered by ballots, with the counts of the warps and blocks before.  A warp takes up to 32 moves at a time: their
 // addresses a lane each, then their rows in 16-byte pieces, several a lane under way.
 #include "common.cuh"
 #include <cooperative_groups.h>
@@ -81,23 +82,33 @@ struct Sums {
     }
 };
 
+#define EV_FEW 128                // keys that are compared with one another
+// bits of a digit: four bins a thread
+__host__ __device__ constexpr int ev_bits(int threads) { return threads == 256 ? 10 : 12; }
+
 template <int THREADS, int PER, bool CLUSTERED>       // PER: keys a thread holds; 0: they are made anew whenever one is asked for
-__global__ void __launch_bounds__(THREADS) evict_kernel(const EvictArgs a) {
-    constexpr int WARPS = THREADS / 32, DEEP = THREADS > 512 ? 4 : 8;    // pieces a lane under way: 64 KB a block or less
-    extern __shared__ int lists[];                                   // destinations and sources, without a cluster
-    __shared__ int sums_of[2][WARPS][3];
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(const EvictArgs a) {
+    constexpr int WARPS = THREADS / 32, BITS = ev_bits(THREADS), BINS = 1 << BITS, DEEP = 4;   // DEEP: pieces a lane under way, 64 KB an SM
+    static_assert(BINS == 4 * THREADS, "four bins a thread");
+    extern __shared__ __align__(16) int lists[];                     // destinations and sources, without a cluster
+    __shared__ __align__(16) int hist[2][BINS];                      // of two digits in turn
+    __shared__ int sums_of[2][WARPS][2], scan[WARPS], found[3], few_n, kth_is[3];
+    __shared__ uint32_t few[EV_FEW];
     const int C = CLUSTERED ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTERED ? (int)cg::this_cluster().block_rank() : 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    reinterpret_cast<int4*>(hist[0])[tid] = make_int4(0, 0, 0, 0);
+    reinterpret_cast<int4*>(hist[1])[tid] = make_int4(0, 0, 0, 0);
+    if (tid == 0) few_n = 0;
     // No early start for the kernel behind this one: attention kernels ask for cached keys ahead of their own wait.
     pdl_wait();
     const int row = blockIdx.x / C, r = row / a.nkv, h = row % a.nkv;
     const int slot = a.slots[r], n = min(a.lens[r], a.limit), k = min(n, max(0, a.keep[r])), newest = a.positions[r];
     const bool alone = slot < 0 || slot >= a.n_slots || n <= 0;      // the same for the whole cluster
-    if (h == 0 && rank == 0 && threadIdx.x == 0) a.new_lens[r] = alone ? a.lens[r] : k;
+    if (h == 0 && rank == 0 && tid == 0) a.new_lens[r] = alone ? a.lens[r] : k;
     if (alone) return;
     const size_t base = ((size_t)slot * a.nkv + h) * a.ld;
     const float* w = a.weights + base;
     const int* places = a.places + base;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // this warp's entries: `run` runs of 32 from w0 on
     const int run = (n + C * THREADS - 1) / (C * THREADS), w0 = (rank * WARPS + warp) * run * 32;
     uint32_t held[PER ? PER : 1];
@@ -108,101 +119,156 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const EvictArgs a) {
         for (int j = 0; j < PER; ++j) {
             const int e = w0 + j * 32 + lane;
             const bool there = j < run && e < n;
-            wv[j] = there ? w[e] : 0.f;
-            pv[j] = there ? places[e] : 0;
+            wv[j] = there ? __ldg(w + e) : 0.f;
+            pv[j] = there ? __ldg(places + e) : 0;
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j) held[j] = weight_key(a, wv[j], pv[j], newest);
     }
-    // f(run, entry, its key, is there such an entry): for every run of the warp, all lanes together
+    // f(entry, its key, is there such an entry): for every run of the warp, all lanes together
     auto each = [&](auto f) {
         if constexpr (PER > 0) {
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                if (j < run) { const int e = w0 + j * 32 + lane; f(j, e, held[j], e < n); }
+                if (j < run) { const int e = w0 + j * 32 + lane; f(e, held[j], e < n); }
         } else {
             for (int j = 0; j < run; ++j) {
                 const int e = w0 + j * 32 + lane;
-                f(j, e, e < n ? weight_key(a, w[e], places[e], newest) : 0u, e < n);
+                f(e, e < n ? weight_key(a, __ldg(w + e), __ldg(places + e), newest) : 0u, e < n);
             }
         }
     };
-    Sums<WARPS, 3, CLUSTERED> sums = {sums_of, 0};
-    int n_moves = 0, total[3], before[3];
+    auto block_or_cluster_sync = [&]() {
+        if constexpr (CLUSTERED) cg::this_cluster().sync();
+        else __syncthreads();
+    };
+    Sums<WARPS, 2, CLUSTERED> sums = {sums_of, 0};
+    int n_moves = 0;
     int *dst = CLUSTERED ? a.moves + (size_t)row * 2 * (a.limit / 2 + 1) : lists, *src = dst + a.limit / 2 + 1;
     if (k < n) {
-        // The k-th greatest key lies in [lo, hi): at least k keys are lo or above, `above` < k are hi or above.
-        unsigned long long lo = 0, hi = 1ull << 32;
-        int above = 0;
-        bool exact = k == 0;                                         // the keys from hi on are just those that stay
-        while (hi - lo > 1 && !exact) {
-            const unsigned long long step = hi - lo > 4 ? (hi - lo) / 4 : 1;
-            const uint32_t t1 = (uint32_t)(lo + step), t2 = (uint32_t)min(lo + 2 * step, hi - 1), t3 = (uint32_t)min(lo + 3 * step, hi - 1);
-            int c[3] = {0, 0, 0};
-            each([&](int, int, uint32_t key, bool there) {
-                c[0] += there && key >= t1;
-                c[1] += there && key >= t2;
-                c[2] += there && key >= t3;
+        // The k-th greatest key has the digits of `high` down to bit `shift`; of the `in` keys that have them `left` stay.
+        uint32_t high = 0;
+        int shift = 32, left = k, in = n;
+        block_or_cluster_sync();
+        for (int digit = 0; shift > 0 && in > EV_FEW && k > 0; ++digit) {
+            const int bits = min(BITS, shift), was = shift;
+            shift -= bits;
+            int* mine = hist[digit & 1];
+            each([&](int, uint32_t key, bool there) {
+                if (there && (was == 32 || key >> was == high >> was)) atomicAdd(&mine[key >> shift & ((1 << bits) - 1)], 1);
             });
+            block_or_cluster_sync();
+            // bins from the top down, four a thread; counts are whole numbers: any order of adding gives the same
+            const int at = THREADS - 1 - tid;
+            int4 c = make_int4(0, 0, 0, 0);
+            for (int q = 0; q < C; ++q) {
+                const int4* from = reinterpret_cast<const int4*>(mine);
+                if constexpr (CLUSTERED) from = cg::this_cluster().map_shared_rank(from, q);
+                const int4 x = from[at];
+                c.x += x.x; c.y += x.y; c.z += x.z; c.w += x.w;
+            }
+            const int sum = c.x + c.y + c.z + c.w;
+            int s = sum;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) c[i] = __reduce_add_sync(0xffffffffu, c[i]);
-            sums.of(c, total, before);
-            if (total[2] == k || total[1] == k || total[0] == k) {
-                hi = total[2] == k ? t3 : (total[1] == k ? t2 : t1);
-                exact = true;
-            } else if (total[2] > k) { lo = t3; }
-            else if (total[1] > k) { lo = t2; hi = t3; above = total[2]; }
-            else if (total[0] > k) { lo = t1; hi = t2; above = total[1]; }
-            else { hi = t1; above = total[0]; }
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            if (lane == 31) scan[warp] = s;
+            __syncthreads();
+            const int earlier = __reduce_add_sync(0xffffffffu, lane < warp && lane < WARPS ? scan[lane] : 0);
+            int above = earlier + s - sum;
+            if (above < left && left <= above + sum) {                 // one thread's bins hold it
+                int bin = 4 * at + 3, here = c.w;
+                if (left > above + here) { above += here; --bin; here = c.z; }
+                if (left > above + here) { above += here; --bin; here = c.y; }
+                if (left > above + here) { above += here; --bin; here = c.x; }
+                found[0] = bin;
+                found[1] = left - above;
+                found[2] = here;
+            }
+            block_or_cluster_sync();                                   // histograms are read, `found` is there
+            high |= (uint32_t)found[0] << shift;
+            left = found[1];
+            in = found[2];
+            if (digit + 2 < (32 + BITS - 1) / BITS) reinterpret_cast<int4*>(mine)[tid] = make_int4(0, 0, 0, 0);   // for the digit after the next
         }
-        // what stays: keys from hi on, and of those that are lo the first `left`
-        const int left = exact ? 0 : k - above;
-        const uint32_t from = (uint32_t)hi, kth = (uint32_t)lo;
-        const bool none_above = hi >> 32 || k == 0;                  // hi is above every key
-        int tie = 0;
-        if (!exact) {
-            int c[3] = {0, 0, 0};
-            each([&](int, int, uint32_t key, bool there) { c[0] += __popc(__ballot_sync(0xffffffffu, there && key == kth)); });
+        int equal = in;                                                // keys that are the one itself, once all digits are there
+        if (shift > 0 && k > 0) {
+            // few enough: a key with g greater ones and q equal ones is the one if g < left <= g + q
+            each([&](int, uint32_t key, bool there) {
+                if (there && (shift == 32 || key >> shift == high >> shift)) {
+                    if constexpr (CLUSTERED) {
+                        cg::cluster_group cluster = cg::this_cluster();
+                        cluster.map_shared_rank(few, 0)[atomicAdd(cluster.map_shared_rank(&few_n, 0), 1)] = key;
+                    } else few[atomicAdd(&few_n, 1)] = key;
+                }
+            });
+            if constexpr (CLUSTERED) {
+                cg::this_cluster().sync();
+                if (rank > 0 && tid < in) few[tid] = cg::this_cluster().map_shared_rank(few, 0)[tid];
+            }
+            __syncthreads();
+            if (tid < EV_FEW) {
+                const uint32_t mine = tid < in ? few[tid] : 0u;
+                int g = 0, q = 0;
+                for (int i = 0; i < in; ++i) {
+                    const uint32_t other = few[i];
+                    g += other > mine;
+                    q += other == mine;
+                }
+                if (tid < in && g < left && left <= g + q) { kth_is[0] = (int)mine; kth_is[1] = left - g; kth_is[2] = q; }
+            }
+            __syncthreads();
+            high = (uint32_t)kth_is[0];
+            left = kth_is[1];
+            equal = kth_is[2];
+        }
+        // What stays: keys above `high`, and of those that equal it the first `left`.  Bit j: the entry of run j stays.
+        const bool some = k > 0 && left < equal;                       // only some of the equal ones: they are numbered
+        int total[2], before[2], c[2] = {0, 0}, tie = 0;
+        if (some) {
+            each([&](int, uint32_t key, bool there) { c[0] += __popc(__ballot_sync(0xffffffffu, there && key == high)); });
             sums.of(c, total, before);
             tie = before[0];
         }
         const uint32_t below = (1u << lane) - 1;
         auto stays = [&](uint32_t key, bool there, int& t) -> bool {
-            bool in = there && !none_above && key >= from;
-            if (!exact) {
-                const uint32_t all = __ballot_sync(0xffffffffu, there && key == kth);
-                in = in || (there && key == kth && t + __popc(all & below) < left);
-                t += __popc(all);
-            }
+            if (!some) return there && key >= high && k > 0;
+            const uint32_t all = __ballot_sync(0xffffffffu, there && key == high);
+            const bool in = there && (key > high || (key == high && t + __popc(all & below) < left));
+            t += __popc(all);
             return in;
         };
-        int c[3] = {0, 0, 0}, t2 = tie;
-        each([&](int, int e, uint32_t key, bool there) {
+        int t2 = tie;
+        c[0] = c[1] = 0;                                               // free, late: this lane's, then the warp's
+        each([&](int e, uint32_t key, bool there) {
             const bool in = stays(key, there, t2);
-            c[0] += __popc(__ballot_sync(0xffffffffu, there && e < k && !in));
-            c[1] += __popc(__ballot_sync(0xffffffffu, there && e >= k && in));
+            c[0] += there && e < k && !in;
+            c[1] += e >= k && in;
         });
+#pragma unroll
+        for (int i = 0; i < 2; ++i) c[i] = __reduce_add_sync(0xffffffffu, c[i]);
         sums.of(c, total, before);
         n_moves = total[1];
-        each([&](int, int e, uint32_t key, bool there) {
-            const bool in = stays(key, there, tie), gone = there && e < k && !in, late = there && e >= k && in;
-            const uint32_t f = __ballot_sync(0xffffffffu, gone), l = __ballot_sync(0xffffffffu, late);
-            if (gone) dst[before[0] + __popc(f & below)] = e;
-            if (late) src[before[1] + __popc(l & below)] = e;
+        each([&](int e, uint32_t key, bool there) {
+            const bool in = stays(key, there, tie), front = e < k, moves = there && in != front;
+            const uint32_t m = __ballot_sync(0xffffffffu, moves), f = __ballot_sync(0xffffffffu, front) & m, l = m & ~f;
+            if (moves) (front ? dst : src)[front ? before[0] + __popc(f & below) : before[1] + __popc(l & below)] = e;
             before[0] += __popc(f);
             before[1] += __popc(l);
-            if (in && e < k) {
-                a.weights_out[base + e] = w[e];
-                a.places_out[base + e] = places[e];
+            if (in && front) {
+                a.weights_out[base + e] = __ldg(w + e);
+                a.places_out[base + e] = __ldg(places + e);
             }
         });
-        if constexpr (CLUSTERED) { __threadfence(); cg::this_cluster().sync(); }
-        else __syncthreads();                                        // the lists are whole, and nobody reads another block's sums any more
+        if constexpr (CLUSTERED) __threadfence();
+        block_or_cluster_sync();                                       // the lists are whole, and nobody reads another block's sums any more
     } else {
-        each([&](int, int e, uint32_t, bool there) {
+        each([&](int e, uint32_t, bool there) {
             if (there) {
-                a.weights_out[base + e] = w[e];
-                a.places_out[base + e] = places[e];
+                a.weights_out[base + e] = __ldg(w + e);
+                a.places_out[base + e] = __ldg(places + e);
             }
         });
     }
@@ -211,7 +277,7 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const EvictArgs a) {
     const size_t half = (size_t)a.nkv * a.page_size * a.row_bytes;   // bytes of a page's keys, or values
     const bool wide = a.row_bytes % 16 == 0 && ((uintptr_t)a.kv & 15) == 0;
     auto at = [&](int e) -> size_t {
-        return (size_t)table[e / a.page_size] * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
+        return (size_t)__ldg(table + e / a.page_size) * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
     };
     const int movers = C * WARPS, batch = min(32, (n_moves + movers - 1) / movers);
     unsigned char* kv = (unsigned char*)a.kv;
@@ -222,8 +288,8 @@ __global__ void __launch_bounds__(THREADS) evict_kernel(const EvictArgs a) {
             const int e = dst[i0 + lane], f = src[i0 + lane];
             to = (long long)at(e);
             from = (long long)at(f);
-            a.weights_out[base + e] = w[f];
-            a.places_out[base + e] = places[f];
+            a.weights_out[base + e] = __ldg(w + f);
+            a.places_out[base + e] = __ldg(places + f);
         }
         const int row_pieces = wide ? a.row_bytes / 16 : a.row_bytes, pieces = 2 * row_pieces, all = m * pieces;
         for (int p0 = 0; p0 < all; p0 += 32 * DEEP) {
