@@ -29,10 +29,12 @@ struct EvictArgs {
     const int* keep;             // [R]
     const int* positions;        // [R]: the place of the newest token
     int* new_lens;               // [R]
-    int* moves;                  // [R * nkv][2][limit / 2 + 1]: destinations, sources
+    int* moves;                  // [R * nkv][ev_list(limit)]: how many, destinations, sources
     long long ld;
     int n_slots, max_blocks, R, nkv, page_size, row_bytes, protect_first, protect_last, limit;
 };
+
+__host__ __device__ inline size_t ev_list(int limit) { return 1 + 2 * ((size_t)limit / 2 + 1); }
 
 // A weight as an unsigned number of the same order.
 __device__ __forceinline__ uint32_t weight_key(const EvictArgs& a, float w, int place, int newest) {
@@ -82,15 +84,72 @@ struct Sums {
     }
 };
 
+// Moves of row (request, kv head) `row` by the warp `mover` of `movers`: `batch` (up to 32) at a time, a lane each for their addresses.  Rows are
+// pieces of 16 bytes, K and V one after the other; or, where they are not made of those, bytes.
+template <int DEEP>                  // pieces a lane under way
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int row, const int* dst, const int* src, int n_moves, int mover, int movers, int batch) {
+    const int lane = threadIdx.x & 31, r = row / a.nkv, h = row % a.nkv;
+    const size_t base = ((size_t)a.slots[r] * a.nkv + h) * a.ld;
+    const int* table = a.block_table + (size_t)r * a.max_blocks;
+    const size_t half = (size_t)a.nkv * a.page_size * a.row_bytes;   // bytes of a page's keys, or values
+    const bool wide = a.row_bytes % 16 == 0 && ((uintptr_t)a.kv & 15) == 0;
+    auto at = [&](int e) -> size_t {
+        return (size_t)__ldg(table + e / a.page_size) * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
+    };
+    unsigned char* kv = (unsigned char*)a.kv;
+    // `lanes` of the warp share a move, `side` moves side by side: a power of two that fits its pieces
+    int lanes = 32;
+    while (lanes > 1 && (wide ? a.row_bytes / 8 : 2 * a.row_bytes) % lanes) lanes >>= 1;
+    const int side = 32 / lanes;
+    for (int i0 = mover * batch; i0 < n_moves; i0 += movers * batch) {
+        const int m = min(batch, n_moves - i0);
+        long long to = 0, from = 0;
+        if (lane < m) {
+            const int e = dst[i0 + lane], f = src[i0 + lane];
+            to = (long long)at(e);
+            from = (long long)at(f);
+            a.weights_out[base + e] = __ldg(a.weights + base + f);
+            a.places_out[base + e] = __ldg(a.places + base + f);
+        }
+        const int row_pieces = wide ? a.row_bytes / 16 : a.row_bytes;
+        for (int c = lane & (lanes - 1); c < 2 * row_pieces; c += lanes) {
+            unsigned char* mine = kv + (c < row_pieces ? (size_t)c : half / (wide ? 16 : 1) + (c - row_pieces)) * (wide ? 16 : 1);
+            for (int k0 = 0; k0 < m; k0 += DEEP * side) {
+                uint4 v[DEEP];
+#pragma unroll
+                for (int j = 0; j < DEEP; ++j) {
+                    const int k = k0 + j * side + lane / lanes;
+                    const unsigned char* get = mine + __shfl_sync(0xffffffffu, from, k < m ? k : 0);
+                    if (k < m) {
+                        if (wide) v[j] = *reinterpret_cast<const uint4*>(get);
+                        else v[j].x = *get;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < DEEP; ++j) {
+                    const int k = k0 + j * side + lane / lanes;
+                    unsigned char* put = mine + __shfl_sync(0xffffffffu, to, k < m ? k : 0);
+                    if (k < m) {
+                        if (wide) *reinterpret_cast<uint4*>(put) = v[j];
+                        else *put = (unsigned char)v[j].x;
+                    }
+                }
+            }
+        }
+    }
+}
+
 #define EV_FEW 128                // keys that are compared with one another
 // bits of a digit: four bins a thread
-__host__ __device__ constexpr int ev_bits(int threads) { return threads == 256 ? 10 : 12; }
+__host__ __device__ constexpr int ev_bits(int threads) { return threads == 256 ? 10 : (threads == 512 ? 11 : 12); }
 
-template <int THREADS, int PER, bool CLUSTERED>       // PER: keys a thread holds; 0: they are made anew whenever one is asked for
+// PER: keys a thread holds; 0: they are made anew whenever one is asked for.  FUSED: the block makes the moves, too.
+template <int THREADS, int PER, bool CLUSTERED, bool FUSED>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(const EvictArgs a) {
-    constexpr int WARPS = THREADS / 32, BITS = ev_bits(THREADS), BINS = 1 << BITS, DEEP = 4;   // DEEP: pieces a lane under way, 64 KB an SM
+    constexpr int WARPS = THREADS / 32, BITS = ev_bits(THREADS), BINS = 1 << BITS;
     static_assert(BINS == 4 * THREADS, "four bins a thread");
-    extern __shared__ __align__(16) int lists[];                     // destinations and sources, without a cluster
+    static_assert(!(CLUSTERED && FUSED), "a cluster's lists are in global memory");
+    extern __shared__ __align__(16) int lists[];                     // destinations and sources, where the block itself moves
     __shared__ __align__(16) int hist[2][BINS];                      // of two digits in turn
     __shared__ int sums_of[2][WARPS][2], scan[WARPS], found[3], few_n, kth_is[3];
     __shared__ uint32_t few[EV_FEW];
@@ -113,17 +172,24 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
     const int run = (n + C * THREADS - 1) / (C * THREADS), w0 = (rank * WARPS + warp) * run * 32;
     uint32_t held[PER ? PER : 1];
     if constexpr (PER > 0) {
-        float wv[PER];
-        int pv[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const int e = w0 + j * 32 + lane;
-            const bool there = j < run && e < n;
-            wv[j] = there ? __ldg(w + e) : 0.f;
-            pv[j] = there ? __ldg(places + e) : 0;
+        for (int j0 = 0; j0 < PER; j0 += 8) {                        // eight of each under way: as many as there are registers for
+            float wv[8];
+            int pv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = min(w0 + (j0 + j) * 32 + lane, n - 1);   // no branch: the loads leave together
+                wv[j] = __ldg(w + e);
+                pv[j] = __ldg(places + e);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) held[j0 + j] = weight_key(a, wv[j], pv[j], newest);
         }
-#pragma unroll
-        for (int j = 0; j < PER; ++j) held[j] = weight_key(a, wv[j], pv[j], newest);
+    }
+    // What lies before the new length, as if it stayed: moves come over it.
+    for (int e = rank * THREADS + tid; e < k; e += C * THREADS) {
+        a.weights_out[base + e] = __ldg(w + e);
+        a.places_out[base + e] = __ldg(places + e);
     }
     // f(entry, its key, is there such an entry): for every run of the warp, all lanes together
     auto each = [&](auto f) {
@@ -144,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
     };
     Sums<WARPS, 2, CLUSTERED> sums = {sums_of, 0};
     int n_moves = 0;
-    int *dst = CLUSTERED ? a.moves + (size_t)row * 2 * (a.limit / 2 + 1) : lists, *src = dst + a.limit / 2 + 1;
+    int *dst = FUSED ? lists : a.moves + (size_t)row * ev_list(a.limit) + 1, *src = dst + a.limit / 2 + 1;
     if (k < n) {
         // The k-th greatest key has the digits of `high` down to bit `shift`; of the `in` keys that have them `left` stay.
         uint32_t high = 0;
@@ -209,15 +275,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
                 if (rank > 0 && tid < in) few[tid] = cg::this_cluster().map_shared_rank(few, 0)[tid];
             }
             __syncthreads();
-            if (tid < EV_FEW) {
-                const uint32_t mine = tid < in ? few[tid] : 0u;
-                int g = 0, q = 0;
-                for (int i = 0; i < in; ++i) {
-                    const uint32_t other = few[i];
-                    g += other > mine;
-                    q += other == mine;
+            // a candidate a warp at a time, compared with all of them by the lanes
+            for (int i = warp; i < in; i += WARPS) {
+                const uint32_t mine = few[i];
+                int c = 0;                                             // greater, and equal << 16
+#pragma unroll
+                for (int j = 0; j < EV_FEW / 32; ++j) {
+                    const uint32_t other = few[lane + 32 * j];
+                    if (lane + 32 * j < in) c += (other > mine ? 1 : 0) + (other == mine ? 1 << 16 : 0);
                 }
-                if (tid < in && g < left && left <= g + q) { kth_is[0] = (int)mine; kth_is[1] = left - g; kth_is[2] = q; }
+                c = __reduce_add_sync(0xffffffffu, c);
+                const int g = c & 0xffff, q = c >> 16;
+                if (lane == 0 && g < left && left <= g + q) { kth_is[0] = (int)mine; kth_is[1] = left - g; kth_is[2] = q; }
             }
             __syncthreads();
             high = (uint32_t)kth_is[0];
@@ -257,91 +326,61 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
             if (moves) (front ? dst : src)[front ? before[0] + __popc(f & below) : before[1] + __popc(l & below)] = e;
             before[0] += __popc(f);
             before[1] += __popc(l);
-            if (in && front) {
-                a.weights_out[base + e] = __ldg(w + e);
-                a.places_out[base + e] = __ldg(places + e);
-            }
         });
-        if constexpr (CLUSTERED) __threadfence();
         block_or_cluster_sync();                                       // the lists are whole, and nobody reads another block's sums any more
-    } else {
-        each([&](int e, uint32_t, bool there) {
-            if (there) {
-                a.weights_out[base + e] = __ldg(w + e);
-                a.places_out[base + e] = __ldg(places + e);
-            }
-        });
     }
-    // The moves.  Rows are `pieces` pieces of 16 bytes, K and V one after the other; or, where rows are not made of those, bytes.
-    const int* table = a.block_table + (size_t)r * a.max_blocks;
-    const size_t half = (size_t)a.nkv * a.page_size * a.row_bytes;   // bytes of a page's keys, or values
-    const bool wide = a.row_bytes % 16 == 0 && ((uintptr_t)a.kv & 15) == 0;
-    auto at = [&](int e) -> size_t {
-        return (size_t)__ldg(table + e / a.page_size) * 2 * half + ((size_t)h * a.page_size + e % a.page_size) * a.row_bytes;
-    };
-    const int movers = C * WARPS, batch = min(32, (n_moves + movers - 1) / movers);
-    unsigned char* kv = (unsigned char*)a.kv;
-    for (int i0 = (rank * WARPS + warp) * batch; i0 < n_moves; i0 += movers * batch) {
-        const int m = min(batch, n_moves - i0);
-        long long to = 0, from = 0;
-        if (lane < m) {
-            const int e = dst[i0 + lane], f = src[i0 + lane];
-            to = (long long)at(e);
-            from = (long long)at(f);
-            a.weights_out[base + e] = __ldg(w + f);
-            a.places_out[base + e] = __ldg(places + f);
-        }
-        const int row_pieces = wide ? a.row_bytes / 16 : a.row_bytes, pieces = 2 * row_pieces, all = m * pieces;
-        for (int p0 = 0; p0 < all; p0 += 32 * DEEP) {
-            uint4 v[DEEP];
-            long long put[DEEP];
-#pragma unroll
-            for (int j = 0; j < DEEP; ++j) {
-                const int p = p0 + 32 * j + lane, i = min(p / pieces, m - 1), c = p % pieces;
-                const size_t off = (c < row_pieces ? 0 : half) + (size_t)(c < row_pieces ? c : c - row_pieces) * (wide ? 16 : 1);
-                const long long get = __shfl_sync(0xffffffffu, from, i);
-                put[j] = __shfl_sync(0xffffffffu, to, i);
-                if (p < all) {
-                    if (wide) v[j] = *reinterpret_cast<const uint4*>(kv + get + off);
-                    else v[j].x = kv[get + off];
-                }
-                put[j] = p < all ? put[j] + (long long)off : -1;
-            }
-#pragma unroll
-            for (int j = 0; j < DEEP; ++j)
-                if (put[j] >= 0) {
-                    if (wide) *reinterpret_cast<uint4*>(kv + put[j]) = v[j];
-                    else kv[put[j]] = (unsigned char)v[j].x;
-                }
-        }
-    }
+    if constexpr (FUSED) move_rows<4>(a, row, dst, src, n_moves, warp, WARPS, min(32, (n_moves + WARPS - 1) / WARPS));
+    else if (rank == 0 && tid == 0) a.moves[(size_t)row * ev_list(a.limit)] = n_moves;
+    if constexpr (FUSED) __threadfence();
+}
+
+// The moves of a row that evict_kernel has listed.  (Bulk copies through shared memory, a row each, take 28 us where this takes
+// EVMOVES: the unit that makes them is bound by their number.)  grid (blocks that share a row's moves, R * nkv)
+#define EV_MOVERS 2               // blocks an SM
+__global__ void __launch_bounds__(256, EV_MOVERS) evict_moves_kernel(const EvictArgs a) {
+    pdl_wait();                                                      // no early start for the kernel behind, as above
+    const int* list = a.moves + (size_t)blockIdx.y * ev_list(a.limit);
+    const int n = list[0], movers = gridDim.x * 8;
+    move_rows<8>(a, blockIdx.y, list + 1, list + 2 + a.limit / 2, n, blockIdx.x * 8 + (threadIdx.x >> 5), movers,
+                 min(32, (n + movers - 1) / movers));
     __threadfence();
 }
 
-// moves: scratch of R * nkv * 2 * (max_context / 2 + 1) ints, used with clusters.  cluster: blocks a (request, kv head), 1, 2, 4 or 8.
+// moves: scratch of R * nkv * (2 * (max_context / 2) + 3) ints where max_context is above 2,048.  cluster: blocks a (request, kv
+// head), 1, 2, 4 or 8; one holds up to 16,384 keys.
 extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, const int* places, float* weights_out, int* places_out,
                                 int ld, int n_slots, const int* slots, const int* block_table, int max_blocks, const int* lens,
                                 const int* keep, const int* positions, int* new_lens, int R, int nkv, int d, int page_size,
                                 int protect_first, int protect_last, int max_context, int* moves, int cluster, void* stream) {
     if (R <= 0) return 0;
     if (nkv < 1 || d < 1 || page_size < 1 || max_context < 1 || max_context > ld || cluster < 1 || cluster > 8 || (cluster & (cluster - 1)) ||
-        (long long)R * nkv * cluster > 0x7fffffffll)
+        (long long)R * nkv * cluster > 0x7fffffffll || (max_context > 256 * 8 && (long long)R * nkv > 65535))
         return RG_ERR_UNSUPPORTED;
     const int limit = (int)min((long long)max_context, (long long)max_blocks * page_size);
     const EvictArgs a = {kv, weights, places, weights_out, places_out, slots, block_table, lens, keep, positions, new_lens, moves, ld, n_slots,
                          max_blocks, R, nkv, page_size, d * elem_bytes, protect_first, protect_last, limit};
-    // Up to 2,048 entries 256 threads hold them, up to 16,384 a thousand, a cluster up to eight times as many; lists of moves are in
-    // shared memory but for clusters.
-    const dim3 grid((unsigned)(R * nkv * cluster));
-    const int lists = 2 * (limit / 2 + 1) * (int)sizeof(int);
-#define RG_EV(T, P, CL, SMEM) { if (SMEM > 48 * 1024) { \
-        cudaError_t ce = cudaFuncSetAttribute(evict_kernel<T, P, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); \
-        if (ce != cudaSuccess) return (int)ce; } \
-    return rg_launch(evict_kernel<T, P, CL>, grid, dim3(T), SMEM, (cudaStream_t)stream, cluster, a); }
-    if (cluster == 1 && limit <= 256 * 8) RG_EV(256, 8, false, lists)
-    if (cluster == 1 && limit <= 1024 * 16) RG_EV(1024, 16, false, lists)
-    if (cluster == 1) return RG_ERR_UNSUPPORTED;
-    if (limit <= cluster * 1024 * 16) RG_EV(1024, 16, true, 0)
-    RG_EV(1024, 0, true, 0)
+    // Up to 2,048 entries 256 threads hold the keys and make the moves.  Above, a thousand threads hold up to 16,384, a cluster up to
+    // eight times as many, and the moves are a second kernel's, so that all SMs take part however few heads there are (64 heads of
+    // 8,192 to 16,384 entries, 2,048 of which stay: EVFIGURES).
+    const unsigned rows = (unsigned)(R * nkv);
+#define RG_EV(T, P, CL, FU, SMEM) e = rg_launch(evict_kernel<T, P, CL, FU>, dim3(rows * (CL ? cluster : 1)), dim3(T), SMEM, s, CL ? cluster : 1, a)
+    const cudaStream_t s = (cudaStream_t)stream;
+    int e;
+    if (max_context <= 256 * 8) {
+        RG_EV(256, 8, false, true, 2 * (limit / 2 + 1) * sizeof(int));
+        return e;
+    }
+    if (cluster == 1) {
+        if (limit > 1024 * 16) return RG_ERR_UNSUPPORTED;
+        RG_EV(1024, 16, false, false, 0);
+    } else if (limit <= cluster * 1024 * 16) RG_EV(1024, 16, true, false, 0);
+    else RG_EV(1024, 0, true, false, 0);
 #undef RG_EV
+    if (e) return e;
+    int dev = 0, sms = 0;
+    cudaError_t ce = cudaGetDevice(&dev);
+    if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (ce != cudaSuccess) return (int)ce;
+    const int share = max(1, min((limit / 2 + 31) / 32, sms * EV_MOVERS / (int)rows));
+    return rg_launch(evict_moves_kernel, dim3(share, rows), dim3(256), 0, s, 1, a);
 }

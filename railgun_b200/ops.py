@@ -2379,11 +2379,13 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     new_lens = torch.empty(R, dtype=torch.int32, device=kv_cache.device)
     if max_context == 0:
         return new_lens.copy_(torch.minimum(lens, keep))
-    # a block holds up to 16,384 keys; a cluster of them takes more, and makes the moves faster where heads are few
+    # a block holds up to 16,384 keys, a cluster of up to eight more
     cluster = 1
-    while cluster < 8 and (max_context > 16384 * cluster or (R * nkv * cluster * 2 <= num_sms(kv_cache.device) and max_context > 2048)):
+    while cluster < 8 and max_context > 16384 * cluster:
         cluster *= 2
-    moves = torch.empty(R * nkv * 2 * (max_context // 2 + 1) if cluster > 1 else 0, dtype=torch.int32, device=kv_cache.device)
+    fused = max_context <= 2048                  # otherwise the moves are listed, and a second kernel's
+    moves = torch.empty(0 if fused else R * nkv * (2 * (max_context // 2) + 3), dtype=torch.int32, device=kv_cache.device)
+    _COUNTER.value += 0 if fused else 1
     _ok(_fn("evict", "rg_evict_entries")(
         _ptr(kv_cache), c_int(kv_cache.element_size()), _ptr(weights), _ptr(places), _ptr(weights_out), _ptr(places_out),
         c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(lens), _ptr(keep),
