@@ -479,14 +479,15 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
 }
 
 // ---------------------------------------------------------------------------------------------------
+static size_t pg_smem(int d) { return (size_t)((PG_Q + 2 * PG_K) * pg_row(d) + PG_Q * PG_LD + PG_Q) * sizeof(float); }
+
 static int launch_parts_general(const PartArgs& a, int dtype, cudaStream_t s) {
     const long long blocks = part_blocks(a);
     if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     if (blocks == 0) return 0;
-    const size_t smem = (size_t)((PG_Q + 2 * PG_K) * pg_row(a.d) + PG_Q * PG_LD + PG_Q) * sizeof(float);
+    const size_t smem = pg_smem(a.d);
     const bool vec = a.d % 4 == 0 && (((uintptr_t)a.kv) & (dtype == RG_DTYPE_F32 ? 15 : 7)) == 0;
-#define RG_PG(A, DP, VEC) { cudaError_t e = cudaFuncSetAttribute(parts_general_kernel<A, DP, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-    if (e != cudaSuccess) return (int)e; \
+#define RG_PG(A, DP, VEC) { RG_ALLOW_SMEM((parts_general_kernel<A, DP, VEC>), pg_smem(256)) \
     return rg_launch(parts_general_kernel<A, DP, VEC>, dim3((unsigned)blocks), dim3(PG_THREADS), smem, s, 1, a); }
 #define RG_PG_WIDTH(A, VEC) { if (a.d <= 32) RG_PG(A, 32, VEC) if (a.d <= 64) RG_PG(A, 64, VEC) RG_PG(A, 128, VEC) }
     if (dtype == RG_DTYPE_F32) { if (vec) RG_PG_WIDTH(float, true) RG_PG_WIDTH(float, false) }
@@ -524,8 +525,7 @@ static int launch_parts_mma(const PartArgs& a, int num_pages, int* err, cudaStre
     int e = make_kv_map(&map, a.kv, num_pages, a.nkv, a.page_size, a.d, a.page_size < 16 ? a.page_size : 16);
     if (e) return e;
 #define RG_PM(P) { constexpr int smem = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
-    cudaError_t ce = cudaFuncSetAttribute(parts_mma_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); \
-    if (ce != cudaSuccess) return (int)ce; \
+    RG_ALLOW_SMEM(parts_mma_kernel<P>, smem) \
     return rg_launch(parts_mma_kernel<P>, dim3((unsigned)blocks), dim3(PM_THREADS), smem, s, 1, map, a, err); }
     if (a.d == 64) RG_PM(1)
     if (a.d == 128) RG_PM(2)

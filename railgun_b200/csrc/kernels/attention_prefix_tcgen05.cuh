@@ -355,8 +355,7 @@ static int launch_prefix_tc(const PartArgs& a, int num_pages, int two_parts, int
     if (r != CUDA_SUCCESS) return 20000 + (int)r;
     int e = rg_make_map(&km, a.kv, (unsigned long long)num_pages * 2 * a.nkv * a.page_size, a.d, a.d, a.page_size < PT_STAGE ? a.page_size : PT_STAGE);
     if (e) return e;
-#define RG_PT(P) { cudaError_t ce = cudaFuncSetAttribute(prefix_tc_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, pt_smem(P)); \
-    if (ce != cudaSuccess) return (int)ce; \
+#define RG_PT(P) { RG_ALLOW_SMEM(prefix_tc_kernel<P>, pt_smem(P)) \
     return rg_launch(prefix_tc_kernel<P>, dim3((unsigned)blocks), dim3(PT_THREADS), (size_t)pt_smem(P), s, 1, qm, km, a, tile_rows, two_parts, err); }
     if (a.d == 64) RG_PT(1)
     RG_PT(2)

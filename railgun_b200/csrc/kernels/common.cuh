@@ -123,6 +123,17 @@ struct RgStreamOrder {
     ~RgStreamOrder() { rg_pdl_enabled = saved; }
 };
 
+// Lets `kernel` (one name a place where this stands) have up to `bytes` of dynamic shared memory: told to a device once, not per call.
+#define RG_ALLOW_SMEM(kernel, bytes) { \
+    static unsigned long long rg_told = 0;                           /* one bit per device */ \
+    int rg_dev = 0; \
+    if (cudaGetDevice(&rg_dev) != cudaSuccess || rg_dev < 0 || rg_dev > 63) rg_dev = 63; \
+    if (rg_dev == 63 || !(rg_told >> rg_dev & 1ull)) { \
+        cudaError_t rg_e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(bytes)); \
+        if (rg_e != cudaSuccess) return (int)rg_e; \
+        rg_told |= 1ull << rg_dev; \
+    } }
+
 // Launch through cudaLaunchKernelEx so that the launch can carry attributes (dependent launch, clusters).
 template <typename... KArgs, typename... Args>
 static int rg_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster_x,

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(256, EV_MOVERS) evict_moves_kernel(const Evict
 extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, const int* places, float* weights_out, int* places_out,
                                 int ld, int n_slots, const int* slots, const int* block_table, int max_blocks, const int* lens,
                                 const int* keep, const int* positions, int* new_lens, int R, int nkv, int d, int page_size,
-                                int protect_first, int protect_last, int max_context, int* moves, int cluster, void* stream) {
+                                int protect_first, int protect_last, int max_context, int* moves, int cluster, int sms, void* stream) {
     if (R <= 0) return 0;
     if (nkv < 1 || d < 1 || page_size < 1 || max_context < 1 || max_context > ld || cluster < 1 || cluster > 8 || (cluster & (cluster - 1)) ||
         (long long)R * nkv * cluster > 0x7fffffffll || (max_context > 256 * 8 && (long long)R * nkv > 65535))
@@ -377,10 +377,6 @@ extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, 
     else RG_EV(1024, 0, true, false, 0);
 #undef RG_EV
     if (e) return e;
-    int dev = 0, sms = 0;
-    cudaError_t ce = cudaGetDevice(&dev);
-    if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (ce != cudaSuccess) return (int)ce;
     const int share = max(1, min((limit / 2 + 31) / 32, sms * EV_MOVERS / (int)rows));
     return rg_launch(evict_moves_kernel, dim3(share, rows), dim3(256), 0, s, 1, a);
 }

@@ -82,6 +82,7 @@ __device__ __forceinline__ void tile_scores(float (&sc)[2][4], const float* qs, 
 }
 
 __host__ __device__ inline int kw_row(int d) { return ((d + 3) & ~3) + 4; }
+static size_t kw_smem(int d) { return (size_t)((KW_Q + KW_K) * kw_row(d) + 8 * KW_K) * sizeof(float); }
 
 // grid (query tiles, nkv, R)
 template <typename A>
@@ -558,7 +559,7 @@ static int make_q_map(CUtensorMap* map, const void* q, int T, int q_stride, int 
 }
 
 template <int PIECES>
-static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int max_context, cudaStream_t s) {
+static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int max_context, int sms, cudaStream_t s) {
     constexpr int smem = (4 + kt_b_stages(PIECES)) * KT_TILE * 128 * PIECES + 1024;
     const WeightArgs& w = rows.w;
     CUtensorMap qm, km;
@@ -566,13 +567,8 @@ static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int
     if (e) return e;
     e = rg_make_map(&km, w.kv, (unsigned long long)num_pages * 2 * w.nkv * w.page_size, w.d, w.d, min(w.page_size, KT_TILE));
     if (e) return e;
-    int dev = 0, sms = 0;
-    cudaError_t ce = cudaGetDevice(&dev);
-    if (ce == cudaSuccess) ce = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (ce == cudaSuccess)
-        ce = cudaFuncSetAttribute(key_weights_tc_kernel<PIECES, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (ce == cudaSuccess) ce = cudaFuncSetAttribute(key_weights_tc_kernel<PIECES, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (ce != cudaSuccess) return (int)ce;
+    RG_ALLOW_SMEM((key_weights_tc_kernel<PIECES, false>), smem)
+    RG_ALLOW_SMEM((key_weights_tc_kernel<PIECES, true>), smem)
     e = rg_launch(key_weights_tc_kernel<PIECES, false>, dim3(min(sms, rows.n_items)), dim3(KT_THREADS), smem, s, 1, qm, km, rows);
     if (!e && rows.parts > 1)
         e = rg_launch(join_row_sums_kernel, dim3((unsigned)(((long long)w.T * w.nh + 255) / 256)), dim3(256), 0, s, 1, rows);
@@ -589,7 +585,7 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
                                      int n_slots, const int* slots, const int* block_table, int max_blocks, const int* cu_rows,
                                      const int* starts, const int* fresh, int R, int T, int nh, int nkv, int d, int page_size,
                                      float scale, int max_rows, int max_context, float* z, int row_parts, float* part_ml,
-                                     int entry_parts, float* part_w, int* err, void* stream) {
+                                     int entry_parts, float* part_w, int sms, int* err, void* stream) {
     if (R <= 0 || T <= 0 || max_rows <= 0 || max_context <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_context > weights_ld || R > 65535 || nkv > 65535 ||
         (long long)max_rows * (nh / nkv) > 0x7fffffffll)
@@ -615,14 +611,13 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
         if (n_rows > 0x3fffffffll || n_entries > 0x3fffffffll) return RG_ERR_UNSUPPORTED;
         rows.n_items = (int)n_rows;
         entries.n_items = (int)n_entries;
-        return d == 64 ? launch_key_weights_tc<1>(rows, entries, num_pages, max_context, s)
-                       : launch_key_weights_tc<2>(rows, entries, num_pages, max_context, s);
+        return d == 64 ? launch_key_weights_tc<1>(rows, entries, num_pages, max_context, sms, s)
+                       : launch_key_weights_tc<2>(rows, entries, num_pages, max_context, sms, s);
     }
-    const size_t smem = (size_t)((KW_Q + KW_K) * kw_row(d) + 8 * KW_K) * sizeof(float);
+    const size_t smem = kw_smem(d);
     const dim3 by_query((max_rows * group + KW_Q - 1) / KW_Q, nkv, R), by_entry((max_context + KW_K - 1) / KW_K, nkv, R);
-#define RG_KW(A) { cudaError_t ce = cudaFuncSetAttribute(row_sums_general_kernel<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-    if (ce == cudaSuccess) ce = cudaFuncSetAttribute(entry_sums_general_kernel<A>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); \
-    if (ce != cudaSuccess) return (int)ce; \
+#define RG_KW(A) { RG_ALLOW_SMEM(row_sums_general_kernel<A>, kw_smem(256)) \
+    RG_ALLOW_SMEM(entry_sums_general_kernel<A>, kw_smem(256)) \
     const int e = rg_launch(row_sums_general_kernel<A>, by_query, dim3(KW_THREADS), smem, s, 1, a); \
     return e ? e : rg_launch(entry_sums_general_kernel<A>, by_entry, dim3(KW_THREADS), smem, s, 1, a); }
     if (dtype == RG_DTYPE_F32) RG_KW(float)

@@ -2173,28 +2173,42 @@ def decode_attention(q, q_stride: int, out, kv_cache, block_table, rows, n_token
 
 def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> int:
     """What the operators over rows of single tokens and portions ask of queries and cache; returns the page size."""
-    _dtype_code(q)
+    code, (T, n), s = _dtype_code(q), q.shape if q.dim() == 2 else (0, 0), kv_cache.shape
+    if (_fast is not None and _fast.fits(kv_cache, q.dtype) and len(s) == 5 and s[1] == 2 and s[2] == nkv > 0 and s[3] > 0 and s[4] == d
+            and 0 < d <= 256 and nh > 0 and nh % nkv == 0 and q.is_cuda and n >= nh * d):
+        at, step = q.stride()
+        if step == 1 and at >= n:
+            return s[3]
     _check_rows(q, "q")
     _check(kv_cache, "kv_cache", q.dtype)
     if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
         raise KernelError(f"{what}: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
-    if kv_cache.dim() != 5 or tuple(kv_cache.shape[1:3]) != (2, nkv) or kv_cache.shape[4] != d or kv_cache.shape[3] < 1:
-        raise KernelError(f"kv cache shape {tuple(kv_cache.shape)} does not match heads {nkv} x {d}")
-    if q.shape[1] < nh * d:
-        raise KernelError(f"{what}: q has {q.shape[1]} columns, {nh} heads of {d} need {nh * d}")
-    return kv_cache.shape[3]
+    _check_pages(kv_cache, nkv, d)
+    if n < nh * d:
+        raise KernelError(f"{what}: q has {n} columns, {nh} heads of {d} need {nh * d}")
+    return s[3]
 
 
-def _check_ints(t: torch.Tensor, name: str, shape: tuple) -> None:
+def _check_pages(kv_cache, nkv: int, d: int) -> None:
+    s = kv_cache.shape
+    if len(s) != 5 or s[1] != 2 or s[2] != nkv or s[4] != d or s[3] < 1:
+        raise KernelError(f"kv cache shape {tuple(s)} does not match heads {nkv} x {d}")
+
+
+def _check_ints(t: torch.Tensor, name: str, rows: int | None, cols: int | None = None, table: bool = False) -> None:
+    """int32 [rows], or [rows, cols] of a ``table`` (None: any)."""
     _check(t, name, torch.int32)
-    if t.dim() != len(shape) or any(n is not None and t.shape[i] != n for i, n in enumerate(shape)):
-        raise KernelError(f"{name} is {tuple(t.shape)}, expected {tuple('any' if n is None else n for n in shape)}")
+    s = t.shape
+    if (len(s) != (2 if table else 1) or (rows is not None and s[0] != rows) or (cols is not None and s[1] != cols)):
+        raise KernelError(f"{name} is {tuple(s)}, expected [{rows if rows is not None else 'any'}{', ' if table else ''}"
+                          f"{(cols if cols is not None else 'any') if table else ''}]")
 
 
 def _check_entry_weights(weights: torch.Tensor, name: str, nkv: int, max_context: int, dtype=torch.float32) -> None:
     _check(weights, name, dtype)
-    if weights.dim() != 3 or weights.shape[1] != nkv or weights.shape[2] < max_context:
-        raise KernelError(f"{name} is {tuple(weights.shape)}, expected [slots, {nkv}, at least {max_context}]")
+    s = weights.shape
+    if len(s) != 3 or s[1] != nkv or s[2] < max_context:
+        raise KernelError(f"{name} is {tuple(s)}, expected [slots, {nkv}, at least {max_context}]")
 
 
 def _tc_error_flag(device) -> torch.Tensor:
@@ -2245,10 +2259,10 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     sums are 32-bit and have one order."""
     page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prefix_attention")
     T = q.shape[0]
-    _check_ints(groups, "groups", (None, 3))
-    _check_ints(prefix_table, "prefix_table", (groups.shape[0], None))
-    _check_ints(block_table, "block_table", (T, None))
-    _check_ints(positions, "positions", (T,))
+    _check_ints(groups, "groups", None, 3, table=True)
+    _check_ints(prefix_table, "prefix_table", groups.shape[0], table=True)
+    _check_ints(block_table, "block_table", T, table=True)
+    _check_ints(positions, "positions", T)
     _check_out_view(out, T, nh * d, q.dtype, "prefix_attention")
     if min(max_rows, max_prefix, max_own) < 0:
         raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
@@ -2283,9 +2297,9 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     are not seen.  All sums are 32-bit and have one order."""
     page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
     R = q.shape[0]
-    _check_ints(block_table, "block_table", (R, None))
-    _check_ints(positions, "positions", (R,))
-    _check_ints(slots, "slots", (R,))
+    _check_ints(block_table, "block_table", R, table=True)
+    _check_ints(positions, "positions", R)
+    _check_ints(slots, "slots", R)
     _check_out_view(out, R, nh * d, q.dtype, "weighed_attention")
     if max_context < 0:
         raise KernelError("weighed_attention: max_context is a count")
@@ -2319,12 +2333,12 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     theirs.  ``max_rows``, ``max_context``: the most rows of a request and the most entries a row may see.  All sums are 32-bit and
     have one order."""
     page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prompt_key_weights")
-    _check_ints(slots, "slots", (None,))
+    _check_ints(slots, "slots", None)
     R = slots.shape[0]
-    _check_ints(block_table, "block_table", (R, None))
-    _check_ints(cu_rows, "cu_rows", (R + 1,))
-    _check_ints(starts, "starts", (R,))
-    _check_ints(fresh, "fresh", (R,))
+    _check_ints(block_table, "block_table", R, table=True)
+    _check_ints(cu_rows, "cu_rows", R + 1)
+    _check_ints(starts, "starts", R)
+    _check_ints(fresh, "fresh", R)
     if min(max_rows, max_context) < 0:
         raise KernelError("prompt_key_weights: max_rows and max_context are counts")
     _check_entry_weights(weights, "weights", nkv, max_context)
@@ -2344,7 +2358,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
         _ptr(q), c_int(q.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
         _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(q.shape[0]),
         c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z),
-        c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), _ptr(_tc_error_flag(q.device)), _stream()),
+        c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), c_int(num_sms(q.device)), _ptr(_tc_error_flag(q.device)), _stream()),
         "prompt_key_weights")
 
 
@@ -2360,13 +2374,12 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     negative slot are left alone."""
     _dtype_code(kv_cache)
     _check(kv_cache, "kv_cache")
-    _check_ints(slots, "slots", (None,))
+    _check_ints(slots, "slots", None)
     R = slots.shape[0]
-    if kv_cache.dim() != 5 or tuple(kv_cache.shape[1:3]) != (2, nkv) or kv_cache.shape[4] != d or kv_cache.shape[3] < 1:
-        raise KernelError(f"kv cache shape {tuple(kv_cache.shape)} does not match heads {nkv} x {d}")
-    _check_ints(block_table, "block_table", (R, None))
+    _check_pages(kv_cache, nkv, d)
+    _check_ints(block_table, "block_table", R, table=True)
     for t, name in ((lens, "lens"), (keep, "keep"), (positions, "positions")):
-        _check_ints(t, name, (R,))
+        _check_ints(t, name, R)
     if max_context < 0 or protect_first < 0 or protect_last < 0:
         raise KernelError("evict_entries: max_context, protect_first and protect_last are counts")
     for t, name, dtype in ((weights, "weights", torch.float32), (places, "places", torch.int32),
@@ -2390,7 +2403,7 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
         _ptr(kv_cache), c_int(kv_cache.element_size()), _ptr(weights), _ptr(places), _ptr(weights_out), _ptr(places_out),
         c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(lens), _ptr(keep),
         _ptr(positions), _ptr(new_lens), c_int(R), c_int(nkv), c_int(d), c_int(kv_cache.shape[3]), c_int(protect_first),
-        c_int(protect_last), c_int(max_context), _ptr(moves), c_int(cluster), _stream()), "evict_entries")
+        c_int(protect_last), c_int(max_context), _ptr(moves), c_int(cluster), c_int(num_sms(kv_cache.device)), _stream()), "evict_entries")
     return new_lens
 
 
