@@ -4,6 +4,8 @@
 #include "attention_parts.cuh"
 #include "mma.cuh"
 #include "attention_prefix_tcgen05.cuh"
+#include <cooperative_groups.h>
+namespace cg = cooperative_groups;
 using rgmma::mma_bf16;
 using rgmma::pack_bf16;
 
@@ -29,22 +31,107 @@ template <> struct Quad<bf16> {
     }
 };
 
-__host__ __device__ inline int pg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
+// Where whole rows go: blocks that see all of a row's entries, or share them in a cluster, leave no parts.
+struct RowsArgs {
+    void* out;                   // [T, out_ld]
+    float* weights;              // [n_slots, nkv, weights_ld]
+    const int* slots;            // [T]
+    long long weights_ld;
+    int out_ld, n_slots, runs;   // runs: of 16 entries a block may have (its scores' place in shared memory)
+    float decay;
+};
 
-template <typename A, int DP, bool VEC>
-__global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArgs a) {
+__host__ __device__ inline int pg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
+__host__ __device__ inline int pg_stages(int d) { return d <= 128 ? 2 : 1; }   // tiles of K and V in shared memory: the next one is on its way
+
+// Query r's M and 1 / L from what the blocks of a cluster have ([queries][2] each).
+__device__ __forceinline__ void join_cluster_ml(cg::cluster_group& cluster, float* ml, int r, float& M, float& inv) {
+    const int C = cluster.num_blocks();
+    float m = -INFINITY, L = 0.f;
+    for (int k = 0; k < C; ++k) m = fmaxf(m, cluster.map_shared_rank(ml, k)[r * 2]);
+    M = m == -INFINITY ? 0.f : m;
+    for (int k = 0; k < C; ++k) {
+        const float* from = cluster.map_shared_rank(ml, k) + r * 2;
+        L += exp2f(from[0] - M) * from[1];
+    }
+    inv = L > 0.f ? 1.f / L : 0.f;
+}
+
+// WHOLE: a cluster takes all entries of a row, its prefix's and then its own, and leaves the output, and the weights where b has a
+// place for them (their scores wait in a.scores).
+template <typename A, int DP, bool VEC, bool WHOLE>
+__global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArgs a, const RowsArgs b) {
     extern __shared__ __align__(16) float smem[];
     constexpr int GROUPS = PG_THREADS / DP, COLS = DP == 128 ? 2 : 1;
     PartShare s;
     pdl_wait();
     pdl_trigger();
-    if (!part_share(a, PG_Q, blockIdx.x, s)) return;
-    const int d = a.d, ld = pg_row(d), group = a.nh / a.nkv, tid = threadIdx.x;
+    int P = 0;
+    const int* prefix_table = nullptr;
+    int C = 1, rank = 0;
+    if constexpr (WHOLE) {
+        C = cg::this_cluster().num_blocks();
+        rank = cg::this_cluster().block_rank();
+        const int block = blockIdx.x / C, tile = block % a.own_tiles, tk = block / a.own_tiles;
+        s.row0 = tk / a.nkv; s.kvh = tk % a.nkv; s.q0 = tile * PG_Q; s.nq = min(PG_Q, a.nh / a.nkv - s.q0);
+        s.table = a.block_table + (size_t)s.row0 * a.max_blocks;
+        s.e0 = 0; s.e1 = max(0, own_entries(a, s.row0));
+        prefix_table = prefix_of(a, s.row0, P);
+    } else if (!part_share(a, PG_Q, blockIdx.x, s)) return;
+    const int d = a.d, ld = pg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = pg_stages(d);
     float* qs = smem;                                               // [16][ld]
-    float* ks = qs + PG_Q * ld;                                     // [64][ld]
-    float* vs = ks + PG_K * ld;                                     // [64][ld]
-    float* ps = vs + PG_K * ld;                                     // [16][PG_LD]
+    float* kv0 = qs + PG_Q * ld;                                    // [stages][K [64][ld], V [64][ld]]
+    float* ps = kv0 + stages * 2 * PG_K * ld;                       // [16][PG_LD]
     float* al = ps + PG_Q * PG_LD;                                  // [16]
+    __shared__ long long row_at[2][PG_K];                           // where the rows of a tile are in the cache, -1 behind its end
+    const size_t page_elems = (size_t)2 * a.nkv * a.page_size * d, to_values = (size_t)a.nkv * a.page_size * d;
+    const int prefix_tiles = (P + PG_K - 1) / PG_K, tiles = prefix_tiles + (s.e1 - s.e0 + PG_K - 1) / PG_K;
+    const int per = (tiles + C - 1) / C, tile0 = min(tiles, rank * per), tile1 = min(tiles, tile0 + per);      // this block's
+    // tile's first entry in its list, and how many entries of it there are
+    auto tile_of = [&](int tile, int& e0) -> int {
+        const bool shared = tile < prefix_tiles;                    // entries of the prefix
+        e0 = shared ? tile * PG_K : s.e0 + (tile - prefix_tiles) * PG_K;
+        return min(PG_K, (shared ? P : s.e1) - e0);
+    };
+    auto look_up = [&](int tile) -> long long {                     // threads 0 .. 63: a row each
+        int e0;
+        const int n = tile < tile1 ? tile_of(tile, e0) : 0;
+        if (tid >= n) return -1;
+        const int e = e0 + tid;
+        return (long long)((tile < prefix_tiles ? prefix_table : s.table)[e / a.page_size]) * (long long)page_elems +
+               ((long long)s.kvh * a.page_size + e % a.page_size) * d;
+    };
+    // a thread's pieces of a tile: every 128th
+    const int pieces = VEC ? d / 4 : d, row_first = tid / pieces, piece_first = tid - row_first * pieces, row_step = PG_THREADS / pieces,
+              piece_step = PG_THREADS - row_step * pieces;
+    auto request = [&](int tile, float* ks) {                       // rows behind the end are zeros
+        constexpr int W = VEC ? 4 : 1;
+        float* vs = ks + PG_K * ld;
+        for (int row = row_first, p = piece_first; row < PG_K; p += piece_step, row += row_step) {
+            if (p >= pieces) { p -= pieces; if (++row >= PG_K) break; }
+            const int c = p * W;
+            const long long at = row_at[tile & 1][row];
+            const A* src = (const A*)a.kv + (at < 0 ? 0 : at + c);
+            if constexpr (VEC && sizeof(A) == 4) {
+                rgmma::cp_async16(ks + row * ld + c, src, at >= 0);
+                rgmma::cp_async16(vs + row * ld + c, src + (at < 0 ? 0 : to_values), at >= 0);
+            } else {
+                float4 k4 = {0.f, 0.f, 0.f, 0.f}, v4 = k4;
+                if (at >= 0) {
+                    if constexpr (VEC) { k4 = Quad<A>::load(src); v4 = Quad<A>::load(src + to_values); }
+                    else { k4.x = to_f32(src[0]); v4.x = to_f32(src[to_values]); }
+                }
+                if constexpr (VEC) {
+                    *reinterpret_cast<float4*>(ks + row * ld + c) = k4;
+                    *reinterpret_cast<float4*>(vs + row * ld + c) = v4;
+                } else { ks[row * ld + c] = k4.x; vs[row * ld + c] = v4.x; }
+            }
+        }
+        if (!VEC)                                                   // the scores read four columns at a time
+            for (int i = tid; i < PG_K * (ld - d); i += PG_THREADS) ks[i / (ld - d) * ld + d + i % (ld - d)] = 0.f;
+        rgmma::cp_async_commit();
+    };
+    if (tid < PG_K) { row_at[tile0 & 1][tid] = look_up(tile0); row_at[(tile0 + 1) & 1][tid] = look_up(tile0 + 1); }
     for (int i = tid; i < PG_Q * ld; i += PG_THREADS) {
         const int row = i / ld, c = i - row * ld, qi = s.q0 + row;
         float v = 0.f;
@@ -52,8 +139,13 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
             v = to_f32(((const A*)a.q)[(size_t)(s.row0 + qi / group) * a.q_stride + (s.kvh * group + qi % group) * d + c]) * a.scale_log2;
         qs[i] = v;
     }
-    const size_t page_elems = (size_t)2 * a.nkv * a.page_size * d, to_values = (size_t)a.nkv * a.page_size * d;
     const int qa = tid >> 4, ka = tid & 15;                         // scores: queries 2 qa, 2 qa + 1; entries ka + 16 j
+    float* keep[2];                                                 // where their scores go
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int qi = s.q0 + 2 * qa + i;
+        keep[i] = a.scores && 2 * qa + i < s.nq ? a.scores + ((size_t)(s.row0 + qi / group) * a.nh + s.kvh * group + qi % group) * a.score_ld + ka : nullptr;
+    }
     const int col = tid % DP, part = tid / DP;                      // output: column(s) col (+ 128), entries part + GROUPS j
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float acc[COLS][PG_Q];
@@ -61,30 +153,24 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
     for (int c = 0; c < COLS; ++c)
 #pragma unroll
         for (int i = 0; i < PG_Q; ++i) acc[c][i] = 0.f;
-    for (int e0 = s.e0; e0 < s.e1; e0 += PG_K) {
-        const int n = min(PG_K, s.e1 - e0);
-        __syncthreads();                                            // the last tile's values are read
-        constexpr int W = VEC ? 4 : 1;
-        const int pieces = VEC ? d / 4 : d;
-        for (int i = tid; i < PG_K * pieces; i += PG_THREADS) {     // rows beyond the part are zeros
-            const int row = i / pieces, c = (i - row * pieces) * W;
-            float4 k4 = {0.f, 0.f, 0.f, 0.f}, v4 = k4;
-            if (row < n) {
-                const int e = e0 + row;
-                const A* src = (const A*)a.kv + (size_t)s.table[e / a.page_size] * page_elems +
-                               ((size_t)s.kvh * a.page_size + e % a.page_size) * d + c;
-                if constexpr (VEC) { k4 = Quad<A>::load(src); v4 = Quad<A>::load(src + to_values); }
-                else { k4.x = to_f32(src[0]); v4.x = to_f32(src[to_values]); }
-            }
-            if constexpr (VEC) {
-                *reinterpret_cast<float4*>(ks + row * ld + c) = k4;
-                *reinterpret_cast<float4*>(vs + row * ld + c) = v4;
-            } else { ks[row * ld + c] = k4.x; vs[row * ld + c] = v4.x; }
+    __syncthreads();
+    if (stages == 2 && tile0 < tile1) request(tile0, kv0 + (tile0 & 1) * 2 * PG_K * ld);
+    for (int tile = tile0; tile < tile1; ++tile) {
+        int e0;
+        const bool shared = tile < prefix_tiles;
+        const int n = tile_of(tile, e0);
+        float* ks = kv0 + (stages == 2 ? (tile & 1) * 2 * PG_K * ld : 0);
+        const float* vs = ks + PG_K * ld;
+        if (stages == 1) {
+            __syncthreads();                                        // the last tile's values are read
+            request(tile, ks);
         }
-        if (!VEC)                                                   // the scores read four columns at a time
-            for (int i = tid; i < PG_K * (ld - d); i += PG_THREADS) ks[i / (ld - d) * ld + d + i % (ld - d)] = 0.f;
-        __syncthreads();
+        rgmma::cp_async_wait<0>();
+        __syncthreads();                                            // the tile is there; with two stages the last one is read
+        if (stages == 2 && tile + 1 < tile1) request(tile + 1, kv0 + ((tile + 1) & 1) * 2 * PG_K * ld);
+        const long long at_next = tid < PG_K ? look_up(tile + 2) : -1;
         float sc[2][4] = {};
+#pragma unroll 4
         for (int c = 0; c < d; c += 4) {
             float4 q4[2];
 #pragma unroll
@@ -101,14 +187,11 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int qi = s.q0 + 2 * qa + i;
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int e = ka + 16 * j;
-                if (e >= n) sc[i][j] = -INFINITY;
-                else if (a.scores && 2 * qa + i < s.nq)
-                    a.scores[((size_t)(s.row0 + qi / group) * a.nh + s.kvh * group + qi % group) * a.score_ld + e0 + e] = sc[i][j];
+                if (ka + 16 * j >= n) sc[i][j] = -INFINITY;
+                else if (keep[i] && !shared) keep[i][e0 + 16 * j] = sc[i][j];
                 mx = fmaxf(mx, sc[i][j]);
             }
 #pragma unroll
@@ -126,6 +209,7 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
             if (ka == 0) al[2 * qa + i] = f;
         }
         __syncthreads();
+        if (tid < PG_K) row_at[tile & 1][tid] = at_next;            // requested from after the next barrier
 #pragma unroll
         for (int i = 0; i < PG_Q; ++i) {
             const float f = al[i];
@@ -158,13 +242,54 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
     if constexpr (GROUPS > 1) {                                     // the groups' sums, added in their order
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < PG_Q; ++i) ks[i * PG_THREADS + tid] = acc[0][i];
+        for (int i = 0; i < PG_Q; ++i) kv0[i * PG_THREADS + tid] = acc[0][i];
         __syncthreads();
         if (part == 0) {
 #pragma unroll
             for (int i = 0; i < PG_Q; ++i)
-                for (int g = 1; g < GROUPS; ++g) acc[0][i] += ks[i * PG_THREADS + g * DP + col];
+                for (int g = 1; g < GROUPS; ++g) acc[0][i] += kv0[i * PG_THREADS + g * DP + col];
         }
+    }
+    if constexpr (WHOLE) {
+        __shared__ float fin_ml[PG_Q][2], row_ml[PG_Q][2];          // this block's M and L; the row's M and 1 / L
+        cg::cluster_group cluster = cg::this_cluster();
+        float* fin = kv0;                                           // [16][d]
+        __syncthreads();                                            // the last tile and the groups' sums are read
+        if (part == 0) {
+#pragma unroll
+            for (int i = 0; i < PG_Q; ++i)
+                if (i < s.nq)
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c)
+                        if (col + DP * c < d) fin[i * d + col + DP * c] = acc[c][i];
+        }
+        if (ka == 0)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { fin_ml[2 * qa + i][0] = m[i]; fin_ml[2 * qa + i][1] = l[i]; }
+        cluster.sync();                                             // every block's result is in place
+        if (tid < s.nq) join_cluster_ml(cluster, &fin_ml[0][0], tid, row_ml[tid][0], row_ml[tid][1]);
+        __syncthreads();
+        const int h0 = s.kvh * group + s.q0;
+        for (int idx = rank * PG_THREADS + tid; idx < s.nq * d; idx += C * PG_THREADS) {
+            const int r = idx / d, c = idx - r * d;
+            float sum = 0.f;
+            for (int k = 0; k < C; ++k)
+                sum += exp2f(cluster.map_shared_rank(&fin_ml[0][0], k)[r * 2] - row_ml[r][0]) * cluster.map_shared_rank(fin, k)[r * d + c];
+            ((A*)b.out)[(size_t)s.row0 * b.out_ld + (h0 + r) * d + c] = from_f32<A>(sum * row_ml[r][1]);
+        }
+        const int slot = b.weights ? b.slots[s.row0] : -1;
+        if (slot >= 0 && slot < b.n_slots) {
+            float* to = b.weights + ((size_t)slot * a.nkv + s.kvh) * b.weights_ld;
+            const int first = max(0, tile0 - prefix_tiles) * PG_K, last = min(s.e1, (tile1 - prefix_tiles) * PG_K);   // own entries of this block
+            for (int e = first + tid; e < last; e += PG_THREADS) {
+                const float* sc = a.scores + ((size_t)s.row0 * a.nh + h0) * a.score_ld + e;
+                float sum = 0.f;
+                for (int i = 0; i < s.nq; ++i) sum += exp2f(sc[(size_t)i * a.score_ld] - row_ml[i][0]) * row_ml[i][1];
+                to[e] = (e == s.e1 - 1 ? 0.f : b.decay * to[e]) + sum;
+            }
+        }
+        cluster.sync();                                             // nobody leaves while its results are being read
+        return;
     }
     const int slots = a.prefix_parts + a.own_parts;
     auto place = [&](int row) -> size_t {
@@ -203,6 +328,13 @@ __host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 6
 __host__ __device__ constexpr int pm_stage_bytes(int pieces) { return 16 * 64 * 2 * 2 * pieces; }
 static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1) * pm_stage_bytes(1), "the warps' results fit where the stages were");
 
+// A run of 16 entries from entry e of its list on: one box, or where pages hold 8 tokens two.  One lane.
+__device__ __forceinline__ void load_run(const CUtensorMap* map, const PartArgs& a, uint32_t dst, uint32_t bar, int bytes, int box_shift, int page_a,
+                                         int page_b, int kvh, int e) {
+    mbar_expect_tx(bar, bytes);
+    tma_load_4d_row(dst, map, bar, (page_a * 2 * a.nkv + kvh) * a.page_size + (e & (a.page_size - 1)));
+    if (box_shift == 3) tma_load_4d_row(dst + bytes / 2, map, bar, (page_b * 2 * a.nkv + kvh) * a.page_size);
+}
 __device__ __forceinline__ void ldmatrix_x4_at(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
@@ -210,95 +342,46 @@ __device__ __forceinline__ void ldmatrix_x4_trans_at(uint32_t (&r)[4], uint32_t 
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 
+// A warp's 16 queries and what it has added up over the runs it has seen.
 template <int PIECES>          // the head size in pieces of 64
-__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
-parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, int* err) {
-    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES), KD = D / 16, ND = D / 8;
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t bars[4 * STAGES];
-    __shared__ float ml[4][PM_Q][2];
-    __shared__ int abort_flag;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const uint32_t base = ((smem_addr(smem_raw) + 1023u) & ~1023u) + (uint32_t)(warp * STAGES * STAGE);
-    const uint32_t bar0 = smem_addr(bars) + (uint32_t)(8 * STAGES * warp);
-    if (threadIdx.x == 0) abort_flag = 0;
-    if (lane == 0)
-        for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
-    if (lane == 0) fence_barrier_init();
-    __syncthreads();
-    // beside: the launch before this one is prefix_tc_kernel for the same rows, whose blocks have all waited for what came
-    // before them; it leaves its own parts.  What comes behind this kernel waits for both: the last block waits at its end.
-    if (!a.beside) pdl_wait();
-    pdl_trigger();
-    PartShare sh;
-    const bool closes = a.beside && blockIdx.x == gridDim.x - 1;
-    if (!part_share(a, PM_Q, blockIdx.x, sh)) {
-        if (closes) pdl_wait();
-        return;
-    }
-    const int group = a.nh / a.nkv;
-    const int n_runs = (sh.e1 - sh.e0 + 15) >> 4, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
-    // Page ids of this warp's next 32 runs, one a lane (of both halves of a run where pages hold 8).
-    const int box_shift = a.page_shift < 4 ? 3 : 4, box_rows = 1 << box_shift;
-    int page_a = 0, page_b = 0;
-    auto entry_of = [&](int i) -> int { return sh.e0 + (warp + 4 * i) * 16; };
-    auto fetch_pages = [&](int i0) {
-        const int e = entry_of(i0 + lane);
-        page_a = e < sh.e1 ? sh.table[e >> a.page_shift] : 0;
-        if (box_shift == 3) page_b = e + 8 < sh.e1 ? sh.table[(e + 8) >> a.page_shift] : page_a;   // no such entry: any page
-    };
-    auto issue = [&](int i) {                                         // the whole warp: run i of this warp
-        if ((i & 31) == 0) fetch_pages(i);
-        const int pa = __shfl_sync(0xffffffffu, page_a, i & 31), pb = __shfl_sync(0xffffffffu, page_b, i & 31);
-        if (lane == 0) {
-            const int s = i % STAGES, in_page = entry_of(i) & (a.page_size - 1);
-            const uint32_t bar = bar0 + 8 * s, dst = base + s * STAGE;
-            mbar_expect_tx(bar, STAGE);
-            tma_load_4d_row(dst, &kv_map, bar, (pa * 2 * a.nkv + sh.kvh) * a.page_size + in_page);
-            if (box_shift == 3) tma_load_4d_row(dst + STAGE / 2, &kv_map, bar, (pb * 2 * a.nkv + sh.kvh) * a.page_size);
-        }
-        __syncwarp();
-    };
-    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
-
-    // queries: rows g and g + 8 of the tile
+struct MmaQueries {
+    static constexpr int D = 64 * PIECES, KD = D / 16, ND = D / 8;
     uint32_t qf[KD][4];
-    const int qa = sh.q0 + g, qb = qa + 8;
-    const bool has_a = g < sh.nq, has_b = g + 8 < sh.nq;
-    auto head_of = [&](int qi) -> int { return sh.kvh * group + qi % group; };
-    auto row_of = [&](int qi) -> int { return sh.row0 + qi / group; };
-    {
-        const bf16* ra = has_a ? (const bf16*)a.q + (size_t)row_of(qa) * a.q_stride + head_of(qa) * D + 2 * tq : nullptr;
-        const bf16* rb = has_b ? (const bf16*)a.q + (size_t)row_of(qb) * a.q_stride + head_of(qb) * D + 2 * tq : nullptr;
+    float o[ND][4], m0, m1, l0, l1;                                   // rows g and g + 8 of the tile
+    uint32_t k_line, v_line, sw, k_c, v_c, piece;                     // where this lane's ldmatrix rows are in a stage
+    int lane, g, tq, box_shift;
+
+    // A stage is boxes of 1 << box_shift rows: K's 64-column pieces one after the other, then V's.
+    __device__ __forceinline__ uint32_t line(int r) const {
+        return (uint32_t)((((r >> box_shift) * 2 * PIECES) << box_shift) + (r & ((1 << box_shift) - 1))) * 128u;
+    }
+    __device__ __forceinline__ void init(int lane_, int box_shift_) {
+        lane = lane_; g = lane >> 2; tq = lane & 3; box_shift = box_shift_;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.f;
+        const int kr = (lane & 7) + (lane >> 4) * 8, vr = (lane & 7) + ((lane >> 3) & 1) * 8;   // K as the B operand, V transposed
+        k_line = line(kr);
+        v_line = line(vr) + (uint32_t)(PIECES << box_shift) * 128u;
+        sw = (uint32_t)(lane & 7);
+        k_c = (lane >> 3) & 1;
+        v_c = lane >> 4;
+        piece = (uint32_t)(128 << box_shift);
+    }
+    __device__ __forceinline__ void queries(const bf16* ra, const bf16* rb) {      // rows g and g + 8, null: zeros
 #pragma unroll
         for (int k = 0; k < KD; ++k) {
-            qf[k][0] = has_a ? *reinterpret_cast<const uint32_t*>(ra + k * 16) : 0u;
-            qf[k][1] = has_b ? *reinterpret_cast<const uint32_t*>(rb + k * 16) : 0u;
-            qf[k][2] = has_a ? *reinterpret_cast<const uint32_t*>(ra + k * 16 + 8) : 0u;
-            qf[k][3] = has_b ? *reinterpret_cast<const uint32_t*>(rb + k * 16 + 8) : 0u;
+            qf[k][0] = ra ? *reinterpret_cast<const uint32_t*>(ra + k * 16 + 2 * tq) : 0u;
+            qf[k][1] = rb ? *reinterpret_cast<const uint32_t*>(rb + k * 16 + 2 * tq) : 0u;
+            qf[k][2] = ra ? *reinterpret_cast<const uint32_t*>(ra + k * 16 + 8 + 2 * tq) : 0u;
+            qf[k][3] = rb ? *reinterpret_cast<const uint32_t*>(rb + k * 16 + 8 + 2 * tq) : 0u;
         }
     }
-    float *score_a = nullptr, *score_b = nullptr;
-    if (a.scores) {
-        if (has_a) score_a = a.scores + ((size_t)row_of(qa) * a.nh + head_of(qa)) * a.score_ld + 2 * tq;
-        if (has_b) score_b = a.scores + ((size_t)row_of(qb) * a.nh + head_of(qb)) * a.score_ld + 2 * tq;
-    }
-    float o[ND][4];
-#pragma unroll
-    for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    // where this lane's ldmatrix rows are in a stage: K rows as the B operand, V rows transposed
-    auto line = [&](int r) -> uint32_t { return (uint32_t)((((r >> box_shift) * 2 * PIECES) << box_shift) + (r & (box_rows - 1))) * 128u; };
-    const int kr = (lane & 7) + (lane >> 4) * 8, vr = (lane & 7) + ((lane >> 3) & 1) * 8;
-    const uint32_t k_line = line(kr), v_line = line(vr) + (uint32_t)(PIECES << box_shift) * 128u, sw = (uint32_t)(lane & 7);
-    const uint32_t k_c = (lane >> 3) & 1, v_c = lane >> 4, piece = (uint32_t)(128 << box_shift);
-    bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-        const int s = i % STAGES, e = entry_of(i);
-        const uint32_t st = base + s * STAGE;
-        ok = mbar_wait_all(bar0 + 8 * s, (i / STAGES) & 1, err, 61, &abort_flag);
-        if (!ok) break;
-        const int n = sh.e1 - e;                                      // entries of this run, if below 16
+    // The run in stage `st`, of which n entries are looked at (16 or more: all).  keep(v): the scores of row g, entries
+    // 2 tq + {0, 1, 8, 9}, then those of row g + 8.
+    template <typename Keep>
+    __device__ __forceinline__ void step(uint32_t st, int n, float scale_log2, Keep keep) {
         if (n < 16) {
             // rows of V behind the last entry are what an earlier request left: 0 times an infinity is no number
             for (int j = lane; j < (16 - n) * 8 * PIECES; j += 32) {
@@ -306,6 +389,7 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
                              ::"r"(st + line(r) + (uint32_t)(PIECES << box_shift) * 128u + (c >> 3) * piece + (c & 7) * 16), "r"(0) : "memory");
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the stage's next box comes after these
             __syncwarp();
         }
         float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -316,21 +400,13 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
             mma_bf16(s0, qf[k], b[0], b[1]);
             mma_bf16(s1, qf[k], b[2], b[3]);
         }
-        // rows g (first two of four) and g + 8, entries e + 2 tq + {0, 1} and + 8
         float v[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[j] *= a.scale_log2;
+            v[j] *= scale_log2;
             if (n < 16 && 2 * tq + (j & 1) + ((j & 2) << 2) >= n) v[j] = -INFINITY;
         }
-        if (score_a) {
-            *reinterpret_cast<float2*>(score_a + e) = make_float2(v[0], v[1]);
-            *reinterpret_cast<float2*>(score_a + e + 8) = make_float2(v[2], v[3]);
-        }
-        if (score_b) {
-            *reinterpret_cast<float2*>(score_b + e) = make_float2(v[4], v[5]);
-            *reinterpret_cast<float2*>(score_b + e + 8) = make_float2(v[6], v[7]);
-        }
+        keep(v);
         float x0 = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), x1 = fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7]));
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
         x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2)); x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
@@ -357,43 +433,264 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
             mma_bf16(o[2 * k + 1], p, b[2], b[3]);
         }
         __syncwarp();                                                 // every lane has read the stage
+    }
+    // What the warp has, to shared memory: co [16][D], ml [16][2].
+    __device__ __forceinline__ void leave(float* co, float (*ml)[2]) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+            *reinterpret_cast<float2*>(co + g * D + j * 8 + 2 * tq) = make_float2(o[j][0], o[j][1]);
+            *reinterpret_cast<float2*>(co + (g + 8) * D + j * 8 + 2 * tq) = make_float2(o[j][2], o[j][3]);
+        }
+        if (tq == 0) { ml[g][0] = m0; ml[g][1] = l0; ml[g + 8][0] = m1; ml[g + 8][1] = l1; }
+    }
+};
+// The four warps' results for row r, columns c .. c + 3: unnormalised sum, M and L.
+template <int D>
+__device__ __forceinline__ float4 join_warps(const float* all, const float (*ml)[PM_Q][2], int r, int c, float& M, float& L) {
+    M = -INFINITY;
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][r][0]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = ex2(ml[w][r][0] - ref);
+        const float4 x = *reinterpret_cast<const float4*>(all + (w * PM_Q + r) * D + c);
+        L += f * ml[w][r][1];
+        sum.x += f * x.x; sum.y += f * x.y; sum.z += f * x.z; sum.w += f * x.w;
+    }
+    return sum;
+}
+
+template <int PIECES>
+__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
+parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, int* err) {
+    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t bars[4 * STAGES];
+    __shared__ float ml[4][PM_Q][2];
+    __shared__ int abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t first_stage = (smem_addr(smem_raw) + 1023u) & ~1023u, base = first_stage + (uint32_t)(warp * STAGES * STAGE);
+    const uint32_t bar0 = smem_addr(bars) + (uint32_t)(8 * STAGES * warp);
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
+    // beside: the launch before this one is prefix_tc_kernel for the same rows, whose blocks have all waited for what came
+    // before them; it leaves its own parts.  What comes behind this kernel waits for both: the last block waits at its end.
+    if (!a.beside) pdl_wait();
+    pdl_trigger();
+    PartShare sh;
+    const bool closes = a.beside && blockIdx.x == gridDim.x - 1;
+    if (!part_share(a, PM_Q, blockIdx.x, sh)) {
+        if (closes) pdl_wait();
+        return;
+    }
+    const int group = a.nh / a.nkv;
+    const int n_runs = (sh.e1 - sh.e0 + 15) >> 4, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
+    // Page ids of this warp's next 32 runs, one a lane (of both halves of a run where pages hold 8).
+    const int box_shift = a.page_shift < 4 ? 3 : 4;
+    int page_a = 0, page_b = 0;
+    auto entry_of = [&](int i) -> int { return sh.e0 + (warp + 4 * i) * 16; };
+    auto issue = [&](int i) {                                         // the whole warp: run i of this warp
+        if ((i & 31) == 0) {
+            const int e = entry_of(i + lane);
+            page_a = e < sh.e1 ? sh.table[e >> a.page_shift] : 0;
+            if (box_shift == 3) page_b = e + 8 < sh.e1 ? sh.table[(e + 8) >> a.page_shift] : page_a;   // no such entry: any page
+        }
+        const int pa = __shfl_sync(0xffffffffu, page_a, i & 31), pb = __shfl_sync(0xffffffffu, page_b, i & 31);
+        if (lane == 0) load_run(&kv_map, a, base + (i % STAGES) * STAGE, bar0 + 8 * (i % STAGES), STAGE, box_shift, pa, pb, sh.kvh, entry_of(i));
+        __syncwarp();
+    };
+    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
+
+    MmaQueries<PIECES> w;
+    w.init(lane, box_shift);
+    const int qa = sh.q0 + w.g, qb = qa + 8;
+    auto head_of = [&](int qi) -> int { return sh.kvh * group + qi % group; };
+    auto row_of = [&](int qi) -> int { return sh.row0 + qi / group; };
+    const bool has_a = w.g < sh.nq, has_b = w.g + 8 < sh.nq;
+    w.queries(has_a ? (const bf16*)a.q + (size_t)row_of(qa) * a.q_stride + head_of(qa) * D : nullptr,
+              has_b ? (const bf16*)a.q + (size_t)row_of(qb) * a.q_stride + head_of(qb) * D : nullptr);
+    float *score_a = nullptr, *score_b = nullptr;
+    if (a.scores) {
+        if (has_a) score_a = a.scores + ((size_t)row_of(qa) * a.nh + head_of(qa)) * a.score_ld + 2 * w.tq;
+        if (has_b) score_b = a.scores + ((size_t)row_of(qb) * a.nh + head_of(qb)) * a.score_ld + 2 * w.tq;
+    }
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+        const int s = i % STAGES, e = entry_of(i);
+        ok = mbar_wait_all(bar0 + 8 * s, (i / STAGES) & 1, err, 61, &abort_flag);
+        if (!ok) break;
+        w.step(base + s * STAGE, sh.e1 - e, a.scale_log2, [&](const float (&v)[8]) {
+            if (score_a) {
+                *reinterpret_cast<float2*>(score_a + e) = make_float2(v[0], v[1]);
+                *reinterpret_cast<float2*>(score_a + e + 8) = make_float2(v[2], v[3]);
+            }
+            if (score_b) {
+                *reinterpret_cast<float2*>(score_b + e) = make_float2(v[4], v[5]);
+                *reinterpret_cast<float2*>(score_b + e + 8) = make_float2(v[6], v[7]);
+            }
+        });
         if (i + STAGES < mine) issue(i + STAGES);
     }
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     if (!ok || abort_flag)                                            // give copies in flight time to land
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
     // the four warps' results, through the stages' memory (every copy has landed and been read)
     __syncthreads();
-    float* all = reinterpret_cast<float*>(smem_raw + (((smem_addr(smem_raw) + 1023u) & ~1023u) - smem_addr(smem_raw)));   // [4][16][D]
-    float* co = all + warp * PM_Q * D;
-#pragma unroll
-    for (int j = 0; j < ND; ++j) {
-        *reinterpret_cast<float2*>(co + g * D + j * 8 + 2 * tq) = make_float2(o[j][0], o[j][1]);
-        *reinterpret_cast<float2*>(co + (g + 8) * D + j * 8 + 2 * tq) = make_float2(o[j][2], o[j][3]);
-    }
-    if (tq == 0) { ml[warp][g][0] = m0; ml[warp][g][1] = l0; ml[warp][g + 8][0] = m1; ml[warp][g + 8][1] = l1; }
+    float* all = reinterpret_cast<float*>(smem_raw + (first_stage - smem_addr(smem_raw)));   // [4][16][D]
+    w.leave(all + warp * PM_Q * D, ml[warp]);
     __syncthreads();
     const int slots = a.prefix_parts + a.own_parts;
     for (int idx = threadIdx.x; idx < sh.nq * (D / 4); idx += PM_THREADS) {
         const int r = idx / (D / 4), c = idx % (D / 4) * 4, qi = sh.q0 + r;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[w][r][0]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = ex2(ml[w][r][0] - ref);
-            const float4 x = *reinterpret_cast<const float4*>(all + (w * PM_Q + r) * D + c);
-            L += f * ml[w][r][1];
-            sum.x += f * x.x; sum.y += f * x.y; sum.z += f * x.z; sum.w += f * x.w;
-        }
+        float M, L;
+        const float4 sum = join_warps<D>(all, ml, r, c, M, L);
         const size_t place = ((size_t)row_of(qi) * a.nh + head_of(qi)) * slots + sh.slot;
         *reinterpret_cast<float4*>(a.part_o + place * D + c) = sum;
         if (c == 0) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(M, L);
     }
     if (closes) pdl_wait();
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Few rows, in one launch: a cluster takes a row and up to 16 heads of a kv head and cuts the row's entries (its prefix's, then
+// its own) among its blocks, which join through each other's shared memory.  A prefix is then read once for every row, out
+// of L2; what is saved is the second launch and the parts' trip through memory.  With WEIGH the scores stay in shared memory
+// until the row's sums are known, and the entries' weights are written by the block that read them.
+// grid (cluster, nkv x tiles of heads, T)
+// ---------------------------------------------------------------------------------------------------
+template <int PIECES, bool WEIGH>
+__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
+rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, const RowsArgs b, int* err) {
+    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t bars[4 * STAGES];
+    __shared__ float ml[4][PM_Q][2], fin_ml[PM_Q][2], row_ml[PM_Q][2];
+    __shared__ int abort_flag;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = cluster.num_blocks(), rank = cluster.block_rank();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t first_stage = (smem_addr(smem_raw) + 1023u) & ~1023u, base = first_stage + (uint32_t)(warp * STAGES * STAGE);
+    const uint32_t bar0 = smem_addr(bars) + (uint32_t)(8 * STAGES * warp);
+    float* all = reinterpret_cast<float*>(smem_raw + (first_stage - smem_addr(smem_raw)));   // [4][16][D], then the block's [16][D]
+    float* fin = all + 4 * PM_Q * D;
+    float* scores = all + 4 * STAGES * STAGE / 4;                     // [heads][ld]
+    const int ld = b.runs * 16 + 8;
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(bar0 + 8 * s, 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+    const int t = blockIdx.z, group = a.nh / a.nkv, kvh = blockIdx.y / a.own_tiles, q0 = blockIdx.y % a.own_tiles * PM_Q;
+    const int nq = min(PM_Q, group - q0), h0 = kvh * group + q0;
+    int P = 0;
+    const int* prefix_table = prefix_of(a, t, P);
+    const int own = max(0, own_entries(a, t)), prefix_runs = (P + 15) >> 4, total = prefix_runs + ((own + 15) >> 4);
+    const int per = (total + C - 1) / C, first = min(total, rank * per), last = min(total, first + per);
+    const int n_runs = last - first, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
+    const int* own_table = a.block_table + (size_t)t * a.max_blocks;
+    const int box_shift = a.page_shift < 4 ? 3 : 4;
+    int page_a = 0, page_b = 0;
+    // run i of this warp: its first entry in the list that it is in, and how many entries that list has from there on
+    auto place_of = [&](int i, int& e, int& n) -> const int* {
+        const int run = first + warp + 4 * i;
+        const bool shared = run < prefix_runs;
+        e = (shared ? run : run - prefix_runs) * 16;
+        n = (shared ? P : own) - e;
+        return shared ? prefix_table : own_table;
+    };
+    auto issue = [&](int i) {
+        int e, n;
+        if ((i & 31) == 0) {
+            const int* table = place_of(i + lane, e, n);
+            const bool there = i + lane < mine;
+            page_a = there ? table[e >> a.page_shift] : 0;
+            if (box_shift == 3) page_b = there && n > 8 ? table[(e + 8) >> a.page_shift] : page_a;       // no such entry: any page
+        }
+        const int pa = __shfl_sync(0xffffffffu, page_a, i & 31), pb = __shfl_sync(0xffffffffu, page_b, i & 31);
+        place_of(i, e, n);
+        if (lane == 0) load_run(&kv_map, a, base + (i % STAGES) * STAGE, bar0 + 8 * (i % STAGES), STAGE, box_shift, pa, pb, kvh, e);
+        __syncwarp();
+    };
+    for (int i = 0; i < min(STAGES, mine); ++i) issue(i);
+    MmaQueries<PIECES> w;
+    w.init(lane, box_shift);
+    const bool has_a = w.g < nq, has_b = w.g + 8 < nq;
+    const bf16* q = (const bf16*)a.q + (size_t)t * a.q_stride + (size_t)h0 * D;
+    w.queries(has_a ? q + w.g * D : nullptr, has_b ? q + (w.g + 8) * D : nullptr);
+    bool ok = true;
+    for (int i = 0; i < mine; ++i) {
+        const int s = i % STAGES;
+        int e, n;
+        place_of(i, e, n);
+        ok = mbar_wait_all(bar0 + 8 * s, (i / STAGES) & 1, err, 62, &abort_flag);
+        if (!ok) break;
+        w.step(base + s * STAGE, n, a.scale_log2, [&](const float (&v)[8]) {
+            if constexpr (WEIGH) {
+                float* to = scores + w.g * ld + (warp + 4 * i) * 16 + 2 * w.tq;
+                if (has_a) {
+                    *reinterpret_cast<float2*>(to) = make_float2(v[0], v[1]);
+                    *reinterpret_cast<float2*>(to + 8) = make_float2(v[2], v[3]);
+                }
+                if (has_b) {
+                    *reinterpret_cast<float2*>(to + 8 * ld) = make_float2(v[4], v[5]);
+                    *reinterpret_cast<float2*>(to + 8 * ld + 8) = make_float2(v[6], v[7]);
+                }
+            }
+        });
+        if (i + STAGES < mine) issue(i + STAGES);
+    }
+    if (!ok || abort_flag)                                            // give copies in flight time to land
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    __syncthreads();
+    w.leave(all + warp * PM_Q * D, ml[warp]);
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < nq * (D / 4); idx += PM_THREADS) {
+        const int r = idx / (D / 4), c = idx % (D / 4) * 4;
+        float M, L;
+        *reinterpret_cast<float4*>(fin + r * D + c) = join_warps<D>(all, ml, r, c, M, L);
+        if (c == 0) { fin_ml[r][0] = M; fin_ml[r][1] = L; }
+    }
+    cluster.sync();                                                   // every block's result is in place
+    if (threadIdx.x < nq) join_cluster_ml(cluster, &fin_ml[0][0], threadIdx.x, row_ml[threadIdx.x][0], row_ml[threadIdx.x][1]);
+    __syncthreads();
+    for (int idx = rank * PM_THREADS + threadIdx.x; idx < nq * (D / 4); idx += C * PM_THREADS) {
+        const int r = idx / (D / 4), c = idx % (D / 4) * 4;
+        float4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < C; ++k) {
+            const float f = ex2(cluster.map_shared_rank(&fin_ml[0][0], k)[r * 2] - row_ml[r][0]) * row_ml[r][1];
+            const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(fin, k) + r * D + c);
+            sum.x += f * x.x; sum.y += f * x.y; sum.z += f * x.z; sum.w += f * x.w;
+        }
+        bf16* to = (bf16*)b.out + (size_t)t * b.out_ld + (h0 + r) * D + c;
+        to[0] = __float2bfloat16_rn(sum.x); to[1] = __float2bfloat16_rn(sum.y);
+        to[2] = __float2bfloat16_rn(sum.z); to[3] = __float2bfloat16_rn(sum.w);
+    }
+    if constexpr (WEIGH) {
+        const int slot = b.slots[t];
+        if (slot >= 0 && slot < b.n_slots) {
+            float* to = b.weights + ((size_t)slot * a.nkv + kvh) * b.weights_ld;
+            for (int i = threadIdx.x; i < n_runs * 16; i += PM_THREADS) {
+                const int e = first * 16 + i;
+                if (e >= own) break;
+                const float before = e == own - 1 ? 0.f : b.decay * to[e];
+                float sum = 0.f;
+                for (int r = 0; r < nq; ++r) sum += ex2(scores[r * ld + i] - row_ml[r][0]) * row_ml[r][1];
+                to[e] = before + sum;
+            }
+        }
+    }
+    cluster.sync();                                                   // nobody leaves while its results are being read
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -479,22 +776,26 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
 }
 
 // ---------------------------------------------------------------------------------------------------
-static size_t pg_smem(int d) { return (size_t)((PG_Q + 2 * PG_K) * pg_row(d) + PG_Q * PG_LD + PG_Q) * sizeof(float); }
+static size_t pg_smem(int d) { return (size_t)((PG_Q + pg_stages(d) * 2 * PG_K) * pg_row(d) + PG_Q * PG_LD + PG_Q) * sizeof(float); }
 
-static int launch_parts_general(const PartArgs& a, int dtype, cudaStream_t s) {
-    const long long blocks = part_blocks(a);
+// whole: rows that go to their places, a cluster of blocks each (and tile of heads).
+static int launch_parts_general(const PartArgs& a, int dtype, cudaStream_t s, const RowsArgs* whole = nullptr, int cluster = 1) {
+    const long long blocks = whole ? (long long)a.T * a.nkv * a.own_tiles * cluster : part_blocks(a);
     if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     if (blocks == 0) return 0;
     const size_t smem = pg_smem(a.d);
     const bool vec = a.d % 4 == 0 && (((uintptr_t)a.kv) & (dtype == RG_DTYPE_F32 ? 15 : 7)) == 0;
-#define RG_PG(A, DP, VEC) { RG_ALLOW_SMEM((parts_general_kernel<A, DP, VEC>), pg_smem(256)) \
-    return rg_launch(parts_general_kernel<A, DP, VEC>, dim3((unsigned)blocks), dim3(PG_THREADS), smem, s, 1, a); }
+    const RowsArgs b = whole ? *whole : RowsArgs{};
+#define RG_PG_(A, DP, VEC, W) { RG_ALLOW_SMEM((parts_general_kernel<A, DP, VEC, W>), 160 * 1024) \
+    return rg_launch(parts_general_kernel<A, DP, VEC, W>, dim3((unsigned)blocks), dim3(PG_THREADS), smem, s, cluster, a, b); }
+#define RG_PG(A, DP, VEC) { if (whole) RG_PG_(A, DP, VEC, true) RG_PG_(A, DP, VEC, false) }
 #define RG_PG_WIDTH(A, VEC) { if (a.d <= 32) RG_PG(A, 32, VEC) if (a.d <= 64) RG_PG(A, 64, VEC) RG_PG(A, 128, VEC) }
     if (dtype == RG_DTYPE_F32) { if (vec) RG_PG_WIDTH(float, true) RG_PG_WIDTH(float, false) }
     if (vec) RG_PG_WIDTH(bf16, true)
     RG_PG_WIDTH(bf16, false)
 #undef RG_PG_WIDTH
 #undef RG_PG
+#undef RG_PG_
 }
 
 // The cache as the mma kernel reads it: 64 columns, rows, pieces of 64 columns, K and V; a box of `rows` rows.
@@ -534,6 +835,28 @@ static int launch_parts_mma(const PartArgs& a, int num_pages, int* err, cudaStre
 #undef RG_PM
 }
 
+// Rows by clusters of `cluster` blocks, in one launch; b.weights null: no weights.
+static int launch_rows(const PartArgs& a, const RowsArgs& b, int dtype, int num_pages, int cluster, int* err, cudaStream_t s) {
+    if (cluster > 8) return RG_ERR_UNSUPPORTED;
+    if (!parts_mma_ok(a, dtype, num_pages)) return launch_parts_general(a, dtype, s, &b, cluster);
+    if (a.T > 65535 || a.nkv * a.own_tiles > 65535) return RG_ERR_UNSUPPORTED;
+    CUtensorMap map;
+    int e = make_kv_map(&map, a.kv, num_pages, a.nkv, a.page_size, a.d, a.page_size < 16 ? a.page_size : 16);
+    if (e) return e;
+    const int scores = b.weights ? (a.nh / a.nkv) * (b.runs * 16 + 8) * 4 : 0;
+    const dim3 grid(cluster, a.nkv * a.own_tiles, a.T);
+#define RG_RM(P, W) { constexpr int stages = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
+    RG_ALLOW_SMEM((rows_mma_kernel<P, W>), 227 * 1024 - 2048) \
+    return rg_launch(rows_mma_kernel<P, W>, grid, dim3(PM_THREADS), stages + scores, s, cluster, map, a, b, err); }
+#define RG_RMW(P) { if (b.weights) RG_RM(P, true) else RG_RM(P, false) }
+    if (a.d == 64) RG_RMW(1)
+    if (a.d == 128) RG_RMW(2)
+    if (a.d == 192) RG_RMW(3)
+    RG_RMW(4)
+#undef RG_RMW
+#undef RG_RM
+}
+
 static int launch_parts(const PartArgs& a, int dtype, int num_pages, int* err, cudaStream_t s) {
     return parts_mma_ok(a, dtype, num_pages) ? launch_parts_mma(a, num_pages, err, s) : launch_parts_general(a, dtype, s);
 }
@@ -555,12 +878,13 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
 // [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].  tensor_cores: 1 the prefixes by prefix_tc_kernel, 2 the same with two
-// parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.
+// parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.  cluster: not 0, rows by clusters of so many
+// blocks, which leave no parts.
 extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                    const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
                                    int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,
                                    int own_parts, int own_per, int T, int nh, int nkv, int d, int page_size, float scale,
-                                   float* part_o, float* part_ml, int tensor_cores, int* err, void* stream) {
+                                   float* part_o, float* part_ml, int tensor_cores, int cluster, int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
@@ -572,6 +896,10 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
     a.prefix_limit = (int)min(0x7fffffffll, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
     if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
+    if (cluster) {
+        const RowsArgs b = {out, nullptr, nullptr, 0, out_ld, 0, 0, 0.f};
+        return launch_rows(a, b, dtype, num_pages, cluster, err, (cudaStream_t)stream);
+    }
     if (tensor_cores) {
         if (!prefix_tc_ok(a, dtype, num_pages)) return RG_ERR_UNSUPPORTED;
         const int tile_rows = (tensor_cores == 2 ? 1 : 2) * (PT_SIDE / group);
@@ -598,7 +926,7 @@ extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int 
                                     const int* block_table, int max_blocks, const int* positions, int own_parts, int own_per,
                                     int T, int nh, int nkv, int d, int page_size, float scale, float* part_o, float* part_ml,
                                     float* scores, int score_ld, float* weights, int weights_ld, int n_slots, const int* slots,
-                                    int max_context, float decay, int* err, void* stream) {
+                                    int max_context, float decay, int cluster, int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
@@ -608,6 +936,11 @@ extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int 
     a.own_limit = min(a.own_limit, max_context);
     const int group = nh / nkv;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
+    if (cluster) {                                                   // own_per: the most entries a block may have
+        if (a.own_tiles != 1 || own_per % 16) return RG_ERR_UNSUPPORTED;
+        const RowsArgs b = {out, weights, slots, weights_ld, out_ld, n_slots, own_per / 16, decay};
+        return launch_rows(a, b, dtype, num_pages, cluster, err, (cudaStream_t)stream);
+    }
     int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
     if (e) return e;
     const int chunks = (max_context + WEIGH_CHUNK - 1) / WEIGH_CHUNK;

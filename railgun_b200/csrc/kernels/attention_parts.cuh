@@ -78,10 +78,20 @@ __host__ __device__ inline long long part_blocks(const PartArgs& a) {
 
 // How many parts row t has of either list.
 __device__ __forceinline__ int own_parts_of(const PartArgs& a, int t) { return (max(0, own_entries(a, t)) + a.own_per - 1) / a.own_per; }
-__device__ __forceinline__ int prefix_parts_of(const PartArgs& a, int t) {
+// Row t's prefix: its table, and how many entries it has (none: 0).
+__device__ __forceinline__ const int* prefix_of(const PartArgs& a, int t, int& entries) {
     for (int g = 0; g < a.n_groups; ++g) {                          // a handful of groups
         const int i = t - a.groups[g * 3];
-        if (i >= 0 && i < a.groups[g * 3 + 1]) return (max(0, prefix_entries(a, g)) + a.prefix_per - 1) / a.prefix_per;
+        if (i >= 0 && i < a.groups[g * 3 + 1]) {
+            entries = max(0, prefix_entries(a, g));
+            return a.prefix_table + (size_t)g * a.prefix_blocks;
+        }
     }
-    return 0;
+    entries = 0;
+    return nullptr;
+}
+__device__ __forceinline__ int prefix_parts_of(const PartArgs& a, int t) {
+    int entries;
+    prefix_of(a, t, entries);
+    return (entries + a.prefix_per - 1) / a.prefix_per;
 }

@@ -2228,6 +2228,24 @@ def _row_maps_ok(q, kv_cache, scale: float) -> bool:
             and kv_cache.data_ptr() % 16 == 0 and scale > 0 and kv_cache.numel() // kv_cache.shape[4] < (1 << 31) - 1)
 
 
+def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0) -> int:
+    """How many blocks, a cluster, share each of ``blocks`` (row, kv head, tile of heads) of up to ``longest`` entries and leave nothing
+    to be joined; 0: the entries go in parts that another kernel joins.  ``fast``: by rows_mma_kernel; ``heads`` > 0: whose scores
+    wait in shared memory."""
+    cluster = 1
+    while cluster < 8 and blocks * cluster * 2 <= 256 and longest > 64 * cluster:
+        cluster *= 2
+    per = -(-longest // cluster)
+    if not fast:
+        return cluster if per <= 448 else 0
+    if blocks * cluster > 296:                   # several waves: two blocks an SM have to fit
+        most = min(640, 3600 // max(heads, 1))
+    else:
+        most = 2048 if blocks * cluster >= 100 else 640
+        most = min(most, 28000 // max(heads, 1))
+    return cluster if per <= most else 0
+
+
 def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int) -> tuple:
     """(parts, entries a part) of prefixes of up to ``longest`` entries, of which ``blocks`` thread blocks, one an SM, read a
     part each (two each where ``tensor_cores`` is 2): whole tiles of 128 entries, as many parts as fill the GPU once."""
@@ -2267,24 +2285,30 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     if min(max_rows, max_prefix, max_own) < 0:
         raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
     n_groups, G = groups.shape[0], nh // nkv
-    longest, tensor_cores = max_prefix if n_groups and max_rows else 0, 0
-    if (q.dtype == torch.bfloat16 and d in (64, 128) and 16 < max_rows * G and G <= 128 and longest >= 256 and _row_maps_ok(q, kv_cache, scale)):
-        # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
-        side = 128 // G
-        tensor_cores = 1 if max_rows > side else 2
-        p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, num_sms(q.device), tensor_cores)
+    longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
+    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, kv_cache, scale)
+    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast)
+    if cluster:
+        p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
     else:
-        p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest)
-    o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own)
-    slots = T * nh * (p_parts + o_parts)
-    parts = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
-    _COUNTER.value += 2 if tensor_cores and o_parts else 1         # the parts, and the kernel that joins them
+        if fast and d <= 128 and 16 < max_rows * G and G <= 128 and longest >= 256:
+            # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
+            side = 128 // G
+            tensor_cores = 1 if max_rows > side else 2
+            p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, num_sms(q.device), tensor_cores)
+        else:
+            p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest)
+        o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own)
+        slots = T * nh * (p_parts + o_parts)
+        scratch = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
+        part_ml = scratch.data_ptr() + 4 * slots * d
+        _COUNTER.value += 2 if tensor_cores and o_parts else 1         # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_prefix_attention")(
         _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(prefix_table),
         c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(parts), c_void_p(parts.data_ptr() + 4 * slots * d),
-        c_int(tensor_cores), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
+        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml),
+        c_int(tensor_cores), c_int(cluster), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
 
 
 def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, nh: int, nkv: int, d: int, scale: float,
@@ -2304,17 +2328,26 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     if max_context < 0:
         raise KernelError("weighed_attention: max_context is a count")
     _check_entry_weights(weights, "weights", nkv, max_context)
-    n_parts, per = attention_parts(R * nkv * -(-(nh // nkv) // 16), max_context)
-    rows, score_ld = R * nh, -(-max_context // 64) * 64
-    scratch = torch.empty(rows * (n_parts * (d + 2) + score_ld), dtype=torch.float32, device=q.device)
-    part_ml = scratch.data_ptr() + 4 * rows * n_parts * d
-    _COUNTER.value += 1                          # the parts, and the kernel that joins them
+    G, score_ld, scratch, part_ml, scores = nh // nkv, -(-max_context // 64) * 64, None, 0, 0
+    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, kv_cache, scale)
+    cluster = rows_cluster(R * nkv, max_context, fast, G) if G <= 16 else 0
+    if cluster:
+        n_parts, per = cluster, -(-(max_context or 1) // (16 * cluster)) * 16
+        floats = 0 if fast else R * nh * score_ld
+    else:
+        n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context)
+        floats = R * nh * (n_parts * (d + 2) + score_ld)
+        _COUNTER.value += 1                      # the parts, and the kernel that joins them
+    if floats:
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+        part_ml = scratch.data_ptr() + (0 if cluster else 4 * R * nh * n_parts * d)
+        scores = part_ml + (0 if cluster else 8 * R * nh * n_parts)
     _ok(_fn("attention_parts", "rg_weighed_attention")(
         _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)),
         _ptr(block_table), c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_void_p(part_ml + 8 * rows * n_parts), c_int(score_ld),
-        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), _ptr(_tc_error_flag(q.device)), _stream()),
-        "weighed_attention")
+        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_void_p(scores), c_int(score_ld),
+        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), c_int(cluster),
+        _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
 
 def key_weight_parts(items: int, tiles: int, room: int = 592) -> int:
