@@ -190,16 +190,18 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const We
 // tensor cores.  Both passes have one structure and differ in what stays and what streams:
 //   row sums:    128 lanes = queries (rows x heads of a kv head), keys stream by;   m, l of a row run in its thread
 //   entry sums:  128 lanes = entries, queries stream by;   w[e] is a sum over columns, again inside a thread: no exchange
-// A block has two such tiles of 128 (a "side" each: its own accumulator and four warps), which share the streamed tiles,
-// so a streamed tile is fetched once for 256 lanes.  Per streamed tile of 128 and side: S = A B^T in 128 columns of tensor
-// memory, two buffers a side, then one pass of exponentials over it while the tensor core works on the next.  Blocks are
-// persistent: items (kv head, 256 lanes, part of what streams) are dealt out in turn, the heaviest first, and loads and products
-// run on across items.
+// A block has two such tiles of 128 (a "side" each: its own accumulator, issuing warp and four warps of exponentials), which
+// share the streamed tiles, so a streamed tile is fetched once for 256 lanes; where only one tile is left, the sides take
+// every other streamed tile of it.  Per streamed tile of 128 and side: S = A B^T in 128 columns of tensor memory, two
+// buffers a side, then one pass of exponentials over it while the tensor core works on the next.  Blocks are persistent:
+// items (kv head, 256 lanes, part of what streams) are dealt out in turn, the heaviest first.  The loading warp works out
+// what an item is and leaves it in shared memory with the item's first tiles; loads, products and exponentials run on
+// across items.
 //
 // What bounds it: one 2^x an element and pass.  128 x 128 of them take 1,024 cycles of a scheduler's MUFU, the products of a
 // tile 520 of the tensor core (head size 128).
 // ---------------------------------------------------------------------------------------------------
-#define KT_THREADS 320             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9: MMA issue, tensor memory
+#define KT_THREADS 352             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
 #define KT_TILE 128
 __host__ __device__ constexpr int kt_b_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 
@@ -216,8 +218,9 @@ struct KtArgs {
 
 struct KtItem {
     int r, kvh, part, row0, rows, start, entries;
-    int m0, n_m;                 // first lane tile, how many of the two there are
+    int m0, n_m;                 // first lane tile, how many of the two there are (0: the end)
     int b0, n_b;                 // streamed tiles b0, b0 + parts, ..
+    int slot, fresh;
 };
 
 template <bool ENTRIES>
@@ -227,6 +230,8 @@ __device__ __forceinline__ bool kt_item(const KtArgs& a, int i, KtItem& t) {
     t.kvh = rest / a.parts % a.w.nkv;
     t.r = rest / a.parts / a.w.nkv;
     rows_of(a.w, t.r, t.row0, t.rows, t.start, t.entries);
+    t.slot = ENTRIES ? a.w.slots[t.r] : 0;
+    t.fresh = ENTRIES ? a.w.fresh[t.r] : 0;
     if (t.entries <= 0) return false;
     const int q_tiles = (t.rows + a.tile_rows - 1) / a.tile_rows;
     if (ENTRIES) {
@@ -243,7 +248,7 @@ __device__ __forceinline__ bool kt_item(const KtArgs& a, int i, KtItem& t) {
     }
     t.n_b = t.n_b > t.part ? (t.n_b - t.part + a.parts - 1) / a.parts : 0;
     t.b0 += t.part;
-    return t.n_m > 0;
+    return t.n_m > 0 && (!ENTRIES || a.part_w || (t.slot >= 0 && t.slot < a.w.n_slots));
 }
 
 // q_map: 64 columns x heads x rows, a box of 64 x group x tile_rows; kv_map: the cache as rows of the head size, a box of
@@ -255,20 +260,25 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     constexpr int NB = kt_b_stages(PIECES);
     constexpr uint32_t PIECE = KT_TILE * 128, TILE = PIECE * PIECES;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, sA = base, sB = sA + 4 * TILE;   // two stages of two tiles; NB tiles
-    __shared__ __align__(8) uint64_t bars[4 + 2 * NB + 8];
+    __shared__ __align__(8) uint64_t bars[4 + 2 * NB + 8 + 2];
     // -z of a streamed tile's columns and their positions: a copy for every warp, so that warps wait for nothing but tiles
     __shared__ __align__(16) float col_z[ENTRIES ? 8 : 1][2][KT_TILE];
     __shared__ __align__(16) int col_p[ENTRIES ? 8 : 1][2][KT_TILE];
+    __shared__ float other_ml[ENTRIES ? 1 : KT_TILE][2];             // side 1's results for side 0, where they share a tile
+    __shared__ KtItem items[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
+    // a_full: an item and its lane tiles; s_full, s_empty: side 0's two buffers, side 1's; x_full, x_empty: other_ml
     const uint32_t a_full = smem_addr(bars), a_empty = a_full + 16, b_full = a_empty + 16, b_empty = b_full + 8 * NB,
-                   s_full = b_empty + 8 * NB, s_empty = s_full + 32;   // s_full, s_empty: side 0's two buffers, side 1's
+                   s_full = b_empty + 8 * NB, s_empty = s_full + 32, x_full = s_empty + 32, x_empty = x_full + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.w.nh / a.w.nkv;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int i = 0; i < 2; ++i) { mbar_init(a_full + 8 * i, 1); mbar_init(a_empty + 8 * i, 1); }
-        for (int i = 0; i < NB; ++i) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(a_full + 8 * i, 1); mbar_init(a_empty + 8 * i, 2 + 8); }   // both issuers, eight warps
+        for (int i = 0; i < NB; ++i) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 2); }
         for (int i = 0; i < 4; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_empty + 8 * i, KT_TILE); }
+        mbar_init(x_full, KT_TILE);
+        mbar_init(x_empty, KT_TILE);
         fence_barrier_init();
     }
     if (warp == 9) tmem_alloc(&tmem_slot, 512u);
@@ -280,13 +290,18 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     pdl_trigger();
     bool ok = true;
     KtItem t = {};
+    // Does side g work on streamed tile b of this item?  With one lane tile the sides take turns.
+    auto mine_is = [&](int g, int b) -> bool { return t.n_m == 2 || (ENTRIES ? g == 0 : (b & 1) == g); };
     if (warp == 8) {
         // ---- loads
         const int box_rows = min(a.w.page_size, KT_TILE), boxes = KT_TILE / box_rows, box = lane % boxes, piece = lane / boxes;
         const bool mine = piece < PIECES;                            // a box of a piece of the head each
-        auto load_keys = [&](uint32_t dst, uint32_t bar, int tile) {
+        auto page_of = [&](int tile) -> int {                        // behind the entries: any page
             const int e = tile * KT_TILE + box * box_rows;
-            const int page = a.w.block_table[(size_t)t.r * a.w.max_blocks + (e < t.entries ? e >> a.page_shift : 0)];   // behind: any page
+            return a.w.block_table[(size_t)t.r * a.w.max_blocks + (e < t.entries ? e >> a.page_shift : 0)];
+        };
+        auto load_keys = [&](uint32_t dst, uint32_t bar, int tile, int page) {
+            const int e = tile * KT_TILE + box * box_rows;
             if (mine)
                 tma_load_2d(dst + piece * PIECE + box * box_rows * 128, &kv_map, bar, 64 * piece,
                             (page * 2 * a.w.nkv + t.kvh) * a.w.page_size + (e & (a.w.page_size - 1)));
@@ -297,101 +312,137 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const uint32_t q_bytes = (uint32_t)(PIECES * 128 * group * a.tile_rows);
         const uint32_t a_bytes = ENTRIES ? TILE : q_bytes, b_bytes = ENTRIES ? q_bytes : TILE;
         int ai = 0, bi = 0;
-        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
-            if (!kt_item<ENTRIES>(a, i, t) || t.n_b == 0) continue;
+        for (int i = blockIdx.x; ok; i += gridDim.x) {
+            const bool end = i >= a.n_items;
+            if (end) t.n_m = t.n_b = 0;
+            else if (!kt_item<ENTRIES>(a, i, t)) continue;
             const int sa = ai & 1;
+            int page[2] = {0, 0};
+            if (ENTRIES && t.n_b) { page[0] = page_of(t.m0); page[1] = page_of(t.m0 + t.n_m - 1); }
+            if (!ENTRIES && t.n_b) page[0] = page_of(t.b0);
             if (ai > 1) ok = mbar_wait_all(a_empty + 8 * sa, ((ai >> 1) & 1) ^ 1, a.err, 71, &abort_flag);
             if (!ok) break;
-            if (lane == 0) mbar_expect_tx(a_full + 8 * sa, (uint32_t)t.n_m * a_bytes);
+            if (lane == 0) {
+                items[sa] = t;
+                if (t.n_b) mbar_expect_tx(a_full + 8 * sa, (uint32_t)t.n_m * a_bytes);
+                else mbar_arrive(a_full + 8 * sa);
+            }
             __syncwarp();
-            for (int g = 0; g < t.n_m; ++g) {
-                if (ENTRIES) load_keys(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g);
+            ++ai;
+            if (end) break;
+            for (int g = 0; g < t.n_m && t.n_b; ++g) {
+                if (ENTRIES) load_keys(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g, page[g]);
                 else load_queries(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g);
             }
-            ++ai;
+            int page_next = page[0];
             for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
-                const int sb = bi % NB;
+                const int sb = bi % NB, tile = t.b0 + b * a.parts, page_now = page_next;
+                if (!ENTRIES && b + 1 < t.n_b) page_next = page_of(tile + a.parts);
                 if (bi >= NB) ok = mbar_wait_all(b_empty + 8 * sb, ((bi / NB) & 1) ^ 1, a.err, 72, &abort_flag);
                 if (!ok) break;
                 if (lane == 0) mbar_expect_tx(b_full + 8 * sb, b_bytes);
                 __syncwarp();
-                if (ENTRIES) load_queries(sB + sb * TILE, b_full + 8 * sb, t.b0 + b * a.parts);
-                else load_keys(sB + sb * TILE, b_full + 8 * sb, t.b0 + b * a.parts);
+                if (ENTRIES) load_queries(sB + sb * TILE, b_full + 8 * sb, tile);
+                else load_keys(sB + sb * TILE, b_full + 8 * sb, tile, page_now);
             }
         }
-    } else if (warp == 9) {
-        // ---- products: the whole warp walks and waits, one elected lane issues
+    } else if (warp == 9 || warp == 10) {
+        // ---- products of a side: the whole warp walks and waits, one elected lane issues
         constexpr uint32_t idesc = make_idesc(KT_TILE, KT_TILE, false);
+        const int g = warp - 9;
         const bool issuer = elect_one();
-        int ai = 0, bi = 0;
-        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
-            if (!kt_item<ENTRIES>(a, i, t) || t.n_b == 0) continue;
+        int si = 0, bi = 0;                                          // tiles of this side; streamed tiles
+        for (int ai = 0; ok; ++ai) {
             const int sa = ai & 1;
             ok = mbar_wait_all(a_full + 8 * sa, (ai >> 1) & 1, a.err, 73, &abort_flag);
+            if (!ok) break;
+            t.n_m = items[sa].n_m;
+            t.n_b = items[sa].n_b;
+            if (t.n_m == 0) break;
+            const uint32_t at = sA + (2 * sa + (t.n_m == 2 ? g : 0)) * TILE;
             for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
-                const int sb = bi % NB, buf = bi & 1;
+                const int sb = bi % NB;
                 ok = mbar_wait_all(b_full + 8 * sb, (bi / NB) & 1, a.err, 74, &abort_flag);
-                for (int g = 0; g < 2 && ok; ++g) {
-                    if (bi > 1) ok = mbar_wait_all(s_empty + 16 * g + 8 * buf, ((bi >> 1) & 1) ^ 1, a.err, 75, &abort_flag);
+                if (ok && mine_is(g, b)) {
+                    const int buf = si & 1;
+                    if (si > 1) ok = mbar_wait_all(s_empty + 16 * g + 8 * buf, ((si >> 1) & 1) ^ 1, a.err, 75, &abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     if (issuer) {
-                        if (g < t.n_m) {
 #pragma unroll
-                            for (int x = 0; x < PIECES; ++x) {
-                                const uint64_t ad = desc_k_major(sA + (2 * sa + g) * TILE + x * PIECE), bd = desc_k_major(sB + sb * TILE + x * PIECE);
+                        for (int x = 0; x < PIECES; ++x) {
+                            const uint64_t ad = desc_k_major(at + x * PIECE), bd = desc_k_major(sB + sb * TILE + x * PIECE);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    tc_mma(tmem + 256u * g + 128u * buf, ad + 2u * k, bd + 2u * k, idesc, x + k > 0 ? 1u : 0u);
-                            }
+                            for (int k = 0; k < 4; ++k)
+                                tc_mma(tmem + 256u * g + 128u * buf, ad + 2u * k, bd + 2u * k, idesc, x + k > 0 ? 1u : 0u);
                         }
                         tc_commit(s_full + 16 * g + 8 * buf);
+                        tc_commit(b_empty + 8 * sb);
                     }
-                    __syncwarp();
-                }
-                if (!ok) break;
-                if (issuer) {
-                    tc_commit(b_empty + 8 * sb);
-                    if (b == t.n_b - 1) tc_commit(a_empty + 8 * sa);
-                }
+                    ++si;
+                } else if (ok && lane == 0) mbar_arrive(b_empty + 8 * sb);
                 __syncwarp();
             }
-            ++ai;
+            if (!ok) break;
+            if (issuer) tc_commit(a_empty + 8 * sa);                 // once every product of the item is done
+            __syncwarp();
         }
-    } else {
+    } else if (warp < 8) {
         // ---- exponentials: thread = lane of the accumulator
         const int g = warp >> 2, row = threadIdx.x & 127;
         const uint32_t tmem_row = tmem + 256u * g + ((uint32_t)((warp & 3) * 32) << 16);
         const uint64_t scale2 = pack2(a.w.scale_log2, a.w.scale_log2);
-        int bi = 0;
-        for (int i = blockIdx.x; i < a.n_items && ok; i += gridDim.x) {
-            if (!kt_item<ENTRIES>(a, i, t)) continue;
-            const bool there = g < t.n_m;
-            if (ENTRIES) {
-                const int e = (t.m0 + g) * KT_TILE + row;
-                // columns lane + 32 j of a streamed tile: their queries' z and positions (-1: no query)
-                float z_next[4];
-                int p_next[4];
-                auto columns = [&](int b) {
+        int si = 0, ai = 0, xi = 0;
+        auto next_item = [&](KtItem& to) -> bool {
+            if (!mbar_wait_all(a_full + 8 * (ai & 1), (ai >> 1) & 1, a.err, 78, &abort_flag)) return false;
+            to = items[ai & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(a_empty + 8 * (ai & 1));
+            ++ai;
+            return true;
+        };
+        if (ENTRIES) {
+            // columns lane + 32 j of a streamed tile: their queries' z and positions (-1: no query)
+            float z_next[4];
+            int p_next[4];
+            KtItem n = {};
+            float before_next = 0.f;
+            auto columns = [&](const KtItem& x, int b) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int c = lane + 32 * j, r = (t.b0 + b * a.parts) * a.tile_rows + c / group;
-                        p_next[j] = there && c < a.tile_rows * group && r < t.rows && b < t.n_b ? t.start + r : -1;
-                        z_next[j] = p_next[j] >= 0 ? a.w.z[(size_t)(t.row0 + r) * a.w.nh + t.kvh * group + c % group] : 0.f;
-                    }
-                };
-                columns(0);
+                for (int j = 0; j < 4; ++j) {
+                    const int c = lane + 32 * j, r = (x.b0 + b * a.parts) * a.tile_rows + c / group;
+                    p_next[j] = g < x.n_m && c < a.tile_rows * group && r < x.rows && b < x.n_b ? x.start + r : -1;
+                    z_next[j] = p_next[j] >= 0 ? a.w.z[(size_t)(x.row0 + r) * a.w.nh + x.kvh * group + c % group] : 0.f;
+                }
+            };
+            auto place = [&](const KtItem& x) -> float* { return a.w.weights + ((size_t)x.slot * a.w.nkv + x.kvh) * a.w.weights_ld; };
+            // the next item, and what of it takes a trip to memory: asked for while this one's last tile is worked on
+            auto look_ahead = [&]() -> bool {
+                if (!next_item(n)) return false;
+                columns(n, 0);
+                const int e = (n.m0 + g) * KT_TILE + row;
+                before_next = !a.part_w && g < n.n_m && e < min(n.entries, n.fresh) ? place(n)[e] : 0.f;
+                return true;
+            };
+            ok = look_ahead();
+            while (ok && n.n_m > 0) {
+                t = n;
+                const float before = before_next;
+                const bool there = g < t.n_m;
+                const int e = (t.m0 + g) * KT_TILE + row;
                 uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-                for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
-                    const int buf = bi & 1;
+                if (t.n_b == 0 || !there) ok = look_ahead();
+                for (int b = 0; b < t.n_b && there && ok; ++b, ++si) {
+                    const int buf = si & 1;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         col_z[warp][buf][lane + 32 * j] = -z_next[j];
                         col_p[warp][buf][lane + 32 * j] = p_next[j];
                     }
                     __syncwarp();                                    // they are there (and every lane is done with those before)
-                    columns(b + 1);
-                    ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (bi >> 1) & 1, a.err, 76, &abort_flag);
+                    if (b + 1 < t.n_b) columns(t, b + 1);
+                    else ok = look_ahead();
+                    if (ok) ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (si >> 1) & 1, a.err, 76, &abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     const float4* z4 = reinterpret_cast<const float4*>(col_z[warp][buf]);
@@ -399,32 +450,42 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                     const int r0 = (t.b0 + b * a.parts) * a.tile_rows, cols = min(a.tile_rows, t.rows - r0) * group;
                     // every column a query that sees every entry of this tile?
                     const bool edge = cols < KT_TILE || t.start + r0 < (t.m0 + g + 1) * KT_TILE - 1;
-                    auto chunk = [&](auto edge_c, int c) {
+                    uint32_t v[2][32];
+                    auto chunk = [&](auto edge_c, int c, const uint32_t (&x)[32]) {
                         constexpr bool EDGE = decltype(edge_c)::value;
-                        uint32_t v[32];
-                        tc_ld32(tmem_row + 128u * buf + 32u * c, v);
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
                             const float4 z = z4[(32 * c + j) >> 2];
-                            float x[4];
-                            unpack2(fma2(pack2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), scale2, pack2(z.x, z.y)), x[0], x[1]);
-                            unpack2(fma2(pack2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3])), scale2, pack2(z.z, z.w)), x[2], x[3]);
+                            float y[4];
+                            unpack2(fma2(pack2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), scale2, pack2(z.x, z.y)), y[0], y[1]);
+                            unpack2(fma2(pack2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), scale2, pack2(z.z, z.w)), y[2], y[3]);
                             if (EDGE) {
                                 const int4 p = p4[(32 * c + j) >> 2];
-                                if (p.x < e) x[0] = -INFINITY;
-                                if (p.y < e) x[1] = -INFINITY;
-                                if (p.z < e) x[2] = -INFINITY;
-                                if (p.w < e) x[3] = -INFINITY;
+                                if (p.x < e) y[0] = -INFINITY;
+                                if (p.y < e) y[1] = -INFINITY;
+                                if (p.z < e) y[2] = -INFINITY;
+                                if (p.w < e) y[3] = -INFINITY;
                             }
-                            sum2[j / 4 % 2 * 2] = add2(sum2[j / 4 % 2 * 2], pack2(ex2(x[0]), ex2(x[1])));
-                            sum2[j / 4 % 2 * 2 + 1] = add2(sum2[j / 4 % 2 * 2 + 1], pack2(ex2(x[2]), ex2(x[3])));
+                            sum2[j / 4 % 2 * 2] = add2(sum2[j / 4 % 2 * 2], pack2(ex2(y[0]), ex2(y[1])));
+                            sum2[j / 4 % 2 * 2 + 1] = add2(sum2[j / 4 % 2 * 2 + 1], pack2(ex2(y[2]), ex2(y[3])));
                         }
                     };
-                    if (there) {
-                        if (edge) { for (int c = 0; c < (cols + 31) / 32; ++c) chunk(std::true_type{}, c); }
-                        else {
+                    // the next 32 columns are on their way while these are worked on
+                    const uint32_t from = tmem_row + 128u * buf;
+                    tc_ld32_nowait(from, v[0]);
+                    tc_ld_wait_for(v[0]);
+                    if (edge) {
+                        const int chunks = (cols + 31) / 32;
+                        for (int c = 0; c < chunks; ++c) {
+                            chunk(std::true_type{}, c, v[0]);
+                            if (c + 1 < chunks) { tc_ld32_nowait(from + 32u * (c + 1), v[0]); tc_ld_wait_for(v[0]); }
+                        }
+                    } else {
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) chunk(std::false_type{}, c);
+                        for (int c = 0; c < 4; ++c) {
+                            if (c < 3) tc_ld32_nowait(from + 32u * (c + 1), v[(c + 1) & 1]);
+                            chunk(std::false_type{}, c, v[c & 1]);
+                            if (c < 3) tc_ld_wait_for(v[(c + 1) & 1]);
                         }
                     }
                     tc_fence_before();
@@ -433,70 +494,99 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 if (there && e < t.entries && ok) {
                     float x, y;
                     unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), x, y);
-                    if (a.part_w) {
-                        a.part_w[(((size_t)t.part * a.w.R + t.r) * a.w.nkv + t.kvh) * a.w.limit + e] = x + y;
-                    } else {
-                        const int slot = a.w.slots[t.r];
-                        if (slot >= 0 && slot < a.w.n_slots) {
-                            float* w = a.w.weights + ((size_t)slot * a.w.nkv + t.kvh) * a.w.weights_ld + e;
-                            *w = (e < a.w.fresh[t.r] ? *w : 0.f) + (x + y);
-                        }
-                    }
+                    if (a.part_w) a.part_w[(((size_t)t.part * a.w.R + t.r) * a.w.nkv + t.kvh) * a.w.limit + e] = x + y;
+                    else place(t)[e] = before + (x + y);
                 }
-            } else {
-                const int r = (t.m0 + g) * a.tile_rows + row / group;
-                const bool query = there && row < a.tile_rows * group && r < t.rows;
+            }
+        } else {
+            while (ok) {
+                ok = next_item(t);
+                if (!ok || t.n_m == 0) break;
+                const bool both = t.n_m == 1;                        // both sides work on one tile
+                const int tile = t.m0 + (both ? 0 : g), r = tile * a.tile_rows + row / group;
+                const bool query = row < a.tile_rows * group && r < t.rows;
                 const int sees = min(t.entries, t.start + r + 1);                       // entries that this lane's row sees
-                const int first = min(t.entries, t.start + (t.m0 + g) * a.tile_rows + 1);  // .. and the tile's first row
+                const int first = min(t.entries, t.start + tile * a.tile_rows + 1);     // .. and the tile's first row
                 float ref = -INFINITY, l = 0.f;
-                for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
-                    const int buf = bi & 1, k0 = (t.b0 + b * a.parts) * KT_TILE;
-                    ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (bi >> 1) & 1, a.err, 77, &abort_flag);
+                for (int b = 0; b < t.n_b && ok; ++b) {
+                    if (!mine_is(g, b)) continue;
+                    const int buf = si & 1, k0 = (t.b0 + b * a.parts) * KT_TILE;
+                    ok = mbar_wait_all(s_full + 16 * g + 8 * buf, (si >> 1) & 1, a.err, 77, &abort_flag);
                     if (!ok) break;
+                    ++si;
                     tc_fence_after();
                     // 64 scores at a time under a reference that the first ones seen set: below 2^100 a sum is as good under
                     // any reference, above it the reference is raised.
                     if (__any_sync(0xffffffffu, query && k0 < sees)) {
                         const bool edge = k0 + KT_TILE > first;
+                        uint32_t v[2][2][32];
+                        const uint32_t from = tmem_row + 128u * buf;
+                        tc_ld32_nowait(from, v[0][0]);
+                        tc_ld32_nowait(from + 32u, v[0][1]);
+                        tc_ld_wait_for(v[0][0]);
+                        tc_ld_wait_for(v[0][1]);
+#pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            uint32_t v[2][32];
-                            tc_ld32_nowait(tmem_row + 128u * buf + 64u * c, v[0]);
-                            tc_ld32_nowait(tmem_row + 128u * buf + 64u * c + 32u, v[1]);
-                            tc_ld_wait();
+                            if (c == 0) { tc_ld32_nowait(from + 64u, v[1][0]); tc_ld32_nowait(from + 96u, v[1][1]); }
+                            uint32_t (&x)[2][32] = v[c];
                             if (edge) {
 #pragma unroll
                                 for (int j = 0; j < 64; ++j)
-                                    if (k0 + 64 * c + j >= sees) v[j >> 5][j & 31] = 0xff800000u;
+                                    if (k0 + 64 * c + j >= sees) x[j >> 5][j & 31] = 0xff800000u;
                             }
                             auto pass = [&](float m) -> float {
                                 uint64_t s2[4] = {0ull, 0ull, 0ull, 0ull};
                                 const uint64_t nm2 = pack2(-m, -m);
 #pragma unroll
                                 for (int j = 0; j < 64; j += 2) {
-                                    float x, y;
-                                    unpack2(fma2(pack2(__uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1])), scale2, nm2), x, y);
-                                    s2[j / 2 % 4] = add2(s2[j / 2 % 4], pack2(ex2(x), ex2(y)));
+                                    float y0, y1;
+                                    unpack2(fma2(pack2(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1])), scale2, nm2), y0, y1);
+                                    s2[j / 2 % 4] = add2(s2[j / 2 % 4], pack2(ex2(y0), ex2(y1)));
                                 }
-                                float x, y;
-                                unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), x, y);
-                                return x + y;
+                                float y0, y1;
+                                unpack2(add2(add2(s2[0], s2[1]), add2(s2[2], s2[3])), y0, y1);
+                                return y0 + y1;
                             };
-                            float sum = pass(ref == -INFINITY ? 0.f : ref);
-                            if (__any_sync(0xffffffffu, query && (ref == -INFINITY || !(sum < 0x1p100f)))) {
+                            float sum = 0.f;
+                            bool raise = __any_sync(0xffffffffu, query && ref == -INFINITY);
+                            if (!raise) {
+                                sum = pass(ref == -INFINITY ? 0.f : ref);
+                                raise = __any_sync(0xffffffffu, query && !(sum < 0x1p100f));
+                            }
+                            if (raise) {
                                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                                for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j >> 5][j & 31]));
+                                for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j >> 5][j & 31]));
                                 const float m = fmaxf(ref, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.w.scale_log2);
                                 if (m > ref) { l *= ex2(ref - m); ref = m; }            // ref -inf: l is 0
                                 sum = pass(ref == -INFINITY ? 0.f : ref);
                             }
                             l += sum;
+                            if (c == 0) { tc_ld_wait_for(v[1][0]); tc_ld_wait_for(v[1][1]); }
                         }
                     }
                     tc_fence_before();
                     mbar_arrive(s_empty + 16 * g + 8 * buf);
                 }
-                if (query && ok) {
+                if (!ok) break;
+                if (both) {                                          // side 1's result goes to side 0
+                    if (g == 1) {
+                        if (xi > 0) ok = mbar_wait_all(x_empty, (xi & 1) ^ 1, a.err, 79, &abort_flag);
+                        if (!ok) break;
+                        other_ml[row][0] = ref;
+                        other_ml[row][1] = l;
+                        mbar_arrive(x_full);
+                    } else {
+                        ok = mbar_wait_all(x_full, xi & 1, a.err, 80, &abort_flag);
+                        if (!ok) break;
+                        const float m = other_ml[row][0], n = fmaxf(ref, m), base_m = n == -INFINITY ? 0.f : n;
+                        l = l * ex2(ref - base_m) + other_ml[row][1] * ex2(m - base_m);
+                        ref = n;
+                        mbar_arrive(x_empty);
+                    }
+                    ++xi;
+                }
+                if (query && !(both && g == 1)) {
                     const size_t at = (size_t)(t.row0 + r) * a.w.nh + t.kvh * group + row % group;
                     if (a.parts == 1) a.w.z[at] = l > 0.f ? ref + log2f(l) : INFINITY;
                     else *reinterpret_cast<float2*>(a.part_ml + (at * a.parts + t.part) * 2) = make_float2(ref, l);
