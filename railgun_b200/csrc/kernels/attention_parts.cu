@@ -434,10 +434,13 @@ struct MmaQueries {
         }
         __syncwarp();                                                 // every lane has read the stage
     }
-    // What the warp has, to shared memory: co [16][D], ml [16][2].
-    __device__ __forceinline__ void leave(float* co, float (*ml)[2]) {
+    __device__ __forceinline__ void sums() {                         // of the weights, over the four lanes of a row
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    }
+    // What the warp has, to shared memory: co [16][D], ml [16][2].
+    __device__ __forceinline__ void leave(float* co, float (*ml)[2]) {
+        sums();
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
             *reinterpret_cast<float2*>(co + g * D + j * 8 + 2 * tq) = make_float2(o[j][0], o[j][1]);
@@ -715,21 +718,51 @@ __device__ __forceinline__ void join_ml(const PartArgs& a, int t, int h, int n_p
     M = ms;
 }
 
+// The output of row t and head h.  The block's four warps take every fourth part, four columns a lane; their sums are added in
+// their order.
+#define JOIN_PARTS 512            // factors kept at a time
 template <typename A>
 __device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __restrict__ out, int out_ld) {
-    const int slots = a.prefix_parts + a.own_parts, d = a.d;
-    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n_own = own_parts_of(a, t), n = n_prefix + n_own;
+    __shared__ float factor[JOIN_PARTS];
+    __shared__ float4 sums[JOIN_THREADS / 32][64];
+    const int slots = a.prefix_parts + a.own_parts, d = a.d, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_of(a, t);
     float M, L;
-    join_ml(a, t, h, n_prefix, n_own, M, L);
+    join_ml(a, t, h, n_prefix, n - n_prefix, M, L);
     const float inv = L > 0.f ? 1.f / L : 0.f;
     const size_t base = ((size_t)t * a.nh + h) * slots;
-    for (int c = threadIdx.x; c < d; c += JOIN_THREADS) {
-        float acc = 0.f;
-        for (int i = 0; i < n; ++i) {
-            const size_t slot = base + (i < n_prefix ? i : a.prefix_parts + i - n_prefix);
-            acc += exp2f(a.part_ml[slot * 2] - M) * a.part_o[slot * d + c];
+    auto slot_of = [&](int i) -> size_t { return base + (i < n_prefix ? i : a.prefix_parts + i - n_prefix); };
+    const bool quads = d % 4 == 0;
+    float4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int i0 = 0; i0 < n; i0 += JOIN_PARTS) {
+        const int m = min(JOIN_PARTS, n - i0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < m; i += JOIN_THREADS) factor[i] = exp2f(a.part_ml[slot_of(i0 + i) * 2] - M) * inv;
+        __syncthreads();
+#pragma unroll 4
+        for (int i = warp; i < m; i += JOIN_THREADS / 32) {
+            const float f = factor[i];
+            const float* from = a.part_o + slot_of(i0 + i) * d;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = 4 * lane + 128 * k;
+                if (c >= d) continue;
+                float4 x = {0.f, 0.f, 0.f, 0.f};
+                if (quads) x = *reinterpret_cast<const float4*>(from + c);
+                else { x.x = from[c]; if (c + 1 < d) x.y = from[c + 1]; if (c + 2 < d) x.z = from[c + 2]; if (c + 3 < d) x.w = from[c + 3]; }
+                acc[k].x += f * x.x; acc[k].y += f * x.y; acc[k].z += f * x.z; acc[k].w += f * x.w;
+            }
         }
-        out[(size_t)t * out_ld + h * d + c] = from_f32<A>(acc * inv);
+    }
+    sums[warp][lane] = acc[0];
+    sums[warp][lane + 32] = acc[1];
+    __syncthreads();
+    A* to = out + (size_t)t * out_ld + h * d;
+    for (int c = threadIdx.x; c < d; c += JOIN_THREADS) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; ++w) v += reinterpret_cast<const float*>(&sums[w][0])[c];
+        to[c] = from_f32<A>(v);
     }
 }
 
@@ -740,9 +773,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const PartArgs a, A*
     join_row(a, blockIdx.x / a.nh, blockIdx.x % a.nh, out, out_ld);
 }
 
-// Blocks 0 .. T nh - 1 join a row and head; the others add up the weights of 512 entries of a row and kv head:
+// Blocks 0 .. T nh - 1 join a row and head; the others add up the weights of 512 entries of a row and kv head, four a thread:
 //   w[e] = decay w[e] + sum_h 2^(s_h(e) - M_h) / L_h,   the newest entry's w not read
-#define WEIGH_CHUNK 512
+#define WEIGH_CHUNK (4 * JOIN_THREADS)
+#define WEIGH_HEADS 64
 template <typename A>
 __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A* __restrict__ out, int out_ld,
                                                              float* __restrict__ weights, long long weights_ld, int n_slots,
@@ -753,26 +787,35 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
     if (b < a.T * a.nh) { join_row(a, b / a.nh, b % a.nh, out, out_ld); return; }
     b -= a.T * a.nh;
     const int chunk = b % chunks, kvh = b / chunks % a.nkv, t = b / chunks / a.nkv, group = a.nh / a.nkv;
-    const int n = own_entries(a, t), e0 = chunk * WEIGH_CHUNK, slot = slots[t];
-    if (e0 >= n || slot < 0 || slot >= n_slots) return;
-    __shared__ float sM[256], sI[256];
+    const int n = own_entries(a, t), e = chunk * WEIGH_CHUNK + 4 * threadIdx.x, slot = slots[t];
+    if (chunk * WEIGH_CHUNK >= n || slot < 0 || slot >= n_slots) return;
+    __shared__ float sM[WEIGH_HEADS], sI[WEIGH_HEADS];
     const int n_own = own_parts_of(a, t), warp = threadIdx.x >> 5;
-    for (int g0 = 0; g0 < group; g0 += 256) {                        // heads of a kv head, up to 256 at a time
+    float* w = weights + ((size_t)slot * a.nkv + kvh) * weights_ld;
+    float before[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) before[j] = e + j < n - 1 ? decay * w[e + j] : 0.f;
+    for (int g0 = 0; g0 < group; g0 += WEIGH_HEADS) {                // heads of a kv head, so many at a time
+        const int heads = min(group - g0, WEIGH_HEADS);
         __syncthreads();
-        for (int g = g0 + warp; g < min(group, g0 + 256); g += JOIN_THREADS / 32) {
+        for (int g = warp; g < heads; g += JOIN_THREADS / 32) {
             float M, L;
-            join_ml(a, t, kvh * group + g, 0, n_own, M, L);
-            if ((threadIdx.x & 31) == 0) { sM[g - g0] = M; sI[g - g0] = 1.f / L; }
+            join_ml(a, t, kvh * group + g0 + g, 0, n_own, M, L);
+            if ((threadIdx.x & 31) == 0) { sM[g] = M; sI[g] = L > 0.f ? 1.f / L : 0.f; }
         }
         __syncthreads();
-        float* w = weights + ((size_t)slot * a.nkv + kvh) * weights_ld;
-        for (int e = e0 + threadIdx.x; e < min(n, e0 + WEIGH_CHUNK); e += JOIN_THREADS) {
-            const float* sc = a.scores + ((size_t)t * a.nh + kvh * group) * a.score_ld + e;
-            float sum = 0.f;
-            for (int g = g0; g < min(group, g0 + 256); ++g) sum += exp2f(sc[(size_t)g * a.score_ld] - sM[g - g0]) * sI[g - g0];
-            w[e] = (g0 > 0 ? w[e] : (e == n - 1 ? 0.f : decay * w[e])) + sum;
+        if (e >= n) continue;
+        const float* sc = a.scores + ((size_t)t * a.nh + kvh * group + g0) * a.score_ld + e;   // rows of whole 64 entries
+#pragma unroll 4
+        for (int g = 0; g < heads; ++g) {
+            const float4 s = *reinterpret_cast<const float4*>(sc + (size_t)g * a.score_ld);
+            sum[0] += exp2f(s.x - sM[g]) * sI[g]; sum[1] += exp2f(s.y - sM[g]) * sI[g];
+            sum[2] += exp2f(s.z - sM[g]) * sI[g]; sum[3] += exp2f(s.w - sM[g]) * sI[g];
         }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (e + j < n) w[e + j] = before[j] + sum[j];
 }
 
 // ---------------------------------------------------------------------------------------------------

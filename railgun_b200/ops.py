@@ -2171,14 +2171,15 @@ def decode_attention(q, q_stride: int, out, kv_cache, block_table, rows, n_token
         _stream()), "decode_attention")
 
 
-def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> int:
-    """What the operators over rows of single tokens and portions ask of queries and cache; returns the page size."""
+def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> tuple:
+    """What the operators over rows of single tokens and portions ask of queries and cache; returns q's rows, how far they are
+    apart, the pages and the page size."""
     code, (T, n), s = _dtype_code(q), q.shape if q.dim() == 2 else (0, 0), kv_cache.shape
     if (_fast is not None and _fast.fits(kv_cache, q.dtype) and len(s) == 5 and s[1] == 2 and s[2] == nkv > 0 and s[3] > 0 and s[4] == d
             and 0 < d <= 256 and nh > 0 and nh % nkv == 0 and q.is_cuda and n >= nh * d):
         at, step = q.stride()
         if step == 1 and at >= n:
-            return s[3]
+            return T, at, s[0], s[3]
     _check_rows(q, "q")
     _check(kv_cache, "kv_cache", q.dtype)
     if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
@@ -2186,7 +2187,7 @@ def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> int:
     _check_pages(kv_cache, nkv, d)
     if n < nh * d:
         raise KernelError(f"{what}: q has {n} columns, {nh} heads of {d} need {nh * d}")
-    return s[3]
+    return T, q.stride(0), s[0], s[3]
 
 
 def _check_pages(kv_cache, nkv: int, d: int) -> None:
@@ -2221,11 +2222,10 @@ def _tc_error_flag(device) -> torch.Tensor:
     return err
 
 
-def _row_maps_ok(q, kv_cache, scale: float) -> bool:
-    """Can TMA read these rows of queries, and pages of this size, in tiles?"""
-    page_size = kv_cache.shape[3]
-    return (page_size >= 8 and page_size & (page_size - 1) == 0 and q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0
-            and kv_cache.data_ptr() % 16 == 0 and scale > 0 and kv_cache.numel() // kv_cache.shape[4] < (1 << 31) - 1)
+def _row_maps_ok(q, step: int, kv_cache, pages: int, nkv: int, page_size: int, scale: float) -> bool:
+    """Can TMA read these rows of queries, ``step`` apart, and pages of this size in tiles?"""
+    return (page_size >= 8 and page_size & (page_size - 1) == 0 and step % 8 == 0 and (q.data_ptr() | kv_cache.data_ptr()) % 16 == 0
+            and scale > 0 and pages * 2 * nkv * page_size < (1 << 31) - 1)
 
 
 def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0) -> int:
@@ -2255,12 +2255,11 @@ def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int) -> tupl
 
 
 def attention_parts(blocks: int, longest: int, room: int = 444, least: int = 128) -> tuple:
-    """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would
-    read a list in one part each: as many parts as fill the GPU once (``room`` blocks, three an SM), of whole tiles of 64
-    entries and at least ``least``."""
+    """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would read a list in
+    one part each: until there are ``room`` blocks (444: three an SM), of whole tiles of 64 entries and at least ``least``."""
     if longest <= 0:
         return 0, 64
-    parts = max(1, min(-(-longest // least), room // max(1, blocks)))
+    parts = max(1, min(-(-longest // least), -(-room // max(1, blocks))))
     per = -(--(-longest // parts) // 64) * 64
     return -(-longest // per), per
 
@@ -2275,8 +2274,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     entry at all the output is 0.  ``max_rows``, ``max_prefix``, ``max_own``: the most rows and prefix entries that a group, and
     own entries that a row, may have (``groups`` and ``positions`` stay on the device); what lies beyond is not seen.  All
     sums are 32-bit and have one order."""
-    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prefix_attention")
-    T = q.shape[0]
+    T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prefix_attention")
     _check_ints(groups, "groups", None, 3, table=True)
     _check_ints(prefix_table, "prefix_table", groups.shape[0], table=True)
     _check_ints(block_table, "block_table", T, table=True)
@@ -2286,7 +2284,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
         raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
     n_groups, G = groups.shape[0], nh // nkv
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
-    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, kv_cache, scale)
+    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
     cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast)
     if cluster:
         p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
@@ -2304,7 +2302,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
         part_ml = scratch.data_ptr() + 4 * slots * d
         _COUNTER.value += 2 if tensor_cores and o_parts else 1         # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_prefix_attention")(
-        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(prefix_table),
+        _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(prefix_table),
         c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
         c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml),
@@ -2319,8 +2317,7 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     decay * weight + the sum, over the query heads of each kv head, of the softmax weight that e got from them.  The entry
     ``positions[r]`` is new: its earlier weight is not read.  ``max_context``: the most entries a row may see; entries beyond
     are not seen.  All sums are 32-bit and have one order."""
-    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
-    R = q.shape[0]
+    R, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
     _check_ints(block_table, "block_table", R, table=True)
     _check_ints(positions, "positions", R)
     _check_ints(slots, "slots", R)
@@ -2328,24 +2325,26 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     if max_context < 0:
         raise KernelError("weighed_attention: max_context is a count")
     _check_entry_weights(weights, "weights", nkv, max_context)
-    G, score_ld, scratch, part_ml, scores = nh // nkv, -(-max_context // 64) * 64, None, 0, 0
-    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, kv_cache, scale)
+    G, score_ld, scores, part_o, part_ml = nh // nkv, -(-max_context // 64) * 64, 0, 0, 0
+    fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
     cluster = rows_cluster(R * nkv, max_context, fast, G) if G <= 16 else 0
     if cluster:
         n_parts, per = cluster, -(-(max_context or 1) // (16 * cluster)) * 16
         floats = 0 if fast else R * nh * score_ld
     else:
-        n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context)
+        # lists may be far shorter than the longest: several waves of parts even that out
+        n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context, *((1500, 512) if fast else ()))
         floats = R * nh * (n_parts * (d + 2) + score_ld)
         _COUNTER.value += 1                      # the parts, and the kernel that joins them
     if floats:
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-        part_ml = scratch.data_ptr() + (0 if cluster else 4 * R * nh * n_parts * d)
-        scores = part_ml + (0 if cluster else 8 * R * nh * n_parts)
+        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)      # scores, and parts behind them
+        scores = scratch.data_ptr()
+        part_o = scores + 4 * R * nh * score_ld
+        part_ml = part_o + 4 * R * nh * n_parts * d
     _ok(_fn("attention_parts", "rg_weighed_attention")(
-        _ptr(q), c_int(q.stride(0)), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)),
+        _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)),
         _ptr(block_table), c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_void_p(scores), c_int(score_ld),
+        c_int(page_size), c_float(scale), c_void_p(part_o), c_void_p(part_ml), c_void_p(scores), c_int(score_ld),
         _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), c_int(cluster),
         _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
@@ -2365,7 +2364,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     ``fresh[r]`` on are new, their earlier weight is not read.  Entries that no row sees, and requests without rows, keep
     theirs.  ``max_rows``, ``max_context``: the most rows of a request and the most entries a row may see.  All sums are 32-bit and
     have one order."""
-    page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prompt_key_weights")
+    T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prompt_key_weights")
     _check_ints(slots, "slots", None)
     R = slots.shape[0]
     _check_ints(block_table, "block_table", R, table=True)
@@ -2375,9 +2374,9 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     if min(max_rows, max_context) < 0:
         raise KernelError("prompt_key_weights: max_rows and max_context are counts")
     _check_entry_weights(weights, "weights", nkv, max_context)
-    T, G, row_parts, entry_parts = q.shape[0], nh // nkv, 0, 0
+    G, row_parts, entry_parts = nh // nkv, 0, 0
     floats = n_z = -(-T * nh // 4) * 4
-    if q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, kv_cache, scale):
+    if q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale):
         # tiles of 128 queries and of 128 entries: one kind stays, two at a time, and the other streams by in parts
         q_tiles, e_tiles = -(-max_rows // (128 // G)), -(-max_context // 128)
         row_parts = key_weight_parts(R * nkv * -(-q_tiles // 2), e_tiles)
@@ -2388,8 +2387,8 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     part_w = part_ml + (8 * T * nh * row_parts if row_parts > 1 else 0)
     _COUNTER.value += 1 + (row_parts > 1) + (entry_parts > 1)      # the rows' sums, then the entries', and what joins their parts
     _ok(_fn("key_weights", "rg_prompt_key_weights")(
-        _ptr(q), c_int(q.stride(0)), _ptr(kv_cache), c_int(kv_cache.shape[0]), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
-        _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(q.shape[0]),
+        _ptr(q), c_int(step), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
+        _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(T),
         c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z),
         c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), c_int(num_sms(q.device)), _ptr(_tc_error_flag(q.device)), _stream()),
         "prompt_key_weights")
