@@ -324,7 +324,10 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 // ---------------------------------------------------------------------------------------------------
 #define PM_THREADS 128
 #define PM_Q 16
-__host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 6 : (pieces == 3 ? 2 : 3); }
+// Runs of a warp's ring, and blocks an SM.  Head size 64: four and three (six and two, 12 % slower: 64 requests on 2,000 entries
+// 70 against 63 us); 128: three and two (two and three are level, and 9 % slower for one request on 32,768).
+__host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 4 : (pieces == 3 ? 2 : 3); }
+__host__ __device__ constexpr int pm_blocks(int pieces) { return pieces == 1 ? 3 : (pieces == 2 ? 2 : 1); }
 __host__ __device__ constexpr int pm_stage_bytes(int pieces) { return 16 * 64 * 2 * 2 * pieces; }
 static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1) * pm_stage_bytes(1), "the warps' results fit where the stages were");
 
@@ -469,7 +472,7 @@ __device__ __forceinline__ float4 join_warps(const float* all, const float (*ml)
 }
 
 template <int PIECES>
-__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES))
 parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, int* err) {
     constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
     extern __shared__ unsigned char smem_raw[];
@@ -570,7 +573,7 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
 // grid (cluster, nkv x tiles of heads, T)
 // ---------------------------------------------------------------------------------------------------
 template <int PIECES, bool WEIGH>
-__global__ void __launch_bounds__(PM_THREADS, PIECES <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES))
 rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, const RowsArgs b, int* err) {
     constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
     extern __shared__ unsigned char smem_raw[];

@@ -2254,12 +2254,17 @@ def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int) -> tupl
     return -(-longest // per), per
 
 
-def attention_parts(blocks: int, longest: int, room: int = 444, least: int = 128) -> tuple:
+def attention_parts(blocks: int, longest: int, d: int, fast: bool, sms: int) -> tuple:
     """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would read a list in
-    one part each: until there are ``room`` blocks (444: three an SM), of whole tiles of 64 entries and at least ``least``."""
+    one part each: so many that the blocks fill the GPU a whole number of times, the fewest times that leave no part with
+    more than 1,024 entries (lists may be far shorter than the longest: several waves even that out); whole tiles of 64 entries, 256
+    at least (by the general kernel, which is bound by its arithmetic, 512 and 128)."""
     if longest <= 0:
         return 0, 64
-    parts = max(1, min(-(-longest // least), -(-room // max(1, blocks))))
+    resident, least, most = (sms * (3 if d == 64 else (2 if d == 128 else 1)), 256, 1024) if fast else (3 * sms, 128, 512)
+    enough = -(-longest // most)
+    waves = max(1, -(-blocks * enough // resident))
+    parts = max(1, min(waves * resident // max(1, blocks), -(-longest // least)))
     per = -(--(-longest // parts) // 64) * 64
     return -(-longest // per), per
 
@@ -2286,6 +2291,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
     cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast)
+    sms = num_sms(q.device)
     if cluster:
         p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
     else:
@@ -2293,10 +2299,10 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
             # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
             side = 128 // G
             tensor_cores = 1 if max_rows > side else 2
-            p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, num_sms(q.device), tensor_cores)
+            p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, sms, tensor_cores)
         else:
-            p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest)
-        o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own)
+            p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest, d, fast, sms)
+        o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own, d, fast, sms)
         slots = T * nh * (p_parts + o_parts)
         scratch = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
         part_ml = scratch.data_ptr() + 4 * slots * d
@@ -2332,8 +2338,7 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         n_parts, per = cluster, -(-(max_context or 1) // (16 * cluster)) * 16
         floats = 0 if fast else R * nh * score_ld
     else:
-        # lists may be far shorter than the longest: several waves of parts even that out
-        n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context, *((1500, 512) if fast else ()))
+        n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context, d, fast, num_sms(q.device))
         floats = R * nh * (n_parts * (d + 2) + score_ld)
         _COUNTER.value += 1                      # the parts, and the kernel that joins them
     if floats:
