@@ -5,11 +5,14 @@
 // its own softmax threads, accumulator and issuing warp; K and V tiles of 128 entries (TMA through the prefix's table, one
 // box a page and 64 columns, 128-byte swizzle) are fetched once for both.  With up to 128 queries the sides take a part
 // each of their own instead, so that two chains of scores, exponentials and products are under way on the SM either way.
-// Per side and tile of 128 entries:
-//   S = Q K^T            tcgen05.mma, M 128 x N 128 x K head size, into 128 TMEM columns
-//   softmax              128 threads, one query each, 64 entries at a time; the reference maximum is raised only when 64
-//                        weights sum to more than 2^8
-//   O += P V             tcgen05.mma, M 128 x N head size x K 64, twice: P as bfloat16 in TMEM over the scores it was made from
+// Per side and 64 entries j:
+//   S(j) = Q K^T         tcgen05.mma, M 128 x N 64 x K head size, into one of two buffers of 64 TMEM columns
+//   softmax              128 threads, one query each; the reference maximum is raised only when the 64 weights sum to more than 2^8
+//   O += P(j) V          tcgen05.mma, M 128 x N head size x K 64: P as bfloat16 in TMEM over the scores it was made from
+// S(j + 2) is issued behind O += P(j) V, which reads the buffer that it goes to, so S(j + 1) is there when the threads are done
+// with j: the exponentials never wait for a product of their own side.  (With one buffer of 128 columns and N 128, the faster
+// shape by 260 to 392 cycles for 64 entries, a side's scores, exponentials and products are one chain: 65,536 entries for
+// 512 queries a kv head OLDLONG us.)
 // There is no mask but the end of a part: rows of V behind it get zeros in shared memory, scores behind it -infinity.
 //
 // Rounding: P to bfloat16 (2^-9 of each weight; the sum of weights is of the unrounded ones), all sums in 32-bit.
@@ -46,8 +49,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t sQ = base, sK0 = sQ + 2 * TILE, sV0 = sK0 + NK * TILE, bars = sV0 + NV * TILE;
     const uint32_t q_full = bars, k_full0 = bars + 8, k_empty0 = k_full0 + 8 * NK, v_full0 = k_empty0 + 8 * NK, v_empty0 = v_full0 + 8 * NV,
-                   s_full0 = v_empty0 + 8 * NV, p_full0 = s_full0 + 16, p_free0 = p_full0 + 32;    // per side; per side and half stage
-    static_assert(8 + 16 * (NK + NV) + 16 + 64 <= 256, "the barriers have 256 bytes");
+                   s_full0 = v_empty0 + 8 * NV, p_full0 = s_full0 + 32, p_free0 = p_full0 + 32;    // per side and half stage
+    static_assert(8 + 16 * (NK + NV) + 32 + 64 <= 256, "the barriers have 256 bytes");
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -80,8 +83,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         mbar_init(q_full, 1);
         for (int s = 0; s < NK; ++s) { mbar_init(k_full0 + 8 * s, 1); mbar_init(k_empty0 + 8 * s, users); }
         for (int s = 0; s < NV; ++s) { mbar_init(v_full0 + 8 * s, 1); mbar_init(v_empty0 + 8 * s, users); }
-        for (int s = 0; s < 2; ++s) mbar_init(s_full0 + 8 * s, 1);
-        for (int b = 0; b < 4; ++b) { mbar_init(p_full0 + 8 * b, PT_SIDE); mbar_init(p_free0 + 8 * b, 1); }
+        for (int b = 0; b < 4; ++b) { mbar_init(s_full0 + 8 * b, 1); mbar_init(p_full0 + 8 * b, PT_SIDE); mbar_init(p_free0 + 8 * b, 1); }
         fence_barrier_init();
     }
     if (warp == 9) tmem_alloc(&tmem_base_slot, 512u);
@@ -136,25 +138,26 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
     } else if (warp == 9 || warp == 10) {
         // ---- MMA issue of one side.  The whole warp walks the loop and waits; one elected lane issues.
-        const int s = warp - 9, n_kt = s ? n_kt1 : n_kt0, n_st = s ? n_st1 : n_st0;
+        const int s = warp - 9, n_kt = s ? n_kt1 : n_kt0;
         const uint32_t tmem_s = tmem + 256u * s, tmem_o = tmem_s + 128u, q_at = sQ + (two_parts ? 0 : s) * TILE;
-        constexpr uint32_t idesc_s = make_idesc(PT_SIDE, PT_STAGE, false), idesc_o = make_idesc(PT_SIDE, D, true);
+        constexpr uint32_t idesc_s = make_idesc(PT_SIDE, PT_BN, false), idesc_o = make_idesc(PT_SIDE, D, true);
         const bool issuer = elect_one();
-        auto wait_k = [&](int J) -> bool {
-            const int b = stage_of(s, J);
+        auto wait_k = [&](int j) -> bool {                            // K of pass j: of its stage's first pass
+            if (j & 1) return true;
+            const int b = stage_of(s, j >> 1);
             return mbar_wait_all(k_full0 + 8 * (b % NK), (b / NK) & 1, err, 54, &abort_flag);
         };
-        auto issue_s = [&](int J) {                                   // K(J) is there
-            const int st = stage_of(s, J) % NK;
+        auto issue_s = [&](int j) {                                   // K(j) is there
+            const int st = stage_of(s, j >> 1) % NK, half = j & 1;
             if (issuer) {
 #pragma unroll
                 for (int x = 0; x < PIECES; ++x) {
-                    const uint64_t qd = desc_k_major(q_at + x * PIECE), kd = desc_k_major(sK0 + st * TILE + x * PIECE);
+                    const uint64_t qd = desc_k_major(q_at + x * PIECE), kd = desc_k_major(sK0 + st * TILE + x * PIECE + half * SUB);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma(tmem_s, qd + 2u * k, kd + 2u * k, idesc_s, x + k > 0 ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) tc_mma(tmem_s + (uint32_t)(half * PT_BN), qd + 2u * k, kd + 2u * k, idesc_s, x + k > 0 ? 1u : 0u);
                 }
-                tc_commit(s_full0 + 8 * s);
-                tc_commit(k_empty0 + 8 * st);
+                tc_commit(s_full0 + 16 * s + 8 * half);
+                if (half == 1 || j == n_kt - 1) tc_commit(k_empty0 + 8 * st);
             }
             __syncwarp();
         };
@@ -162,6 +165,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         if (ok) ok = mbar_wait_all(q_full, 0, err, 53, &abort_flag);
         if (ok) ok = wait_k(0);
         if (ok) { tc_fence_after(); issue_s(0); }
+        if (ok && n_kt > 1) issue_s(1);                               // the same stage
         for (int j = 0; j < n_kt && ok; ++j) {
             const int J = j >> 1, half = j & 1, b = stage_of(s, J), st = b % NV;
             if (half == 0) ok = mbar_wait_all(v_full0 + 8 * st, (b / NV) & 1, err, 55, &abort_flag);
@@ -176,8 +180,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the product reads them
                 __syncwarp();
             }
-            const bool next = (half == 1 || j == n_kt - 1) && J + 1 < n_st;
-            if (ok && next) ok = wait_k(J + 1);
+            const bool next = j + 2 < n_kt;
+            if (ok && next) ok = wait_k(j + 2);
             if (ok) ok = mbar_wait_all(p_full0 + 16 * s + 8 * half, J & 1, err, 56, &abort_flag);
             if (!ok) break;
             tc_fence_after();
@@ -191,8 +195,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                 if (half == 1 || j == n_kt - 1) tc_commit(v_empty0 + 8 * st);
             }
             __syncwarp();
-            // S(J + 1) over the scores and weights of this stage: the tensor core takes it up after the product that reads them
-            if (next) issue_s(J + 1);
+            // S(j + 2) over the scores and weights of this pass: the tensor core takes it up after the product that reads them
+            if (next) issue_s(j + 2);
         }
     } else if (warp < 8 && (warp < 4 || n_kt1 > 0)) {
         // ---- softmax and output: thread = query
@@ -208,11 +212,9 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         for (int j = 0; j < n_kt && ok; ++j) {
             const int J = j >> 1, half = j & 1, n = e1 - e0 - j * PT_BN;
             const uint32_t tmem_s = tmem_sg + (uint32_t)(half * PT_BN);
-            if (half == 0) {
-                ok = mbar_wait_all(s_full0 + 8 * s, J & 1, err, 57, &abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-            }
+            ok = mbar_wait_all(s_full0 + 16 * s + 8 * half, J & 1, err, 57, &abort_flag);
+            if (!ok) break;
+            tc_fence_after();
             if (idle) { mbar_arrive(p_full + 8 * half); continue; }   // its lanes of P are scores: lanes have no say in one another
             uint32_t pk[PT_BN / 2];
             auto exp_pass = [&](auto edge_c, float ms) -> float {
