@@ -25,7 +25,7 @@
 #define PT_SIDE 128                // queries of a side
 #define PT_BN 64                   // entries of a softmax pass
 #define PT_STAGE 128               // entries of a K or V stage
-#define PT_THREADS 352             // warps 0-3, 4-7: softmax of side 0, 1; 8: TMA; 9, 10: MMA issue of side 0, 1
+#define PT_THREADS 384             // warps 0-3, 4-7: softmax of side 0, 1; 8, 10: TMA of K (and Q), of V; 9, 11: MMA issue of side 0, 1
 __host__ __device__ constexpr int pt_k_stages(int pieces) { return pieces == 1 ? 5 : 3; }
 __host__ __device__ constexpr int pt_v_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 __host__ __device__ constexpr int pt_smem(int pieces) {
@@ -73,8 +73,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     };
     const int n_kt0 = passes_of(0), n_kt1 = passes_of(1), n_st0 = (n_kt0 + 1) / 2, n_st1 = (n_kt1 + 1) / 2;
     if (n_kt0 == 0) return;                                           // nothing for side 0: nothing at all
-    // A stage of the stream belongs to both sides, or in turn to either; stage number of side s's J-th tile:
-    auto stage_of = [&](int s, int J) -> int { return two_parts ? (s ? 2 * J + 1 : J + min(J, n_st1)) : J; };
+    // A stage of the stream belongs to both sides, or in turn to either while side 1 has some
     const int n_stages = two_parts ? n_st0 + n_st1 : n_st0;
 
     if (threadIdx.x == 0) {
@@ -93,8 +92,8 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     // side s: scores and weights in columns [256 s, 256 s + 128), O in [256 s + 128, 256 s + 128 + D)
     const uint32_t tmem = tmem_base_slot;
 
-    if (warp == 8) {
-        // ---- producer.  A stage is 128 / box_rows boxes for each 64 columns; lane l has box l % boxes of piece l / boxes.
+    if (warp == 8 || warp == 10) {
+        // ---- producers of K and of V.  A stage is 128 / box_rows boxes for each 64 columns; lane l has box l % boxes of piece l / boxes.
         const int box_rows = min(a.page_size, PT_STAGE), boxes = PT_STAGE / box_rows, box = lane % boxes, piece = lane / boxes;
         const bool mine = piece < PIECES;
         const int* table = a.prefix_table + (size_t)g_id * a.prefix_blocks;
@@ -109,9 +108,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const int e = first_of(s) + J * PT_STAGE + box * box_rows;
             return b < n_stages ? table[(e < end_of(s) ? e : first_of(s)) >> a.page_shift] : 0;
         };
-        if (lane == 0) mbar_expect_tx(q_full, (uint32_t)((n_kt1 && !two_parts ? 2 : 1) * PIECES * 128 * group * tile_rows));
+        const int kv = warp == 10 ? 1 : 0, n = kv ? NV : NK;
+        if (kv == 0 && lane == 0) mbar_expect_tx(q_full, (uint32_t)((n_kt1 && !two_parts ? 2 : 1) * PIECES * 128 * group * tile_rows));
         __syncwarp();
-        if (lane < 2 * PIECES) {
+        if (kv == 0 && lane < 2 * PIECES) {
             const int s = lane / PIECES, x = lane % PIECES;
             if (s == 0 || (n_kt1 && !two_parts))
                 tma_load_3d(sQ + s * TILE + x * PIECE, &q_map, q_full, 64 * x, kvh * group, row0 + (tile0 + s) * tile_rows);
@@ -123,80 +123,88 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             tile_of(b, s, J);
             const int page = page_next, e = first_of(s) + J * PT_STAGE + box * box_rows, in_page = e & (a.page_size - 1);
             page_next = page_of(b + 1);
-#pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                const int n = kv ? NV : NK, st = b % n, u = b / n;
-                const uint32_t full = (kv ? v_full0 : k_full0) + 8 * st, empty = (kv ? v_empty0 : k_empty0) + 8 * st;
-                if (u > 0) ok = mbar_wait_all(empty, (u & 1) ^ 1, err, 51 + kv, &abort_flag);
-                if (!ok) break;
-                if (lane == 0) mbar_expect_tx(full, TILE);
-                __syncwarp();
-                if (mine)
-                    tma_load_2d((kv ? sV0 : sK0) + st * TILE + piece * PIECE + box * box_rows * 128, &kv_map, full, 64 * piece,
-                                ((page * 2 + kv) * a.nkv + kvh) * a.page_size + in_page);
-            }
+            const int st = b % n, u = b / n;
+            const uint32_t full = (kv ? v_full0 : k_full0) + 8 * st, empty = (kv ? v_empty0 : k_empty0) + 8 * st;
+            if (u > 0) ok = mbar_wait_all(empty, (u & 1) ^ 1, err, 51 + kv, &abort_flag);
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(full, TILE);
+            __syncwarp();
+            if (mine)
+                tma_load_2d((kv ? sV0 : sK0) + st * TILE + piece * PIECE + box * box_rows * 128, &kv_map, full, 64 * piece,
+                            ((page * 2 + kv) * a.nkv + kvh) * a.page_size + in_page);
         }
-    } else if (warp == 9 || warp == 10) {
-        // ---- MMA issue of one side.  The whole warp walks the loop and waits; one elected lane issues.
-        const int s = warp - 9, n_kt = s ? n_kt1 : n_kt0;
-        const uint32_t tmem_s = tmem + 256u * s, tmem_o = tmem_s + 128u, q_at = sQ + (two_parts ? 0 : s) * TILE;
+    } else if (warp == 9 || warp == 11) {
+        // ---- MMA issue of one side.  The whole warp walks the loop and waits; one elected lane issues.  The loop is lean: its
+        // instructions share a scheduler with two warps of exponentials, and what it does between two products is time that
+        // the tensor core may stand still.
+        const int s = warp == 11, n_kt = s ? n_kt1 : n_kt0, n_st = (n_kt + 1) >> 1;
+        const uint32_t tmem_s = tmem + 256u * s, tmem_o = tmem_s + 128u;
         constexpr uint32_t idesc_s = make_idesc(PT_SIDE, PT_BN, false), idesc_o = make_idesc(PT_SIDE, D, true);
         const bool issuer = elect_one();
-        auto wait_k = [&](int j) -> bool {                            // K of pass j: of its stage's first pass
-            if (j & 1) return true;
-            const int b = stage_of(s, j >> 1);
-            return mbar_wait_all(k_full0 + 8 * (b % NK), (b / NK) & 1, err, 54, &abort_flag);
+        const uint64_t qd = desc_k_major(sQ + (two_parts ? 0 : s) * TILE);
+        // where this side's K and V tiles are in their rings: stage and phase, `step` stages of the stream from one to the next
+        int ki = two_parts ? s : 0, vi = ki, k_phase = 0, v_phase = 0;
+        auto step = [&](int J) -> int { return two_parts && (s || J < n_st1) ? 2 : 1; };   // from tile J to tile J + 1
+        auto ahead = [&](int& i, int& phase, int by, int n) {
+            i += by;
+            if (i >= n) { i -= n; phase ^= 1; }
         };
-        auto issue_s = [&](int j) {                                   // K(j) is there
-            const int st = stage_of(s, j >> 1) % NK, half = j & 1;
+        auto issue_s = [&](int half, bool last) {                     // the next pass's scores: K is there
             if (issuer) {
+                const uint64_t kd = desc_k_major(sK0 + ki * TILE + half * SUB);
 #pragma unroll
-                for (int x = 0; x < PIECES; ++x) {
-                    const uint64_t qd = desc_k_major(q_at + x * PIECE), kd = desc_k_major(sK0 + st * TILE + x * PIECE + half * SUB);
+                for (int x = 0; x < PIECES; ++x)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc_mma(tmem_s + (uint32_t)(half * PT_BN), qd + 2u * k, kd + 2u * k, idesc_s, x + k > 0 ? 1u : 0u);
-                }
+                    for (int k = 0; k < 4; ++k)
+                        tc_mma(tmem_s + (uint32_t)(half * PT_BN), qd + (PIECE >> 4) * x + 2u * k, kd + (PIECE >> 4) * x + 2u * k, idesc_s, x + k > 0 ? 1u : 0u);
                 tc_commit(s_full0 + 16 * s + 8 * half);
-                if (half == 1 || j == n_kt - 1) tc_commit(k_empty0 + 8 * st);
+                if (last) tc_commit(k_empty0 + 8 * ki);
             }
             __syncwarp();
         };
         bool ok = n_kt > 0;
         if (ok) ok = mbar_wait_all(q_full, 0, err, 53, &abort_flag);
-        if (ok) ok = wait_k(0);
-        if (ok) { tc_fence_after(); issue_s(0); }
-        if (ok && n_kt > 1) issue_s(1);                               // the same stage
-        for (int j = 0; j < n_kt && ok; ++j) {
-            const int J = j >> 1, half = j & 1, b = stage_of(s, J), st = b % NV;
-            if (half == 0) ok = mbar_wait_all(v_full0 + 8 * st, (b / NV) & 1, err, 55, &abort_flag);
-            const int over0 = end_of(s) - first_of(s) - j * PT_BN;    // entries of this pass, if below 64
-            if (ok && over0 < PT_BN) {
-                // rows of V behind the part may be anything: their weights are 0, and 0 times an infinity is no number
-                for (int i = lane; i < (PT_BN - over0) * 8 * PIECES; i += 32) {
-                    const int key = over0 + i / (8 * PIECES), c = i % (8 * PIECES);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
-                                 ::"r"(sV0 + st * TILE + half * SUB + (c >> 3) * PIECE + key * 128 + (c & 7) * 16), "r"(0) : "memory");
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the product reads them
-                __syncwarp();
-            }
-            const bool next = j + 2 < n_kt;
-            if (ok && next) ok = wait_k(j + 2);
-            if (ok) ok = mbar_wait_all(p_full0 + 16 * s + 8 * half, J & 1, err, 56, &abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            if (issuer) {
+        if (ok) ok = mbar_wait_all(k_full0 + 8 * ki, 0, err, 54, &abort_flag);
+        if (ok) { tc_fence_after(); issue_s(0, n_kt == 1); }
+        if (ok && n_kt > 1) issue_s(1, true);                         // the same stage
+        const int tail = end_of(s) - first_of(s) - (n_kt - 1) * PT_BN;    // entries of the last pass
+        for (int J = 0; J < n_st && ok; ++J) {
+            ok = mbar_wait_all(v_full0 + 8 * vi, v_phase, err, 55, &abort_flag);
+            if (J + 1 < n_st) ahead(ki, k_phase, step(J), NK);
 #pragma unroll
-                for (int k = 0; k < PT_BN / 16; ++k) {                // 16 entries: 16 rows of V, 8 cells of P
-                    const uint64_t vd = desc_mn_major(sV0 + st * TILE + half * SUB + (uint32_t)k * 2048u, PIECE);
-                    tc_mma_a_tmem(tmem_o, tmem_s + (uint32_t)(half * PT_BN + k * 8), vd, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+            for (int half = 0; half < 2; ++half) {
+                const int j = 2 * J + half;
+                if (!ok || j >= n_kt) break;
+                if (j == n_kt - 1 && tail < PT_BN) {
+                    // rows of V behind the part may be anything: their weights are 0, and 0 times an infinity is no number (both
+                    // sides may write the same zeros)
+                    for (int i = lane; i < (PT_BN - tail) * 8 * PIECES; i += 32) {
+                        const int key = tail + i / (8 * PIECES), c = i % (8 * PIECES);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};"
+                                     ::"r"(sV0 + vi * TILE + half * SUB + (c >> 3) * PIECE + key * 128 + (c & 7) * 16), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the product reads them
+                    __syncwarp();
                 }
-                tc_commit(p_free0 + 16 * s + 8 * half);
-                if (half == 1 || j == n_kt - 1) tc_commit(v_empty0 + 8 * st);
+                const bool next = j + 2 < n_kt;
+                if (half == 0 && next) ok = mbar_wait_all(k_full0 + 8 * ki, k_phase, err, 54, &abort_flag);
+                if (ok) ok = mbar_wait_all(p_full0 + 16 * s + 8 * half, J & 1, err, 56, &abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                if (issuer) {
+                    const uint64_t vd = desc_mn_major(sV0 + vi * TILE + half * SUB, PIECE);
+#pragma unroll
+                    for (int k = 0; k < PT_BN / 16; ++k)              // 16 entries: 16 rows of V, 8 cells of P
+                        tc_mma_a_tmem(tmem_o, tmem_s + (uint32_t)(half * PT_BN + k * 8), vd + 128u * k, idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                    tc_commit(p_free0 + 16 * s + 8 * half);
+                    if (half == 1 || j == n_kt - 1) tc_commit(v_empty0 + 8 * vi);
+                }
+                __syncwarp();
+                // the scores of pass j + 2 over the scores and weights of this one: the tensor core takes them up after the product
+                // that reads them
+                if (next) issue_s(half, half == 1 || j + 2 == n_kt - 1);
             }
-            __syncwarp();
-            // S(j + 2) over the scores and weights of this pass: the tensor core takes it up after the product that reads them
-            if (next) issue_s(j + 2);
+            ahead(vi, v_phase, step(J), NV);
         }
     } else if (warp < 8 && (warp < 4 || n_kt1 > 0)) {
         // ---- softmax and output: thread = query
