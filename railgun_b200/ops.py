@@ -2246,10 +2246,17 @@ def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0) -> int:
     return cluster if per <= most else 0
 
 
-def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int) -> tuple:
+def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int, own: int, d: int) -> tuple:
     """(parts, entries a part) of prefixes of up to ``longest`` entries, of which ``blocks`` thread blocks, one an SM, read a
-    part each (two each where ``tensor_cores`` is 2): whole tiles of 128 entries, as many parts as fill the GPU once."""
-    parts = max(1, sms // max(1, blocks)) * tensor_cores
+    part each (two each where ``tensor_cores`` is 2): whole tiles of 128 entries, as many parts as fill their share of the GPU once.
+    The rows' ``own`` entries (all kv heads', at most) are read beside them by the SMs that are left: a tile takes a block some 1.9 us at
+    head size 128 and 1.4 at 64, an own entry an SM 4 d bytes of 43 a ns, and half of the most are there on average.  64 rows
+    on 8,192 with up to 512 of their own: 44 us on all SMs, 40 / 37 / 46 on 0.6 / 0.45 / 0.3 of them; with 16 of their own on
+    32,768: 57 on all, 68 on 0.6."""
+    tiles = blocks * (longest / 128) * (0.9 + d / 128) * 1000 / tensor_cores
+    share = max(0.45, tiles / (tiles + own * 4 * d / 43 / 2) + 0.05)
+    share = 1.0 if share > 0.85 else share
+    parts = max(1, int(sms * share) // max(1, blocks)) * tensor_cores
     per = -(--(-longest // parts) // 128) * 128
     return -(-longest // per), per
 
@@ -2299,7 +2306,8 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
             # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
             side = 128 // G
             tensor_cores = 1 if max_rows > side else 2
-            p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, sms, tensor_cores)
+            p_parts, p_per = prefix_parts(n_groups * nkv * -(-max_rows // (2 * side)), longest, sms, tensor_cores,
+                                          T * nkv * max_own, d)
         else:
             p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest, d, fast, sms)
         o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own, d, fast, sms)
