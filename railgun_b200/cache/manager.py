@@ -88,7 +88,7 @@ def _lib():
         lib.rg_cache_set_chunk.argtypes = [c_void_p, c_int, c_int]
         for name in ("add_request", "release", "has", "num_computed", "slot"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong]
-        for name in ("reserve", "commit"):
+        for name in ("reserve", "commit", "shrink"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong, c_int]
         lib.rg_cache_can_reserve.argtypes = [c_void_p, c_longlong, c_int, c_int]
         lib.rg_cache_table.argtypes = [c_void_p, c_longlong, c_int, c_void_p, c_int]
@@ -231,6 +231,13 @@ class PageAllocator:
         code = self._lib.rg_cache_commit(self._h, req_id, int(new_len))
         if code:
             self._raise(code, f"commit({req_id}, {new_len})")
+
+    def shrink(self, req_id: int, new_len: int) -> None:
+        """The request keeps its entries 0 .. new_len - 1 only (``ops.evict_entries``): the pages behind them go back, and
+        its position becomes ``new_len``.  Groups with windows or chunks, which go by position, refuse."""
+        code = self._lib.rg_cache_shrink(self._h, req_id, int(new_len))
+        if code:
+            self._raise(code, f"shrink({req_id}, {new_len})")
 
     def release(self, req_id: int) -> None:
         code = self._lib.rg_cache_release(self._h, req_id)

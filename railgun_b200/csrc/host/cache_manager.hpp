@@ -204,6 +204,27 @@ public:
         return CACHE_OK;
     }
 
+    // The request keeps entries [0, new_len) only (the others were evicted, those that stayed moved to the front): the pages
+    // behind go back.  Not for groups that give pages back by position.
+    int shrink(int64_t id, int new_len) {
+        auto it = reqs_.find(id);
+        if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;
+        CacheRequest& r = it->second;
+        for (size_t g = 0; g < groups_.size(); ++g)
+            if (new_len < 0 || groups_[g].window > 0 || groups_[g].chunk > 0 || new_len > (int)r.tables[g].size() * groups_[g].page_size)
+                return CACHE_BAD_ARGUMENT;
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            const size_t keep = (size_t)(new_len + groups_[g].page_size - 1) / groups_[g].page_size;
+            while (r.tables[g].size() > keep) {
+                const int st = free_page(groups_[g], r.tables[g].back());
+                if (st != CACHE_OK) return st;
+                r.tables[g].pop_back();
+            }
+        }
+        records_[r.slot].num_computed = new_len;
+        return CACHE_OK;
+    }
+
     // The request ends (finished, aborted or preempted): all pages and the slot come back.
     int release(int64_t id) {
         auto it = reqs_.find(id);

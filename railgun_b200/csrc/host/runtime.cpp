@@ -30,6 +30,7 @@ int rg_cache_can_reserve(void* h, long long id, int new_len, int spare) {
     RG_GUARD(return ((CacheManager*)h)->can_reserve(id, new_len, spare) ? 1 : 0)
 }
 int rg_cache_commit(void* h, long long id, int new_len) { RG_GUARD(return ((CacheManager*)h)->commit(id, new_len)) }
+int rg_cache_shrink(void* h, long long id, int new_len) { RG_GUARD(return ((CacheManager*)h)->shrink(id, new_len)) }
 int rg_cache_release(void* h, long long id) { RG_GUARD(return ((CacheManager*)h)->release(id)) }
 int rg_cache_has(void* h, long long id) { return ((CacheManager*)h)->has(id) ? 1 : 0; }
 int rg_cache_num_computed(void* h, long long id) {

@@ -21,7 +21,7 @@ struct EvictArgs {
     void* kv;                    // [pages, 2, nkv, page_size, d], `row_bytes` a row
     const float* weights;        // [n_slots, nkv, ld]
     const int* places;           // [n_slots, nkv, ld]
-    float* weights_out;
+    float* weights_out;          // may be the weights themselves, and so the places
     int* places_out;
     const int* slots;            // [R]
     const int* block_table;      // [R, max_blocks]
@@ -108,8 +108,8 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int row, const int
             const int e = dst[i0 + lane], f = src[i0 + lane];
             to = (long long)at(e);
             from = (long long)at(f);
-            a.weights_out[base + e] = __ldg(a.weights + base + f);
-            a.places_out[base + e] = __ldg(a.places + base + f);
+            a.weights_out[base + e] = __ldcg(a.weights + base + f);
+            a.places_out[base + e] = __ldcg(a.places + base + f);
         }
         const int row_pieces = wide ? a.row_bytes / 16 : a.row_bytes;
         for (int c = lane & (lanes - 1); c < 2 * row_pieces; c += lanes) {
@@ -179,18 +179,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int e = min(w0 + (j0 + j) * 32 + lane, n - 1);   // no branch: the loads leave together
-                wv[j] = __ldg(w + e);
-                pv[j] = __ldg(places + e);
+                wv[j] = __ldcg(w + e);
+                pv[j] = __ldcg(places + e);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) held[j0 + j] = weight_key(a, wv[j], pv[j], newest);
         }
     }
-    // What lies before the new length, as if it stayed: moves come over it.
-    for (int e = rank * THREADS + tid; e < k; e += C * THREADS) {
-        a.weights_out[base + e] = __ldg(w + e);
-        a.places_out[base + e] = __ldg(places + e);
-    }
+    // What lies before the new length, as if it stayed (moves come over it); in place it is there already, and what moves
+    // comes from where nothing is written.
+    if (a.weights_out != a.weights || a.places_out != a.places)
+        for (int e = rank * THREADS + tid; e < k; e += C * THREADS) {
+            a.weights_out[base + e] = __ldcg(w + e);
+            a.places_out[base + e] = __ldcg(places + e);
+        }
     // f(entry, its key, is there such an entry): for every run of the warp, all lanes together
     auto each = [&](auto f) {
         if constexpr (PER > 0) {
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
         } else {
             for (int j = 0; j < run; ++j) {
                 const int e = w0 + j * 32 + lane;
-                f(e, e < n ? weight_key(a, __ldg(w + e), __ldg(places + e), newest) : 0u, e < n);
+                f(e, e < n ? weight_key(a, __ldcg(w + e), __ldcg(places + e), newest) : 0u, e < n);
             }
         }
     };

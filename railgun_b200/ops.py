@@ -2414,8 +2414,8 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     ``protect_first`` or above ``positions[r]`` - ``protect_last`` (``positions``: the newest token's place), or whose weight is no number, count as
     infinitely heavy.  K and V rows behind the new length move, in place, into entries before it that got free, the i-th into
     the i-th, so what stays is entries 0 .. new length - 1 and no more rows move than have to; the pages behind may be
-    given back.  Weights and places of the entries that stay go to ``weights_out`` and ``places_out`` (other buffers of these shapes;
-    what lies behind the new length there is left alone).  Returns the new lengths [R] int32, min(lens, keep).  Requests with a
+    given back (``PageAllocator.shrink``).  Weights and places of the entries that stay go to ``weights_out`` and ``places_out``: the same
+    buffers, or others of these shapes that share no memory with them; what lies behind the new length there is left alone.  Returns the new lengths [R] int32, min(lens, keep).  Requests with a
     negative slot are left alone."""
     _dtype_code(kv_cache)
     _check(kv_cache, "kv_cache")
@@ -2432,8 +2432,6 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
         _check_entry_weights(t, name, nkv, max_context, dtype)
         if t.shape != weights.shape:
             raise KernelError(f"{name} is {tuple(t.shape)}, weights {tuple(weights.shape)}")
-    if weights_out.data_ptr() == weights.data_ptr() or places_out.data_ptr() == places.data_ptr():
-        raise KernelError("evict_entries: weights and places go to other buffers than their own")
     new_lens = torch.empty(R, dtype=torch.int32, device=kv_cache.device)
     if max_context == 0:
         return new_lens.copy_(torch.minimum(lens, keep))

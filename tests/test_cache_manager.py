@@ -151,3 +151,32 @@ def test_groups_get_the_page_geometry_they_ask_for():
     assert [len(cm.alloc.block_table(1, g)) for g in range(3)] == [2, 3, 2]
     assert [cm.alloc.free_pages(g) for g in range(3)] == [14, 9, 14]
     cm.alloc.check()
+
+
+def test_shrink_gives_the_pages_behind_back():
+    a = PageAllocator([4, 8], [10, 6], [0, 0], 2)
+    a.add_request(1)
+    a.reserve(1, 30)
+    a.commit(1, 30)
+    assert a.free_pages(0) == 2 and a.free_pages(1) == 2
+    before = a.block_table(1, 0).tolist()
+    a.shrink(1, 9)
+    assert a.block_table(1, 0).tolist() == before[:3] and a.num_computed(1) == 9
+    assert a.free_pages(0) == 7 and a.free_pages(1) == 4
+    a.check()
+    a.shrink(1, 12)                                    # within what it has: no page more, no page less
+    assert a.free_pages(0) == 7 and a.num_computed(1) == 12
+    for bad in (-1, 13, 100):
+        with pytest.raises(CacheError):
+            a.shrink(1, bad)
+    with pytest.raises(CacheError):
+        a.shrink(2, 1)
+    a.reserve(1, 20)                                   # and it grows again
+    a.shrink(1, 0)
+    assert a.free_pages(0) == 10 and a.free_pages(1) == 6
+    a.check()
+    b = PageAllocator([4], [10], [6], 1)
+    b.add_request(1)
+    b.reserve(1, 8)
+    with pytest.raises(CacheError):
+        b.shrink(1, 4)                                 # a window goes by position

@@ -310,12 +310,17 @@ def test_evict_entries(nkv, d, page, lens, keep, kind, dtype):
     newest = [2 * most - r for r in range(R)]
     first, last = (3, 40) if kind != "ties" else (0, 0)
     want = plain_evict(cache, weights, places, slots, lens, keep, newest, first, last)
-    w_out, p_out = weights.clone(), places.clone()
+    w_out, p_out, before = weights.clone(), places.clone(), cache.kv.clone()
     new = ops.evict_entries(cache.kv, weights, places, w_out, p_out, i32(slots), cache.table, i32(lens), i32(keep), i32(newest), nkv, d,
                             first, last, max_context=most)
     assert new.tolist() == want[3]
     assert same(w_out, want[1]) and torch.equal(p_out, want[2])
     assert same(cache.kv, want[0])
+    # in place: the same but for what lies behind the new lengths, which stays as it was
+    cache.kv.copy_(before)
+    ops.evict_entries(cache.kv, weights, places, weights, places, i32(slots), cache.table, i32(lens), i32(keep), i32(newest), nkv, d,
+                      first, last, max_context=most)
+    assert same(weights, want[1]) and torch.equal(places, want[2]) and same(cache.kv, want[0])
 
 
 @pytest.mark.parametrize("n,keep", [(70000, 30000), (420000, 1234)])
@@ -411,7 +416,7 @@ BAD = [("q", lambda a: a["q"].cpu(), "pwk"), ("q", lambda a: a["q"].half(), "pwk
        ("table", lambda a: a["table"][:1], "pwke"), ("pos", lambda a: a["pos"][:1], "pwke"), ("pos", lambda a: a["pos"].float(), "pwke"),
        ("groups", lambda a: a["groups"][:, :2].contiguous(), "p"), ("ptable", lambda a: a["table"], "p"), ("slots", lambda a: a["slots"][:1], "wke"),
        ("w", lambda a: a["w"].double(), "wke"), ("w", lambda a: a["w"][:, :, :30].contiguous(), "wke"), ("w", lambda a: a["w"][:, :1].contiguous(), "wke"),
-       ("w2", lambda a: a["w"], "e"), ("p2", lambda a: a["p"], "e"), ("p", lambda a: a["p"].float(), "e"), ("keep", lambda a: a["keep"][:1], "e"),
+       ("w2", lambda a: a["w2"][:, :, :30].contiguous(), "e"), ("p2", lambda a: a["p2"].float(), "e"), ("p", lambda a: a["p"].float(), "e"), ("keep", lambda a: a["keep"][:1], "e"),
        ("lens", lambda a: a["lens"].long(), "e"), ("cu", lambda a: a["cu"][:2], "k"), ("nh", lambda a: 3, "pwk"), ("nkv", lambda a: 0, "pwk"),
        ("n", lambda a: -1, "pwke")]
 
