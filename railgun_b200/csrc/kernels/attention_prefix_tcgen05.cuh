@@ -12,7 +12,7 @@
 // S(j + 2) is issued behind O += P(j) V, which reads the buffer that it goes to, so S(j + 1) is there when the threads are done
 // with j: the exponentials never wait for a product of their own side.  (With one buffer of 128 columns and N 128, the faster
 // shape by 260 to 392 cycles for 64 entries, a side's scores, exponentials and products are one chain: 65,536 entries for
-// 512 queries a kv head OLDLONG us.)
+// 512 queries a kv head 189 us, 171 with two.)
 // There is no mask but the end of a part: rows of V behind it get zeros in shared memory, scores behind it -infinity.
 //
 // Rounding: P to bfloat16 (2^-9 of each weight; the sum of weights is of the unrounded ones), all sums in 32-bit.

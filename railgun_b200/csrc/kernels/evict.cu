@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
     if constexpr (FUSED) __threadfence();
 }
 
-// The moves of a row that evict_kernel has listed.  (Bulk copies through shared memory, a row each, take 28 us where this takes
-// EVMOVES: the unit that makes them is bound by their number.)  grid (blocks that share a row's moves, R * nkv)
+// The moves of a row that evict_kernel has listed.  (Bulk copies through shared memory, a row each, are slower, 48 us for the
+// whole of eight prompts against 39: the unit that makes them is bound by their number.)  grid (blocks that share a row's moves, R * nkv)
 #define EV_MOVERS 2               // blocks an SM
 __global__ void __launch_bounds__(256, EV_MOVERS) evict_moves_kernel(const EvictArgs a) {
     pdl_wait();                                                      // no early start for the kernel behind, as above
@@ -363,7 +363,7 @@ extern "C" int rg_evict_entries(void* kv, int elem_bytes, const float* weights, 
                          max_blocks, R, nkv, page_size, d * elem_bytes, protect_first, protect_last, limit};
     // Up to 2,048 entries 256 threads hold the keys and make the moves.  Above, a thousand threads hold up to 16,384, a cluster up to
     // eight times as many, and the moves are a second kernel's, so that all SMs take part however few heads there are (64 heads of
-    // 8,192 to 16,384 entries, 2,048 of which stay: EVFIGURES).
+    // 8,192 to 16,384 entries, 2,048 of which stay: 39 us, 44 with clusters of two that move what they have chosen).
     const unsigned rows = (unsigned)(R * nkv);
 #define RG_EV(T, P, CL, FU, SMEM) e = rg_launch(evict_kernel<T, P, CL, FU>, dim3(rows * (CL ? cluster : 1)), dim3(T), SMEM, s, CL ? cluster : 1, a)
     const cudaStream_t s = (cudaStream_t)stream;

@@ -2362,7 +2362,7 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
 
-def key_weight_parts(items: int, tiles: int, room: int = int(os.environ.get("KW_ROOM", 592)), least: int = int(os.environ.get("KW_LEAST", 4))) -> int:
+def key_weight_parts(items: int, tiles: int, room: int = 592, least: int = 4) -> int:
     """Parts that the streamed side of ``prompt_key_weights`` is cut into: until there are four items an SM, of four tiles at
     least."""
     return max(1, min(-(-room // max(1, items)), -(-tiles // least), 32))
