@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const We
 // share the streamed tiles, so a streamed tile is fetched once for 256 lanes; where only one tile is left, the sides take
 // every other streamed tile of it.  Per streamed tile of 128 and side: S = A B^T in 128 columns of tensor memory, two
 // buffers a side, then one pass of exponentials over it while the tensor core works on the next.  Blocks are persistent:
-// items (kv head, 256 lanes, part of what streams) are dealt out in turn, the heaviest first.  The loading warp works out
+// items (kv head, 256 lanes, part of what streams) are dealt out to and fro, the heaviest first.  The loading warp works out
 // what an item is and leaves it in shared memory with the item's first tiles; loads, products and exponentials run on
 // across items.
 //
@@ -312,8 +312,11 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const uint32_t q_bytes = (uint32_t)(PIECES * 128 * group * a.tile_rows);
         const uint32_t a_bytes = ENTRIES ? TILE : q_bytes, b_bytes = ENTRIES ? q_bytes : TILE;
         int ai = 0, bi = 0;
-        for (int i = blockIdx.x; ok; i += gridDim.x) {
-            const bool end = i >= a.n_items;
+        for (int round = 0; ok; ++round) {
+            // to and fro: who got the heaviest of one round gets the lightest of the next
+            const int i = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            const bool end = round * (int)gridDim.x >= a.n_items;
+            if (!end && i >= a.n_items) continue;
             if (end) t.n_m = t.n_b = 0;
             else if (!kt_item<ENTRIES>(a, i, t)) continue;
             const int sa = ai & 1;

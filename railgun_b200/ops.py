@@ -2362,10 +2362,10 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
 
-def key_weight_parts(items: int, tiles: int, room: int = 592, least: int = 4) -> int:
-    """Parts that the streamed side of ``prompt_key_weights`` is cut into: until there are four items an SM, of four tiles at
-    least."""
-    return max(1, min(-(-room // max(1, items)), -(-tiles // least), 32))
+def key_weight_parts(items: int, tiles: int) -> int:
+    """Parts that the streamed side of ``prompt_key_weights`` is cut into: until there are 256 items, not quite two an SM, which
+    the kernel deals out to and fro, of four tiles at least.  (Four an SM: 80 us for 2,048 rows of a prompt against 70, one: 80.)"""
+    return max(1, min(-(-256 // max(1, items)), -(-tiles // 4), 32))
 
 
 def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts, fresh, nh: int, nkv: int, d: int, scale: float,
