@@ -141,7 +141,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, int row, const int
 
 #define EV_FEW 128                // keys that are compared with one another
 // bits of a digit: four bins a thread
-__host__ __device__ constexpr int ev_bits(int threads) { return threads == 256 ? 10 : (threads == 512 ? 11 : 12); }
+__host__ __device__ constexpr int ev_bits(int threads) { return threads == 256 ? 10 : 12; }
 
 // PER: keys a thread holds; 0: they are made anew whenever one is asked for.  FUSED: the block makes the moves, too.
 template <int THREADS, int PER, bool CLUSTERED, bool FUSED>
@@ -164,7 +164,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
     const int slot = a.slots[r], n = min(a.lens[r], a.limit), k = min(n, max(0, a.keep[r])), newest = a.positions[r];
     const bool alone = slot < 0 || slot >= a.n_slots || n <= 0;      // the same for the whole cluster
     if (h == 0 && rank == 0 && tid == 0) a.new_lens[r] = alone ? a.lens[r] : k;
-    if (alone) return;
+    if (alone) {                                                      // the kernel that moves goes by the number of moves
+        if constexpr (!FUSED)
+            if (rank == 0 && tid == 0) a.moves[(size_t)row * ev_list(a.limit)] = 0;
+        return;
+    }
     const size_t base = ((size_t)slot * a.nkv + h) * a.ld;
     const float* w = a.weights + base;
     const int* places = a.places + base;
