@@ -44,7 +44,8 @@ struct RowsArgs {
 __host__ __device__ inline int pg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
 __host__ __device__ inline int pg_stages(int d) { return d <= 128 ? 2 : 1; }   // tiles of K and V in shared memory: the next one is on its way
 
-// Query r's M and 1 / L from what the blocks of a cluster have ([queries][2] each).
+// Query r's M and 1 / L (0 where no entry is seen; no number where a score is none) from what the blocks of a cluster have
+// ([queries][2] each).
 __device__ __forceinline__ void join_cluster_ml(cg::cluster_group& cluster, float* ml, int r, float& M, float& inv) {
     const int C = cluster.num_blocks();
     float m = -INFINITY, L = 0.f;
@@ -54,7 +55,7 @@ __device__ __forceinline__ void join_cluster_ml(cg::cluster_group& cluster, floa
         const float* from = cluster.map_shared_rank(ml, k) + r * 2;
         L += exp2f(from[0] - M) * from[1];
     }
-    inv = L > 0.f ? 1.f / L : 0.f;
+    inv = L == 0.f ? 0.f : 1.f / L;
 }
 
 // WHOLE: a cluster takes all entries of a row, its prefix's and then its own, and leaves the output, and the weights where b has a
@@ -570,7 +571,7 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
 // its own) among its blocks, which join through each other's shared memory.  A prefix is then read once for every row, out
 // of L2; what is saved is the second launch and the parts' trip through memory.  With WEIGH the scores stay in shared memory
 // until the row's sums are known, and the entries' weights are written by the block that read them.
-// grid (cluster, nkv x tiles of heads, T)
+// grid (T clusters, nkv x tiles of heads)
 // ---------------------------------------------------------------------------------------------------
 template <int PIECES, bool WEIGH>
 __global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES))
@@ -597,7 +598,7 @@ rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, co
     __syncthreads();
     pdl_wait();
     pdl_trigger();
-    const int t = blockIdx.z, group = a.nh / a.nkv, kvh = blockIdx.y / a.own_tiles, q0 = blockIdx.y % a.own_tiles * PM_Q;
+    const int t = blockIdx.x / C, group = a.nh / a.nkv, kvh = blockIdx.y / a.own_tiles, q0 = blockIdx.y % a.own_tiles * PM_Q;
     const int nq = min(PM_Q, group - q0), h0 = kvh * group + q0;
     int P = 0;
     const int* prefix_table = prefix_of(a, t, P);
@@ -732,7 +733,7 @@ __device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __r
     const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_of(a, t);
     float M, L;
     join_ml(a, t, h, n_prefix, n - n_prefix, M, L);
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     const size_t base = ((size_t)t * a.nh + h) * slots;
     auto slot_of = [&](int i) -> size_t { return base + (i < n_prefix ? i : a.prefix_parts + i - n_prefix); };
     const bool quads = d % 4 == 0;
@@ -804,7 +805,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
         for (int g = warp; g < heads; g += JOIN_THREADS / 32) {
             float M, L;
             join_ml(a, t, kvh * group + g0 + g, 0, n_own, M, L);
-            if ((threadIdx.x & 31) == 0) { sM[g] = M; sI[g] = L > 0.f ? 1.f / L : 0.f; }
+            if ((threadIdx.x & 31) == 0) { sM[g] = M; sI[g] = L == 0.f ? 0.f : 1.f / L; }
         }
         __syncthreads();
         if (e >= n) continue;
@@ -885,12 +886,12 @@ static int launch_parts_mma(const PartArgs& a, int num_pages, int* err, cudaStre
 static int launch_rows(const PartArgs& a, const RowsArgs& b, int dtype, int num_pages, int cluster, int* err, cudaStream_t s) {
     if (cluster > 8) return RG_ERR_UNSUPPORTED;
     if (!parts_mma_ok(a, dtype, num_pages)) return launch_parts_general(a, dtype, s, &b, cluster);
-    if (a.T > 65535 || a.nkv * a.own_tiles > 65535) return RG_ERR_UNSUPPORTED;
+    if (a.nkv * a.own_tiles > 65535 || (long long)cluster * a.T > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     CUtensorMap map;
     int e = make_kv_map(&map, a.kv, num_pages, a.nkv, a.page_size, a.d, a.page_size < 16 ? a.page_size : 16);
     if (e) return e;
     const int scores = b.weights ? (a.nh / a.nkv) * (b.runs * 16 + 8) * 4 : 0;
-    const dim3 grid(cluster, a.nkv * a.own_tiles, a.T);
+    const dim3 grid(cluster * a.T, a.nkv * a.own_tiles);
 #define RG_RM(P, W) { constexpr int stages = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
     RG_ALLOW_SMEM((rows_mma_kernel<P, W>), 227 * 1024 - 2048) \
     return rg_launch(rows_mma_kernel<P, W>, grid, dim3(PM_THREADS), stages + scores, s, cluster, map, a, b, err); }
@@ -937,7 +938,7 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
                         own_parts, own_per) || n_groups < 0 || prefix_parts < 0 || prefix_per < 1 || out_ld < nh * d)
         return RG_ERR_UNSUPPORTED;
     const int group = nh / nkv;
-    a.prefix_table = prefix_table; a.prefix_blocks = prefix_blocks; a.groups = groups; a.n_groups = n_groups;
+    a.prefix_table = prefix_table; a.prefix_blocks = prefix_blocks; a.groups = groups; a.n_groups = n_groups; a.max_rows = max_rows;
     a.prefix_parts = prefix_parts; a.prefix_per = prefix_per;
     a.prefix_limit = (int)min(0x7fffffffll, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
     if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;

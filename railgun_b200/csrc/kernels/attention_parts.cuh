@@ -25,6 +25,7 @@ struct PartArgs {
     int prefix_parts, prefix_per, own_parts, own_per;   // parts of either list and entries a part
     int prefix_tiles, own_tiles;                        // query tiles of a group, of a row's kv head
     int prefix_limit, own_limit;                        // the most entries that tables, parts and scratch have room for
+    int max_rows;                                       // rows of a group that a launch is sized for
     int T, nh, nkv, d, page_size, page_shift;           // page_shift: log2 of the page size, or -1
     float scale_log2;
     int beside;                  // the kernel before this one writes nothing that this one reads, and the other way round
@@ -40,6 +41,11 @@ struct PartShare {
 // How many entries of its own row t sees, and how many group g's prefix has; never more than there is room for.
 __device__ __forceinline__ int own_entries(const PartArgs& a, int t) { return min(a.positions[t] + 1, a.own_limit); }
 __device__ __forceinline__ int prefix_entries(const PartArgs& a, int g) { return min(a.groups[g * 3 + 2], a.prefix_limit); }
+// Rows of group g: no more than a launch is sized for.
+__device__ __forceinline__ int group_rows(const PartArgs& a, int g) {
+    const int row0 = a.groups[g * 3];
+    return row0 < 0 ? 0 : min(min(a.groups[g * 3 + 1], a.max_rows), a.T - row0);
+}
 
 // Block b of a launch: the prefixes' parts first, their blocks numbered part by part within (tile, kv head, group).
 // false: there is nothing to do (a shorter prefix or fewer rows than the launch was sized for).
@@ -50,7 +56,7 @@ __device__ __forceinline__ bool part_share(const PartArgs& a, int tile_queries, 
         const int part = b % a.prefix_parts, tile = b / a.prefix_parts % a.prefix_tiles;
         const int gk = b / a.prefix_parts / a.prefix_tiles, g = gk / a.nkv;
         s.row0 = a.groups[g * 3];
-        const int rows = s.row0 < 0 ? 0 : min(a.groups[g * 3 + 1], a.T - s.row0), entries = prefix_entries(a, g);
+        const int rows = group_rows(a, g), entries = prefix_entries(a, g);
         s.kvh = gk % a.nkv;
         s.q0 = tile * tile_queries;
         s.nq = min(tile_queries, rows * group - s.q0);
@@ -82,7 +88,7 @@ __device__ __forceinline__ int own_parts_of(const PartArgs& a, int t) { return (
 __device__ __forceinline__ const int* prefix_of(const PartArgs& a, int t, int& entries) {
     for (int g = 0; g < a.n_groups; ++g) {                          // a handful of groups
         const int i = t - a.groups[g * 3];
-        if (i >= 0 && i < a.groups[g * 3 + 1]) {
+        if (i >= 0 && i < group_rows(a, g)) {
             entries = max(0, prefix_entries(a, g));
             return a.prefix_table + (size_t)g * a.prefix_blocks;
         }

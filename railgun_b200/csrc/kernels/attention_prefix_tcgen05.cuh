@@ -62,7 +62,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     pdl_wait();                                                      // tables, lengths and queries may come from the kernel before
     pdl_trigger();
     const int row0 = a.groups[g_id * 3], entries = prefix_entries(a, g_id);
-    const int rows = row0 < 0 ? 0 : min(a.groups[g_id * 3 + 1], a.T - row0);
+    const int rows = group_rows(a, g_id);
     const int tile0 = blk * sides;                                    // of tile_rows rows each
     // what side s looks at: its part's entries [e0, e1), in passes of 64 and stages of 128
     auto first_of = [&](int s) -> int { return (two_parts ? 2 * part + s : part) * a.prefix_per; };

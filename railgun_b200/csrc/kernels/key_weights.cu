@@ -20,12 +20,13 @@ struct WeightArgs {
     long long weights_ld;
     int q_stride, max_blocks, n_slots, T, R, nh, nkv, d, page_size, limit;   // limit: the most entries there is room for
     float scale_log2;
+    int max_rows;                // the most rows of a request
 };
 
 // Request r's rows and entries, cut to what there is room for.
 __device__ __forceinline__ void rows_of(const WeightArgs& a, int r, int& row0, int& rows, int& start, int& entries) {
     row0 = max(0, a.cu_rows[r]);
-    rows = min(a.cu_rows[r + 1], a.T) - row0;
+    rows = min(min(a.cu_rows[r + 1], a.T) - row0, a.max_rows);
     start = a.starts[r];
     entries = rows > 0 && start >= 0 ? min(start + rows, a.limit) : 0;
 }
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(KW_THREADS) row_sums_general_kernel(const Weig
         for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         const int qi = q0 + 2 * qa + i;
         if (ka == 0 && 2 * qa + i < nq)                             // no weight at all: every 2^(s - z) is 0
-            a.z[(size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group] = L > 0.f ? ms + log2f(L) : INFINITY;
+            a.z[(size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group] = L == 0.f ? INFINITY : ms + log2f(L);
     }
 }
 
@@ -591,7 +592,7 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
                 }
                 if (query && !(both && g == 1)) {
                     const size_t at = (size_t)(t.row0 + r) * a.w.nh + t.kvh * group + row % group;
-                    if (a.parts == 1) a.w.z[at] = l > 0.f ? ref + log2f(l) : INFINITY;
+                    if (a.parts == 1) a.w.z[at] = l == 0.f ? INFINITY : ref + log2f(l);
                     else *reinterpret_cast<float2*>(a.part_ml + (at * a.parts + t.part) * 2) = make_float2(ref, l);
                 }
             }
@@ -623,7 +624,7 @@ __global__ void __launch_bounds__(256) join_row_sums_kernel(const KtArgs a) {
         l = l * ex2(m - ref) + x.y * ex2(x.x - ref);
         m = n;
     }
-    a.w.z[i] = l > 0.f ? m + log2f(l) : INFINITY;
+    a.w.z[i] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // The weights from the second pass's parts, in the parts' order.  grid (entries / 256, nkv, R)
@@ -685,7 +686,7 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
         return RG_ERR_UNSUPPORTED;
     const WeightArgs a = {q, kv, block_table, cu_rows, starts, fresh, slots, weights, z, weights_ld, q_stride, max_blocks, n_slots, T, R,
                           nh, nkv, d, page_size, (int)min((long long)max_context, (long long)max_blocks * page_size),
-                          scale * 1.4426950408889634f};
+                          scale * 1.4426950408889634f, max_rows};
     const cudaStream_t s = (cudaStream_t)stream;
     const int group = nh / nkv;
     if (row_parts > 0) {

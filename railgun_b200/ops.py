@@ -2375,8 +2375,8 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     (already in the cache) its softmax weights.  To ``weights`` [slots, nkv, at least max_context] float32, at ``slots[r]`` (negative: rows
     whose weights nobody keeps), entry e's sum over the rows and the query heads of each kv head is added; entries from
     ``fresh[r]`` on are new, their earlier weight is not read.  Entries that no row sees, and requests without rows, keep
-    theirs.  ``max_rows``, ``max_context``: the most rows of a request and the most entries a row may see.  All sums are 32-bit and
-    have one order."""
+    theirs.  ``max_rows``, ``max_context``: the most rows of a request and the most entries a row may see; rows and entries beyond
+    are left out.  All sums are 32-bit and have one order."""
     T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prompt_key_weights")
     _check_ints(slots, "slots", None)
     R = slots.shape[0]
@@ -2434,7 +2434,7 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
             raise KernelError(f"{name} is {tuple(t.shape)}, weights {tuple(weights.shape)}")
     new_lens = torch.empty(R, dtype=torch.int32, device=kv_cache.device)
     if max_context == 0:
-        return new_lens.copy_(torch.minimum(lens, keep))
+        return new_lens.copy_(lens)
     # a block holds up to 16,384 keys, a cluster of up to eight more
     cluster = 1
     while cluster < 8 and max_context > 16384 * cluster:

@@ -479,3 +479,101 @@ def test_in_a_captured_graph():
         w = torch.zeros_like(weights)
         step(outs[2], outs[3], w)
         assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]) and torch.equal(w, weights)
+
+
+# ---- at the edges of what a call says -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("most", [2500, 20000])
+def test_evict_leaves_requests_alone_in_long_contexts(most):
+    """Requests without entries or without a slot, next to one that has both, where another kernel makes the moves."""
+    from railgun_b200 import ops
+    nkv, d, page, lens, slots = 2, 64, 16, [0, 2400, 300, 2500], [3, -1, 5, 0]
+    g = torch.Generator(device=DEV).manual_seed(most)
+    cache = Cache(lens, nkv, d, page, torch.bfloat16, g, width=-(-most // page))
+    weights = torch.empty(5, nkv, most, device=DEV).exponential_(generator=g)
+    places = torch.arange(most, device=DEV, dtype=torch.int32).expand(5, nkv, most).contiguous()
+    w_out, p_out = weights.clone(), places.clone()               # there are slots 0 .. 4
+    want = plain_evict(cache, weights, places, [s if 0 <= s < 5 else -1 for s in slots], lens, [100] * 4, lens, 4, 8)
+    new = ops.evict_entries(cache.kv, weights, places, w_out, p_out, i32(slots), cache.table, i32(lens), i32([100] * 4), i32(lens), nkv, d, 4, 8,
+                            max_context=most)
+    assert new.tolist() == want[3] == [0, 2400, 300, 100]
+    assert same(w_out, want[1]) and torch.equal(p_out, want[2]) and same(cache.kv, want[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_rows(dtype):
+    """More rows than a grid has blocks in its second and third dimension."""
+    from railgun_b200 import ops
+    T, nh, nkv, d, page = 66000, 2, 1, 64, 8
+    g = torch.Generator(device=DEV).manual_seed(5)
+    kv = torch.randn(3, 2, nkv, page, d, device=DEV, generator=g).to(dtype)
+    q = queries(T, nh, d, dtype, g)
+    table = torch.randint(0, 3, (T, 1), device=DEV, generator=g, dtype=torch.int32)
+    n = torch.randint(0, page + 1, (T,), device=DEV, generator=g)
+    outs = [torch.empty(T, nh * d, dtype=dtype, device=DEV) for _ in range(2)]
+    weights, slots = torch.zeros(T, nkv, page, device=DEV), torch.arange(T, device=DEV, dtype=torch.int32)
+    pos = (n - 1).to(torch.int32)
+    ops.weighed_attention(q, outs[0], kv, weights, slots, table, pos, nh, nkv, d, 0.125, max_context=page)
+    ops.prefix_attention(q, outs[1], kv, table[:0], i32([]).view(0, 3), table, pos, nh, nkv, d, 0.125, max_rows=0, max_prefix=0, max_own=page)
+    K, V = (kv[table[:, 0].long(), i, 0].double() for i in range(2))
+    s = q.double().view(T, nh, d) @ K.transpose(1, 2) * 0.125
+    p = torch.nan_to_num(torch.softmax(s.masked_fill(torch.arange(page, device=DEV) >= n[:, None, None], float("-inf")), -1))
+    bound = out_error(q.reshape(-1, d), kv[:, 0, 0].reshape(1, -1, d).double(), V, page, 0.125, dtype)
+    for out in outs:
+        assert (out.double().view(T, nh, d) - p @ V).abs().max().item() <= bound
+    w_bound = 2 * (weight_error(q.reshape(-1, d), kv[:, 0, 0].reshape(1, -1, d).double(), page, 0.125, dtype) + (nh + 3) * U)
+    assert (weights[:, 0].double() - p.sum(1)).abs().max().item() <= w_bound
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,prefix,own", [(40, 700, 900), (5, 70, 40)])
+def test_rows_beyond_what_a_call_says_are_not_seen(rows, prefix, own, dtype):
+    from railgun_b200 import ops
+    nh, nkv, d, page, most = 8, 2, 64, 16, rows - 2
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    cache = Cache([prefix, prefix] + [own] * rows, nkv, d, page, dtype, g)
+    q, tables, pos = queries(rows, nh, d, dtype, g), cache.table[:2].contiguous(), i32([own - 1] * rows)
+    own_table = cache.table[2:].contiguous()
+
+    def run(groups, max_rows):
+        out = torch.empty(rows, nh * d, dtype=dtype, device=DEV)
+        ops.prefix_attention(q, out, cache.kv, tables, i32(groups), own_table, pos, nh, nkv, d, 0.125, max_rows=max_rows, max_prefix=prefix, max_own=own)
+        return out
+    want = run([[0, most, prefix], [rows, 0, 0]], most)
+    assert torch.equal(run([[0, rows, prefix], [-1, 5, prefix]], most), want)      # more rows than max_rows; no such first row
+    # portions: the third request's rows come to more than max_rows
+    few, outs = min(2, rows - 1), []
+    for last in (1 + few, rows):
+        w = torch.zeros(3, nkv, own + 8, device=DEV)
+        ops.prompt_key_weights(q, cache.kv, w, i32([0, 1, 2]), cache.table[2:5].contiguous(), i32([0, 1, 1, last]), i32([5, 0, own // 2]),
+                               i32([0, 0, 0]), nh, nkv, d, 0.125, max_rows=few, max_context=own)
+        outs.append(w)
+    assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [40, 700, 5000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_score_that_is_no_number_is_seen(bad, n, dtype):
+    """An entry that a row sees and whose score is no number, or infinite: the row's results for its kv head are no numbers, as a
+    softmax gives them; other heads, rows and requests are none the worse."""
+    from railgun_b200 import ops
+    nh, nkv, d, page, R = 8, 2, 64, 16, 3
+    g = torch.Generator(device=DEV).manual_seed(n)
+    cache = Cache([n] * R, nkv, d, page, dtype, g)
+    q, pos, slots = queries(R, nh, d, dtype, g).abs(), i32([n - 1] * R), i32([0, 1, 2])
+    args = (nh, nkv, d, 0.125)
+
+    def run():
+        outs = [torch.empty(R, nh * d, dtype=dtype, device=DEV) for _ in range(2)]
+        w1, w2 = (torch.zeros(R, nkv, n, device=DEV) for _ in range(2))
+        ops.prefix_attention(q, outs[0], cache.kv, cache.table[:1].contiguous(), i32([[0, 0, 0]]), cache.table, pos, *args, max_rows=0, max_prefix=0,
+                             max_own=n)
+        ops.weighed_attention(q, outs[1], cache.kv, w1, slots, cache.table, pos, *args, max_context=n)
+        ops.prompt_key_weights(q, cache.kv, w2, slots, cache.table, i32([0, 1, 2, 3]), pos, i32([0, 0, 0]), *args, max_rows=1, max_context=n)
+        return [o.view(R, nkv, -1) for o in outs] + [w1, w2]
+    before = run()
+    cache.kv[cache.table[1, 25 // page].long(), 0, 1, 25 % page, 3] = bad
+    for x, y in zip(before, run()):
+        hit = torch.zeros(R, nkv, dtype=torch.bool, device=DEV)
+        hit[1, 1] = True
+        assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], x[~hit])
