@@ -31,87 +31,124 @@ __device__ __forceinline__ void rows_of(const WeightArgs& a, int r, int& row0, i
     entries = rows > 0 && start >= 0 ? min(start + rows, a.limit) : 0;
 }
 
+// A pass of which parts are joined afterwards.
+struct KtArgs {
+    WeightArgs w;
+    float* part_ml;              // [T, nh, row_parts, 2]
+    float* part_w;               // [parts of the second pass, R, nkv, limit]; null: the weights themselves are written
+    int row_parts, parts;        // of the first pass, and of this one: what streams, dealt out in turn
+    // the tensor cores' kernel
+    int* err;
+    int blocks, n_items;         // 256 lanes each, of the longest request
+    int tile_rows;               // rows of a query tile: 128 / group
+    int page_shift;
+};
+
 // ---------------------------------------------------------------------------------------------------
-// Any head size up to 256, any page size, 32-bit or bfloat16 storage, all arithmetic in 32-bit.  16 queries (rows x heads
-// of a kv head) by 64 entries at a time, 2 x 4 a thread.
+// Any head size up to 256, any page size, 32-bit or bfloat16 storage, all arithmetic in 32-bit.  16 or 64 queries (rows x heads
+// of a kv head) by 64 entries at a time, 2 x 4 or 8 x 4 a thread: eight of them read 12 quads of shared memory for 128
+// multiply-adds, two of them 6 for 32.  What bounds it is arithmetic, and with few blocks the trip to memory before every tile:
+// 32-bit, 32 heads on 8 of 128, 256 rows 58 us, 2,048 rows 1.6 ms (21 TFLOP/s over both passes).  (16 queries at a time, single
+// numbers loaded and one block for all rows that see a tile: 691 us for the 256 rows.)
 // ---------------------------------------------------------------------------------------------------
 #define KW_THREADS 128
-#define KW_Q 16
 #define KW_K 64
+#define KW_FEW 32                  // queries a kv head up to which 16 at a time waste less than they read
 
-template <typename A>
-__device__ __forceinline__ void load_queries(const WeightArgs& a, float* qs, int ld, int row0, int kvh, int q0, int nq) {
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ float4 load4(const bf16* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+
+// ROWS rows of d numbers, from `at` (-1: zeros), times f; to rows of ld, zeros up to the next four columns.
+template <typename A, bool VEC, int ROWS>
+__device__ __forceinline__ void load_rows(float* to, int ld, int d, const A* from, const long long* at, float f) {
+    const int pieces = VEC ? d / 4 : (d + 3) & ~3, step = KW_THREADS / pieces, odd = KW_THREADS - step * pieces;
+#pragma unroll 4
+    for (int row = threadIdx.x / pieces, p = threadIdx.x % pieces; row < ROWS; p += odd, row += step) {
+        if (p >= pieces) { p -= pieces; if (++row >= ROWS) break; }
+        const long long x = at[row];
+        if (VEC) {
+            float4 v = {0.f, 0.f, 0.f, 0.f};
+            if (x >= 0) v = load4(from + x + 4 * p);
+            *reinterpret_cast<float4*>(to + row * ld + 4 * p) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        } else to[row * ld + p] = x >= 0 && p < d ? to_f32(from[x + p]) * f : 0.f;
+    }
+}
+// Where query qi of (request's first row, kv head) and entry e are.
+__device__ __forceinline__ long long query_at(const WeightArgs& a, int row0, int kvh, int qi) {
     const int group = a.nh / a.nkv;
-    for (int i = threadIdx.x; i < KW_Q * ld; i += KW_THREADS) {
-        const int row = i / ld, c = i - row * ld, qi = q0 + row;
-        float v = 0.f;
-        if (row < nq && c < a.d)
-            v = to_f32(((const A*)a.q)[(size_t)(row0 + qi / group) * a.q_stride + (kvh * group + qi % group) * a.d + c]) * a.scale_log2;
-        qs[i] = v;
-    }
+    return (long long)(row0 + qi / group) * a.q_stride + (kvh * group + qi % group) * a.d;
 }
-template <typename A>
-__device__ __forceinline__ void load_keys(const WeightArgs& a, float* ks, int ld, const int* table, int kvh, int e0, int n) {
-    const size_t page_elems = (size_t)2 * a.nkv * a.page_size * a.d;
-    for (int i = threadIdx.x; i < KW_K * ld; i += KW_THREADS) {
-        const int row = i / ld, c = i - row * ld, e = e0 + row;
-        float v = 0.f;
-        if (row < n && c < a.d)
-            v = to_f32(((const A*)a.kv)[(size_t)table[e / a.page_size] * page_elems + ((size_t)kvh * a.page_size + e % a.page_size) * a.d + c]);
-        ks[i] = v;
-    }
+__device__ __forceinline__ long long key_at(const WeightArgs& a, const int* table, int kvh, int e) {
+    return (long long)table[e / a.page_size] * 2 * a.nkv * a.page_size * a.d + ((long long)kvh * a.page_size + e % a.page_size) * a.d;
 }
-__device__ __forceinline__ void tile_scores(float (&sc)[2][4], const float* qs, const float* ks, int ld, int d, int qa, int ka) {
+template <int QI>
+__device__ __forceinline__ void tile_scores(float (&sc)[QI][4], const float* qs, const float* ks, int ld, int d, int qa, int ka) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < QI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+#pragma unroll 2
     for (int c = 0; c < d; c += 4) {
-        float4 q4[2];
+        float4 k4[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (2 * qa + i) * ld + c);
+        for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const float4*>(ks + (ka + 16 * j) * ld + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float4 k4 = *reinterpret_cast<const float4*>(ks + (ka + 16 * j) * ld + c);
+        for (int i = 0; i < QI; ++i) {
+            const float4 q4 = *reinterpret_cast<const float4*>(qs + (QI * qa + i) * ld + c);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                sc[i][j] += q4[i].x * k4.x; sc[i][j] += q4[i].y * k4.y;
-                sc[i][j] += q4[i].z * k4.z; sc[i][j] += q4[i].w * k4.w;
+            for (int j = 0; j < 4; ++j) {
+                sc[i][j] += q4.x * k4[j].x; sc[i][j] += q4.y * k4[j].y;
+                sc[i][j] += q4.z * k4[j].z; sc[i][j] += q4.w * k4[j].w;
             }
         }
     }
 }
 
 __host__ __device__ inline int kw_row(int d) { return ((d + 3) & ~3) + 4; }
-static size_t kw_smem(int d) { return (size_t)((KW_Q + KW_K) * kw_row(d) + 8 * KW_K) * sizeof(float); }
+static size_t kw_smem(int d, int queries) { return (size_t)((queries + KW_K) * kw_row(d) + 8 * KW_K) * sizeof(float); }
 
-// grid (query tiles, nkv, R)
-template <typename A>
-__global__ void __launch_bounds__(KW_THREADS) row_sums_general_kernel(const WeightArgs a) {
+// grid (query tiles x parts of the entries, nkv, R)
+template <typename A, bool VEC, int QI>
+__global__ void __launch_bounds__(KW_THREADS) row_sums_general_kernel(const KtArgs k) {
     extern __shared__ __align__(16) float smem[];
+    constexpr int QT = 8 * QI;
+    __shared__ long long at[KW_K];
+    static_assert(QT <= KW_K, "the queries' places fit");
+    const WeightArgs& a = k.w;
     pdl_wait();
     pdl_trigger();
-    const int r = blockIdx.z, kvh = blockIdx.y, group = a.nh / a.nkv, q0 = blockIdx.x * KW_Q;
+    const int r = blockIdx.z, kvh = blockIdx.y, group = a.nh / a.nkv, q0 = blockIdx.x / k.parts * QT, part = blockIdx.x % k.parts, tid = threadIdx.x;
     int row0, rows, start, entries;
     rows_of(a, r, row0, rows, start, entries);
-    const int nq = min(KW_Q, rows * group - q0);
+    const int nq = min(QT, rows * group - q0);
     if (nq <= 0 || entries <= 0) return;
-    const int ld = kw_row(a.d), qa = threadIdx.x >> 4, ka = threadIdx.x & 15;
-    float *qs = smem, *ks = smem + KW_Q * ld;
-    load_queries<A>(a, qs, ld, row0, kvh, q0, nq);
+    const int ld = kw_row(a.d), qa = tid >> 4, ka = tid & 15;
+    float *qs = smem, *ks = smem + QT * ld;
+    if (tid < QT) at[tid] = tid < nq ? query_at(a, row0, kvh, q0 + tid) : -1;
+    __syncthreads();
+    load_rows<A, VEC, QT>(qs, ld, a.d, (const A*)a.q, at, a.scale_log2);
     const int* table = a.block_table + (size_t)r * a.max_blocks;
     const int last = min(entries, start + (q0 + nq - 1) / group + 1);          // what the tile's last row sees
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    for (int e0 = 0; e0 < last; e0 += KW_K) {
-        const int n = min(KW_K, last - e0);
-        __syncthreads();
-        load_keys<A>(a, ks, ld, table, kvh, e0, n);
-        __syncthreads();
-        float sc[2][4];
-        tile_scores(sc, qs, ks, ld, a.d, qa, ka);
+    auto look_up = [&](int e0) -> long long { return tid < KW_K && e0 + tid < last ? key_at(a, table, kvh, e0 + tid) : -1; };
+    long long at_next = look_up(part * KW_K);
+    float m[QI], l[QI];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int sees = min(n, start + (q0 + 2 * qa + i) / group + 1 - e0);
+    for (int i = 0; i < QI; ++i) { m[i] = -INFINITY; l[i] = 0.f; }
+    for (int e0 = part * KW_K; e0 < last; e0 += k.parts * KW_K) {
+        __syncthreads();                                             // the last tile is read
+        if (tid < KW_K) at[tid] = at_next;
+        __syncthreads();
+        load_rows<A, VEC, KW_K>(ks, ld, a.d, (const A*)a.kv, at, 1.f);
+        at_next = look_up(e0 + k.parts * KW_K);
+        __syncthreads();
+        float sc[QI][4];
+        tile_scores<QI>(sc, qs, ks, ld, a.d, qa, ka);
+#pragma unroll
+        for (int i = 0; i < QI; ++i) {
+            const int sees = min(last, start + (q0 + QI * qa + i) / group + 1) - e0;
             float mx = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -127,7 +164,7 @@ __global__ void __launch_bounds__(KW_THREADS) row_sums_general_kernel(const Weig
         }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < QI; ++i) {
         float M = m[i];
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
@@ -135,54 +172,72 @@ __global__ void __launch_bounds__(KW_THREADS) row_sums_general_kernel(const Weig
         float L = l[i] * exp2f(m[i] - ms);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        const int qi = q0 + 2 * qa + i;
-        if (ka == 0 && 2 * qa + i < nq)                             // no weight at all: every 2^(s - z) is 0
-            a.z[(size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group] = L == 0.f ? INFINITY : ms + log2f(L);
+        const int qi = q0 + QI * qa + i;
+        if (ka == 0 && QI * qa + i < nq) {
+            const size_t to = (size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group;
+            if (k.parts > 1) *reinterpret_cast<float2*>(k.part_ml + (to * k.parts + part) * 2) = make_float2(M, L);
+            else a.z[to] = L == 0.f ? INFINITY : ms + log2f(L);       // no weight at all: every 2^(s - z) is 0
+        }
     }
 }
 
-// grid (tiles of entries, nkv, R)
-template <typename A>
-__global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const WeightArgs a) {
+// grid (tiles of entries x parts of the queries, nkv, R)
+template <typename A, bool VEC, int QI>
+__global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const KtArgs k) {
     extern __shared__ __align__(16) float smem[];
+    constexpr int QT = 8 * QI;
+    __shared__ long long at[KW_K];
+    const WeightArgs& a = k.w;
     pdl_wait();
     pdl_trigger();
-    const int r = blockIdx.z, kvh = blockIdx.y, group = a.nh / a.nkv, e0 = blockIdx.x * KW_K, slot = a.slots[r];
+    const int r = blockIdx.z, kvh = blockIdx.y, group = a.nh / a.nkv, e0 = blockIdx.x / k.parts * KW_K, part = blockIdx.x % k.parts, tid = threadIdx.x;
+    const int slot = a.slots[r];
     int row0, rows, start, entries;
     rows_of(a, r, row0, rows, start, entries);
     const int n = min(KW_K, entries - e0);
     if (n <= 0 || slot < 0 || slot >= a.n_slots) return;
-    const int ld = kw_row(a.d), qa = threadIdx.x >> 4, ka = threadIdx.x & 15;
-    float *qs = smem, *ks = qs + KW_Q * ld, *part = ks + KW_K * ld;            // part [8][64]
-    load_keys<A>(a, ks, ld, a.block_table + (size_t)r * a.max_blocks, kvh, e0, n);
+    const int ld = kw_row(a.d), qa = tid >> 4, ka = tid & 15;
+    float *qs = smem, *ks = qs + QT * ld, *sums = ks + KW_K * ld;              // sums [8][64]
+    if (tid < KW_K) at[tid] = tid < n ? key_at(a, a.block_table + (size_t)r * a.max_blocks, kvh, e0 + tid) : -1;
+    __syncthreads();
+    load_rows<A, VEC, KW_K>(ks, ld, a.d, (const A*)a.kv, at, 1.f);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int q0 = max(0, e0 - start) * group; q0 < rows * group; q0 += KW_Q) {  // from the first row that sees entry e0
-        const int nq = min(KW_Q, rows * group - q0);
+    for (int q0 = max(0, e0 - start) * group + part * QT; q0 < rows * group; q0 += k.parts * QT) {  // from the first row that sees entry e0
         __syncthreads();
-        load_queries<A>(a, qs, ld, row0, kvh, q0, nq);
+        if (tid < QT) at[tid] = q0 + tid < rows * group ? query_at(a, row0, kvh, q0 + tid) : -1;
         __syncthreads();
-        float sc[2][4];
-        tile_scores(sc, qs, ks, ld, a.d, qa, ka);
+        load_rows<A, VEC, QT>(qs, ld, a.d, (const A*)a.q, at, a.scale_log2);
+        float z[QI];
+        int sees[QI];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (2 * qa + i >= nq) continue;
-            const int qi = q0 + 2 * qa + i, sees = start + qi / group + 1 - e0;
-            const float z = a.z[(size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group];
+        for (int i = 0; i < QI; ++i) {
+            const int qi = q0 + QI * qa + i;
+            const bool query = qi < rows * group;
+            z[i] = query ? a.z[(size_t)(row0 + qi / group) * a.nh + kvh * group + qi % group] : 0.f;
+            sees[i] = query ? start + qi / group + 1 - e0 : 0;
+        }
+        __syncthreads();
+        float sc[QI][4];
+        tile_scores<QI>(sc, qs, ks, ld, a.d, qa, ka);
+#pragma unroll
+        for (int i = 0; i < QI; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (ka + 16 * j < sees) sum[j] += exp2f(sc[i][j] - z);
-        }
+                if (ka + 16 * j < sees[i]) sum[j] += exp2f(sc[i][j] - z[i]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[qa * KW_K + ka + 16 * j] = sum[j];
+    for (int j = 0; j < 4; ++j) sums[qa * KW_K + ka + 16 * j] = sum[j];
     __syncthreads();
-    float* w = a.weights + ((size_t)slot * a.nkv + kvh) * a.weights_ld + e0;
-    if (threadIdx.x < n) {
-        float v = e0 + (int)threadIdx.x < a.fresh[r] ? w[threadIdx.x] : 0.f;
+    if (tid < n) {
         float added = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) added += part[i * KW_K + threadIdx.x];
-        w[threadIdx.x] = v + added;
+        for (int i = 0; i < 8; ++i) added += sums[i * KW_K + tid];
+        const int e = e0 + tid;
+        if (k.part_w) k.part_w[(((size_t)part * a.R + r) * a.nkv + kvh) * a.limit + e] = added;
+        else {
+            float* w = a.weights + ((size_t)slot * a.nkv + kvh) * a.weights_ld + e;
+            *w = (e < a.fresh[r] ? *w : 0.f) + added;
+        }
     }
 }
 
@@ -205,17 +260,6 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const We
 #define KT_THREADS 352             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
 #define KT_TILE 128
 __host__ __device__ constexpr int kt_b_stages(int pieces) { return pieces == 1 ? 4 : 2; }
-
-struct KtArgs {
-    WeightArgs w;
-    float* part_ml;              // [T, nh, parts of the first pass, 2]
-    float* part_w;               // [parts of the second pass, R, nkv, limit]; null: the weights themselves are written
-    int* err;
-    int blocks, parts, n_items;  // 256 lanes each, of the longest request; parts of what streams
-    int row_parts;               // parts of the first pass
-    int tile_rows;               // rows of a query tile: 128 / group
-    int page_shift;
-};
 
 struct KtItem {
     int r, kvh, part, row0, rows, start, entries;
@@ -652,6 +696,15 @@ static int make_q_map(CUtensorMap* map, const void* q, int T, int q_stride, int 
     return r == CUDA_SUCCESS ? 0 : 20000 + (int)r;
 }
 
+static int join_rows(const KtArgs& a, cudaStream_t s) {
+    if (a.parts == 1) return 0;
+    return rg_launch(join_row_sums_kernel, dim3((unsigned)(((long long)a.w.T * a.w.nh + 255) / 256)), dim3(256), 0, s, 1, a);
+}
+static int join_entries(const KtArgs& a, int max_context, cudaStream_t s) {
+    if (a.parts == 1) return 0;
+    return rg_launch(join_entry_sums_kernel, dim3((max_context + 255) / 256, a.w.nkv, a.w.R), dim3(256), 0, s, 1, a);
+}
+
 template <int PIECES>
 static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int max_context, int sms, cudaStream_t s) {
     constexpr int smem = (4 + kt_b_stages(PIECES)) * KT_TILE * 128 * PIECES + 1024;
@@ -664,43 +717,58 @@ static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int
     RG_ALLOW_SMEM((key_weights_tc_kernel<PIECES, false>), smem)
     RG_ALLOW_SMEM((key_weights_tc_kernel<PIECES, true>), smem)
     e = rg_launch(key_weights_tc_kernel<PIECES, false>, dim3(min(sms, rows.n_items)), dim3(KT_THREADS), smem, s, 1, qm, km, rows);
-    if (!e && rows.parts > 1)
-        e = rg_launch(join_row_sums_kernel, dim3((unsigned)(((long long)w.T * w.nh + 255) / 256)), dim3(256), 0, s, 1, rows);
+    if (!e) e = join_rows(rows, s);
     if (!e) e = rg_launch(key_weights_tc_kernel<PIECES, true>, dim3(min(sms, entries.n_items)), dim3(KT_THREADS), smem, s, 1, qm, km, entries);
-    if (!e && entries.parts > 1)
-        e = rg_launch(join_entry_sums_kernel, dim3((max_context + 255) / 256, w.nkv, w.R), dim3(256), 0, s, 1, entries);
-    return e;
+    return e ? e : join_entries(entries, max_context, s);
 }
 
-// max_rows: the most rows of a request; max_context: the most entries a row sees.  Scratch: z [T, nh]; for the tensor cores'
-// kernels (row_parts > 0; the caller has seen to what they take) part_ml [T, nh, row_parts, 2] where row_parts > 1 and part_w
-// [entry_parts, R, nkv, max_context] where entry_parts > 1.
+template <typename A, bool VEC, int QI>
+static int launch_key_weights_general(const KtArgs& rows, const KtArgs& entries, int max_rows, int max_context, cudaStream_t s) {
+    const WeightArgs& w = rows.w;
+    const size_t smem = kw_smem(w.d, 8 * QI);
+    const long long q_tiles = ((long long)max_rows * (w.nh / w.nkv) + 8 * QI - 1) / (8 * QI), e_tiles = (max_context + KW_K - 1) / KW_K;
+    if (q_tiles * rows.parts > 0x7fffffffll || e_tiles * entries.parts > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    RG_ALLOW_SMEM((row_sums_general_kernel<A, VEC, QI>), kw_smem(256, 8 * QI))
+    RG_ALLOW_SMEM((entry_sums_general_kernel<A, VEC, QI>), kw_smem(256, 8 * QI))
+    int e = rg_launch(row_sums_general_kernel<A, VEC, QI>, dim3((unsigned)(q_tiles * rows.parts), w.nkv, w.R), dim3(KW_THREADS), smem, s, 1, rows);
+    if (!e) e = join_rows(rows, s);
+    if (!e)
+        e = rg_launch(entry_sums_general_kernel<A, VEC, QI>, dim3((unsigned)(e_tiles * entries.parts), w.nkv, w.R), dim3(KW_THREADS), smem, s, 1,
+                      entries);
+    return e ? e : join_entries(entries, max_context, s);
+}
+
+// max_rows: the most rows of a request; max_context: the most entries a row sees.  Scratch: z [T, nh], part_ml [T, nh, row_parts,
+// 2] where row_parts > 1 and part_w [entry_parts, R, nkv, max_context] where entry_parts > 1.
 extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv, int num_pages, int dtype, float* weights, int weights_ld,
                                      int n_slots, const int* slots, const int* block_table, int max_blocks, const int* cu_rows,
                                      const int* starts, const int* fresh, int R, int T, int nh, int nkv, int d, int page_size,
                                      float scale, int max_rows, int max_context, float* z, int row_parts, float* part_ml,
-                                     int entry_parts, float* part_w, int sms, int* err, void* stream) {
+                                     int entry_parts, float* part_w, int tensor_cores, int sms, int* err, void* stream) {
     if (R <= 0 || T <= 0 || max_rows <= 0 || max_context <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_context > weights_ld || R > 65535 || nkv > 65535 ||
-        (long long)max_rows * (nh / nkv) > 0x7fffffffll)
+        (long long)max_rows * (nh / nkv) > 0x7fffffffll || row_parts < 1 || entry_parts < 1)
         return RG_ERR_UNSUPPORTED;
     const WeightArgs a = {q, kv, block_table, cu_rows, starts, fresh, slots, weights, z, weights_ld, q_stride, max_blocks, n_slots, T, R,
                           nh, nkv, d, page_size, (int)min((long long)max_context, (long long)max_blocks * page_size),
                           scale * 1.4426950408889634f, max_rows};
     const cudaStream_t s = (cudaStream_t)stream;
     const int group = nh / nkv;
-    if (row_parts > 0) {
+    KtArgs rows = {a, part_ml, nullptr, row_parts, row_parts}, entries = rows;
+    entries.parts = entry_parts;
+    entries.part_w = entry_parts > 1 ? part_w : nullptr;
+    if (tensor_cores) {
         int shift = -1;
         for (int b = 3; b < 31; ++b) if (page_size == (1 << b)) shift = b;
         if (dtype != RG_DTYPE_BF16 || (d != 64 && d != 128) || group > KT_TILE || shift < 0 || q_stride % 8 || ((uintptr_t)q & 15) ||
-            ((uintptr_t)kv & 15) || scale <= 0.f || entry_parts < 1 || (long long)num_pages * 2 * nkv * page_size > 0x7fffffffll)
+            ((uintptr_t)kv & 15) || scale <= 0.f || (long long)num_pages * 2 * nkv * page_size > 0x7fffffffll)
             return RG_ERR_UNSUPPORTED;
-        KtArgs rows = {a, part_ml, nullptr, err, 0, row_parts, 0, row_parts, KT_TILE / group, shift}, entries = rows;
+        rows.err = entries.err = err;
+        rows.page_shift = entries.page_shift = shift;
+        rows.tile_rows = entries.tile_rows = KT_TILE / group;
         const long long q_tiles = (max_rows + rows.tile_rows - 1) / rows.tile_rows, e_tiles = (max_context + KT_TILE - 1) / KT_TILE;
         rows.blocks = (int)((q_tiles + 1) / 2);
         entries.blocks = (int)((e_tiles + 1) / 2);
-        entries.parts = entry_parts;
-        entries.part_w = entry_parts > 1 ? part_w : nullptr;
         const long long n_rows = (long long)rows.blocks * R * nkv * row_parts, n_entries = (long long)entries.blocks * R * nkv * entry_parts;
         if (n_rows > 0x3fffffffll || n_entries > 0x3fffffffll) return RG_ERR_UNSUPPORTED;
         rows.n_items = (int)n_rows;
@@ -708,13 +776,11 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
         return d == 64 ? launch_key_weights_tc<1>(rows, entries, num_pages, max_context, sms, s)
                        : launch_key_weights_tc<2>(rows, entries, num_pages, max_context, sms, s);
     }
-    const size_t smem = kw_smem(d);
-    const dim3 by_query((max_rows * group + KW_Q - 1) / KW_Q, nkv, R), by_entry((max_context + KW_K - 1) / KW_K, nkv, R);
-#define RG_KW(A) { RG_ALLOW_SMEM(row_sums_general_kernel<A>, kw_smem(256)) \
-    RG_ALLOW_SMEM(entry_sums_general_kernel<A>, kw_smem(256)) \
-    const int e = rg_launch(row_sums_general_kernel<A>, by_query, dim3(KW_THREADS), smem, s, 1, a); \
-    return e ? e : rg_launch(entry_sums_general_kernel<A>, by_entry, dim3(KW_THREADS), smem, s, 1, a); }
-    if (dtype == RG_DTYPE_F32) RG_KW(float)
-    RG_KW(bf16)
+    const bool vec = d % 4 == 0 && q_stride % 4 == 0 && (((uintptr_t)q | (uintptr_t)kv) & (dtype == RG_DTYPE_F32 ? 15 : 7)) == 0;
+#define RG_KW(A, V) { if (max_rows * group <= KW_FEW) return launch_key_weights_general<A, V, 2>(rows, entries, max_rows, max_context, s); \
+    return launch_key_weights_general<A, V, 8>(rows, entries, max_rows, max_context, s); }
+    if (dtype == RG_DTYPE_F32) { if (vec) RG_KW(float, true) RG_KW(float, false) }
+    if (vec) RG_KW(bf16, true)
+    RG_KW(bf16, false)
 #undef RG_KW
 }

@@ -2362,10 +2362,13 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
 
-def key_weight_parts(items: int, tiles: int) -> int:
-    """Parts that the streamed side of ``prompt_key_weights`` is cut into: until there are 256 items, not quite two an SM, which
-    the kernel deals out to and fro, of four tiles at least.  (Four an SM: 80 us for 2,048 rows of a prompt against 70, one: 80.)"""
-    return max(1, min(-(-256 // max(1, items)), -(-tiles // 4), 32))
+def key_weight_parts(items: int, tiles: int, tensor_cores: bool = True) -> int:
+    """Parts that the streamed side of ``prompt_key_weights`` is cut into.  Tensor cores: until there are 256 items, not quite two an SM,
+    which the kernel deals out to and fro, of four tiles at least.  (Four an SM: 80 us for 2,048 rows of a prompt against 70, one:
+    80.)  The general kernel: 592 blocks, four an SM (8 rows of 4 requests on 4,000 entries each in 32-bit 164 us; two an SM 237,
+    six 183)."""
+    room, least = (256, 4) if tensor_cores else (592, 1)
+    return max(1, min(-(-room // max(1, items)), -(-tiles // least), 32))
 
 
 def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts, fresh, nh: int, nkv: int, d: int, scale: float,
@@ -2387,14 +2390,16 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     if min(max_rows, max_context) < 0:
         raise KernelError("prompt_key_weights: max_rows and max_context are counts")
     _check_entry_weights(weights, "weights", nkv, max_context)
-    G, row_parts, entry_parts = nh // nkv, 0, 0
-    floats = n_z = -(-T * nh // 4) * 4
-    if q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale):
+    G, n_z = nh // nkv, -(-T * nh // 4) * 4
+    tensor_cores = q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
+    if tensor_cores:
         # tiles of 128 queries and of 128 entries: one kind stays, two at a time, and the other streams by in parts
-        q_tiles, e_tiles = -(-max_rows // (128 // G)), -(-max_context // 128)
-        row_parts = key_weight_parts(R * nkv * -(-q_tiles // 2), e_tiles)
-        entry_parts = key_weight_parts(R * nkv * -(-e_tiles // 2), q_tiles)
-        floats += (T * nh * row_parts * 2 if row_parts > 1 else 0) + (R * nkv * max_context * entry_parts if entry_parts > 1 else 0)
+        q_tiles, e_tiles, at_a_time = -(-max_rows // (128 // G)), -(-max_context // 128), 2
+    else:
+        q_tiles, e_tiles, at_a_time = -(-max_rows * G // (16 if max_rows * G <= 32 else 64)), -(-max_context // 64), 1
+    row_parts = key_weight_parts(R * nkv * -(-q_tiles // at_a_time), e_tiles, tensor_cores)
+    entry_parts = key_weight_parts(R * nkv * -(-e_tiles // at_a_time), q_tiles, tensor_cores)
+    floats = n_z + (T * nh * row_parts * 2 if row_parts > 1 else 0) + (R * nkv * max_context * entry_parts if entry_parts > 1 else 0)
     z = torch.empty(floats, dtype=torch.float32, device=q.device)
     part_ml = z.data_ptr() + 4 * n_z
     part_w = part_ml + (8 * T * nh * row_parts if row_parts > 1 else 0)
@@ -2403,7 +2408,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
         _ptr(q), c_int(step), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
         _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(T),
         c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z),
-        c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), c_int(num_sms(q.device)), _ptr(_tc_error_flag(q.device)), _stream()),
+        c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), c_int(1 if tensor_cores else 0), c_int(num_sms(q.device)), _ptr(_tc_error_flag(q.device)), _stream()),
         "prompt_key_weights")
 
 
