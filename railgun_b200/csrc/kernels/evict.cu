@@ -13,6 +13,10 @@
 // a step needs 7 to 8 steps to get there: 14 us of 53 for clusters of two on 16,384 keys.)  Then free entries and late ones
 // are numbered by ballots, with the counts of the warps and blocks before.  A warp takes up to 32 moves at a time: their
 // addresses a lane each, then their rows in 16-byte pieces, several a lane under way.
+//
+// What bounds it: the digits, one after the other, each a barrier or three away from the next; then, with many moves, memory.  8 prompts
+// of 8,192 to 16,384 entries down to 2,048 in 8 kv heads of 128: 40 us, 15 of them the choice, 24 the moves of 83 MB (3.4 TB/s
+// from a cold cache); 64 requests of 1,040 down to 1,024 in 8 heads of 64: 9.7 us, one launch.
 #include "common.cuh"
 #include <cooperative_groups.h>
 namespace cg = cooperative_groups;

@@ -255,7 +255,10 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const Kt
 // across items.
 //
 // What bounds it: one 2^x an element and pass.  128 x 128 of them take 1,024 cycles of a scheduler's MUFU, the products of a
-// tile 520 of the tensor core (head size 128).
+// tile 520 of the tensor core (head size 128).  The MUFU is busy for six tenths of a pass, waits for a tile's scores and uneven items
+// take the rest: 2,048 rows of 32 heads on 8 of 128 70 us, 8,192 rows 864 (318 TFLOP/s counted once, twice that are done).  The
+// last 1 to 33 rows of 8 prompts of 3,000 to 6,000 entries at head size 64 57 us: a lane without a query still costs a 2^x.
+// (Entries as lanes and queries as columns in both passes, with sums over columns in registers: 110 us.)
 // ---------------------------------------------------------------------------------------------------
 #define KT_THREADS 352             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
 #define KT_TILE 128
