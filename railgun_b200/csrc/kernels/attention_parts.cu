@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 // brings.  What bounds it is memory: every entry's K and V are read once for up to 16 queries.  64 requests on 4,096 entries each,
 // 32 heads on 8, with their weights: 190 us at head size 128 (5.7 TB/s, 89 % of what a copy reaches), 112 at 64 (5.0 TB/s); on 1 to
 // 4,096 entries at head size 128 106 us, some 12 of which are the tail of unequal blocks and the kernel that joins.  (Blocks that
-// stay and take several parts each: 202 to 214 us for the equal lists.)
+// stay and take several parts each: 202 to 214 us for the equal lists.)  One request on 32,768 entries: 33 us.
 //
 // A block is four warps that share nothing until they join at the end.  A warp takes every fourth run of 16 entries: one TMA
 // box of K and V together (a four-dimensional map: 64 columns, rows, 64-column pieces of the head, K and V; pages of 8 take
@@ -578,7 +578,7 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
 // of L2; what is saved is the second launch and the parts' trip through memory.  With WEIGH the scores stay in shared memory
 // until the row's sums are known, and the entries' weights are written by the block that read them.  What bounds it is the launch,
 // one trip to memory for the table and one for the entries: one request on 1,024 entries at head size 64 with weights 5.7 us
-// (9.5 in parts that a second kernel joins), on 32,768 at 128 33 us; 4 rows on 1,024 shared and 64 own entries 8.7 us.
+// (7.8 in parts that a second kernel joins); 4 rows on 1,024 shared and 64 own entries at 128 8.7 (10.0 in parts).
 // grid (T clusters, nkv x tiles of heads)
 // ---------------------------------------------------------------------------------------------------
 template <int PIECES, bool WEIGH>

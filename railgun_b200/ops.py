@@ -2228,21 +2228,24 @@ def _row_maps_ok(q, step: int, kv_cache, pages: int, nkv: int, page_size: int, s
             and scale > 0 and pages * 2 * nkv * page_size < (1 << 31) - 1)
 
 
-def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0) -> int:
+def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: bool = False) -> int:
     """How many blocks, a cluster, share each of ``blocks`` (row, kv head, tile of heads) of up to ``longest`` entries and leave nothing
     to be joined; 0: the entries go in parts that another kernel joins.  ``fast``: by rows_mma_kernel; ``heads`` > 0: whose scores
-    wait in shared memory."""
+    wait in shared memory; ``shared``: entries that parts would read once for several rows.  32 heads on 8 of 128, rows against
+    parts: one row with weights on 1,024 / 2,048 / 3,136 / 4,096 entries 6.8 to 8.8, 8.4 to 8.7, 11.0 to 9.6, 11.7 to 9.4 us; four
+    rows on 8,192 63 to 31; 64 on 512 / 1,024 34.7 to 36.3, 79 to 58 (one block an SM is left by its scores); 128 rows that
+    share 64 / 256 / 512 of 64 more 22 to 29, 31 to 28, 43 to 31."""
     cluster = 1
     while cluster < 8 and blocks * cluster * 2 <= 256 and longest > 64 * cluster:
         cluster *= 2
-    per = -(-longest // cluster)
+    per, running = -(-longest // cluster), blocks * cluster
     if not fast:
         return cluster if per <= 448 else 0
-    if blocks * cluster > 296:                   # several waves: two blocks an SM have to fit
-        most = min(640, 3600 // max(heads, 1))
-    else:
-        most = 2048 if blocks * cluster >= 100 else 640
-        most = min(most, 28000 // max(heads, 1))
+    most = {1: 640, 2: 512, 4: 400, 8: 320}[cluster]
+    if heads:
+        most = min(most, (3600 if running >= 100 else 28000) // heads)
+    if shared:
+        most = most * 296 // max(296, running)   # by the waves of blocks: each reads again what parts share
     return cluster if per <= most else 0
 
 
@@ -2297,7 +2300,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     n_groups, G = groups.shape[0], nh // nkv
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
-    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast)
+    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast, shared=longest > 0)
     sms = num_sms(q.device)
     if cluster:
         p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
