@@ -780,26 +780,69 @@ __device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __r
     }
 }
 
+// The same by one warp, parts in their order, where there are up to 32 of them: a part's factor a lane.
 template <typename A>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const PartArgs a, A* __restrict__ out, int out_ld) {
-    pdl_wait();
-    pdl_trigger();
-    join_row(a, blockIdx.x / a.nh, blockIdx.x % a.nh, out, out_ld);
+__device__ __forceinline__ void join_row_warp(const PartArgs& a, int t, int h, A* __restrict__ out, int out_ld) {
+    const int slots = a.prefix_parts + a.own_parts, d = a.d, lane = threadIdx.x & 31;
+    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_of(a, t);
+    const size_t base = ((size_t)t * a.nh + h) * slots;
+    const int slot = lane < n_prefix ? lane : a.prefix_parts + lane - n_prefix;
+    float2 ml = {-INFINITY, 0.f};
+    if (lane < n) ml = *reinterpret_cast<const float2*>(a.part_ml + (base + slot) * 2);
+    const float M = warp_max(ml.x), e = exp2f(ml.x - (M == -INFINITY ? 0.f : M)), L = warp_sum(ml.y * e);
+    const float factor = L == 0.f ? 0.f : e / L;
+    A* to = out + (size_t)t * out_ld + h * d;
+    for (int c0 = 0; c0 < d; c0 += 128) {
+        const int c = c0 + 4 * lane;
+        float4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const float f = __shfl_sync(0xffffffffu, factor, i);
+            const float* from = a.part_o + (base + (i < n_prefix ? i : a.prefix_parts + i - n_prefix)) * d + c;
+            float4 x = {0.f, 0.f, 0.f, 0.f};
+            if (d % 4 == 0) { if (c < d) x = *reinterpret_cast<const float4*>(from); }
+            else { if (c < d) x.x = from[0]; if (c + 1 < d) x.y = from[1]; if (c + 2 < d) x.z = from[2]; if (c + 3 < d) x.w = from[3]; }
+            acc.x += f * x.x; acc.y += f * x.y; acc.z += f * x.z; acc.w += f * x.w;
+        }
+        if (c < d) to[c] = from_f32<A>(acc.x);
+        if (c + 1 < d) to[c + 1] = from_f32<A>(acc.y);
+        if (c + 2 < d) to[c + 2] = from_f32<A>(acc.z);
+        if (c + 3 < d) to[c + 3] = from_f32<A>(acc.w);
+    }
+}
+// Rows and heads of a block: one, or one a warp where there are enough to fill the GPU and few parts (211 rows of 32 heads in five
+// parts: 19 us with one a block, bound by instructions).
+static int join_heads(const PartArgs& a) {
+    return a.prefix_parts + a.own_parts <= 32 && (long long)a.T * a.nh >= 592 ? JOIN_THREADS / 32 : 1;
+}
+static unsigned join_blocks(const PartArgs& a) { return (unsigned)(((long long)a.T * a.nh + join_heads(a) - 1) / join_heads(a)); }
+template <typename A>
+__device__ __forceinline__ void join_block(const PartArgs& a, int b, int heads, A* __restrict__ out, int out_ld) {
+    const int i = heads == 1 ? b : b * heads + (int)(threadIdx.x >> 5), t = i / a.nh, h = i % a.nh;
+    if (heads == 1) join_row(a, t, h, out, out_ld);
+    else if (t < a.T) join_row_warp(a, t, h, out, out_ld);
 }
 
-// Blocks 0 .. T nh - 1 join a row and head; the others add up the weights of 512 entries of a row and kv head, four a thread:
+template <typename A>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const PartArgs a, int heads, A* __restrict__ out, int out_ld) {
+    pdl_wait();
+    pdl_trigger();
+    join_block(a, blockIdx.x, heads, out, out_ld);
+}
+
+// The first `joins` blocks join rows and heads; the others add up the weights of 512 entries of a row and kv head, four a thread:
 //   w[e] = decay w[e] + sum_h 2^(s_h(e) - M_h) / L_h,   the newest entry's w not read
 #define WEIGH_CHUNK (4 * JOIN_THREADS)
 #define WEIGH_HEADS 64
 template <typename A>
-__global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A* __restrict__ out, int out_ld,
+__global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, int joins, int heads, A* __restrict__ out, int out_ld,
                                                              float* __restrict__ weights, long long weights_ld, int n_slots,
                                                              const int* __restrict__ slots, int chunks, float decay) {
     pdl_wait();
     pdl_trigger();
     int b = blockIdx.x;
-    if (b < a.T * a.nh) { join_row(a, b / a.nh, b % a.nh, out, out_ld); return; }
-    b -= a.T * a.nh;
+    if (b < joins) { join_block(a, b, heads, out, out_ld); return; }
+    b -= joins;
     const int chunk = b % chunks, kvh = b / chunks % a.nkv, t = b / chunks / a.nkv, group = a.nh / a.nkv;
     const int n = own_entries(a, t), e = chunk * WEIGH_CHUNK + 4 * threadIdx.x, slot = slots[t];
     if (chunk * WEIGH_CHUNK >= n || slot < 0 || slot >= n_slots) return;
@@ -810,9 +853,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
 #pragma unroll
     for (int j = 0; j < 4; ++j) before[j] = e + j < n - 1 ? decay * w[e + j] : 0.f;
     for (int g0 = 0; g0 < group; g0 += WEIGH_HEADS) {                // heads of a kv head, so many at a time
-        const int heads = min(group - g0, WEIGH_HEADS);
+        const int some = min(group - g0, WEIGH_HEADS);
         __syncthreads();
-        for (int g = warp; g < heads; g += JOIN_THREADS / 32) {
+        for (int g = warp; g < some; g += JOIN_THREADS / 32) {
             float M, L;
             join_ml(a, t, kvh * group + g0 + g, 0, n_own, M, L);
             if ((threadIdx.x & 31) == 0) { sM[g] = M; sI[g] = L == 0.f ? 0.f : 1.f / L; }
@@ -821,7 +864,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, A
         if (e >= n) continue;
         const float* sc = a.scores + ((size_t)t * a.nh + kvh * group + g0) * a.score_ld + e;   // rows of whole 64 entries
 #pragma unroll 4
-        for (int g = 0; g < heads; ++g) {
+        for (int g = 0; g < some; ++g) {
             const float4 s = *reinterpret_cast<const float4*>(sc + (size_t)g * a.score_ld);
             sum[0] += exp2f(s.x - sM[g]) * sI[g]; sum[1] += exp2f(s.y - sM[g]) * sI[g];
             sum[2] += exp2f(s.z - sM[g]) * sI[g]; sum[3] += exp2f(s.w - sM[g]) * sI[g];
@@ -974,8 +1017,8 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
         if (e) return e;
     }
     if (dtype == RG_DTYPE_F32)
-        return rg_launch(join_kernel<float>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
-    return rg_launch(join_kernel<bf16>, dim3(T * nh), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);
+        return rg_launch(join_kernel<float>, dim3(join_blocks(a)), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, join_heads(a), (float*)out, out_ld);
+    return rg_launch(join_kernel<bf16>, dim3(join_blocks(a)), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, join_heads(a), (bf16*)out, out_ld);
 }
 
 // Single tokens with the weights of their entries.  weights [n_slots, nkv, weights_ld]; scores [T, nh, score_ld] is scratch.
@@ -1001,11 +1044,11 @@ extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int 
     int e = launch_parts(a, dtype, num_pages, err, (cudaStream_t)stream);
     if (e) return e;
     const int chunks = (max_context + WEIGH_CHUNK - 1) / WEIGH_CHUNK;
-    const long long blocks = (long long)T * nh + (long long)T * nkv * chunks;
+    const long long blocks = join_blocks(a) + (long long)T * nkv * chunks;
     if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     if (dtype == RG_DTYPE_F32)
-        return rg_launch(weigh_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out,
-                         out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
-    return rg_launch(weigh_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out,
-                     out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
+        return rg_launch(weigh_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a,
+                         (int)join_blocks(a), join_heads(a), (float*)out, out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
+    return rg_launch(weigh_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a,
+                     (int)join_blocks(a), join_heads(a), (bf16*)out, out_ld, weights, (long long)weights_ld, n_slots, slots, chunks, decay);
 }
