@@ -333,10 +333,17 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 #define PM_Q 16
 // Runs of a warp's ring, and blocks an SM.  Head size 64: four and three (six and two, 12 % slower: 64 requests on 2,000 entries
 // 70 against 63 us); 128: three and two (two and three are level, and 9 % slower for one request on 32,768).
-__host__ __device__ constexpr int pm_stages(int pieces) { return pieces == 1 ? 4 : (pieces == 3 ? 2 : 3); }
-__host__ __device__ constexpr int pm_blocks(int pieces) { return pieces == 1 ? 3 : (pieces == 2 ? 2 : 1); }
+// Brief: a warp has no more than two runs, and there are more blocks than fit at once, which then come and go: 128 requests' tokens on
+// 100 entries 23.7 us (27.1 with the other), on 128 at head size 64 14.7 (17.1); with few blocks it is level or slower.
+__host__ __device__ constexpr int pm_stages(int pieces, bool brief) {
+    return brief ? (pieces == 1 ? 2 : 2) : (pieces == 1 ? 4 : (pieces == 3 ? 2 : 3));
+}
+__host__ __device__ constexpr int pm_blocks(int pieces, bool brief) {
+    return brief ? (pieces == 1 ? 5 : 3) : (pieces == 1 ? 3 : (pieces == 2 ? 2 : 1));
+}
+static bool pm_brief(int d, long long entries, long long blocks) { return entries <= 128 && blocks > 148 * pm_blocks(d / 64, false); }
 __host__ __device__ constexpr int pm_stage_bytes(int pieces) { return 16 * 64 * 2 * 2 * pieces; }
-static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1) * pm_stage_bytes(1), "the warps' results fit where the stages were");
+static_assert(4 * 4 * 16 * 64 <= 4 * pm_stages(1, true) * pm_stage_bytes(1), "the warps' results fit where the stages were");
 
 // A run of 16 entries from entry e of its list on: one box, or where pages hold 8 tokens two.  One lane.
 __device__ __forceinline__ void load_run(const CUtensorMap* map, const PartArgs& a, uint32_t dst, uint32_t bar, int bytes, int box_shift, int page_a,
@@ -478,10 +485,10 @@ __device__ __forceinline__ float4 join_warps(const float* all, const float (*ml)
     return sum;
 }
 
-template <int PIECES>
-__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES))
+template <int PIECES, bool BRIEF>
+__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES, BRIEF))
 parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, int* err) {
-    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
+    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES, BRIEF), STAGE = pm_stage_bytes(PIECES);
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bars[4 * STAGES];
     __shared__ float ml[4][PM_Q][2];
@@ -581,10 +588,10 @@ parts_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, i
 // (7.8 in parts that a second kernel joins); 4 rows on 1,024 shared and 64 own entries at 128 8.7 (10.0 in parts).
 // grid (T clusters, nkv x tiles of heads)
 // ---------------------------------------------------------------------------------------------------
-template <int PIECES, bool WEIGH>
-__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES))
+template <int PIECES, bool WEIGH, bool BRIEF>
+__global__ void __launch_bounds__(PM_THREADS, pm_blocks(PIECES, BRIEF))
 rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, const RowsArgs b, int* err) {
-    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES), STAGE = pm_stage_bytes(PIECES);
+    constexpr int D = 64 * PIECES, STAGES = pm_stages(PIECES, BRIEF), STAGE = pm_stage_bytes(PIECES);
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t bars[4 * STAGES];
     __shared__ float ml[4][PM_Q][2], fin_ml[PM_Q][2], row_ml[PM_Q][2];
@@ -925,13 +932,14 @@ static int launch_parts_mma(const PartArgs& a, int num_pages, int* err, cudaStre
     CUtensorMap map;
     int e = make_kv_map(&map, a.kv, num_pages, a.nkv, a.page_size, a.d, a.page_size < 16 ? a.page_size : 16);
     if (e) return e;
-#define RG_PM(P) { constexpr int smem = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
-    RG_ALLOW_SMEM(parts_mma_kernel<P>, smem) \
-    return rg_launch(parts_mma_kernel<P>, dim3((unsigned)blocks), dim3(PM_THREADS), smem, s, 1, map, a, err); }
-    if (a.d == 64) RG_PM(1)
-    if (a.d == 128) RG_PM(2)
-    if (a.d == 192) RG_PM(3)
-    RG_PM(4)
+#define RG_PM(P, B) { constexpr int smem = 4 * pm_stages(P, B) * pm_stage_bytes(P) + 1024; \
+    RG_ALLOW_SMEM((parts_mma_kernel<P, B>), smem) \
+    return rg_launch(parts_mma_kernel<P, B>, dim3((unsigned)blocks), dim3(PM_THREADS), smem, s, 1, map, a, err); }
+    const bool brief = pm_brief(a.d, max(a.n_groups ? a.prefix_per : 0, a.own_per), blocks);
+    if (a.d == 64) { if (brief) RG_PM(1, true) else RG_PM(1, false) }
+    if (a.d == 128) { if (brief) RG_PM(2, true) else RG_PM(2, false) }
+    if (a.d == 192) RG_PM(3, false)
+    RG_PM(4, false)
 #undef RG_PM
 }
 
@@ -945,14 +953,15 @@ static int launch_rows(const PartArgs& a, const RowsArgs& b, int dtype, int num_
     if (e) return e;
     const int scores = b.weights ? (a.nh / a.nkv) * (b.runs * 16 + 8) * 4 : 0;
     const dim3 grid(cluster * a.T, a.nkv * a.own_tiles);
-#define RG_RM(P, W) { constexpr int stages = 4 * pm_stages(P) * pm_stage_bytes(P) + 1024; \
-    RG_ALLOW_SMEM((rows_mma_kernel<P, W>), 227 * 1024 - 2048) \
-    return rg_launch(rows_mma_kernel<P, W>, grid, dim3(PM_THREADS), stages + scores, s, cluster, map, a, b, err); }
-#define RG_RMW(P) { if (b.weights) RG_RM(P, true) else RG_RM(P, false) }
-    if (a.d == 64) RG_RMW(1)
-    if (a.d == 128) RG_RMW(2)
-    if (a.d == 192) RG_RMW(3)
-    RG_RMW(4)
+#define RG_RM(P, W, B) { constexpr int stages = 4 * pm_stages(P, B) * pm_stage_bytes(P) + 1024; \
+    RG_ALLOW_SMEM((rows_mma_kernel<P, W, B>), 227 * 1024 - 2048) \
+    return rg_launch(rows_mma_kernel<P, W, B>, grid, dim3(PM_THREADS), stages + scores, s, cluster, map, a, b, err); }
+#define RG_RMW(P, B) { if (b.weights) RG_RM(P, true, B) else RG_RM(P, false, B) }
+    const bool brief = pm_brief(a.d, ((long long)a.prefix_limit + a.own_limit + cluster - 1) / cluster, (long long)grid.x * grid.y);
+    if (a.d == 64) { if (brief) RG_RMW(1, true) else RG_RMW(1, false) }
+    if (a.d == 128) { if (brief) RG_RMW(2, true) else RG_RMW(2, false) }
+    if (a.d == 192) RG_RMW(3, false)
+    RG_RMW(4, false)
 #undef RG_RMW
 #undef RG_RM
 }
