@@ -2228,13 +2228,13 @@ def _row_maps_ok(q, step: int, kv_cache, pages: int, nkv: int, page_size: int, s
             and scale > 0 and pages * 2 * nkv * page_size < (1 << 31) - 1)
 
 
-def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: bool = False) -> int:
+def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: int = 0, d: int = 128) -> int:
     """How many blocks, a cluster, share each of ``blocks`` (row, kv head, tile of heads) of up to ``longest`` entries and leave nothing
     to be joined; 0: the entries go in parts that another kernel joins.  ``fast``: by rows_mma_kernel; ``heads`` > 0: whose scores
-    wait in shared memory; ``shared``: entries that parts would read once for several rows.  32 heads on 8 of 128, rows against
+    wait in shared memory; ``shared``: so many of the entries parts would read once for several rows.  32 heads on 8 of 128, rows against
     parts: one row with weights on 1,024 / 2,048 / 3,136 / 4,096 entries 6.8 to 8.8, 8.4 to 8.7, 11.0 to 9.6, 11.7 to 9.4 us; four
-    rows on 8,192 63 to 31; 64 on 512 / 1,024 34.7 to 36.3, 79 to 58 (one block an SM is left by its scores); 128 rows that
-    share 64 / 256 / 512 of 64 more 22 to 29, 31 to 28, 43 to 31."""
+    rows on 8,192 63 to 31; 64 on 512 / 1,024 34.7 to 36.3, 79 to 58 (one block an SM is left by its scores); 48 that share 15 of
+    up to 196 / 128 of 144 / 256 of 512 11.6 to 13.9, 12.3 to 11.6, 18.2 to 16.0; 231 62 to 66 where 128 of 628 are shared."""
     cluster = 1
     while cluster < 8 and blocks * cluster * 2 <= 256 and longest > 64 * cluster:
         cluster *= 2
@@ -2244,8 +2244,8 @@ def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: 
     most = {1: 640, 2: 512, 4: 400, 8: 320}[cluster]
     if heads:
         most = min(most, (3600 if running >= 100 else 28000) // heads)
-    if shared:
-        most = most * 296 // max(296, running)   # by the waves of blocks: each reads again what parts share
+    if shared > 640 * cluster or (per > 128 and running > (444 if d == 64 else 296) and 4 * shared > longest - shared):
+        return 0                                 # more than one wave of blocks: each reads again what parts share
     return cluster if per <= most else 0
 
 
@@ -2300,7 +2300,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     n_groups, G = groups.shape[0], nh // nkv
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
-    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast, shared=longest > 0)
+    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast, shared=longest, d=d)
     sms = num_sms(q.device)
     if cluster:
         p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
