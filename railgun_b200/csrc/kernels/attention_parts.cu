@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 // bfloat16, head sizes 64, 128, 192 and 256, pages of 8 tokens or a larger power of two: mma.sync m16n8k16 on tiles that TMA
 // brings.  What bounds it is memory: every entry's K and V are read once for up to 16 queries.  64 requests on 4,096 entries each,
 // 32 heads on 8, with their weights: 190 us at head size 128 (5.7 TB/s, 89 % of what a copy reaches), 112 at 64 (5.0 TB/s); on 1 to
-// 4,096 entries at head size 128 106 us, some 12 of which are the tail of unequal blocks and the kernel that joins.  (Blocks that
+// 4,096 entries at head size 128 104 us, some 10 of which are the tail of unequal blocks and the kernel that joins.  (Blocks that
 // stay and take several parts each: 202 to 214 us for the equal lists.)  One request on 32,768 entries: 33 us.
 //
 // A block is four warps that share nothing until they join at the end.  A warp takes every fourth run of 16 entries: one TMA
@@ -717,8 +717,8 @@ rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, co
 
 // ---------------------------------------------------------------------------------------------------
 // Joining the parts of a row and head, and adding up the weights of a row's entries over the heads of a kv head.  Short kernels
-// that are bound by their trips to memory: 64 rows of 32 heads in parts of 128 numbers 11 us from a cold cache, 64 requests'
-// weights of 1 to 4,096 entries from 32 heads' scores 17 (25 MB read).
+// that are bound by their trips to memory: 64 rows of 32 heads in parts of 128 numbers 9.7 us from a cold cache, 64 requests'
+// outputs and weights of 1 to 4,096 entries from 32 heads' scores 14 (25 MB read).
 // ---------------------------------------------------------------------------------------------------
 #define JOIN_THREADS 128
 

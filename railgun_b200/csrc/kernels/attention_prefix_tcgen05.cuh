@@ -13,7 +13,7 @@
 // with j: the exponentials never wait for a product of their own side.  (With one buffer of 128 columns and N 128, the faster
 // shape by 260 to 392 cycles for 64 entries, a side's scores, exponentials and products are one chain: 65,536 entries for
 // 512 queries a kv head 189 us, 171 with two.)
-// What bounds it: 65,536 entries for 128 rows of 32 heads on 8 of 128 take 161 us with the rows' 256 own entries beside them, 1,010
+// What bounds it: 65,536 entries for 128 rows of 32 heads on 8 of 128 take 155 us with the rows' 256 own entries beside them, 1,010
 // TFLOP/s while the tiles run (59 % of what a dense product reaches): N 64 scores cost the tensor core 49 cycles where 33 would
 // do, and the hand-over between products and exponentials the rest.
 // There is no mask but the end of a part: rows of V behind it get zeros in shared memory, scores behind it -infinity.
