@@ -23,7 +23,7 @@ typedef int (*Launcher)(u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u
                         u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64, u64,
                         u64, u64, u64, u64, u64, u64, float, float, float, float, float, float, float, float);
 
-static PyObject *s_data_ptr, *s_is_cuda, *s_is_contiguous, *s_dtype;
+static PyObject *s_data_ptr, *s_is_cuda, *s_is_contiguous, *s_dtype, *s_shape;
 
 // call(address, arguments..): what `integer`, `pointer`, `ptr` and `real` give (None: a null pointer)
 static PyObject* fc_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -121,6 +121,28 @@ static PyObject* fc_fits(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return PyBool_FromLong(ok);
 }
 
+// shaped(tensor, dtype or None, sizes..): does it fit, with as many dimensions, of these sizes (None: any)?
+static PyObject* fc_shaped(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    if (n < 2) {
+        PyErr_SetString(PyExc_TypeError, "shaped: a tensor, a type and sizes");
+        return nullptr;
+    }
+    PyObject* x = fc_fits(self, a, 2);
+    if (x != Py_True) return x;
+    PyObject* shape = PyObject_GetAttr(a[0], s_shape);
+    if (!shape) { Py_DECREF(x); return nullptr; }
+    bool ok = PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) == n - 2;
+    for (Py_ssize_t i = 0; ok && i < n - 2; ++i) {
+        if (a[i + 2] == Py_None) continue;
+        const long long want = PyLong_AsLongLong(a[i + 2]), have = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i));
+        if (PyErr_Occurred()) { Py_DECREF(shape); Py_DECREF(x); return nullptr; }
+        ok = want == have;
+    }
+    Py_DECREF(shape);
+    Py_DECREF(x);
+    return PyBool_FromLong(ok);
+}
+
 static PyMethodDef methods[] = {
     {"call", (PyCFunction)(void (*)(void))fc_call, METH_FASTCALL, "call(address, *numbers) -> int"},
     {"ptr", fc_ptr, METH_O, "the address of a tensor's first element; 0 for None"},
@@ -128,6 +150,7 @@ static PyMethodDef methods[] = {
     {"pointer", fc_pointer, METH_O, "its argument, an address; 0 for None"},
     {"real", fc_real, METH_O, "its argument, a number, as a float"},
     {"fits", (PyCFunction)(void (*)(void))fc_fits, METH_FASTCALL, "is it a contiguous CUDA tensor of this type (None: any)?"},
+    {"shaped", (PyCFunction)(void (*)(void))fc_shaped, METH_FASTCALL, "does it fit, and has it these sizes (None: any)?"},
     {nullptr, nullptr, 0, nullptr}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "fastcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -137,6 +160,7 @@ PyMODINIT_FUNC PyInit_fastcall(void) {
     s_is_cuda = PyUnicode_InternFromString("is_cuda");
     s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
     s_dtype = PyUnicode_InternFromString("dtype");
-    if (!s_data_ptr || !s_is_cuda || !s_is_contiguous || !s_dtype) return nullptr;
+    s_shape = PyUnicode_InternFromString("shape");
+    if (!s_data_ptr || !s_is_cuda || !s_is_contiguous || !s_dtype || !s_shape) return nullptr;
     return PyModule_Create(&module);
 }

@@ -899,6 +899,8 @@ def talking_prefill_flash(qc: torch.Tensor, cache: torch.Tensor, block_table: to
 
 
 def _check_out_view(out, T: int, n: int, dtype, what: str):
+    if _fast is not None and _fast.shaped(out, dtype, T, n):
+        return
     if not out.is_cuda or out.dtype != dtype or out.dim() != 2 or out.shape != (T, n) or out.stride(1) != 1:
         raise KernelError(f"{what}: out must be a CUDA [{T}, {n}] view of {dtype} with unit column stride")
 
@@ -2174,17 +2176,19 @@ def decode_attention(q, q_stride: int, out, kv_cache, block_table, rows, n_token
 def _check_rows_of(q, nh: int, nkv: int, d: int, kv_cache, what: str) -> tuple:
     """What the operators over rows of single tokens and portions ask of queries and cache; returns q's rows, how far they are
     apart, the pages and the page size."""
-    code, (T, n), s = _dtype_code(q), q.shape if q.dim() == 2 else (0, 0), kv_cache.shape
-    if (_fast is not None and _fast.fits(kv_cache, q.dtype) and len(s) == 5 and s[1] == 2 and s[2] == nkv > 0 and s[3] > 0 and s[4] == d
-            and 0 < d <= 256 and nh > 0 and nh % nkv == 0 and q.is_cuda and n >= nh * d):
-        at, step = q.stride()
-        if step == 1 and at >= n:
+    dtype = q.dtype
+    if (_fast is not None and (dtype is torch.bfloat16 or dtype is torch.float32) and _fast.shaped(kv_cache, dtype, None, 2, nkv, None, d)
+            and 0 < d <= 256 and 0 < nkv and nh > 0 and nh % nkv == 0 and q.is_cuda and q.dim() == 2):
+        (T, n), (at, step), s = q.shape, q.stride(), kv_cache.shape
+        if step == 1 and at >= n >= nh * d and s[3] > 0:
             return T, at, s[0], s[3]
+    _dtype_code(q)
     _check_rows(q, "q")
     _check(kv_cache, "kv_cache", q.dtype)
     if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
         raise KernelError(f"{what}: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
     _check_pages(kv_cache, nkv, d)
+    (T, n), s = q.shape, kv_cache.shape
     if n < nh * d:
         raise KernelError(f"{what}: q has {n} columns, {nh} heads of {d} need {nh * d}")
     return T, q.stride(0), s[0], s[3]
@@ -2198,6 +2202,8 @@ def _check_pages(kv_cache, nkv: int, d: int) -> None:
 
 def _check_ints(t: torch.Tensor, name: str, rows: int | None, cols: int | None = None, table: bool = False) -> None:
     """int32 [rows], or [rows, cols] of a ``table`` (None: any)."""
+    if _fast is not None and (_fast.shaped(t, torch.int32, rows, cols) if table else _fast.shaped(t, torch.int32, rows)):
+        return
     _check(t, name, torch.int32)
     s = t.shape
     if (len(s) != (2 if table else 1) or (rows is not None and s[0] != rows) or (cols is not None and s[1] != cols)):
@@ -2205,11 +2211,15 @@ def _check_ints(t: torch.Tensor, name: str, rows: int | None, cols: int | None =
                           f"{(cols if cols is not None else 'any') if table else ''}]")
 
 
-def _check_entry_weights(weights: torch.Tensor, name: str, nkv: int, max_context: int, dtype=torch.float32) -> None:
-    _check(weights, name, dtype)
+def _check_entry_weights(weights: torch.Tensor, name: str, nkv: int, max_context: int, dtype=torch.float32) -> tuple:
+    """[slots, nkv, at least max_context]; returns how many slots, and numbers a head."""
     s = weights.shape
+    if len(s) == 3 and s[1] == nkv and s[2] >= max_context and _fast is not None and _fast.fits(weights, dtype):
+        return s[0], s[2]
+    _check(weights, name, dtype)
     if len(s) != 3 or s[1] != nkv or s[2] < max_context:
         raise KernelError(f"{name} is {tuple(s)}, expected [slots, {nkv}, at least {max_context}]")
+    return s[0], s[2]
 
 
 def _tc_error_flag(device) -> torch.Tensor:
@@ -2228,6 +2238,7 @@ def _row_maps_ok(q, step: int, kv_cache, pages: int, nkv: int, page_size: int, s
             and scale > 0 and pages * 2 * nkv * page_size < (1 << 31) - 1)
 
 
+@functools.lru_cache(maxsize=4096)
 def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: int = 0, d: int = 128) -> int:
     """How many blocks, a cluster, share each of ``blocks`` (row, kv head, tile of heads) of up to ``longest`` entries and leave nothing
     to be joined; 0: the entries go in parts that another kernel joins.  ``fast``: by rows_mma_kernel; ``heads`` > 0: whose scores
@@ -2249,6 +2260,7 @@ def rows_cluster(blocks: int, longest: int, fast: bool, heads: int = 0, shared: 
     return cluster if per <= most else 0
 
 
+@functools.lru_cache(maxsize=4096)
 def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int, own: int, d: int) -> tuple:
     """(parts, entries a part) of prefixes of up to ``longest`` entries, of which ``blocks`` thread blocks, one an SM, read a
     part each (two each where ``tensor_cores`` is 2): whole tiles of 128 entries, as many parts as fill their share of the GPU once.
@@ -2264,6 +2276,7 @@ def prefix_parts(blocks: int, longest: int, sms: int, tensor_cores: int, own: in
     return -(-longest // per), per
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_parts(blocks: int, longest: int, d: int, fast: bool, sms: int) -> tuple:
     """(parts, entries a part) that lists of up to ``longest`` entries are cut into where ``blocks`` thread blocks would read a list in
     one part each: so many that the blocks fill the GPU a whole number of times, the fewest times that leave no part with
@@ -2300,11 +2313,11 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     n_groups, G = groups.shape[0], nh // nkv
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
-    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast, shared=longest, d=d)
-    sms = num_sms(q.device)
+    cluster = rows_cluster(T * nkv * -(-G // 16), longest + max_own, fast, 0, longest, d)
     if cluster:
         p_parts, p_per, o_parts, o_per = 1, longest or 1, 1, max_own or 1
     else:
+        sms = num_sms(q.device)
         if fast and d <= 128 and 16 < max_rows * G and G <= 128 and longest >= 256:
             # sides of 128 queries, two a block; groups that fill one side only have their blocks take two parts
             side = 128 // G
@@ -2341,7 +2354,7 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     _check_out_view(out, R, nh * d, q.dtype, "weighed_attention")
     if max_context < 0:
         raise KernelError("weighed_attention: max_context is a count")
-    _check_entry_weights(weights, "weights", nkv, max_context)
+    n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
     G, score_ld, scores, part_o, part_ml = nh // nkv, -(-max_context // 64) * 64, 0, 0, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
     cluster = rows_cluster(R * nkv, max_context, fast, G) if G <= 16 else 0
@@ -2361,10 +2374,11 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
         _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)),
         _ptr(block_table), c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),
         c_int(page_size), c_float(scale), c_void_p(part_o), c_void_p(part_ml), c_void_p(scores), c_int(score_ld),
-        _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), c_int(max_context), c_float(decay), c_int(cluster),
+        _ptr(weights), c_int(ld), c_int(n_slots), _ptr(slots), c_int(max_context), c_float(decay), c_int(cluster),
         _ptr(_tc_error_flag(q.device)), _stream()), "weighed_attention")
 
 
+@functools.lru_cache(maxsize=4096)
 def key_weight_parts(items: int, tiles: int, tensor_cores: bool = True) -> int:
     """Parts that the streamed side of ``prompt_key_weights`` is cut into.  Tensor cores: until there are 256 items, not quite two an SM,
     which the kernel deals out to and fro, of four tiles at least.  (Four an SM: 80 us for 2,048 rows of a prompt against 70, one:
@@ -2392,7 +2406,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     _check_ints(fresh, "fresh", R)
     if min(max_rows, max_context) < 0:
         raise KernelError("prompt_key_weights: max_rows and max_context are counts")
-    _check_entry_weights(weights, "weights", nkv, max_context)
+    n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
     G, n_z = nh // nkv, -(-T * nh // 4) * 4
     tensor_cores = q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
     if tensor_cores:
@@ -2408,7 +2422,7 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     part_w = part_ml + (8 * T * nh * row_parts if row_parts > 1 else 0)
     _COUNTER.value += 1 + (row_parts > 1) + (entry_parts > 1)      # the rows' sums, then the entries', and what joins their parts
     _ok(_fn("key_weights", "rg_prompt_key_weights")(
-        _ptr(q), c_int(step), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(weights), c_int(weights.shape[2]), c_int(weights.shape[0]),
+        _ptr(q), c_int(step), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(weights), c_int(ld), c_int(n_slots),
         _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(fresh), c_int(R), c_int(T),
         c_int(nh), c_int(nkv), c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), _ptr(z),
         c_int(row_parts), c_void_p(part_ml), c_int(entry_parts), c_void_p(part_w), c_int(1 if tensor_cores else 0), c_int(num_sms(q.device)), _ptr(_tc_error_flag(q.device)), _stream()),
@@ -2435,8 +2449,10 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
         _check_ints(t, name, R)
     if max_context < 0 or protect_first < 0 or protect_last < 0:
         raise KernelError("evict_entries: max_context, protect_first and protect_last are counts")
-    for t, name, dtype in ((weights, "weights", torch.float32), (places, "places", torch.int32),
-                           (weights_out, "weights_out", torch.float32), (places_out, "places_out", torch.int32)):
+    n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
+    for t, name, dtype in ((places, "places", torch.int32), (weights_out, "weights_out", torch.float32), (places_out, "places_out", torch.int32)):
+        if _fast is not None and _fast.shaped(t, dtype, n_slots, nkv, ld):
+            continue
         _check_entry_weights(t, name, nkv, max_context, dtype)
         if t.shape != weights.shape:
             raise KernelError(f"{name} is {tuple(t.shape)}, weights {tuple(weights.shape)}")
@@ -2448,11 +2464,11 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     while cluster < 8 and max_context > 16384 * cluster:
         cluster *= 2
     fused = max_context <= 2048                  # otherwise the moves are listed, and a second kernel's
-    moves = torch.empty(0 if fused else R * nkv * (2 * (max_context // 2) + 3), dtype=torch.int32, device=kv_cache.device)
+    moves = None if fused else torch.empty(R * nkv * (2 * (max_context // 2) + 3), dtype=torch.int32, device=kv_cache.device)
     _COUNTER.value += 0 if fused else 1
     _ok(_fn("evict", "rg_evict_entries")(
         _ptr(kv_cache), c_int(kv_cache.element_size()), _ptr(weights), _ptr(places), _ptr(weights_out), _ptr(places_out),
-        c_int(weights.shape[2]), c_int(weights.shape[0]), _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(lens), _ptr(keep),
+        c_int(ld), c_int(n_slots), _ptr(slots), _ptr(block_table), c_int(block_table.shape[1]), _ptr(lens), _ptr(keep),
         _ptr(positions), _ptr(new_lens), c_int(R), c_int(nkv), c_int(d), c_int(kv_cache.shape[3]), c_int(protect_first),
         c_int(protect_last), c_int(max_context), _ptr(moves), c_int(cluster), c_int(num_sms(kv_cache.device)), _stream()), "evict_entries")
     return new_lens
