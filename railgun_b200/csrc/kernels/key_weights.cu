@@ -260,11 +260,12 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const Kt
 // last 1 to 33 rows of 8 prompts of 3,000 to 6,000 entries at head size 64 57 us: a lane without a query still costs a 2^x.
 // (Entries as lanes and queries as columns in both passes, with sums over columns in registers: 110 us.)
 // ---------------------------------------------------------------------------------------------------
-#define KT_THREADS 352             // warps 0-3, 4-7: sides 0, 1; 8: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
+#define KT_THREADS 384             // warps 0-3, 4-7: sides 0, 1; 8, 11: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
 #define KT_TILE 128
+__host__ __device__ constexpr int kt_a_stages(int pieces) { return pieces == 1 ? 4 : 2; }      // of two tiles each
 __host__ __device__ constexpr int kt_b_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 
-struct KtItem {
+struct alignas(16) KtItem {             // read in quads
     int r, kvh, part, row0, rows, start, entries;
     int m0, n_m;                 // first lane tile, how many of the two there are (0: the end)
     int b0, n_b;                 // streamed tiles b0, b0 + parts, ..
@@ -305,24 +306,24 @@ template <int PIECES, bool ENTRIES>
 __global__ void __launch_bounds__(KT_THREADS, 1)
 key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap kv_map, const KtArgs a) {
     extern __shared__ unsigned char smem_raw[];
-    constexpr int NB = kt_b_stages(PIECES);
+    constexpr int NA = kt_a_stages(PIECES), NB = kt_b_stages(PIECES);
     constexpr uint32_t PIECE = KT_TILE * 128, TILE = PIECE * PIECES;
-    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, sA = base, sB = sA + 4 * TILE;   // two stages of two tiles; NB tiles
-    __shared__ __align__(8) uint64_t bars[4 + 2 * NB + 8 + 2];
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u, sA = base, sB = sA + 2 * NA * TILE;   // NA stages of two tiles; NB tiles
+    __shared__ __align__(8) uint64_t bars[3 * NA + 2 * NB + 8 + 2];
     // -z of a streamed tile's columns and their positions: a copy for every warp, so that warps wait for nothing but tiles
     __shared__ __align__(16) float col_z[ENTRIES ? 8 : 1][2][KT_TILE];
     __shared__ __align__(16) int col_p[ENTRIES ? 8 : 1][2][KT_TILE];
     __shared__ float other_ml[ENTRIES ? 1 : KT_TILE][2];             // side 1's results for side 0, where they share a tile
-    __shared__ KtItem items[2];
+    __shared__ KtItem items[NA];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    // a_full: an item and its lane tiles; s_full, s_empty: side 0's two buffers, side 1's; x_full, x_empty: other_ml
-    const uint32_t a_full = smem_addr(bars), a_empty = a_full + 16, b_full = a_empty + 16, b_empty = b_full + 8 * NB,
+    // i_full: an item; a_full: its lane tiles as well; s_full, s_empty: side 0's two buffers, side 1's; x_full, x_empty: other_ml
+    const uint32_t i_full = smem_addr(bars), a_full = i_full + 8 * NA, a_empty = a_full + 8 * NA, b_full = a_empty + 8 * NA, b_empty = b_full + 8 * NB,
                    s_full = b_empty + 8 * NB, s_empty = s_full + 32, x_full = s_empty + 32, x_empty = x_full + 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.w.nh / a.w.nkv;
     if (threadIdx.x == 0) {
         abort_flag = 0;
-        for (int i = 0; i < 2; ++i) { mbar_init(a_full + 8 * i, 1); mbar_init(a_empty + 8 * i, 2 + 8); }   // both issuers, eight warps
+        for (int i = 0; i < NA; ++i) { mbar_init(i_full + 8 * i, 1); mbar_init(a_full + 8 * i, 1); mbar_init(a_empty + 8 * i, 2 + 8); }   // both issuers, eight warps
         for (int i = 0; i < NB; ++i) { mbar_init(b_full + 8 * i, 1); mbar_init(b_empty + 8 * i, 2); }
         for (int i = 0; i < 4; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_empty + 8 * i, KT_TILE); }
         mbar_init(x_full, KT_TILE);
@@ -340,13 +341,39 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
     KtItem t = {};
     // Does side g work on streamed tile b of this item?  With one lane tile the sides take turns.
     auto mine_is = [&](int g, int b) -> bool { return t.n_m == 2 || (ENTRIES ? g == 0 : (b & 1) == g); };
-    if (warp == 8) {
-        // ---- loads
+    if (warp == 8 || warp == 11) {
+        // ---- loads.  Both warps walk through the items, each issues half of the boxes (one takes some 85 cycles of a warp).
+        const int half = warp == 11;
         const int box_rows = min(a.w.page_size, KT_TILE), boxes = KT_TILE / box_rows, box = lane % boxes, piece = lane / boxes;
-        const bool mine = piece < PIECES;                            // a box of a piece of the head each
-        auto page_of = [&](int tile) -> int {                        // behind the entries: any page
+        const bool mine = piece < PIECES && (ENTRIES || (lane & 1) == half);   // a box of a piece of the head each
+        // Items are looked up by all lanes, 32 of this block's rounds at a time, and page ids asked for an item, or four streamed
+        // tiles, ahead: a look-up takes as long as a tile's exponentials.
+        KtItem held = {}, n = {};
+        int r0 = -32;
+        uint32_t left = 0;
+        auto next_item = [&]() {
+            while (left == 0) {
+                r0 += 32;
+                if ((long long)r0 * gridDim.x >= a.n_items) { n = KtItem{}; return; }
+                // to and fro: who got the heaviest of one round gets the lightest of the next
+                const int i = (r0 + lane) * gridDim.x + (lane & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                left = __ballot_sync(0xffffffffu, i < a.n_items && kt_item<ENTRIES>(a, i, held));
+            }
+            const int from = __ffs(left) - 1;
+            left &= left - 1;
+            auto get = [&](int v) -> int { return __shfl_sync(0xffffffffu, v, from); };
+            n.r = get(held.r); n.kvh = get(held.kvh); n.part = get(held.part); n.row0 = get(held.row0); n.rows = get(held.rows);
+            n.start = get(held.start); n.entries = get(held.entries); n.m0 = get(held.m0); n.n_m = get(held.n_m); n.b0 = get(held.b0);
+            n.n_b = get(held.n_b); n.slot = get(held.slot); n.fresh = get(held.fresh);
+        };
+        auto page_of = [&](const KtItem& x, int tile) -> int {       // behind the entries: any page
             const int e = tile * KT_TILE + box * box_rows;
-            return a.w.block_table[(size_t)t.r * a.w.max_blocks + (e < t.entries ? e >> a.page_shift : 0)];
+            return x.n_b > 0 ? a.w.block_table[(size_t)x.r * a.w.max_blocks + (e < x.entries ? e >> a.page_shift : 0)] : 0;
+        };
+        constexpr int AHEAD = ENTRIES ? 1 : 4;
+        auto first_pages = [&](const KtItem& x, int (&page)[AHEAD]) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) page[j] = page_of(x, ENTRIES ? x.m0 + (x.n_m == 2 ? half : 0) : x.b0 + j * a.parts);
         };
         auto load_keys = [&](uint32_t dst, uint32_t bar, int tile, int page) {
             const int e = tile * KT_TILE + box * box_rows;
@@ -359,42 +386,53 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         };
         const uint32_t q_bytes = (uint32_t)(PIECES * 128 * group * a.tile_rows);
         const uint32_t a_bytes = ENTRIES ? TILE : q_bytes, b_bytes = ENTRIES ? q_bytes : TILE;
-        int ai = 0, bi = 0;
-        for (int round = 0; ok; ++round) {
-            // to and fro: who got the heaviest of one round gets the lightest of the next
-            const int i = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            const bool end = round * (int)gridDim.x >= a.n_items;
-            if (!end && i >= a.n_items) continue;
-            if (end) t.n_m = t.n_b = 0;
-            else if (!kt_item<ENTRIES>(a, i, t)) continue;
-            const int sa = ai & 1;
-            int page[2] = {0, 0};
-            if (ENTRIES && t.n_b) { page[0] = page_of(t.m0); page[1] = page_of(t.m0 + t.n_m - 1); }
-            if (!ENTRIES && t.n_b) page[0] = page_of(t.b0);
-            if (ai > 1) ok = mbar_wait_all(a_empty + 8 * sa, ((ai >> 1) & 1) ^ 1, a.err, 71, &abort_flag);
+        int page[AHEAD], bi = 0;
+        next_item();
+        first_pages(n, page);
+        for (int ai = 0; ok; ++ai) {
+            t = n;
+            const int sa = ai % NA;
+            if (ai >= NA) ok = mbar_wait_all(a_empty + 8 * sa, ((ai / NA) & 1) ^ 1, a.err, 71, &abort_flag);
             if (!ok) break;
-            if (lane == 0) {
+            if (half == 0 && lane == 0) {
                 items[sa] = t;
+                mbar_arrive(i_full + 8 * sa);
                 if (t.n_b) mbar_expect_tx(a_full + 8 * sa, (uint32_t)t.n_m * a_bytes);
                 else mbar_arrive(a_full + 8 * sa);
             }
             __syncwarp();
-            ++ai;
-            if (end) break;
-            for (int g = 0; g < t.n_m && t.n_b; ++g) {
-                if (ENTRIES) load_keys(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g, page[g]);
-                else load_queries(sA + (2 * sa + g) * TILE, a_full + 8 * sa, t.m0 + g);
+            if (t.n_m == 0) break;                                   // the end
+            if (t.n_b && half < t.n_m) {                             // a lane tile each
+                if (ENTRIES) load_keys(sA + (2 * sa + half) * TILE, a_full + 8 * sa, t.m0 + half, page[0]);
+                else load_queries(sA + (2 * sa + half) * TILE, a_full + 8 * sa, t.m0 + half);
             }
-            int page_next = page[0];
-            for (int b = 0; b < t.n_b && ok; ++b, ++bi) {
-                const int sb = bi % NB, tile = t.b0 + b * a.parts, page_now = page_next;
-                if (!ENTRIES && b + 1 < t.n_b) page_next = page_of(tile + a.parts);
-                if (bi >= NB) ok = mbar_wait_all(b_empty + 8 * sb, ((bi / NB) & 1) ^ 1, a.err, 72, &abort_flag);
-                if (!ok) break;
-                if (lane == 0) mbar_expect_tx(b_full + 8 * sb, b_bytes);
-                __syncwarp();
-                if (ENTRIES) load_queries(sB + sb * TILE, b_full + 8 * sb, tile);
-                else load_keys(sB + sb * TILE, b_full + 8 * sb, tile, page_now);
+            next_item();
+            if (ENTRIES || t.n_b == 0) first_pages(n, page);
+            for (int b0 = 0; b0 < t.n_b && ok; b0 += AHEAD) {
+                int page_next[AHEAD];
+                if (!ENTRIES) {
+                    if (b0 + AHEAD >= t.n_b) first_pages(n, page_next);
+                    else
+#pragma unroll
+                        for (int j = 0; j < AHEAD; ++j) page_next[j] = page_of(t, t.b0 + (b0 + AHEAD + j) * a.parts);
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    if (b0 + j >= t.n_b || !ok) break;
+                    const int sb = bi % NB, tile = t.b0 + (b0 + j) * a.parts;
+                    if (!ENTRIES || half == 0) {
+                        if (bi >= NB) ok = mbar_wait_all(b_empty + 8 * sb, ((bi / NB) & 1) ^ 1, a.err, 72, &abort_flag);
+                        if (!ok) break;
+                        if (half == 0 && lane == 0) mbar_expect_tx(b_full + 8 * sb, b_bytes);
+                        __syncwarp();
+                        if (ENTRIES) load_queries(sB + sb * TILE, b_full + 8 * sb, tile);
+                        else load_keys(sB + sb * TILE, b_full + 8 * sb, tile, page[j]);
+                    }
+                    ++bi;
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j)
+                    if (!ENTRIES) page[j] = page_next[j];
             }
         }
     } else if (warp == 9 || warp == 10) {
@@ -404,8 +442,8 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const bool issuer = elect_one();
         int si = 0, bi = 0;                                          // tiles of this side; streamed tiles
         for (int ai = 0; ok; ++ai) {
-            const int sa = ai & 1;
-            ok = mbar_wait_all(a_full + 8 * sa, (ai >> 1) & 1, a.err, 73, &abort_flag);
+            const int sa = ai % NA;
+            ok = mbar_wait_all(a_full + 8 * sa, (ai / NA) & 1, a.err, 73, &abort_flag);
             if (!ok) break;
             t.n_m = items[sa].n_m;
             t.n_b = items[sa].n_b;
@@ -445,10 +483,10 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
         const uint64_t scale2 = pack2(a.w.scale_log2, a.w.scale_log2);
         int si = 0, ai = 0, xi = 0;
         auto next_item = [&](KtItem& to) -> bool {
-            if (!mbar_wait_all(a_full + 8 * (ai & 1), (ai >> 1) & 1, a.err, 78, &abort_flag)) return false;
-            to = items[ai & 1];
+            if (!mbar_wait_all(i_full + 8 * (ai % NA), (ai / NA) & 1, a.err, 78, &abort_flag)) return false;
+            to = items[ai % NA];
             __syncwarp();
-            if (lane == 0) mbar_arrive(a_empty + 8 * (ai & 1));
+            if (lane == 0) mbar_arrive(a_empty + 8 * (ai % NA));
             ++ai;
             return true;
         };
@@ -458,12 +496,20 @@ key_weights_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_co
             int p_next[4];
             KtItem n = {};
             float before_next = 0.f;
+            int c_row[4], c_z[4];                                    // their rows in the tile, and where z is from the tile's first row's on
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = lane + 32 * j;
+                c_row[j] = c < a.tile_rows * group ? c / group : 0x3fffffff;
+                c_z[j] = c / group * a.w.nh + c % group;
+            }
             auto columns = [&](const KtItem& x, int b) {
+                const int r0 = (x.b0 + b * a.parts) * a.tile_rows, rows = g < x.n_m && b < x.n_b ? x.rows - r0 : 0;
+                const float* z = a.w.z + (size_t)(x.row0 + r0) * a.w.nh + x.kvh * group;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int c = lane + 32 * j, r = (x.b0 + b * a.parts) * a.tile_rows + c / group;
-                    p_next[j] = g < x.n_m && c < a.tile_rows * group && r < x.rows && b < x.n_b ? x.start + r : -1;
-                    z_next[j] = p_next[j] >= 0 ? a.w.z[(size_t)(x.row0 + r) * a.w.nh + x.kvh * group + c % group] : 0.f;
+                    p_next[j] = c_row[j] < rows ? x.start + r0 + c_row[j] : -1;
+                    z_next[j] = c_row[j] < rows ? z[c_z[j]] : 0.f;
                 }
             };
             auto place = [&](const KtItem& x) -> float* { return a.w.weights + ((size_t)x.slot * a.w.nkv + x.kvh) * a.w.weights_ld; };
@@ -710,7 +756,7 @@ static int join_entries(const KtArgs& a, int max_context, cudaStream_t s) {
 
 template <int PIECES>
 static int launch_key_weights_tc(KtArgs rows, KtArgs entries, int num_pages, int max_context, int sms, cudaStream_t s) {
-    constexpr int smem = (4 + kt_b_stages(PIECES)) * KT_TILE * 128 * PIECES + 1024;
+    constexpr int smem = (2 * kt_a_stages(PIECES) + kt_b_stages(PIECES)) * KT_TILE * 128 * PIECES + 1024;
     const WeightArgs& w = rows.w;
     CUtensorMap qm, km;
     int e = make_q_map(&qm, w.q, w.T, w.q_stride, w.nh, w.d, w.nh / w.nkv, rows.tile_rows);
