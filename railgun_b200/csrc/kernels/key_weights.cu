@@ -250,15 +250,16 @@ __global__ void __launch_bounds__(KW_THREADS) entry_sums_general_kernel(const Kt
 // share the streamed tiles, so a streamed tile is fetched once for 256 lanes; where only one tile is left, the sides take
 // every other streamed tile of it.  Per streamed tile of 128 and side: S = A B^T in 128 columns of tensor memory, two
 // buffers a side, then one pass of exponentials over it while the tensor core works on the next.  Blocks are persistent:
-// items (kv head, 256 lanes, part of what streams) are dealt out to and fro, the heaviest first.  The loading warp works out
-// what an item is and leaves it in shared memory with the item's first tiles; loads, products and exponentials run on
-// across items.
+// items (kv head, 256 lanes, part of what streams) are dealt out to and fro, the heaviest first.  Two loading warps work out
+// what an item is, look up its pages and fetch its first tiles while earlier ones are worked on (a ring of items); loads,
+// products and exponentials run on across items.  (One warp that looked up one item and one tile at a time: the last 1 to 33 rows
+// of 8 prompts 57 us, 54 now; 8,192 rows 861, 779 now.)
 //
 // What bounds it: one 2^x an element and pass.  128 x 128 of them take 1,024 cycles of a scheduler's MUFU, the products of a
 // tile 520 of the tensor core (head size 128).  The MUFU is busy for six tenths of a pass, waits for a tile's scores and uneven items
-// take the rest: 2,048 rows of 32 heads on 8 of 128 70 us, 8,192 rows 864 (318 TFLOP/s counted once, twice that are done).  The
-// last 1 to 33 rows of 8 prompts of 3,000 to 6,000 entries at head size 64 57 us: a lane without a query still costs a 2^x.
-// (Entries as lanes and queries as columns in both passes, with sums over columns in registers: 110 us.)
+// take the rest: 2,048 rows of 32 heads on 8 of 128 70 us, 8,192 rows 779 (353 TFLOP/s counted once, twice that are done).  The
+// last 1 to 33 rows of 8 prompts of 3,000 to 6,000 entries at head size 64 54 us: a lane without a query still costs a 2^x.
+// (Entries as lanes and queries as columns in both passes, with sums over columns in registers: 110.)
 // ---------------------------------------------------------------------------------------------------
 #define KT_THREADS 384             // warps 0-3, 4-7: sides 0, 1; 8, 11: TMA; 9, 10: MMA issue of sides 0, 1 (9: tensor memory)
 #define KT_TILE 128

@@ -2381,10 +2381,10 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
 @functools.lru_cache(maxsize=4096)
 def key_weight_parts(items: int, tiles: int, tensor_cores: bool = True) -> int:
     """Parts that the streamed side of ``prompt_key_weights`` is cut into.  Tensor cores: until there are 256 items, not quite two an SM,
-    which the kernel deals out to and fro, of four tiles at least.  (Four an SM: 80 us for 2,048 rows of a prompt against 70, one:
-    80.)  The general kernel: 592 blocks, four an SM (8 rows of 4 requests on 4,000 entries each in 32-bit 164 us; two an SM 237,
+    which the kernel deals out to and fro, of two tiles at least.  (2,048 rows of a prompt 70 us, with half as many items 90, with
+    twice as many 75; 80 rows behind 1,630 entries 18.8, in parts of four tiles 21.4.)  The general kernel: 592 blocks, four an SM (8 rows of 4 requests on 4,000 entries each in 32-bit 164 us; two an SM 237,
     six 183)."""
-    room, least = (256, 4) if tensor_cores else (592, 1)
+    room, least = (256, 2) if tensor_cores else (592, 1)
     return max(1, min(-(-room // max(1, items)), -(-tiles // least), 32))
 
 
