@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
 #define PM_Q 16
 // Runs of a warp's ring, and blocks an SM.  Head size 64: four and three (six and two, 12 % slower: 64 requests on 2,000 entries
 // 70 against 63 us); 128: three and two (two and three are level, and 9 % slower for one request on 32,768).
-// Brief: a warp has no more than two runs, and there are more blocks than fit at once, which then come and go: 128 requests' tokens on
+// Brief: a warp has no more than two runs, and there are more blocks than 148 SMs hold at once, which then come and go: 128 requests' tokens on
 // 100 entries 23.7 us (27.1 with the other), on 128 at head size 64 14.7 (17.1); with few blocks it is level or slower.
 __host__ __device__ constexpr int pm_stages(int pieces, bool brief) {
     return brief ? (pieces == 1 ? 2 : 2) : (pieces == 1 ? 4 : (pieces == 3 ? 2 : 3));

@@ -577,3 +577,56 @@ def test_a_score_that_is_no_number_is_seen(bad, n, dtype):
         hit = torch.zeros(R, nkv, dtype=torch.bool, device=DEV)
         hit[1, 1] = True
         assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], x[~hit])
+
+
+# ---- head sizes that are no multiples of four, queries on odd addresses --------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,d,page", [(4, 2, 5, 7), (3, 1, 33, 16), (2, 1, 130, 8), (6, 3, 255, 4), (9, 1, 1, 3)])
+def test_odd_head_sizes(nh, nkv, d, page, dtype):
+    for scene in ("three groups", "long"):
+        test_prefix_attention(nh, nkv, d, page, scene, dtype)
+    test_weighed_attention(nh, nkv, d, page, [64, 63, 65, 1, 0, 200], dtype)
+    test_prompt_key_weights(nh, nkv, d, page, [70, 129, 2], [0, 300, 63], [0, 300, 0], dtype)
+    test_prompt_key_weights(nh, nkv, d, page, [3, 0, 1], [0, 5, 64], [0, 5, 64], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,d", [(8, 2, 64), (8, 2, 128), (4, 1, 48)])
+def test_queries_on_odd_addresses(nh, nkv, d, dtype):
+    """The same numbers one column further on, where no wide load can read them: the same results but for their rounding."""
+    from railgun_b200 import ops
+    R, n, P, page = 5, 150, 90, 16
+    g = torch.Generator(device=DEV).manual_seed(d)
+    cache = Cache([P] + [n] * R, nkv, d, page, dtype, g)
+    q = torch.randn(R, nh * d, device=DEV, generator=g).to(dtype)
+    odd = torch.empty(R, nh * d + 9, dtype=dtype, device=DEV)[:, 1:nh * d + 1]
+    odd.copy_(q)
+    tables, table, pos, slots = cache.table[:1].contiguous(), cache.table[1:].contiguous(), i32([n - 1] * R), i32(list(range(R)))
+    args, outs = (nh, nkv, d, d ** -0.5), []
+    for x in (q, odd):
+        a, b = (out_view(R, nh * d, dtype) for _ in range(2))
+        w1, w2 = (torch.zeros(R, nkv, n, device=DEV) for _ in range(2))
+        ops.prefix_attention(x, a, cache.kv, tables, i32([[0, R, P]]), table, pos, *args, max_rows=R, max_prefix=P, max_own=n)
+        ops.weighed_attention(x, b, cache.kv, w1, slots, table, pos, *args, max_context=n)
+        ops.prompt_key_weights(x, cache.kv, w2, slots, table, i32(list(range(R + 1))), pos, i32([0] * R), *args, max_rows=1, max_context=n)
+        outs.append((a, b, w1, w2))
+    for r in range(R):
+        K, V = cache.entries(1 + r, n)
+        Kp, Vp = cache.entries(0, P)
+        mine = q[r].reshape(nh, d)
+        both = torch.cat([Kp, K], 1), torch.cat([Vp, V], 1)
+        assert (outs[0][0][r].double() - outs[1][0][r].double()).abs().max() <= 2 * out_error(mine, *both, P + n, d ** -0.5, dtype)
+        assert (outs[0][1][r].double() - outs[1][1][r].double()).abs().max() <= 2 * out_error(mine, K, V, n, d ** -0.5, dtype)
+        for i in (2, 3):
+            x, y = outs[0][i][r].double(), outs[1][i][r].double()
+            assert ((x - y).abs() / y).max() <= 2 * (weight_error(mine, K, n, d ** -0.5, dtype) + (nh + 3) * U)
+
+
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 128, 256), (4, 4, 64, 512), (128, 1, 64, 16), (160, 1, 64, 16), (96, 1, 128, 32), (130, 2, 128, 8)])
+def test_large_pages_and_many_heads(nh, nkv, d, page):
+    """Pages longer than a tile, and as many query heads on a kv head as a tile has rows, or more."""
+    for scene in ("three groups", "many rows", "long"):
+        test_prefix_attention(nh, nkv, d, page, scene, torch.bfloat16)
+    test_weighed_attention(nh, nkv, d, page, [2049, 3, 700], torch.bfloat16)
+    test_prompt_key_weights(nh, nkv, d, page, [70, 129, 2], [0, 300, 63], [0, 300, 0], torch.bfloat16)
+    test_prompt_key_weights(nh, nkv, d, page, [33, 64], [1000, 191], [2000, 0], torch.bfloat16)
