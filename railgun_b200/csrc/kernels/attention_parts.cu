@@ -973,7 +973,9 @@ static int launch_parts(const PartArgs& a, int dtype, int num_pages, int* err, c
 static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void* kv, const int* block_table, int max_blocks,
                            const int* positions, int T, int nh, int nkv, int d, int page_size, float scale, float* part_o,
                            float* part_ml, int own_parts, int own_per) {
-    if (T < 0 || d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || own_parts < 0 || own_per < 1) return false;
+    if (T < 0 || d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || own_parts < 0 || own_per < 1 ||
+        ((uintptr_t)part_o & 15) || ((uintptr_t)part_ml & 7))        // outputs are read in fours, (m, l) in pairs
+        return false;
     a = PartArgs{};
     a.q = q; a.q_stride = q_stride; a.kv = kv; a.block_table = block_table; a.max_blocks = max_blocks; a.positions = positions;
     a.T = T; a.nh = nh; a.nkv = nkv; a.d = d; a.page_size = page_size; a.scale_log2 = scale * 1.4426950408889634f;
@@ -986,7 +988,8 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 }
 
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
-// [T, nh, prefix_parts + own_parts, d] and part_ml [.., 2].  tensor_cores: 1 the prefixes by prefix_tc_kernel, 2 the same with two
+// [T, nh, prefix_parts + own_parts, d] on a 16-byte boundary and part_ml [.., 2] on one of 8.  tensor_cores: 1 the prefixes by
+// prefix_tc_kernel, 2 the same with two
 // parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.  cluster: not 0, rows by clusters of so many
 // blocks, which leave no parts.
 extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
@@ -1041,6 +1044,7 @@ extern "C" int rg_weighed_attention(const void* q, int q_stride, void* out, int 
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
                         own_parts, own_per) || max_context > score_ld || max_context > weights_ld || out_ld < nh * d)
         return RG_ERR_UNSUPPORTED;
+    if (score_ld % 4 || ((uintptr_t)scores & 15)) return RG_ERR_UNSUPPORTED;   // read in fours
     a.scores = scores; a.score_ld = score_ld;
     a.own_limit = min(a.own_limit, max_context);
     const int group = nh / nkv;

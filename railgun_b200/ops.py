@@ -2292,6 +2292,12 @@ def attention_parts(blocks: int, longest: int, d: int, fast: bool, sms: int) -> 
     return -(-longest // per), per
 
 
+def _floats_before_ml(parts: int, d: int) -> int:
+    """Numbers that the outputs of ``parts`` parts take in scratch, in whole 16 bytes: behind them lie the parts' (m, l), which are
+    read two at a time."""
+    return -(-parts * d // 4) * 4
+
+
 def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positions, nh: int, nkv: int, d: int, scale: float,
                      max_rows: int, max_prefix: int, max_own: int) -> None:
     """Attention of single tokens whose requests share prefixes: ``out`` [T, nh * d], row t of ``q`` [T, at least nh * d] (head h
@@ -2328,8 +2334,9 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
             p_parts, p_per = attention_parts(n_groups * nkv * -(-max_rows * G // 16), longest, d, fast, sms)
         o_parts, o_per = attention_parts(T * nkv * -(-G // 16), max_own, d, fast, sms)
         slots = T * nh * (p_parts + o_parts)
-        scratch = torch.empty(slots * (d + 2), dtype=torch.float32, device=q.device)
-        part_ml = scratch.data_ptr() + 4 * slots * d
+        before_ml = _floats_before_ml(slots, d)
+        scratch = torch.empty(before_ml + 2 * slots, dtype=torch.float32, device=q.device)
+        part_ml = scratch.data_ptr() + 4 * before_ml
         _COUNTER.value += 2 if tensor_cores and o_parts else 1         # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_prefix_attention")(
         _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(prefix_table),
@@ -2360,16 +2367,17 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     cluster = rows_cluster(R * nkv, max_context, fast, G) if G <= 16 else 0
     if cluster:
         n_parts, per = cluster, -(-(max_context or 1) // (16 * cluster)) * 16
-        floats = 0 if fast else R * nh * score_ld
+        if not fast:
+            scratch = torch.empty(R * nh * score_ld, dtype=torch.float32, device=q.device)
+            scores = scratch.data_ptr()
     else:
         n_parts, per = attention_parts(R * nkv * -(-G // 16), max_context, d, fast, num_sms(q.device))
-        floats = R * nh * (n_parts * (d + 2) + score_ld)
-        _COUNTER.value += 1                      # the parts, and the kernel that joins them
-    if floats:
-        scratch = torch.empty(floats, dtype=torch.float32, device=q.device)      # scores, and parts behind them
+        n_scores, before_ml = R * nh * score_ld, _floats_before_ml(R * nh * n_parts, d)
+        scratch = torch.empty(n_scores + before_ml + 2 * R * nh * n_parts, dtype=torch.float32, device=q.device)
         scores = scratch.data_ptr()
-        part_o = scores + 4 * R * nh * score_ld
-        part_ml = part_o + 4 * R * nh * n_parts * d
+        part_o = scores + 4 * n_scores
+        part_ml = part_o + 4 * before_ml
+        _COUNTER.value += 1                      # the parts, and the kernel that joins them
     _ok(_fn("attention_parts", "rg_weighed_attention")(
         _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)),
         _ptr(block_table), c_int(block_table.shape[1]), _ptr(positions), c_int(n_parts), c_int(per), c_int(R), c_int(nh), c_int(nkv), c_int(d),

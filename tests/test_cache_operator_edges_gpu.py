@@ -1,0 +1,84 @@
+"""Operators over the cache at the edges of their sizes: odd head sizes in parts, lists longer than a call's counts, many groups,
+and outputs held to bounds of their own size."""
+import pytest
+import torch
+
+from test_cache_operators_gpu import DEV, TYPES, U, Cache, i32, no_wait_gave_up, out_view, queries, same, softmax, weight_error  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def attended(q, K, V, scale, dtype):
+    """One row's softmax weights [nkv, G, n] and output [nkv, G, d] in 64 bits, and how far each number of the kernels' output may be
+    off: the weights by ``weight_error`` and, where the tensor cores multiply them (bfloat16, head sizes in 64s), by their rounding; sums of
+    n products in 32 bits; the output's own rounding.  A rounding to bfloat16, of 8 significant bits, is at most 2^-8 of a number
+    (1 + 2^-8 lies half way between 1 and 1 + 2^-7)."""
+    nkv, n = K.shape[0], K.shape[1]
+    nh, d = q.shape
+    p = softmax(q.double().view(nkv, nh // nkv, d) @ K.transpose(1, 2) * scale)
+    out = p @ V
+    if n == 0:
+        return p, out, torch.zeros_like(out)
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else U
+    rounded = half if dtype == torch.bfloat16 and d % 64 == 0 else 0.0
+    off = (p @ V.abs()) * (weight_error(q, K, n, scale, dtype) + (2 * n + 8) * U + rounded)
+    return p, out, off + half * (out.abs() + off)
+
+
+def run_weighed(lens, nh, nkv, d, page, dtype, seed):
+    from railgun_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    R, most, G, scale = len(lens), max(lens), nh // nkv, d ** -0.5
+    cache = Cache(lens, nkv, d, page, dtype, g)
+    q, out, slots = queries(R, nh, d, dtype, g), out_view(R, nh * d, dtype), torch.randperm(R, device=DEV, generator=g)
+    weights = torch.rand(R, nkv, most, device=DEV, generator=g)
+    before = weights.clone()
+    ops.weighed_attention(q, out, cache.kv, weights, slots.int(), cache.table, i32([n - 1 for n in lens]), nh, nkv, d, scale, max_context=most,
+                          decay=0.75)
+    for r, n in enumerate(lens):
+        K, V = cache.entries(r, n)
+        mine, s = q[r].reshape(nh, d), int(slots[r])
+        p, want, off = attended(mine, K, V, scale, dtype)
+        assert ((out[r].double().view(nkv, G, d) - want).abs() <= off).all(), r
+        if n:
+            w = p.sum(1)
+            w[:, :-1] += 0.75 * before[s, :, :n - 1].double()
+            assert ((weights[s, :, :n].double() - w).abs() <= w * (weight_error(mine, K, n, scale, dtype) + (G + 3) * U)).all(), r
+        assert torch.equal(weights[s, :, n:], before[s, :, n:])
+
+
+def run_prefix(groups, own, nh, nkv, d, page, dtype, seed):
+    """groups: (rows, prefix entries); rows behind them belong to none."""
+    from railgun_b200 import ops
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    T, G, scale, prefixes = len(own), nh // nkv, d ** -0.5, [p for _, p in groups]
+    cache = Cache(prefixes + own, nkv, d, page, dtype, g)
+    q, out, first, table, of = queries(T, nh, d, dtype, g), out_view(T, nh * d, dtype), 0, [], {}
+    for i, (n, p) in enumerate(groups):
+        table.append([first, n, p])
+        of.update({t: i for t in range(first, first + n)})
+        first += n
+    ops.prefix_attention(q, out, cache.kv, cache.table[:len(groups)].contiguous(), i32(table).view(-1, 3), cache.table[len(groups):].contiguous(),
+                         i32([n - 1 for n in own]), nh, nkv, d, scale, max_rows=max(n for n, _ in groups), max_prefix=max(prefixes),
+                         max_own=max(own))
+    lists = {}
+    for t in range(T):
+        i = of.get(t)
+        if i not in lists:
+            lists[i] = cache.entries(i or 0, prefixes[i] if i is not None else 0)
+        K, V = (torch.cat(x, 1) for x in zip(lists[i], cache.entries(len(groups) + t, own[t])))
+        _, want, off = attended(q[t].reshape(nh, d), K, V, scale, dtype)
+        assert ((out[t].double().view(nkv, G, d) - want).abs() <= off).all(), t
+
+
+# ---- odd numbers of rows, heads, parts and columns: parts whose (m, l) start behind an odd number of numbers -------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,nh,nkv,d,most", [(201, 3, 3, 5, 450), (601, 1, 1, 5, 500), (199, 3, 1, 33, 450), (593, 1, 1, 255, 300)])
+def test_odd_parts_of_weighed_attention(R, nh, nkv, d, most, dtype):
+    run_weighed([most - 7 * i % most for i in range(R)], nh, nkv, d, 16, dtype, R + d)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,nh,nkv,d,prefix,own", [(199, 3, 1, 33, 600, 100), (199, 3, 1, 33, 500, 100), (601, 1, 1, 5, 700, 40)])
+def test_odd_parts_of_prefix_attention(T, nh, nkv, d, prefix, own, dtype):
+    run_prefix([(T - 2, prefix)], [7 * i % (own + 1) for i in range(T)], nh, nkv, d, 16, dtype, T + d)
