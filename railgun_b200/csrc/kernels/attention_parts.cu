@@ -285,11 +285,12 @@ __global__ void __launch_bounds__(PG_THREADS) parts_general_kernel(const PartArg
         if (slot >= 0 && slot < b.n_slots) {
             float* to = b.weights + ((size_t)slot * a.nkv + s.kvh) * b.weights_ld;
             const int first = max(0, tile0 - prefix_tiles) * PG_K, last = min(s.e1, (tile1 - prefix_tiles) * PG_K);   // own entries of this block
+            const int newest = a.positions[s.row0];                   // behind what there is room for: none of them is new
             for (int e = first + tid; e < last; e += PG_THREADS) {
                 const float* sc = a.scores + ((size_t)s.row0 * a.nh + h0) * a.score_ld + e;
                 float sum = 0.f;
                 for (int i = 0; i < s.nq; ++i) sum += exp2f(sc[(size_t)i * a.score_ld] - row_ml[i][0]) * row_ml[i][1];
-                to[e] = (e == s.e1 - 1 ? 0.f : b.decay * to[e]) + sum;
+                to[e] = (e == newest ? 0.f : b.decay * to[e]) + sum;
             }
         }
         cluster.sync();                                             // nobody leaves while its results are being read
@@ -702,10 +703,11 @@ rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, co
         const int slot = b.slots[t];
         if (slot >= 0 && slot < b.n_slots) {
             float* to = b.weights + ((size_t)slot * a.nkv + kvh) * b.weights_ld;
+            const int newest = a.positions[t];                        // behind what there is room for: none of them is new
             for (int i = threadIdx.x; i < n_runs * 16; i += PM_THREADS) {
                 const int e = first * 16 + i;
                 if (e >= own) break;
-                const float before = e == own - 1 ? 0.f : b.decay * to[e];
+                const float before = e == newest ? 0.f : b.decay * to[e];
                 float sum = 0.f;
                 for (int r = 0; r < nq; ++r) sum += ex2(scores[r * ld + i] - row_ml[r][0]) * row_ml[r][1];
                 to[e] = before + sum;
@@ -838,7 +840,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const PartArgs a, in
 }
 
 // The first `joins` blocks join rows and heads; the others add up the weights of 512 entries of a row and kv head, four a thread:
-//   w[e] = decay w[e] + sum_h 2^(s_h(e) - M_h) / L_h,   the newest entry's w not read
+//   w[e] = decay w[e] + sum_h 2^(s_h(e) - M_h) / L_h,   w[positions[t]], the newest entry's, not read
 #define WEIGH_CHUNK (4 * JOIN_THREADS)
 #define WEIGH_HEADS 64
 template <typename A>
@@ -851,14 +853,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) weigh_kernel(const PartArgs a, i
     if (b < joins) { join_block(a, b, heads, out, out_ld); return; }
     b -= joins;
     const int chunk = b % chunks, kvh = b / chunks % a.nkv, t = b / chunks / a.nkv, group = a.nh / a.nkv;
-    const int n = own_entries(a, t), e = chunk * WEIGH_CHUNK + 4 * threadIdx.x, slot = slots[t];
+    const int n = own_entries(a, t), newest = a.positions[t], e = chunk * WEIGH_CHUNK + 4 * threadIdx.x, slot = slots[t];
     if (chunk * WEIGH_CHUNK >= n || slot < 0 || slot >= n_slots) return;
     __shared__ float sM[WEIGH_HEADS], sI[WEIGH_HEADS];
     const int n_own = own_parts_of(a, t), warp = threadIdx.x >> 5;
     float* w = weights + ((size_t)slot * a.nkv + kvh) * weights_ld;
     float before[4], sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) before[j] = e + j < n - 1 ? decay * w[e + j] : 0.f;
+    for (int j = 0; j < 4; ++j) before[j] = e + j < n && e + j != newest ? decay * w[e + j] : 0.f;
     for (int g0 = 0; g0 < group; g0 += WEIGH_HEADS) {                // heads of a kv head, so many at a time
         const int some = min(group - g0, WEIGH_HEADS);
         __syncthreads();
@@ -989,9 +991,8 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
 // [T, nh, prefix_parts + own_parts, d] on a 16-byte boundary and part_ml [.., 2] on one of 8.  tensor_cores: 1 the prefixes by
-// prefix_tc_kernel, 2 the same with two
-// parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.  cluster: not 0, rows by clusters of so many
-// blocks, which leave no parts.
+// prefix_tc_kernel, 2 the same with two parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.  cluster:
+// not 0, rows by clusters of so many blocks, which leave no parts.
 extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                    const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
                                    int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,

@@ -2353,7 +2353,7 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     max_context] float32, request r's at ``slots[r]`` (negative: a row whose weights nobody keeps): entry e's becomes
     decay * weight + the sum, over the query heads of each kv head, of the softmax weight that e got from them.  The entry
     ``positions[r]`` is new: its earlier weight is not read.  ``max_context``: the most entries a row may see; entries beyond
-    are not seen.  All sums are 32-bit and have one order."""
+    are not seen (where the new one is among them, no weight is dropped).  All sums are 32-bit and have one order."""
     R, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
     _check_ints(block_table, "block_table", R, table=True)
     _check_ints(positions, "positions", R)

@@ -82,3 +82,37 @@ def test_odd_parts_of_weighed_attention(R, nh, nkv, d, most, dtype):
 @pytest.mark.parametrize("T,nh,nkv,d,prefix,own", [(199, 3, 1, 33, 600, 100), (199, 3, 1, 33, 500, 100), (601, 1, 1, 5, 700, 40)])
 def test_odd_parts_of_prefix_attention(T, nh, nkv, d, prefix, own, dtype):
     run_prefix([(T - 2, prefix)], [7 * i % (own + 1) for i in range(T)], nh, nkv, d, 16, dtype, T + d)
+
+
+# ---- lists longer than a call's counts ---------------------------------------------------------------------------------------
+# which kernels: few and many rows in 32-bit, few and many in bfloat16, more heads on one than a cluster's block takes
+WEIGHED = [(torch.float32, 8, 2, 64, 3, 90), (torch.float32, 8, 2, 64, 3, 5000), (torch.bfloat16, 8, 2, 64, 2, 700),
+           (torch.bfloat16, 8, 2, 128, 40, 2000), (torch.bfloat16, 40, 1, 64, 2, 300), (torch.float32, 20, 1, 24, 2, 130)]
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,d,R,most", WEIGHED)
+@pytest.mark.parametrize("cut", ["max_context", "table"])
+def test_an_entry_is_new_by_its_position(dtype, nh, nkv, d, R, most, cut):
+    """The last entry that a call has room for is not new where the row's position lies behind it: its weight goes on."""
+    from railgun_b200 import ops
+    page, G, scale, decay = 16, nh // nkv, d ** -0.5, 0.5
+    most = -(-most // page) * page                                    # whole pages: a table of so many has room for no more
+    g = torch.Generator(device=DEV).manual_seed(most)
+    cache = Cache([most + page] * R, nkv, d, page, dtype, g)
+    table = cache.table if cut == "max_context" else cache.table[:, :most // page].contiguous()
+    q, out = queries(R, nh, d, dtype, g), out_view(R, nh * d, dtype)
+    positions = [most - 1 + (1, 0, 2)[r % 3] for r in range(R)]       # the last one that is seen, or behind it
+    weights = 1.0 + torch.rand(R, nkv, most + page, device=DEV, generator=g)
+    before = weights.clone()
+    ops.weighed_attention(q, out, cache.kv, weights, i32(list(range(R))), table, i32(positions), nh, nkv, d, scale,
+                          max_context=most if cut == "max_context" else most + page, decay=decay)
+    for r, at in enumerate(positions):
+        K, V = cache.entries(r, most)
+        mine = q[r].reshape(nh, d)
+        p, want, off = attended(mine, K, V, scale, dtype)
+        assert ((out[r].double().view(nkv, G, d) - want).abs() <= off).all(), r
+        w = p.sum(1) + decay * before[r, :, :most].double()
+        if at == most - 1:
+            w[:, -1] = p.sum(1)[:, -1]
+        assert ((weights[r, :, :most].double() - w).abs() <= w * (weight_error(mine, K, most, scale, dtype) + (G + 3) * U)).all(), r
+        assert torch.equal(weights[r, :, most:], before[r, :, most:])
