@@ -992,21 +992,25 @@ static bool fill_part_args(PartArgs& a, const void* q, int q_stride, const void*
 // Rows of single tokens behind shared prefixes: see attention_parts.cuh for the arguments.  Scratch: part_o
 // [T, nh, prefix_parts + own_parts, d] on a 16-byte boundary and part_ml [.., 2] on one of 8.  tensor_cores: 1 the prefixes by
 // prefix_tc_kernel, 2 the same with two parts a block (groups of up to 128 queries a kv head), 0 everything in one launch.  cluster:
-// not 0, rows by clusters of so many blocks, which leave no parts.
+// not 0, rows by clusters of so many blocks, which leave no parts.  max_prefix, max_own: the most entries of either list that are seen.
 extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                    const int* prefix_table, int prefix_blocks, const int* groups, int n_groups, int max_rows,
                                    int prefix_parts, int prefix_per, const int* block_table, int max_blocks, const int* positions,
                                    int own_parts, int own_per, int T, int nh, int nkv, int d, int page_size, float scale,
-                                   float* part_o, float* part_ml, int tensor_cores, int cluster, int* err, void* stream) {
+                                   float* part_o, float* part_ml, int max_prefix, int max_own, int tensor_cores, int cluster,
+                                   int* err, void* stream) {
     if (T <= 0) return 0;
     PartArgs a;
     if (!fill_part_args(a, q, q_stride, kv, block_table, max_blocks, positions, T, nh, nkv, d, page_size, scale, part_o, part_ml,
-                        own_parts, own_per) || n_groups < 0 || prefix_parts < 0 || prefix_per < 1 || out_ld < nh * d)
+                        own_parts, own_per) || n_groups < 0 || prefix_parts < 0 || prefix_per < 1 || out_ld < nh * d || max_prefix < 0 ||
+        max_own < 0)
         return RG_ERR_UNSUPPORTED;
     const int group = nh / nkv;
     a.prefix_table = prefix_table; a.prefix_blocks = prefix_blocks; a.groups = groups; a.n_groups = n_groups; a.max_rows = max_rows;
     a.prefix_parts = prefix_parts; a.prefix_per = prefix_per;
-    a.prefix_limit = (int)min(0x7fffffffll, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
+    // parts are whole tiles: where they end is behind what the call says may be seen
+    a.prefix_limit = (int)min((long long)max_prefix, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
+    a.own_limit = min(a.own_limit, max_own);
     if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
     if (cluster) {

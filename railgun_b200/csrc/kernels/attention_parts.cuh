@@ -24,7 +24,7 @@ struct PartArgs {
     int q_stride, max_blocks, prefix_blocks, n_groups;
     int prefix_parts, prefix_per, own_parts, own_per;   // parts of either list and entries a part
     int prefix_tiles, own_tiles;                        // query tiles of a group, of a row's kv head
-    int prefix_limit, own_limit;                        // the most entries that tables, parts and scratch have room for
+    int prefix_limit, own_limit;                        // the most entries that the call says, and that tables, parts and scratch have room for
     int max_rows;                                       // rows of a group that a launch is sized for
     int T, nh, nkv, d, page_size, page_shift;           // page_shift: log2 of the page size, or -1
     float scale_log2;

@@ -2342,7 +2342,7 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
         _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(prefix_table),
         c_int(prefix_table.shape[1]), _ptr(groups), c_int(n_groups), c_int(max_rows), c_int(p_parts), c_int(p_per), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(positions), c_int(o_parts), c_int(o_per), c_int(T), c_int(nh), c_int(nkv), c_int(d),
-        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml),
+        c_int(page_size), c_float(scale), _ptr(scratch), c_void_p(part_ml), c_int(max_prefix), c_int(max_own),
         c_int(tensor_cores), c_int(cluster), _ptr(_tc_error_flag(q.device)), _stream()), "prefix_attention")
 
 

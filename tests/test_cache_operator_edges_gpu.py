@@ -116,3 +116,31 @@ def test_an_entry_is_new_by_its_position(dtype, nh, nkv, d, R, most, cut):
             w[:, -1] = p.sum(1)[:, -1]
         assert ((weights[r, :, :most].double() - w).abs() <= w * (weight_error(mine, K, most, scale, dtype) + (G + 3) * U)).all(), r
         assert torch.equal(weights[r, :, most:], before[r, :, most:])
+
+
+# few rows and many in 32-bit and bfloat16; groups of many rows, whose prefixes the tensor cores take, with one or two parts a block
+PREFIXED = [(torch.float32, 4, 2, 64, 3), (torch.float32, 8, 2, 32, 150), (torch.bfloat16, 8, 2, 64, 4), (torch.bfloat16, 20, 1, 256, 2),
+            (torch.bfloat16, 8, 2, 192, 170), (torch.bfloat16, 32, 8, 128, 150), (torch.bfloat16, 32, 8, 64, 60), (torch.bfloat16, 8, 2, 128, 40)]
+
+
+@pytest.mark.parametrize("dtype,nh,nkv,d,T", PREFIXED)
+@pytest.mark.parametrize("max_prefix,max_own", [(0, 0), (0, 70), (130, 0), (1000, 100), (300, 333), (1, 1), (2500, 17)])
+def test_entries_beyond_what_a_call_says_are_not_seen(max_prefix, max_own, dtype, nh, nkv, d, T):
+    """Prefixes and own lists that are longer than a call says: the results are those of lists that end there."""
+    from railgun_b200 import ops
+    page, more = 16, 150
+    g = torch.Generator(device=DEV).manual_seed(max_prefix + T)
+    cache = Cache([max_prefix + more] * 2 + [max_own + more] * T, nkv, d, page, dtype, g)
+    q, tables, own_table = queries(T, nh, d, dtype, g), cache.table[:2].contiguous(), cache.table[2:].contiguous()
+    first = T // 2
+
+    def run(prefix, own):
+        out = out_view(T, nh * d, dtype)
+        ops.prefix_attention(q, out, cache.kv, tables, i32([[0, first, prefix[0]], [first, T - first, prefix[1]]]), own_table, i32(own), nh, nkv,
+                             d, d ** -0.5, max_rows=T - first, max_prefix=max_prefix, max_own=max_own)
+        return out
+    lens = [(max_own + more - 1) * (r % 4) // 3 for r in range(T)]       # positions, some behind what the call says
+    over = run([max_prefix + more, max_prefix + 1], lens)
+    assert torch.equal(over, run([max_prefix, max_prefix], [min(n, max_own - 1) for n in lens]))
+    if max_prefix + max_own == 0:
+        assert not over.any()
