@@ -165,9 +165,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 4 : 1) evict_kernel(
     // No early start for the kernel behind this one: attention kernels ask for cached keys ahead of their own wait.
     pdl_wait();
     const int row = blockIdx.x / C, r = row / a.nkv, h = row % a.nkv;
-    const int slot = a.slots[r], n = min(a.lens[r], a.limit), k = min(n, max(0, a.keep[r])), newest = a.positions[r];
-    const bool alone = slot < 0 || slot >= a.n_slots || n <= 0;      // the same for the whole cluster
-    if (h == 0 && rank == 0 && tid == 0) a.new_lens[r] = alone ? a.lens[r] : k;
+    const int slot = a.slots[r], n = a.lens[r], k = min(n, max(0, a.keep[r])), newest = a.positions[r];
+    // Left alone, the same for the whole cluster; also a request with more entries than there is room for: its newest ones would go
+    // without having been looked at.
+    const bool alone = slot < 0 || slot >= a.n_slots || n <= 0 || n > a.limit;
+    if (h == 0 && rank == 0 && tid == 0) a.new_lens[r] = alone ? n : k;
     if (alone) {                                                      // the kernel that moves goes by the number of moves
         if constexpr (!FUSED)
             if (rank == 0 && tid == 0) a.moves[(size_t)row * ev_list(a.limit)] = 0;

@@ -2445,8 +2445,10 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     infinitely heavy.  K and V rows behind the new length move, in place, into entries before it that got free, the i-th into
     the i-th, so what stays is entries 0 .. new length - 1 and no more rows move than have to; the pages behind may be
     given back (``PageAllocator.shrink``).  Weights and places of the entries that stay go to ``weights_out`` and ``places_out``: the same
-    buffers, or others of these shapes that share no memory with them; what lies behind the new length there is left alone.  Returns the new lengths [R] int32, min(lens, keep).  Requests with a
-    negative slot are left alone."""
+    buffers, or others of these shapes that share no memory with them; what lies behind the new length there is left alone.
+    ``max_context``: the most entries a request may have (``lens`` stays on the device).  Returns the new lengths [R] int32: min(lens,
+    keep), or lens for requests that are left alone: those with a negative slot, and those with more entries than ``max_context`` or than
+    their table has room for, of which no choice could be made (other buffers get nothing of them)."""
     _dtype_code(kv_cache)
     _check(kv_cache, "kv_cache")
     _check_ints(slots, "slots", None)
@@ -2465,7 +2467,7 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
         if t.shape != weights.shape:
             raise KernelError(f"{name} is {tuple(t.shape)}, weights {tuple(weights.shape)}")
     new_lens = torch.empty(R, dtype=torch.int32, device=kv_cache.device)
-    if max_context == 0:
+    if max_context == 0:                         # every request has none, or is left alone
         return new_lens.copy_(lens)
     # a block holds up to 16,384 keys, a cluster of up to eight more
     cluster = 1

@@ -3,7 +3,8 @@ and outputs held to bounds of their own size."""
 import pytest
 import torch
 
-from test_cache_operators_gpu import DEV, TYPES, U, Cache, i32, no_wait_gave_up, out_view, queries, same, softmax, weight_error  # noqa: F401
+from test_cache_operators_gpu import (DEV, TYPES, U, Cache, i32, no_wait_gave_up, out_view, plain_evict, queries, same, softmax,  # noqa: F401
+                                      weight_error)
 
 pytestmark = pytest.mark.gpu
 
@@ -144,3 +145,33 @@ def test_entries_beyond_what_a_call_says_are_not_seen(max_prefix, max_own, dtype
     assert torch.equal(over, run([max_prefix, max_prefix], [min(n, max_own - 1) for n in lens]))
     if max_prefix + max_own == 0:
         assert not over.any()
+
+
+@pytest.mark.parametrize("most", [0, 1, 90, 2048, 2500, 20000])
+def test_evict_leaves_longer_requests_alone(most):
+    """A request with more entries than a call has room for: choosing among some of them could drop those that are protected."""
+    from railgun_b200 import ops
+    nkv, d, page = 2, 64, 16
+    lens = [most, most + 1, most + 40, max(0, most - 1)]
+    keep = [max(1, n // 3) for n in lens]
+    g = torch.Generator(device=DEV).manual_seed(most)
+    cache = Cache(lens, nkv, d, page, torch.bfloat16, g, width=1)
+    weights = torch.empty(4, nkv, most + 40, device=DEV).exponential_(generator=g)
+    places = torch.arange(most + 40, device=DEV, dtype=torch.int32).expand(4, nkv, most + 40).contiguous()
+    want = plain_evict(cache, weights, places, [0, -1, -1, 3], lens, keep, [n - 1 for n in lens], 2, 5)
+    got = weights.clone(), places.clone()
+    new = ops.evict_entries(cache.kv, weights, places, *got, i32([0, 1, 2, 3]), cache.table, i32(lens), i32(keep), i32([n - 1 for n in lens]),
+                            nkv, d, 2, 5, max_context=most)
+    assert new.tolist() == [min(most, keep[0]), most + 1, most + 40, min(lens[3], keep[3])]
+    assert same(got[0], want[1]) and torch.equal(got[1], want[2]) and same(cache.kv, want[0])
+    # the table has room for fewer entries than the call
+    if most >= 90:
+        narrow = cache.table[:, :2].contiguous()
+        kv, w, p = cache.kv.clone(), weights.clone(), places.clone()
+        new = ops.evict_entries(cache.kv, weights, places, weights, places, i32([0, 1, 2, 3]), narrow, i32([33, 32, most, 34]), i32([8] * 4),
+                                i32([32, 31, most - 1, 33]), nkv, d, 2, 5, max_context=most)
+        assert new.tolist() == [33, 8, most, 34]
+        for r in (0, 2, 3):
+            assert torch.equal(weights[r], w[r]) and torch.equal(places[r], p[r])
+            mine = cache.table[r, :-(-lens[r] // page)].long()
+            assert same(cache.kv[mine], kv[mine])
