@@ -175,3 +175,13 @@ def test_evict_leaves_longer_requests_alone(most):
             assert torch.equal(weights[r], w[r]) and torch.equal(places[r], p[r])
             mine = cache.table[r, :-(-lens[r] // page)].long()
             assert same(cache.kv[mine], kv[mine])
+
+
+# ---- many groups ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_groups,nh,nkv,d,prefix,own", [(48, 8, 2, 64, 300, 40), (70, 4, 2, 32, 90, 20), (33, 32, 8, 128, 700, 60), (130, 2, 1, 64, 40, 5)])
+def test_many_groups(n_groups, nh, nkv, d, prefix, own, dtype):
+    """Parallel samples: dozens of groups of a few rows, some without rows or entries, rows of no group behind them."""
+    groups = [((i * 5 + 3) % 9, 0 if i % 11 == 4 else prefix - 7 * i % prefix) for i in range(n_groups)]
+    T = sum(n for n, _ in groups) + 3
+    run_prefix(groups, [3 * i % (own + 1) for i in range(T)], nh, nkv, d, 16, dtype, n_groups + d)
