@@ -1011,7 +1011,7 @@ extern "C" int rg_prefix_attention(const void* q, int q_stride, void* out, int o
     // parts are whole tiles: where they end is behind what the call says may be seen
     a.prefix_limit = (int)min((long long)max_prefix, min((long long)prefix_blocks * page_size, (long long)prefix_parts * prefix_per));
     a.own_limit = min(a.own_limit, max_own);
-    if ((long long)max_rows * group > 0x7fffffffll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+    if ((long long)max_rows * group > 0x7fffff00ll || (long long)T * nh > 0x7fffffffll) return RG_ERR_UNSUPPORTED;   // rounded up to tiles below
     a.own_tiles = (group + PG_Q - 1) / PG_Q;
     if (cluster) {
         const RowsArgs b = {out, nullptr, nullptr, 0, out_ld, 0, 0, 0.f};

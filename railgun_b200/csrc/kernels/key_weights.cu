@@ -797,7 +797,7 @@ extern "C" int rg_prompt_key_weights(const void* q, int q_stride, const void* kv
                                      int entry_parts, float* part_w, int tensor_cores, int sms, int* err, void* stream) {
     if (R <= 0 || T <= 0 || max_rows <= 0 || max_context <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_context > weights_ld || R > 65535 || nkv > 65535 ||
-        (long long)max_rows * (nh / nkv) > 0x7fffffffll || row_parts < 1 || entry_parts < 1)
+        (long long)max_rows * (nh / nkv) > 0x7fffff00ll || max_context > 0x7fffff00 || row_parts < 1 || entry_parts < 1)
         return RG_ERR_UNSUPPORTED;
     const WeightArgs a = {q, kv, block_table, cu_rows, starts, fresh, slots, weights, z, weights_ld, q_stride, max_blocks, n_slots, T, R,
                           nh, nkv, d, page_size, (int)min((long long)max_context, (long long)max_blocks * page_size),

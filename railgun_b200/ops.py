@@ -2314,8 +2314,8 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     _check_ints(block_table, "block_table", T, table=True)
     _check_ints(positions, "positions", T)
     _check_out_view(out, T, nh * d, q.dtype, "prefix_attention")
-    if min(max_rows, max_prefix, max_own) < 0:
-        raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts")
+    if min(max_rows, max_prefix, max_own) < 0 or max(max_rows, max_prefix, max_own) >= 1 << 31:
+        raise KernelError("prefix_attention: max_rows, max_prefix and max_own are counts below 2^31")
     n_groups, G = groups.shape[0], nh // nkv
     longest, tensor_cores, scratch, part_ml = max_prefix if n_groups and max_rows else 0, 0, None, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
@@ -2359,8 +2359,8 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     _check_ints(positions, "positions", R)
     _check_ints(slots, "slots", R)
     _check_out_view(out, R, nh * d, q.dtype, "weighed_attention")
-    if max_context < 0:
-        raise KernelError("weighed_attention: max_context is a count")
+    if not 0 <= max_context < 1 << 31:
+        raise KernelError("weighed_attention: max_context is a count below 2^31")
     n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
     G, score_ld, scores, part_o, part_ml = nh // nkv, -(-max_context // 64) * 64, 0, 0, 0
     fast = q.dtype == torch.bfloat16 and d % 64 == 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
@@ -2412,8 +2412,8 @@ def prompt_key_weights(q, kv_cache, weights, slots, block_table, cu_rows, starts
     _check_ints(cu_rows, "cu_rows", R + 1)
     _check_ints(starts, "starts", R)
     _check_ints(fresh, "fresh", R)
-    if min(max_rows, max_context) < 0:
-        raise KernelError("prompt_key_weights: max_rows and max_context are counts")
+    if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
+        raise KernelError("prompt_key_weights: max_rows and max_context are counts below 2^31")
     n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
     G, n_z = nh // nkv, -(-T * nh // 4) * 4
     tensor_cores = q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
@@ -2457,8 +2457,8 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     _check_ints(block_table, "block_table", R, table=True)
     for t, name in ((lens, "lens"), (keep, "keep"), (positions, "positions")):
         _check_ints(t, name, R)
-    if max_context < 0 or protect_first < 0 or protect_last < 0:
-        raise KernelError("evict_entries: max_context, protect_first and protect_last are counts")
+    if min(max_context, protect_first, protect_last) < 0 or max(max_context, protect_first, protect_last) >= 1 << 31:
+        raise KernelError("evict_entries: max_context, protect_first and protect_last are counts below 2^31")
     n_slots, ld = _check_entry_weights(weights, "weights", nkv, max_context)
     for t, name, dtype in ((places, "places", torch.int32), (weights_out, "weights_out", torch.float32), (places_out, "places_out", torch.int32)):
         if _fast is not None and _fast.shaped(t, dtype, n_slots, nkv, ld):

@@ -89,3 +89,28 @@ def test_parts_lie_where_their_loads_can_read_them(calls, T, nh, nkv, d, dtype):
                 assert scores % 16 == 0 and part_o % 16 == 0 and part_ml % 8 == 0
                 assert parts % (T * nh) == 0 and part_o + 4 * parts * d <= part_ml and scores + 4 * T * nh * own <= part_o
     assert seen or T == 2
+
+
+@pytest.mark.parametrize("n", [-1, 1 << 31, 1 << 32, (1 << 32) + 5, 1 << 63])
+@pytest.mark.parametrize("operator,name", [(o, n) for o, names in dict(
+    prefix="max_rows max_prefix max_own", weigh="max_context", prompt="max_rows max_context", evict="max_context protect_first protect_last").items()
+    for n in names.split()])
+def test_counts_that_no_launcher_can_take(calls, operator, name, n):
+    """A launcher's counts are 32-bit: a larger one would arrive as another number, and the call do nothing, or something else."""
+    q, out, kv, table = tensors(3, 2, 1, 16, 8, torch.float32, 3, 4)
+    weights, places = torch.zeros(3, 1, 32), torch.zeros(3, 1, 32, dtype=torch.int32)
+    ints = torch.zeros(3, dtype=torch.int32)
+    if operator == "prefix":
+        f, args, counts = ops.prefix_attention, (q, out, kv, table[:0], torch.zeros(0, 3, dtype=torch.int32), table, ints, 2, 1, 16, 0.25), dict(
+            max_rows=0, max_prefix=0, max_own=32)
+    elif operator == "weigh":
+        f, args, counts = ops.weighed_attention, (q, out, kv, weights, ints, table, ints, 2, 1, 16, 0.25), dict(max_context=32)
+    elif operator == "prompt":
+        f, args, counts = ops.prompt_key_weights, (q, kv, weights, ints, table, torch.zeros(4, dtype=torch.int32), ints, ints, 2, 1, 16, 0.25), dict(
+            max_rows=1, max_context=32)
+    else:
+        f, args, counts = ops.evict_entries, (kv, weights, places, weights, places, ints, table, ints, ints, ints, 1, 16), dict(
+            protect_first=1, protect_last=1, max_context=32)
+    calls(f, *args, **counts)                                          # as it is, it gets to its launcher
+    with pytest.raises(ops.KernelError):
+        f(*args, **{**counts, name: n})
