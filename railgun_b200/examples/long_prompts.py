@@ -146,7 +146,10 @@ class LongPrompts:
             return out
 
         batch.attend = run
-        return ops.argmax(self.forward(batch)).tolist()
+        after = ops.argmax(self.forward(batch)).tolist()
+        for r, e in zip(requests, entries):
+            self.alloc.commit(r, e + 1)
+        return after
 
     # ---- many questions behind one prompt ---------------------------------------------------------------------------
     def answer(self, prompt: Prompt, questions, max_new_tokens: int) -> list:
