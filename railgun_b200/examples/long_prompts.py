@@ -82,6 +82,10 @@ class LongPrompts:
         width = max([1, *(len(t) for t in tables)])
         return self.ints([[*t.tolist(), *[0] * (width - len(t))] for t in tables])
 
+    def check_end(self, tokens: int) -> None:
+        if tokens > self.model.spec.max_position:
+            raise ValueError(f"a text of {tokens} tokens; the model ends at {self.model.spec.max_position}")
+
     def forward(self, batch) -> torch.Tensor:
         logits = self.model.forward(batch, self)
         ops.tc_gemm_check()
@@ -154,14 +158,15 @@ class LongPrompts:
     # ---- many questions behind one prompt ---------------------------------------------------------------------------
     def answer(self, prompt: Prompt, questions, max_new_tokens: int) -> list:
         """Greedy answers to the questions (lists of tokens), all behind ``prompt``."""
-        T = len(questions)
+        T, longest = len(questions), max(len(q) for q in questions) + max_new_tokens
+        self.check_end(prompt.tokens + longest - 1)
         requests = [self.next_request + i for i in range(T)]
         self.next_request += T
         for r in requests:
             self.alloc.add_request(r)
         groups, prefix = self.ints([[0, T, prompt.entries]]), self.table_of([prompt.request])
         answers = [[] for _ in questions]
-        feed, longest = [q[0] for q in questions], max(len(q) for q in questions) + max_new_tokens
+        feed = [q[0] for q in questions]
         for i in range(longest - 1):
             def attend(part, q, out, batch, cache):
                 ops.prefix_attention(q, out, cache.kv, prefix, groups, batch.block_table[0], batch.start_pos, part.nh, part.nkv, part.d,
@@ -178,11 +183,14 @@ class LongPrompts:
     # ---- one prompt goes on within its budget --------------------------------------------------------------------------
     def go_on(self, prompt: Prompt, max_new_tokens: int, decay: float = 1.0) -> list:
         """Greedy tokens behind ``prompt``; a page above the budget the lightest entries go."""
-        out = []
+        self.check_end(prompt.tokens + max_new_tokens)
+        most, out = prompt.entries + max_new_tokens, []
+        if self.budget is not None:
+            most = min(most, self.budget + self.page_size)
+        if most > self.max_entries:
+            raise ValueError(f"{most} entries; there is room for {self.max_entries}")
         for _ in range(max_new_tokens):
             token, entry = prompt.next_token, prompt.entries
-            if entry >= self.max_entries:
-                raise ValueError(f"there is room for {self.max_entries} entries")
             out.append(token)
             for places in self.places:
                 places[prompt.slot, :, entry] = prompt.tokens

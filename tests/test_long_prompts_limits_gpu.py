@@ -27,3 +27,38 @@ def test_the_allocator_knows_what_is_in_the_cache():
         lp.go_on(prompt, n)
         assert lp.alloc.num_computed(prompt.request) == prompt.entries < 30 + 16
     lp.alloc.check()
+
+
+def test_positions_end_where_the_model_ends():
+    """Behind its last position a model has no rotation: nothing is computed there, and nothing has changed."""
+    most = TINY["A"][0]["max_position_embeddings"]
+    first, question = text("A", most - 6, 3)
+    lp = long_prompts("A")
+    prompt = lp.read(first)
+    before = (prompt.tokens, prompt.entries, prompt.next_token, lp.alloc.free_pages())
+    with pytest.raises(ValueError):
+        lp.go_on(prompt, 7)
+    with pytest.raises(ValueError):
+        lp.answer(prompt, [question[:1], question], 5)
+    assert (prompt.tokens, prompt.entries, prompt.next_token, lp.alloc.free_pages()) == before
+    assert [len(a) for a in lp.answer(prompt, [question[:1], question], 4)] == [4, 4]
+    tokens = lp.go_on(prompt, 6)
+    assert len(tokens) == 6 and prompt.tokens == most
+    with pytest.raises(ValueError):
+        lp.go_on(prompt, 1)
+
+
+def test_there_is_room_for_so_many_entries():
+    lp = long_prompts(max_entries=50)
+    prompt = lp.read(text("C", 40)[0])
+    with pytest.raises(ValueError):
+        lp.go_on(prompt, 11)
+    assert prompt.entries == prompt.tokens == 40                        # refused before anything was done
+    assert len(lp.go_on(prompt, 10)) == 10
+    lp = long_prompts(max_entries=46, budget=30, protect_last=4)         # a page above the budget is all that it takes
+    prompt = lp.read(text("C", 46)[0])
+    assert len(lp.go_on(prompt, 60)) == 60
+    lp = long_prompts(max_entries=45, budget=30, protect_last=4)
+    prompt = lp.read(text("C", 45)[0])
+    with pytest.raises(ValueError):
+        lp.go_on(prompt, 60)
