@@ -54,6 +54,8 @@ class LongPrompts:
             spec = arch_spec(config)
             layers = tuple(dataclasses.replace(s, mixer=dataclasses.replace(s.mixer, kind="long_prompt_attention")) for s in spec.layers)
             return dataclasses.replace(spec, layers=layers)
+        if (budget is not None and budget < 1) or min(watch, max_entries) < 1 or min(protect_first, protect_last) < 0:
+            raise ValueError("at least one entry of budget and of room, one row that is watched, and no fewer protected entries than none")
         from ..config.registry import load_config
         arch_spec = load_config(model_dir)[0].model_spec
         self.device, self.dtype = torch.device(device), parse_dtype(dtype)
@@ -158,6 +160,10 @@ class LongPrompts:
     # ---- many questions behind one prompt ---------------------------------------------------------------------------
     def answer(self, prompt: Prompt, questions, max_new_tokens: int) -> list:
         """Greedy answers to the questions (lists of tokens), all behind ``prompt``."""
+        if not questions:
+            return []
+        if any(len(q) < 1 or min(q) < 0 or max(q) >= self.model.vocab_size for q in questions):
+            raise ValueError(f"a question is one token or more, each in [0, {self.model.vocab_size})")
         T, longest = len(questions), max(len(q) for q in questions) + max_new_tokens
         self.check_end(prompt.tokens + longest - 1)
         requests = [self.next_request + i for i in range(T)]

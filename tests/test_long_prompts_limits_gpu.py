@@ -62,3 +62,21 @@ def test_there_is_room_for_so_many_entries():
     prompt = lp.read(text("C", 45)[0])
     with pytest.raises(ValueError):
         lp.go_on(prompt, 60)
+
+
+@pytest.mark.parametrize("bad", [[], [-1], [3, TINY["C"][0]["vocab_size"]], [1 << 40]])
+def test_questions_are_tokens_of_the_model(bad):
+    """A token that the model does not have would be a row of zeros, and answered."""
+    lp = long_prompts()
+    prompt = lp.read(text("C", 20)[0])
+    free = lp.alloc.free_pages()
+    with pytest.raises(ValueError):
+        lp.answer(prompt, [[1, 2], bad], 3)
+    assert lp.alloc.free_pages() == free
+    assert lp.answer(prompt, [], 3) == []
+
+
+@pytest.mark.parametrize("bad", [dict(budget=0), dict(budget=-3), dict(watch=0), dict(protect_first=-1), dict(protect_last=-1), dict(max_entries=0)])
+def test_what_is_asked_of_the_budget(bad):
+    with pytest.raises(ValueError):
+        long_prompts(**bad)
