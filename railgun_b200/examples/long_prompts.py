@@ -111,12 +111,16 @@ class LongPrompts:
             return out
 
         batch.attend = attend
-        prompt = Prompt(request, self.alloc.slot(request), n, n, int(ops.argmax(self.forward(batch))[0]))
-        self.alloc.commit(request, n)
-        for places in self.places:
-            places[prompt.slot, :, :n] = torch.arange(n, dtype=torch.int32, device=self.device)
-        if self.budget is not None and n > self.budget:
-            self.evict([prompt])
+        try:
+            prompt = Prompt(request, self.alloc.slot(request), n, n, int(ops.argmax(self.forward(batch))[0]))
+            self.alloc.commit(request, n)
+            for places in self.places:
+                places[prompt.slot, :, :n] = torch.arange(n, dtype=torch.int32, device=self.device)
+            if self.budget is not None and n > self.budget:
+                self.evict([prompt])
+        except BaseException:
+            self.alloc.release(request)
+            raise
         return prompt
 
     def evict(self, prompts) -> None:
@@ -168,22 +172,26 @@ class LongPrompts:
         self.check_end(prompt.tokens + longest - 1)
         requests = [self.next_request + i for i in range(T)]
         self.next_request += T
-        for r in requests:
-            self.alloc.add_request(r)
-        groups, prefix = self.ints([[0, T, prompt.entries]]), self.table_of([prompt.request])
-        answers = [[] for _ in questions]
-        feed = [q[0] for q in questions]
-        for i in range(longest - 1):
-            def attend(part, q, out, batch, cache):
-                ops.prefix_attention(q, out, cache.kv, prefix, groups, batch.block_table[0], batch.start_pos, part.nh, part.nkv, part.d,
-                                     part.scale, max_rows=T, max_prefix=prompt.entries, max_own=i + 1)
-            after = self.step(requests, feed, [prompt.tokens + i] * T, [i] * T, attend)
-            for t, q in enumerate(questions):
-                if i + 1 >= len(q) and len(answers[t]) < max_new_tokens:
-                    answers[t].append(after[t])
-                feed[t] = q[i + 1] if i + 1 < len(q) else after[t]
-        for r in requests:
-            self.alloc.release(r)
+        try:
+            for r in requests:
+                self.alloc.add_request(r)
+                self.alloc.reserve(r, longest - 1)
+            groups, prefix = self.ints([[0, T, prompt.entries]]), self.table_of([prompt.request])
+            answers = [[] for _ in questions]
+            feed = [q[0] for q in questions]
+            for i in range(longest - 1):
+                def attend(part, q, out, batch, cache):
+                    ops.prefix_attention(q, out, cache.kv, prefix, groups, batch.block_table[0], batch.start_pos, part.nh, part.nkv, part.d,
+                                         part.scale, max_rows=T, max_prefix=prompt.entries, max_own=i + 1)
+                after = self.step(requests, feed, [prompt.tokens + i] * T, [i] * T, attend)
+                for t, q in enumerate(questions):
+                    if i + 1 >= len(q) and len(answers[t]) < max_new_tokens:
+                        answers[t].append(after[t])
+                    feed[t] = q[i + 1] if i + 1 < len(q) else after[t]
+        finally:
+            for r in requests:
+                if self.alloc.has(r):
+                    self.alloc.release(r)
         return answers
 
     # ---- one prompt goes on within its budget --------------------------------------------------------------------------
@@ -195,6 +203,7 @@ class LongPrompts:
             most = min(most, self.budget + self.page_size)
         if most > self.max_entries:
             raise ValueError(f"{most} entries; there is room for {self.max_entries}")
+        self.alloc.reserve(prompt.request, most)        # all there is need for, or nothing is done
         for _ in range(max_new_tokens):
             token, entry = prompt.next_token, prompt.entries
             out.append(token)
@@ -224,8 +233,9 @@ def main(argv=None) -> int:
     ap.add_argument("--questions", type=int, default=8)
     ap.add_argument("--max-tokens", type=int, default=16)
     a = ap.parse_args(argv)
-    lp = LongPrompts(a.model, a.dtype, num_pages=2 * (a.prompt_tokens // 16 + 1) + 64 * a.questions, max_requests=a.questions + 2,
-                     max_entries=a.prompt_tokens + a.max_tokens + 64, budget=a.budget)
+    pages = lambda n: -(-n // 16)  # noqa: E731
+    lp = LongPrompts(a.model, a.dtype, num_pages=pages(a.prompt_tokens + a.max_tokens) + a.questions * pages(5 + a.max_tokens),
+                     max_requests=a.questions + 2, max_entries=a.prompt_tokens + a.max_tokens + 64, budget=a.budget)
     g = torch.Generator().manual_seed(0)
     draw = lambda n: torch.randint(0, lp.model.vocab_size, (n,), generator=g).tolist()  # noqa: E731
     prompt = lp.read(draw(a.prompt_tokens))

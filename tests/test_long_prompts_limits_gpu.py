@@ -80,3 +80,32 @@ def test_questions_are_tokens_of_the_model(bad):
 def test_what_is_asked_of_the_budget(bad):
     with pytest.raises(ValueError):
         long_prompts(**bad)
+
+
+def test_what_fails_gives_everything_back():
+    from railgun_b200.cache.manager import CacheError
+    lp = long_prompts(num_pages=4, max_requests=4)
+    prompt = lp.read(text("C", 30)[0])                                  # two pages of 16
+    for questions, n in (([[1, 2]] * 3, 3), ([[1]], 40), ([[1]] * 4, 2)):  # pages for two, for 32 tokens; slots for three
+        with pytest.raises(CacheError):
+            lp.answer(prompt, questions, n)
+        assert lp.alloc.free_pages() == 2
+    before = (prompt.tokens, prompt.entries, prompt.next_token)
+    with pytest.raises(CacheError):
+        lp.go_on(prompt, 40)
+    assert (prompt.tokens, prompt.entries, prompt.next_token) == before and lp.alloc.free_pages() == 2
+    assert len(lp.answer(prompt, [[1, 2]] * 2, 3)) == 2
+    with pytest.raises(CacheError):
+        lp.read(text("C", 100)[0])
+    lp.prefill_fails = lambda batch: 1 / 0
+    forward, lp.forward = lp.forward, lp.prefill_fails
+    with pytest.raises(ZeroDivisionError):
+        lp.read(text("C", 20)[0])
+    with pytest.raises(ZeroDivisionError):
+        lp.answer(prompt, [[1]], 2)
+    lp.forward = forward
+    assert lp.alloc.free_pages() == 2
+    lp.forget(prompt)
+    lp.alloc.check()
+    prompt = lp.read(text("C", 64)[0])                                  # every page and slot can be had again
+    lp.forget(prompt)
