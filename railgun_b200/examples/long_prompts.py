@@ -128,9 +128,12 @@ class LongPrompts:
         table, slots = self.table_of([p.request for p in prompts]), self.ints([p.slot for p in prompts])
         lens, keep = self.ints([p.entries for p in prompts]), self.ints([self.budget] * len(prompts))
         newest = self.ints([p.tokens - 1 for p in prompts])
+        # more protected entries than the budget holds: of equals the first would stay, but the newest are what is wanted
+        first = min(self.protect_first, self.budget)
+        last = min(self.protect_last, self.budget - first)
         for kv, weights, places in zip(self.kv, self.weights, self.places):
-            ops.evict_entries(kv, weights, places, weights, places, slots, table, lens, keep, newest, self.nkv, self.d, self.protect_first,
-                              self.protect_last, max_context=max(p.entries for p in prompts))
+            ops.evict_entries(kv, weights, places, weights, places, slots, table, lens, keep, newest, self.nkv, self.d, first, last,
+                              max_context=max(p.entries for p in prompts))
         for p in prompts:
             p.entries = min(p.entries, self.budget)
             self.alloc.shrink(p.request, p.entries)

@@ -109,3 +109,18 @@ def test_what_fails_gives_everything_back():
     lp.alloc.check()
     prompt = lp.read(text("C", 64)[0])                                  # every page and slot can be had again
     lp.forget(prompt)
+
+
+@pytest.mark.parametrize("budget,first,last", [(32, 4, 32), (20, 4, 32), (3, 4, 32), (40, 50, 3)])
+def test_the_newest_entries_stay_in_a_small_budget(budget, first, last):
+    """Fewer entries than there are protected ones: the first of the text, and of the others the newest."""
+    lp = long_prompts(budget=budget, protect_first=first, protect_last=last)
+    prompt = lp.read(text("C", 100)[0])
+    head = min(first, budget)
+    for n in (0, 40):
+        lp.go_on(prompt, n)
+        tail = min(last, budget - head)
+        for places in lp.places:
+            for kept in places[prompt.slot, :, :prompt.entries].tolist():
+                assert len(kept) == len(set(kept)) and set(range(head)) <= set(kept)
+                assert set(range(prompt.tokens - tail, prompt.tokens)) <= set(kept)
