@@ -3,7 +3,7 @@ and outputs held to bounds of their own size."""
 import pytest
 import torch
 
-from test_cache_operators_gpu import (DEV, TYPES, U, Cache, i32, no_wait_gave_up, out_view, plain_evict, queries, same, softmax,  # noqa: F401
+from test_cache_operators_gpu import (DEV, HEADS, TYPES, U, Cache, i32, no_wait_gave_up, out_view, plain_evict, queries, same, softmax,  # noqa: F401
                                       weight_error)
 
 pytestmark = pytest.mark.gpu
@@ -185,3 +185,16 @@ def test_many_groups(n_groups, nh, nkv, d, prefix, own, dtype):
     groups = [((i * 5 + 3) % 9, 0 if i % 11 == 4 else prefix - 7 * i % prefix) for i in range(n_groups)]
     T = sum(n for n, _ in groups) + 3
     run_prefix(groups, [3 * i % (own + 1) for i in range(T)], nh, nkv, d, 16, dtype, n_groups + d)
+
+
+# ---- outputs to their own size ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("nh,nkv,d,page", HEADS)
+def test_outputs_are_as_near_as_their_roundings(nh, nkv, d, page, dtype):
+    """A mean over thousands of entries is small: held to what its own weights and values allow, not to the largest value."""
+    run_prefix([(2, 65), (1, 0), (7, 201)], [3, 0, 9, 31, 0, 64, 63, 129, 1, 16, 0, 5], nh, nkv, d, page, dtype, nh + d)
+    run_prefix([(20, 4999), (3, 640)], [i * 37 % 140 for i in range(24)], nh, nkv, d, page, dtype, nh + d + 1)
+    run_prefix([(5, 3001)], [700, 0, 1, 128, 333], nh, nkv, d, page, dtype, nh + d + 2)
+    run_weighed([64, 63, 65, 1, 0, 200], nh, nkv, d, page, dtype, nh + d + 3)
+    run_weighed([5000, 2049, 3, 700], nh, nkv, d, page, dtype, nh + d + 4)
+    run_weighed([i * 53 % 1500 for i in range(70)], nh, nkv, d, page, dtype, nh + d + 5)
