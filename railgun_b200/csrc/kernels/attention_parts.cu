@@ -616,9 +616,10 @@ rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, co
     pdl_trigger();
     const int t = blockIdx.x / C, group = a.nh / a.nkv, kvh = blockIdx.y / a.own_tiles, q0 = blockIdx.y % a.own_tiles * PM_Q;
     const int nq = min(PM_Q, group - q0), h0 = kvh * group + q0;
+    const int newest = a.positions[t];                                // asked for before the groups are looked at
     int P = 0;
     const int* prefix_table = prefix_of(a, t, P);
-    const int own = max(0, own_entries(a, t)), prefix_runs = (P + 15) >> 4, total = prefix_runs + ((own + 15) >> 4);
+    const int own = max(0, min(newest + 1, a.own_limit)), prefix_runs = (P + 15) >> 4, total = prefix_runs + ((own + 15) >> 4);
     const int per = (total + C - 1) / C, first = min(total, rank * per), last = min(total, first + per);
     const int n_runs = last - first, mine = n_runs > warp ? (n_runs - warp + 3) >> 2 : 0;
     const int* own_table = a.block_table + (size_t)t * a.max_blocks;
@@ -703,11 +704,10 @@ rows_mma_kernel(const __grid_constant__ CUtensorMap kv_map, const PartArgs a, co
         const int slot = b.slots[t];
         if (slot >= 0 && slot < b.n_slots) {
             float* to = b.weights + ((size_t)slot * a.nkv + kvh) * b.weights_ld;
-            const int newest = a.positions[t];                        // behind what there is room for: none of them is new
             for (int i = threadIdx.x; i < n_runs * 16; i += PM_THREADS) {
                 const int e = first * 16 + i;
                 if (e >= own) break;
-                const float before = e == newest ? 0.f : b.decay * to[e];
+                const float before = e == newest ? 0.f : b.decay * to[e];   // newest behind what there is room for: none
                 float sum = 0.f;
                 for (int r = 0; r < nq; ++r) sum += ex2(scores[r * ld + i] - row_ml[r][0]) * row_ml[r][1];
                 to[e] = before + sum;
@@ -749,7 +749,8 @@ __device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __r
     __shared__ float factor[JOIN_PARTS];
     __shared__ float4 sums[JOIN_THREADS / 32][64];
     const int slots = a.prefix_parts + a.own_parts, d = a.d, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_of(a, t);
+    const int position = a.positions[t];                              // asked for before the groups are looked at
+    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_at(a, position);
     float M, L;
     join_ml(a, t, h, n_prefix, n - n_prefix, M, L);
     const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -793,7 +794,8 @@ __device__ __forceinline__ void join_row(const PartArgs& a, int t, int h, A* __r
 template <typename A>
 __device__ __forceinline__ void join_row_warp(const PartArgs& a, int t, int h, A* __restrict__ out, int out_ld) {
     const int slots = a.prefix_parts + a.own_parts, d = a.d, lane = threadIdx.x & 31;
-    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_of(a, t);
+    const int position = a.positions[t];                              // asked for before the groups are looked at
+    const int n_prefix = a.prefix_parts ? prefix_parts_of(a, t) : 0, n = n_prefix + own_parts_at(a, position);
     const size_t base = ((size_t)t * a.nh + h) * slots;
     const int slot = lane < n_prefix ? lane : a.prefix_parts + lane - n_prefix;
     float2 ml = {-INFINITY, 0.f};

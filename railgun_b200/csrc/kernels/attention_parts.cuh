@@ -83,32 +83,38 @@ __host__ __device__ inline long long part_blocks(const PartArgs& a) {
 }
 
 // How many parts row t has of either list.
-__device__ __forceinline__ int own_parts_of(const PartArgs& a, int t) { return (max(0, own_entries(a, t)) + a.own_per - 1) / a.own_per; }
-// Row t's prefix: its table, and how many entries it has (none: 0).  Whole warps, all lanes for the same row: a lane looks at every
-// 32nd group, the first group that has the row counts.  (One group after the other in every thread: 48 groups of 4 rows on 64 shared
-// and 32 own entries, 32 heads on 8 of 128, 35.1 us, 23.7 so; 1,000 of 2 rows, 8 heads on 2 of 64, 384 and 54.5; one group 8.7 and 8.8.)
-__device__ __forceinline__ const int* prefix_of(const PartArgs& a, int t, int& entries) {
-    entries = 0;
-    for (int g0 = 0; g0 < a.n_groups; g0 += 32) {
-        const int g = g0 + (int)(threadIdx.x & 31);
-        bool has = false;
-        int e = 0;
-        if (g < a.n_groups) {
-            const int i = t - a.groups[g * 3];
-            has = i >= 0 && i < group_rows(a, g);
-            e = prefix_entries(a, g);
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, has);
-        if (hit) {
-            const int lane = __ffs(hit) - 1;
-            entries = max(0, __shfl_sync(0xffffffffu, e, lane));
-            return a.prefix_table + (size_t)(g0 + lane) * a.prefix_blocks;
-        }
+__device__ __forceinline__ int own_parts_at(const PartArgs& a, int position) {
+    return (max(0, min(position + 1, a.own_limit)) + a.own_per - 1) / a.own_per;
+}
+__device__ __forceinline__ int own_parts_of(const PartArgs& a, int t) { return own_parts_at(a, a.positions[t]); }
+// Row t's group (-1: none), and how many entries its prefix has.  Whole warps, all lanes for the same row: a lane looks at every 32nd
+// group, the first group that has the row counts; a group's three numbers are asked for together.  (One group after the other in every
+// thread: 48 groups of 4 rows on 64 shared and 32 own entries, 32 heads on 8 of 128, 35.1 us, 22.9 so; 1,000 of 2 rows, 8 heads on 2
+// of 64, 384 and 45.9; one group 8.7 and 8.6.)
+__device__ __forceinline__ int group_of(const PartArgs& a, int t, int& entries) {
+    const int lane = threadIdx.x & 31;
+    int g0 = 0, e = 0;
+    unsigned hit = 0;
+#pragma unroll 1
+    for (; !hit && g0 < a.n_groups; g0 += 32) {
+        const int g = g0 + lane;
+        const int* at = a.groups + 3 * (size_t)min(g, a.n_groups - 1);
+        const int row0 = at[0], rows = at[1];
+        e = at[2];
+        const int i = t - row0;
+        hit = __ballot_sync(0xffffffffu, g < a.n_groups && row0 >= 0 && i >= 0 && i < min(rows, a.max_rows));
     }
-    return nullptr;
+    const int first = __ffs(hit) - 1;
+    entries = hit ? max(0, min(__shfl_sync(0xffffffffu, e, first), a.prefix_limit)) : 0;
+    return hit ? g0 - 32 + first : -1;
+}
+// Its table, where there are entries.
+__device__ __forceinline__ const int* prefix_of(const PartArgs& a, int t, int& entries) {
+    const int g = group_of(a, t, entries);
+    return a.prefix_table + (size_t)max(g, 0) * a.prefix_blocks;
 }
 __device__ __forceinline__ int prefix_parts_of(const PartArgs& a, int t) {
     int entries;
-    prefix_of(a, t, entries);
+    group_of(a, t, entries);
     return (entries + a.prefix_per - 1) / a.prefix_per;
 }
