@@ -234,7 +234,9 @@ class PageAllocator:
 
     def shrink(self, req_id: int, new_len: int) -> None:
         """The request keeps its entries 0 .. new_len - 1 only (``ops.evict_entries``): the pages behind them go back, and
-        its position becomes ``new_len``.  Groups with windows or chunks, which go by position, refuse."""
+        its position becomes ``new_len``.  As with ``commit``, the caller says what is there: up to what the pages that it has
+        hold, entries behind the last commit that were written since among them.  Groups with windows or chunks, which go by
+        position, refuse."""
         code = self._lib.rg_cache_shrink(self._h, req_id, int(new_len))
         if code:
             self._raise(code, f"shrink({req_id}, {new_len})")

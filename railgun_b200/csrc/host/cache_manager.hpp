@@ -205,7 +205,7 @@ public:
     }
 
     // The request keeps entries [0, new_len) only (the others were evicted, those that stayed moved to the front): the pages
-    // behind go back.  Not for groups that give pages back by position.
+    // behind go back.  Entries are what the caller says they are, as in commit.  Not for groups that give pages back by position.
     int shrink(int64_t id, int new_len) {
         auto it = reqs_.find(id);
         if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;

@@ -441,7 +441,7 @@ struct MmaQueries {
         for (int j = 0; j < 4; ++j) { v[j] = ex2(v[j] - r0); v[j + 4] = ex2(v[j + 4] - r1); }
         l0 += (v[0] + v[1]) + (v[2] + v[3]);                          // this thread's entries; added up at the end
         l1 += (v[4] + v[5]) + (v[6] + v[7]);
-        // weights to bfloat16 for the second product (the sums above are of the weights before that rounding)
+        // weights to bfloat16, up to 2^-8 of each, for the second product (the sums above are of the weights before that rounding)
         const uint32_t p[4] = {pack_bf16(v[0], v[1]), pack_bf16(v[4], v[5]), pack_bf16(v[2], v[3]), pack_bf16(v[6], v[7])};
 #pragma unroll
         for (int k = 0; k < KD; ++k) {                                // 16 columns at a time

@@ -18,7 +18,7 @@
 // do, and the hand-over between products and exponentials the rest.
 // There is no mask but the end of a part: rows of V behind it get zeros in shared memory, scores behind it -infinity.
 //
-// Rounding: P to bfloat16 (2^-9 of each weight; the sum of weights is of the unrounded ones), all sums in 32-bit.
+// Rounding: P to bfloat16 (up to 2^-8 of each weight; the sum of weights is of the unrounded ones), all sums in 32-bit.
 #pragma once
 #include "attention_parts.cuh"
 #include "packed_f32.cuh"

@@ -21,7 +21,7 @@
 // 160 KB of stages) and tensor memory allow one block per SM.
 //
 // Why two numbers a weight: under a reference that is the row's maximum the largest weight is 1, which bfloat16 holds; under
-// one that is seldom raised it is any number up to 2^8 and loses 2^-9 like the others.  In the 2-norm against 64 bits
+// one that is seldom raised it is any number up to 2^8 and loses up to 2^-8 like the others.  In the 2-norm against 64 bits
 // (2,048 tokens, queries times 0.3 / 1 / 3): one number 2.07e-3 / 2.07e-3 / 2.14e-3, attention_mma.cu 2.07e-3 / 2.02e-3 /
 // 1.76e-3, two numbers 1.56e-3 / 1.61e-3 / 1.65e-3, which is the rounding of the output.  The second product costs 4 to 12 %
 // (2,048 tokens 61 to 68 us, 8,192 651 to 680); raising the reference for every new maximum would read and write O in

@@ -2306,8 +2306,8 @@ def prefix_attention(q, out, kv_cache, prefix_table, groups, block_table, positi
     prefix is row e % page_size of page ``prefix_table[g, e // page_size]``.  Row t sees its own entries 0 ..
     ``positions[t]`` (-1: none) through ``block_table[t]``.  Rows of no group see their own entries alone; where there is no
     entry at all the output is 0.  ``max_rows``, ``max_prefix``, ``max_own``: the most rows and prefix entries that a group, and
-    own entries that a row, may have (``groups`` and ``positions`` stay on the device); what lies beyond is not seen.  All
-    sums are 32-bit and have one order."""
+    own entries that a row, may have (``groups`` and ``positions`` stay on the device); what lies beyond is not seen, and scratch is sized by
+    them.  A score of -infinity is a weight of 0: a row that sees no others gives 0.  All sums are 32-bit and have one order."""
     T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "prefix_attention")
     _check_ints(groups, "groups", None, 3, table=True)
     _check_ints(prefix_table, "prefix_table", groups.shape[0], table=True)
@@ -2353,7 +2353,9 @@ def weighed_attention(q, out, kv_cache, weights, slots, block_table, positions, 
     max_context] float32, request r's at ``slots[r]`` (negative: a row whose weights nobody keeps): entry e's becomes
     decay * weight + the sum, over the query heads of each kv head, of the softmax weight that e got from them.  The entry
     ``positions[r]`` is new: its earlier weight is not read.  ``max_context``: the most entries a row may see; entries beyond
-    are not seen (where the new one is among them, no weight is dropped).  All sums are 32-bit and have one order."""
+    are not seen (where the new one is among them, no weight is dropped).  Scratch goes by it too, not by the lengths: where rows are many
+    or contexts long, R * nh * max_context 32-bit scores, 1 GB for 256 rows of 32 heads with room for 32,768, and their parts.  All sums
+    are 32-bit and have one order."""
     R, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "weighed_attention")
     _check_ints(block_table, "block_table", R, table=True)
     _check_ints(positions, "positions", R)
@@ -2442,9 +2444,9 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     """Of the ``lens[r]`` entries of request r, ``keep[r]`` stay in every kv head: those of greatest weight, ties to the lowest
     entry.  ``places`` [slots, nkv, at least max_context] int32 holds every entry's position in the text; entries at a place below
     ``protect_first`` or above ``positions[r]`` - ``protect_last`` (``positions``: the newest token's place), or whose weight is no number, count as
-    infinitely heavy.  K and V rows behind the new length move, in place, into entries before it that got free, the i-th into
+    infinitely heavy (more of them than stay: the lowest entries).  K and V rows behind the new length move, in place, into entries before it that got free, the i-th into
     the i-th, so what stays is entries 0 .. new length - 1 and no more rows move than have to; the pages behind may be
-    given back (``PageAllocator.shrink``).  Weights and places of the entries that stay go to ``weights_out`` and ``places_out``: the same
+    given back (``PageAllocator.shrink``).  The pages are the requests' own: what another table reads as well would change under it.  Weights and places of the entries that stay go to ``weights_out`` and ``places_out``: the same
     buffers, or others of these shapes that share no memory with them; what lies behind the new length there is left alone.
     ``max_context``: the most entries a request may have (``lens`` stays on the device).  Returns the new lengths [R] int32: min(lens,
     keep), or lens for requests that are left alone: those with a negative slot, and those with more entries than ``max_context`` or than
