@@ -1,0 +1,153 @@
+// What the kernels of attention_tree.cu share: how the work of trees of drafted tokens is cut, and where the parts are left.
+//
+// Request r brings rows cu_rows[r] .. cu_rows[r + 1] - 1, the nodes of its tree, behind starts[r] entries that it has in the
+// cache; node j is entry starts[r] + j.  Row i sees the entries before starts[r] and the nodes whose bit its mask has:
+//   out_ih = sum_e p_ih(e) v_e,  p = softmax over {e < start} and {start + j : bit j of mask i} of scale q_ih . k_e,   no entry: 0
+//
+// An item is (request, kv head, block of queries); query i of a request and kv head is row i / group, head i % group.  An item has
+// ceil(entries / tile) tiles.  All items' tiles, one item after the other, are one line that is cut into as many stretches of `per`
+// tiles as there are workers: whatever the requests' lengths, every worker has the same number of tiles to read.  A stretch
+// may end inside an item; what a worker finds for an item, its part, is left as the unnormalised output o = sum 2^(s - m) v with
+// m = max s and l = sum 2^(s - m), s = scale log2(e) q.k, in 32-bit, and a second kernel joins the parts of every row and head:
+//   out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l,   M = max_parts m
+// A part's numbers lie at (first query of the item in all queries) + worker x (queries of an item): parts along the line never
+// meet, and T x nh + workers x (queries of an item) places are enough.
+#pragma once
+#include "common.cuh"
+
+#define RG_BAD_PAGE 1000              // in the error flag: a table names a page that the cache does not have
+
+struct TreeArgs {
+    const void* q;               // [T, q_stride]: head h of row t at q[t * q_stride + h * d]
+    const void* kv;              // [pages, 2, nkv, page_size, d]
+    const int* block_table;      // [R, max_blocks]
+    const int* cu_rows;          // [R + 1]
+    const int* starts;           // [R]
+    const int* masks;            // [T, words]
+    float* part_o;               // [places, d]
+    float* part_ml;              // [places, 2]
+    long long* plan;             // [R + 1]: tiles of all items before request r's; then `per`
+    int* err;
+    int R, T, max_rows, limit;   // limit: the most entries of a request that are seen
+    int q_stride, max_blocks, words, pages;
+    int nh, nkv, d, page_size, page_shift;      // page_shift: log2 of the page size, or -1
+    int tile, item_queries, workers, least;     // entries of a tile, queries of an item, workers, least tiles of a stretch
+    float scale_log2;
+};
+
+// A request as the kernels see it: rows that take part, entries that are seen, tiles of an item and items of a kv head.
+struct TreeRequest {
+    int row0, rows, start, entries, tiles, blocks;
+};
+__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
+    TreeRequest x;
+    const int row0 = a.cu_rows[r], next = a.cu_rows[r + 1], start = a.starts[r];
+    x.row0 = row0;
+    const long long rows = min((long long)next - row0, (long long)a.max_rows);
+    x.rows = row0 < 0 || start < 0 ? 0 : (int)max(0ll, min(rows, (long long)a.T - row0));
+    x.start = start;
+    x.entries = x.rows ? (int)min((long long)a.limit, (long long)start + x.rows) : 0;
+    x.tiles = (x.entries + a.tile - 1) / a.tile;
+    x.blocks = (int)(((long long)x.rows * (a.nh / a.nkv) + a.item_queries - 1) / a.item_queries);
+    return x;
+}
+__device__ __forceinline__ long long tree_tiles(const TreeArgs& a, const TreeRequest& x) { return (long long)x.tiles * x.blocks * a.nkv; }
+
+// Where a worker is on the line: an item and a tile of it.
+struct TreeWalk {
+    TreeRequest x;
+    int r, item, tile;           // item: kv head x blocks + block of queries
+    __device__ __forceinline__ int kvh() const { return item / x.blocks; }
+    __device__ __forceinline__ int block() const { return item % x.blocks; }
+    __device__ __forceinline__ void skip_empty(const TreeArgs& a) {      // to a request that has tiles (one is known to come)
+        while (x.tiles == 0 || x.blocks == 0) x = tree_request(a, ++r);
+    }
+    // At place `in` of request r's tiles.
+    __device__ __forceinline__ void at(const TreeArgs& a, int r_, long long in) {
+        r = r_;
+        x = tree_request(a, r);
+        item = (int)(in / x.tiles);
+        tile = (int)(in % x.tiles);
+    }
+    // One tile on; `more`: there is one.
+    __device__ __forceinline__ void next(const TreeArgs& a, bool more) {
+        if (++tile < x.tiles) return;
+        tile = 0;
+        if (++item < x.blocks * a.nkv) return;
+        item = 0;
+        if (!more) return;
+        x = tree_request(a, ++r);
+        skip_empty(a);
+    }
+    __device__ __forceinline__ bool last_tile() const { return tile + 1 == x.tiles; }
+    // The first query of the item among all rows' and heads'.
+    __device__ __forceinline__ long long first_query(const TreeArgs& a) const {
+        return (long long)x.row0 * a.nh + (long long)kvh() * x.rows * (a.nh / a.nkv) + (long long)block() * a.item_queries;
+    }
+};
+
+// The whole block, THREADS threads: tiles of all items, and the request (with the place among its tiles) in which each of `n`
+// (up to 2) workers from `first` on begins (r -1: it has nothing).  Block 0 leaves the plan for the joining kernel.
+struct TreeStart {
+    long long total, per;
+    long long in[2];
+    int r[2];
+};
+template <int THREADS>
+__device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, TreeStart& st) {
+    __shared__ long long sums[THREADS / 32 + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto scan = [&](long long v, long long& total) -> long long {       // exclusive, over the block
+        long long x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = x;
+        __syncthreads();
+        long long before = 0;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += sums[w];
+            total += sums[w];
+        }
+        return before + x - v;
+    };
+    long long total = 0, mine = 0, before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
+        const int r = r0 + threadIdx.x;
+        long long some;
+        mine = r < a.R ? tree_tiles(a, tree_request(a, r)) : 0;
+        before = total + scan(mine, some);
+        total += some;
+    }
+    const long long per = max((long long)a.least, (total + a.workers - 1) / a.workers);
+    if (threadIdx.x == 0) {
+        st.total = total;
+        st.per = per;
+        st.r[0] = st.r[1] = -1;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[a.R] = per;
+    const bool once = a.R <= THREADS;                                    // what was found above still stands
+    long long sofar = 0;
+    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
+        const int r = r0 + threadIdx.x;
+        if (!once) {
+            long long some;
+            mine = r < a.R ? tree_tiles(a, tree_request(a, r)) : 0;
+            before = sofar + scan(mine, some);
+            sofar += some;
+        }
+        if (r >= a.R) continue;
+        if (blockIdx.x == 0) a.plan[r] = before;
+        for (int i = 0; i < n; ++i) {
+            const long long at = (first + i) * per - before;
+            if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; }
+        }
+    }
+    __syncthreads();
+}

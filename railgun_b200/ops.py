@@ -11,6 +11,7 @@ import ctypes
 import functools
 import os
 
+import numpy as np
 import torch
 
 from . import log, native
@@ -2486,6 +2487,179 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     return new_lens
 
 
+def _check_here(what: str, *tensors) -> None:
+    """A launch goes to the current device: all its tensors lie there."""
+    here = _current_device()
+    for t in tensors:
+        if t.get_device() != here:
+            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
+
+
+DRAFT_MOST = 4096              # nodes of a tree of drafted tokens
+
+
+def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, starts: torch.Tensor, max_rows: int) -> tuple:
+    """The layout of trees of drafted tokens, made once a step for all layers.  Request r brings rows ``cu_rows[r]`` .. ``cu_rows[r + 1]`` - 1,
+    the nodes of its tree, behind ``starts[r]`` tokens that it has in the cache; ``parents`` [T] int32 holds every node's parent as a
+    number within its request, which is lower than its own (anything else: a root).  Returns ``masks`` [T, ceil(max_rows / 32)]
+    int32, in which bit j % 32 of word j // 32 says that a row sees node j (itself or an ancestor), for ``tree_attention``, and the nodes'
+    ``positions`` [T] int32, starts + how many ancestors there are, for rotations.  ``max_rows``, up to 4,096: the most rows of a
+    request; rows beyond, rows of requests with a negative start and rows of no request get zeros."""
+    _check_ints(parents, "parents", None)
+    _check_ints(starts, "starts", None)
+    T, R = parents.shape[0], starts.shape[0]
+    _check_ints(cu_rows, "cu_rows", R + 1)
+    _check_here("draft_tree", parents, cu_rows, starts)
+    if not 0 <= max_rows <= DRAFT_MOST:
+        raise KernelError(f"draft_tree: up to {DRAFT_MOST} rows a request, not {max_rows}")
+    words = -(-max_rows // 32)
+    masks = torch.empty((T, words), dtype=torch.int32, device=parents.device)
+    positions = torch.empty(T, dtype=torch.int32, device=parents.device)
+    _ok(_fn("drafts", "rg_draft_tree")(_ptr(parents), _ptr(cu_rows), _ptr(starts), c_int(R), c_int(T), c_int(max_rows), _ptr(masks), c_int(words),
+                                       _ptr(positions), _stream()), "draft_tree")
+    return masks, positions
+
+
+def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: int, nkv: int, d: int, scale: float, max_rows: int,
+                   max_context: int) -> None:
+    """Attention of trees of drafted tokens: ``out`` [T, nh * d], row t of ``q`` [T, at least nh * d] (head h at column h * d).  Request r's rows
+    are ``cu_rows[r]`` .. ``cu_rows[r + 1]`` - 1; its entries, through ``block_table[r]``, are ``starts[r]`` of earlier tokens, which all its
+    rows see, and then one for each of its rows (already in the cache), of which a row sees those whose bits ``masks`` [T, words] int32
+    has (``draft_tree``; any other choice will do).  A row that sees nothing gives 0; keys and values that a row does not see have no say
+    in it, whatever they are, and a score of -infinity is a weight of 0.  ``max_rows``, ``max_context``: the most rows of a request, and
+    the most entries (earlier and its own) that are seen; scratch is sized by rows.  Rows beyond ``max_rows``, rows of requests with a
+    negative start and rows of no request are left as they were.  A page that the cache does not have is reported by
+    ``tc_gemm_check``, and the result is invalid.  All sums are 32-bit and have one order."""
+    T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "tree_attention")
+    _check_ints(starts, "starts", None)
+    R = starts.shape[0]
+    _check_ints(cu_rows, "cu_rows", R + 1)
+    _check_ints(block_table, "block_table", R, table=True)
+    _check_ints(masks, "masks", T, table=True)
+    _check_out_view(out, T, nh * d, q.dtype, "tree_attention")
+    _check_here("tree_attention", q, out, kv_cache, block_table, cu_rows, starts, masks)
+    if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
+        raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
+    if T == 0 or R == 0 or max_rows == 0:
+        return
+    sms = num_sms(q.device)
+    queries, workers, least = 16, sms * tree_general_blocks(d), 1
+    places = T * nh + workers * queries
+    before_ml = _floats_before_ml(places, d)
+    before_plan = before_ml + 2 * places
+    scratch = torch.empty(before_plan + 2 * (R + 1), dtype=torch.float32, device=q.device)
+    part_ml = scratch.data_ptr() + 4 * before_ml
+    _COUNTER.value += 1                          # the parts, and the kernel that joins them
+    _ok(_fn("attention_tree", "rg_tree_attention")(
+        _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(block_table),
+        c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(masks), c_int(masks.shape[1]), c_int(R), c_int(T), c_int(nh), c_int(nkv),
+        c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), c_int(workers), c_int(queries), c_int(least), _ptr(scratch),
+        c_void_p(part_ml), c_void_p(part_ml + 8 * places), _ptr(_tc_error_flag(q.device)), _stream()), "tree_attention")
+
+
+def tree_general_blocks(d: int) -> int:
+    """Blocks an SM of the general kernel over trees: what its tiles leave room for in shared memory, and three by its registers."""
+    row = ((d + 3) & ~3) + 4
+    return max(1, min(3, (227 << 10) // (4 * ((16 + (4 if d <= 128 else 2) * 64) * row + 16 * 69) + 2304)))
+
+
+def _cache_list(caches, what: str) -> tuple:
+    """One cache or several of one shape and type, as (list, their addresses, the bytes of an element)."""
+    caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+    if not caches:
+        raise KernelError(f"{what}: no caches")
+    first = caches[0]
+    shape, dtype, fits = first.shape, first.dtype, _fast.shaped if _fast is not None else None
+    for t in caches:
+        if fits is None or not fits(t, dtype, *shape):
+            _check(t, "a cache", dtype)
+            if t.shape != shape:
+                raise KernelError(f"{what}: caches of {tuple(shape)} and {tuple(t.shape)}")
+    _check_here(what, *caches)
+    addresses = (ctypes.c_ulonglong * len(caches))(*[t.data_ptr() for t in caches])
+    return caches, addresses, first.element_size()
+
+
+def _unit(row_bytes: int, addresses) -> int:
+    """The largest of 16, 8, 4, 2 and 1 bytes that rows and addresses are multiples of."""
+    low = row_bytes | 16
+    for a in addresses:
+        low |= a
+    return low & -low
+
+
+def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, max_rows: int) -> tuple:
+    """What the model's own choices confirm of trees of drafted tokens.  Rows, ``starts`` and ``parents`` as in ``draft_tree``; ``tokens`` [T] int32
+    is every node's token, ``chosen`` [T] int32 the token that the model chose behind it (``argmax``, ``sample``).  From node 0 on, the
+    lowest child whose token is the one chosen behind its parent is confirmed, until there is none.  Returns ``counts`` [R] int32, how many
+    nodes are (node 0 is, always), ``path`` [R, max_rows] int32, their numbers, and ``fresh`` [R, max_rows] int32, the tokens chosen
+    behind them: the request's next ``counts[r]`` tokens, the last of which begins its next tree; -1 behind them.  In every
+    cache [pages, .., page, x] of ``caches`` (one, or a list of one shape) the k-th confirmed node's entry moves from starts + its
+    number to starts + k, so that the request has starts + counts entries and what lies behind may be given back
+    (``PageAllocator.shrink``).  The pages are the request's own from ``starts`` on.  ``max_rows``, up to 4,096: the most rows of a request; rows
+    beyond are left out, and requests without rows or with a negative start have a count of 0.  An entry that table or
+    cache do not have does not move, and ``tc_gemm_check`` reports it."""
+    caches, addresses, size = _cache_list(caches, "keep_drafts")
+    shape = caches[0].shape
+    if len(shape) < 3 or caches[0].numel() == 0:
+        raise KernelError(f"keep_drafts: a cache is [pages, .., page, x], not {tuple(shape)}")
+    _check_ints(starts, "starts", None)
+    R = starts.shape[0]
+    _check_ints(parents, "parents", None)
+    T = parents.shape[0]
+    _check_ints(cu_rows, "cu_rows", R + 1)
+    _check_ints(block_table, "block_table", R, table=True)
+    _check_ints(tokens, "tokens", T)
+    _check_ints(chosen, "chosen", T)
+    _check_here("keep_drafts", block_table, cu_rows, starts, parents, tokens, chosen)
+    if not 0 <= max_rows <= DRAFT_MOST:
+        raise KernelError(f"keep_drafts: up to {DRAFT_MOST} rows a request, not {max_rows}")
+    device = starts.device
+    counts = torch.empty(R, dtype=torch.int32, device=device)
+    path = torch.empty((2, R, max_rows), dtype=torch.int32, device=device)
+    pages, page_size, outer = shape[0], shape[-2], caches[0].numel() // (shape[0] * shape[-2] * shape[-1])
+    piece = _unit(shape[-1] * size, addresses)
+    _COUNTER.value += (len(caches) - 1) // 64
+    _ok(_fn("drafts", "rg_keep_drafts")(
+        _at(addresses), c_int(len(caches)), c_int(pages), c_int(outer), c_int(page_size), c_int(shape[-1] * size // piece), c_int(piece),
+        _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(parents), _ptr(tokens), _ptr(chosen), c_int(R), c_int(T),
+        c_int(max_rows), _ptr(counts), _ptr(path), c_void_p(path.data_ptr() + 4 * R * max_rows), c_int(num_sms(device)),
+        _ptr(_tc_error_flag(device)), _stream()), "keep_drafts")
+    return counts, path[0], path[1]
+
+
+def copy_pages(caches, copies) -> None:
+    """Copies of pages in every cache of ``caches`` (one, or a list of one shape and type, [pages, .., page, x]; [slots, ..] of fewer than three
+    dimensions as whole rows).  ``copies`` [n, 3] int32 on the host (what ``PageAllocator.fork`` returns): (from, to, held), the first
+    ``held`` entries of page ``from`` (-1: all of it) to page ``to``; what lies behind them there is left alone.  A page may be
+    copied several times; one that is written is written once and read by no copy, so that their order does not matter (a copy of a
+    page to itself is none).  The copies are arguments of the launch: a captured graph repeats these."""
+    caches, addresses, size = _cache_list(caches, "copy_pages")
+    copies = np.asarray(copies) if len(copies) else np.empty((0, 3), np.int32)
+    if copies.ndim != 2 or copies.shape[1] != 3 or copies.dtype.kind not in "iu" or (
+            copies.dtype != np.int32 and np.abs(copies.astype(np.float64)).max() >= 1 << 31):
+        raise KernelError(f"copy_pages: copies are whole numbers [n, 3] of 32 bits, not {copies.dtype} {copies.shape}")
+    copies = np.ascontiguousarray(copies, dtype=np.int32)
+    shape, numel = caches[0].shape, caches[0].numel()
+    if len(shape) < 1:
+        raise KernelError("copy_pages: a cache is [pages, ..]")
+    if len(copies) == 0:
+        return
+    pages = shape[0]
+    if numel == 0:
+        raise KernelError(f"copy_pages: caches of {tuple(shape)} have no pages to copy")
+    page_size, entry = (shape[-2], shape[-1] * size) if len(shape) >= 3 else (1, numel // pages * size)
+    outer = numel * size // (pages * page_size * entry)
+    _COUNTER.value += -(-len(copies) // 256) * -(-len(caches) // 64) - 1
+    code = _fn("page_copy", "rg_copy_pages")(_at(addresses), c_int(len(caches)), c_int(pages), c_int(outer), c_int(page_size), c_longlong(entry),
+                                             c_int(_unit(entry, addresses)), c_void_p(copies.ctypes.data), c_int(len(copies)),
+                                             c_int(num_sms(caches[0].device)), _stream())
+    if code in (10002, 10003):
+        raise KernelError("copy_pages: " + ("pages and numbers of entries are those of the caches" if code == 10002
+                                            else "a page that is written is written once and read by no copy"))
+    _ok(code, "copy_pages")
+
+
 _tc_err: dict = {}
 TC_GEMM_MIN_ROWS = 1024        # from here the fused tcgen05 gate|up product beats cuBLAS + SiLU-mul (measured)
 
@@ -2871,8 +3045,8 @@ def probe_sm100(device="cuda:0") -> dict:
 
 
 def tc_gemm_check(device=None) -> None:
-    """Raise if a wait inside a tcgen05 product gave up since the last check
-    (synchronises; free when no such product ran since)."""
+    """Raise if a wait inside a tcgen05 product gave up since the last check, or an operator over trees of drafted tokens met a page
+    that its cache does not have (synchronises; free when no such kernel ran since)."""
     global _tc_unchecked
     if not _tc_unchecked:
         return
@@ -2883,6 +3057,8 @@ def tc_gemm_check(device=None) -> None:
         code = int(err.item())
         if code:
             err.zero_()
+            if code == 1000:
+                raise KernelError("a block table names a page or an entry that the cache does not have; the result is invalid")
             who = {1: "the TMA producer", 2: "the MMA issuer", 3: "the epilogue", 4: "the MMA issuer"}.get(
                 code, f"role {code} of the attention kernel")
             raise KernelError(f"a tcgen05 kernel: {who} gave up waiting on a barrier; the result is invalid")
