@@ -1,6 +1,7 @@
 // Attention of trees of drafted tokens over the paged cache and over one another.  attention_tree.cuh says what is computed and
 // how it is cut.
 #include "attention_tree.cuh"
+#include "attention_tree_tcgen05.cuh"
 #include "mma.cuh"
 
 #define TG_THREADS 128
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     __shared__ long long row_at[2][TG_K];                           // where the rows of a tile are in the cache, -1 behind its end
     pdl_wait();
     pdl_trigger();
-    tree_plan<TG_THREADS>(a, blockIdx.x, 1, st);
+    tree_plan<TG_THREADS>(a, blockIdx.x, 1, 0, st);
     if (st.r[0] < 0) return;
     const int d = a.d, ld = tg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = tg_stages(d);
     float* qs = smem;                                               // [16][ld]
@@ -368,11 +369,12 @@ static int launch_tree_general(const TreeArgs& a, int dtype, cudaStream_t s) {
 }
 
 // See attention_tree.cuh for the arguments.  Scratch: plan [R + 1] on an 8-byte boundary, part_o [T nh + workers item_queries, d]
-// on one of 32 bytes and part_ml [.., 2] on one of 8.
+// on one of 32 bytes and part_ml [.., 2] on one of 8.  tensor_cores: 0 tree_general_kernel; 1 tree_tc_kernel, a stretch a side; 2 the same,
+// a stretch for both sides; tile_rows: rows of a side.
 extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                  const int* block_table, int max_blocks, const int* cu_rows, const int* starts, const int* masks, int words,
                                  int R, int T, int nh, int nkv, int d, int page_size, float scale, int max_rows, int max_context,
-                                 int workers, int item_queries, int least, float* part_o, float* part_ml, long long* plan, int* err, void* stream) {
+                                 int blocks, int workers, int item_queries, int least, int tile_rows, int tensor_cores, float* part_o, float* part_ml, long long* plan, int* err, void* stream) {
     if (T <= 0 || R <= 0 || max_rows <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_blocks < 0 || words < 0 || max_context < 0 || out_ld < nh * d ||
         workers < 1 || item_queries < 1 || least < 1 || ((uintptr_t)part_o & 31) || ((uintptr_t)part_ml & 7) || ((uintptr_t)plan & 7) ||
@@ -388,12 +390,12 @@ extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out
     a.part_o = part_o; a.part_ml = part_ml; a.plan = plan; a.err = err;
     a.page_shift = -1;
     for (int b = 0; b < 31; ++b) if (page_size == (1 << b)) a.page_shift = b;
-    if (item_queries != TG_Q) return RG_ERR_UNSUPPORTED;
-    a.tile = TG_K;
-    int e = launch_tree_general(a, dtype, (cudaStream_t)stream);
+    a.tile = tensor_cores ? TT_STAGE : TG_K;
+    if (tensor_cores ? !tree_tc_ok(a, dtype) : item_queries != TG_Q || workers != blocks) return RG_ERR_UNSUPPORTED;
+    int e = tensor_cores ? launch_tree_tc(a, tile_rows, tensor_cores == 2, blocks, (cudaStream_t)stream) : launch_tree_general(a, dtype, (cudaStream_t)stream);
     if (e) return e;
-    const long long blocks = ((long long)T * nh + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
+    const long long joins = ((long long)T * nh + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
     if (dtype == RG_DTYPE_F32)
-        return rg_launch(tree_join_kernel<float>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
-    return rg_launch(tree_join_kernel<bf16>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);
+        return rg_launch(tree_join_kernel<float>, dim3((unsigned)joins), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
+    return rg_launch(tree_join_kernel<bf16>, dim3((unsigned)joins), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);
 }

@@ -87,14 +87,14 @@ struct TreeWalk {
 };
 
 // The whole block, THREADS threads: tiles of all items, and the request (with the place among its tiles) in which each of `n`
-// (up to 2) workers from `first` on begins (r -1: it has nothing).  Block 0 leaves the plan for the joining kernel.
+// (up to 2) workers, `first` and `first` + `apart`, begins (r -1: it has nothing).  Block 0 leaves the plan for the joining kernel.
 struct TreeStart {
     long long total, per;
     long long in[2];
     int r[2];
 };
 template <int THREADS>
-__device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, TreeStart& st) {
+__device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, int apart, TreeStart& st) {
     __shared__ long long sums[THREADS / 32 + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto scan = [&](long long v, long long& total) -> long long {       // exclusive, over the block
@@ -145,7 +145,7 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, T
         if (r >= a.R) continue;
         if (blockIdx.x == 0) a.plan[r] = before;
         for (int i = 0; i < n; ++i) {
-            const long long at = (first + i) * per - before;
+            const long long at = (first + (long long)i * apart) * per - before;
             if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; }
         }
     }

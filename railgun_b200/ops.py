@@ -2542,8 +2542,16 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
     if T == 0 or R == 0 or max_rows == 0:
         return
-    sms = num_sms(q.device)
-    queries, workers, least = 16, sms * tree_general_blocks(d), 1
+    G, blocks, tile_rows, tensor_cores, least = nh // nkv, num_sms(q.device), 0, 0, 1
+    if (q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and block_table.shape[1]
+            and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)):
+        # sides of 128 queries, two a block: a stretch of the work each, or one for both where requests may bring more
+        tensor_cores = 1 if max_rows <= 128 // G else 2
+        tile_rows = min(max_rows, 128 // G)
+        queries, workers = tile_rows * G * tensor_cores, blocks * (3 - tensor_cores)
+    else:
+        queries, workers = 16, blocks * tree_general_blocks(d)
+        blocks = workers
     places = T * nh + workers * queries
     before_ml = _floats_before_ml(places, d)
     before_plan = before_ml + 2 * places
@@ -2553,7 +2561,8 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     _ok(_fn("attention_tree", "rg_tree_attention")(
         _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(block_table),
         c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(masks), c_int(masks.shape[1]), c_int(R), c_int(T), c_int(nh), c_int(nkv),
-        c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), c_int(workers), c_int(queries), c_int(least), _ptr(scratch),
+        c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), c_int(blocks), c_int(workers), c_int(queries), c_int(least),
+        c_int(tile_rows), c_int(tensor_cores), _ptr(scratch),
         c_void_p(part_ml), c_void_p(part_ml + 8 * places), _ptr(_tc_error_flag(q.device)), _stream()), "tree_attention")
 
 
