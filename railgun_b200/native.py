@@ -38,8 +38,10 @@ NVCC_FLAGS = [
 GXX_FLAGS = ["-O2", "-std=c++17", "-shared", "-fPIC", "-Wall"]
 
 
-# Host sources that are Python extension modules rather than libraries of C functions.
-PYTHON_MODULES = ("fastcall",)
+# Host sources that are Python extension modules rather than libraries of C functions, and those among them that use torch's own
+# C++ interface.
+PYTHON_MODULES = ("fastcall", "fasttensor")
+TORCH_MODULES = ("fasttensor",)
 
 
 class NativeBuildError(RuntimeError):
@@ -121,6 +123,15 @@ def _run_with_progress(cmd: list[str], what: str) -> None:
     _say(f"compiled {what} in {time.time() - t0:.1f} s")
 
 
+def _torch_flags() -> list[str]:
+    """Headers and libraries of the torch that runs here; its version is among the flags, so that another torch gets another build."""
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    return [f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}", f"-DRAILGUN_TORCH_{''.join(c if c.isalnum() else '_' for c in torch.__version__)}",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-Wl,--no-as-needed", f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+            "-ltorch", "-lc10"]
+
+
 def library_path(name: str, kind: str) -> tuple[Path, Path, list[str], str]:
     if kind == "kernel":
         src = KERNEL_DIR / f"{name}.cu"
@@ -131,6 +142,8 @@ def library_path(name: str, kind: str) -> tuple[Path, Path, list[str], str]:
         flags = list(GXX_FLAGS)
         if name in PYTHON_MODULES:
             flags.append(f"-I{sysconfig.get_paths()['include']}")
+        if name in TORCH_MODULES:
+            flags += _torch_flags()
         compiler = "g++"
     if not src.exists():
         raise NativeBuildError(f"no source file {src}")
@@ -149,6 +162,8 @@ def build(name: str, kind: str = "kernel") -> Path:
     else:
         if kind == "host" and name in PYTHON_MODULES and not python_headers():
             raise NativeToolMissing(f"{src.name} needs Python's headers (Python.h in {sysconfig.get_paths()['include']})")
+        if kind == "host" and name in TORCH_MODULES and not os.path.exists(next(f for f in flags if f.endswith("/torch/include"))[2:]):
+            raise NativeToolMissing(f"{src.name} needs torch's headers")
         exe = _find("g++", ["/usr/bin/g++"])
     tmp = out.with_suffix(f".tmp{os.getpid()}.so")
     cmd = [exe, *flags, "-o", str(tmp), str(src)]

@@ -49,6 +49,77 @@ else:
         return c_void_p(0 if t is None else t.data_ptr())
 
 
+# The same and more on tensors themselves (csrc/host/fasttensor.cpp), for operators whose time is the host's: built at first use.
+# False: this machine cannot build it.
+_tensors = None
+
+
+def _tensor_calls():
+    global _tensors
+    if _tensors is None:
+        try:
+            _tensors = native.load_module("fasttensor") if _fast is not None else False
+        except native.NativeToolMissing as e:
+            log.warning("some operators check their arguments through Python, which takes up to some 20 us a call longer: %s", e)
+            _tensors = False
+    return _tensors
+
+
+_addresses: dict = {}
+
+
+def _launch(lib_name: str, fn_name: str, kinds: str, *args) -> int:
+    """Call a launcher.  ``kinds``: a letter for each argument, i a whole number, f a float, p a tensor or bytes (where they are), an
+    address or None.  The current stream comes last."""
+    stream = _raw_stream(_current_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
+    if not _tensor_calls():
+        def place(v):
+            if isinstance(v, bytes):
+                v = ctypes.cast(ctypes.c_char_p(v), ctypes.c_void_p).value
+            return _ptr(v) if isinstance(v, torch.Tensor) else c_void_p(v)
+        if len(kinds) != len(args):
+            raise TypeError(f"{fn_name}: {len(args)} arguments for {len(kinds)}")
+        x = [dict(i=c_longlong, f=c_float, p=place)[k](v) for k, v in zip(kinds, args)]
+        return _fn(lib_name, fn_name)(*x, c_void_p(stream))
+    address = _addresses.get(fn_name)
+    if address is None:
+        _fn(lib_name, fn_name)
+        address = _addresses[fn_name] = ctypes.cast(getattr(native.load(lib_name), fn_name), ctypes.c_void_p).value, kinds + "p"
+    else:
+        _COUNTER.value += 1
+    return _tensors.call(*address, *args, stream)
+
+
+def _fits(t, name: str, dtype, here: int, *sizes) -> None:
+    """A contiguous tensor of this type on the current device, of these sizes (None: any)."""
+    if _tensors and _tensors.fits(t, dtype, here, *sizes):
+        return
+    _check(t, name, dtype)
+    if t.get_device() != here:
+        raise KernelError(f"{name} is on {t.device}, the current device is cuda:{here}")
+    if t.dim() != len(sizes) or any(n is not None and n != m for n, m in zip(sizes, t.shape)):
+        raise KernelError(f"{name} is {tuple(t.shape)}, expected [{', '.join('any' if n is None else str(n) for n in sizes)}]")
+
+
+def _rows_fit(t, name: str, dtype, here: int, columns: int) -> tuple:
+    """(rows, elements from one to the next) of a matrix on the current device with unit column stride and at least so many columns."""
+    got = _tensors.rows(t, dtype, here, columns) if _tensors else None
+    if got is None:
+        _check_rows(t, name, dtype)
+        if t.get_device() != here:
+            raise KernelError(f"{name} is on {t.device}, the current device is cuda:{here}")
+        if t.shape[1] < columns:
+            raise KernelError(f"{name} has {t.shape[1]} columns, {columns} are needed")
+        got = t.shape[0], t.stride(0)
+    return got
+
+
+def _new(dtype, here: int, *sizes) -> torch.Tensor:
+    if _tensors:
+        return _tensors.empty(dtype, here, *sizes)
+    return torch.empty(sizes, dtype=dtype, device=torch.device("cuda", here))
+
+
 def _check(t: torch.Tensor, name: str, dtype=None) -> None:
     if _fast is not None and _fast.fits(t, dtype):
         return
@@ -2487,14 +2558,6 @@ def evict_entries(kv_cache, weights, places, weights_out, places_out, slots, blo
     return new_lens
 
 
-def _check_here(what: str, *tensors) -> None:
-    """A launch goes to the current device: all its tensors lie there."""
-    here = _current_device()
-    for t in tensors:
-        if t.get_device() != here:
-            raise KernelError(f"{what}: a tensor on {t.device}, the current device is cuda:{here}")
-
-
 DRAFT_MOST = 4096              # nodes of a tree of drafted tokens
 
 
@@ -2505,18 +2568,17 @@ def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, starts: torch.Tenso
     int32, in which bit j % 32 of word j // 32 says that a row sees node j (itself or an ancestor), for ``tree_attention``, and the nodes'
     ``positions`` [T] int32, starts + how many ancestors there are, for rotations.  ``max_rows``, up to 4,096: the most rows of a
     request; rows beyond, rows of requests with a negative start and rows of no request get zeros."""
-    _check_ints(parents, "parents", None)
-    _check_ints(starts, "starts", None)
+    _tensor_calls()
+    here, i32 = _current_device(), torch.int32
+    _fits(parents, "parents", i32, here, None)
+    _fits(starts, "starts", i32, here, None)
     T, R = parents.shape[0], starts.shape[0]
-    _check_ints(cu_rows, "cu_rows", R + 1)
-    _check_here("draft_tree", parents, cu_rows, starts)
+    _fits(cu_rows, "cu_rows", i32, here, R + 1)
     if not 0 <= max_rows <= DRAFT_MOST:
         raise KernelError(f"draft_tree: up to {DRAFT_MOST} rows a request, not {max_rows}")
     words = -(-max_rows // 32)
-    masks = torch.empty((T, words), dtype=torch.int32, device=parents.device)
-    positions = torch.empty(T, dtype=torch.int32, device=parents.device)
-    _ok(_fn("drafts", "rg_draft_tree")(_ptr(parents), _ptr(cu_rows), _ptr(starts), c_int(R), c_int(T), c_int(max_rows), _ptr(masks), c_int(words),
-                                       _ptr(positions), _stream()), "draft_tree")
+    masks, positions = _new(i32, here, T, words), _new(i32, here, T)
+    _ok(_launch("drafts", "rg_draft_tree", "pppiiipip", parents, cu_rows, starts, R, T, max_rows, masks, words, positions), "draft_tree")
     return masks, positions
 
 
@@ -2530,21 +2592,28 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     the most entries (earlier and its own) that are seen; scratch is sized by rows.  Rows beyond ``max_rows``, rows of requests with a
     negative start and rows of no request are left as they were.  A page that the cache does not have is reported by
     ``tc_gemm_check``, and the result is invalid.  All sums are 32-bit and have one order."""
-    T, step, pages, page_size = _check_rows_of(q, nh, nkv, d, kv_cache, "tree_attention")
-    _check_ints(starts, "starts", None)
+    _tensor_calls()
+    here, i32, dtype = _current_device(), torch.int32, q.dtype
+    code = _dtype_code(q)
+    if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
+        raise KernelError(f"tree_attention: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
+    T, step = _rows_fit(q, "q", dtype, here, nh * d)
+    _fits(kv_cache, "kv_cache", dtype, here, None, 2, nkv, None, d)
+    _fits(starts, "starts", i32, here, None)
     R = starts.shape[0]
-    _check_ints(cu_rows, "cu_rows", R + 1)
-    _check_ints(block_table, "block_table", R, table=True)
-    _check_ints(masks, "masks", T, table=True)
-    _check_out_view(out, T, nh * d, q.dtype, "tree_attention")
-    _check_here("tree_attention", q, out, kv_cache, block_table, cu_rows, starts, masks)
+    _fits(cu_rows, "cu_rows", i32, here, R + 1)
+    _fits(block_table, "block_table", i32, here, R, None)
+    _fits(masks, "masks", i32, here, T, None)
+    out_rows, out_step = _rows_fit(out, "out", dtype, here, nh * d)
+    (pages, _, _, page_size, _), blocks_a_row, words = kv_cache.shape, block_table.shape[1], masks.shape[1]
+    if out_rows != T or out.shape[1] != nh * d or page_size < 1:
+        raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; pages hold {page_size} entries")
     if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
     if T == 0 or R == 0 or max_rows == 0:
         return
     G, blocks, tile_rows, tensor_cores, least = nh // nkv, num_sms(q.device), 0, 0, 1
-    if (q.dtype == torch.bfloat16 and d in (64, 128) and G <= 128 and block_table.shape[1]
-            and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)):
+    if dtype is torch.bfloat16 and d in (64, 128) and G <= 128 and blocks_a_row and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale):
         # sides of 128 queries, two a block: a stretch of the work each, or one for both where requests may bring more
         tensor_cores = 1 if max_rows <= 128 // G else 2
         tile_rows = min(max_rows, 128 // G)
@@ -2555,45 +2624,49 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     places = T * nh + workers * queries
     before_ml = _floats_before_ml(places, d)
     before_plan = before_ml + 2 * places
-    scratch = torch.empty(before_plan + 2 * (R + 1), dtype=torch.float32, device=q.device)
-    part_ml = scratch.data_ptr() + 4 * before_ml
+    scratch = _new(torch.float32, here, before_plan + 2 * (R + 1))
+    part_o = scratch.data_ptr()
     _COUNTER.value += 1                          # the parts, and the kernel that joins them
-    _ok(_fn("attention_tree", "rg_tree_attention")(
-        _ptr(q), c_int(step), _ptr(out), c_int(out.stride(0)), _ptr(kv_cache), c_int(pages), c_int(_dtype_code(q)), _ptr(block_table),
-        c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(masks), c_int(masks.shape[1]), c_int(R), c_int(T), c_int(nh), c_int(nkv),
-        c_int(d), c_int(page_size), c_float(scale), c_int(max_rows), c_int(max_context), c_int(blocks), c_int(workers), c_int(queries), c_int(least),
-        c_int(tile_rows), c_int(tensor_cores), _ptr(scratch),
-        c_void_p(part_ml), c_void_p(part_ml + 8 * places), _ptr(_tc_error_flag(q.device)), _stream()), "tree_attention")
+    _ok(_launch("attention_tree", "rg_tree_attention", "pipipiipipppiiiiiiifiiiiiiiipppp", q, step, out, out_step, kv_cache, pages, code,
+                block_table, blocks_a_row, cu_rows, starts, masks, words, R, T, nh, nkv, d, page_size, scale, max_rows, max_context, blocks, workers, queries, least, tile_rows, tensor_cores,
+                part_o, part_o + 4 * before_ml, part_o + 4 * before_plan, _tc_error_flag(q.device)), "tree_attention")
 
 
+@functools.lru_cache(maxsize=None)
 def tree_general_blocks(d: int) -> int:
     """Blocks an SM of the general kernel over trees: what its tiles leave room for in shared memory, and three by its registers."""
     row = ((d + 3) & ~3) + 4
     return max(1, min(3, (227 << 10) // (4 * ((16 + (4 if d <= 128 else 2) * 64) * row + 16 * 69) + 2304)))
 
 
-def _cache_list(caches, what: str) -> tuple:
-    """One cache or several of one shape and type, as (list, their addresses, the bytes of an element)."""
-    caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+def _cache_list(caches, what: str, here: int) -> tuple:
+    """One cache or several of one shape and type on the current device: (the first one, how many, their addresses as 64-bit numbers in
+    bytes, the bits of all addresses)."""
+    if isinstance(caches, torch.Tensor):
+        caches = (caches,)
+    elif not isinstance(caches, (list, tuple)):
+        caches = list(caches)
     if not caches:
         raise KernelError(f"{what}: no caches")
     first = caches[0]
-    shape, dtype, fits = first.shape, first.dtype, _fast.shaped if _fast is not None else None
-    for t in caches:
-        if fits is None or not fits(t, dtype, *shape):
-            _check(t, "a cache", dtype)
-            if t.shape != shape:
-                raise KernelError(f"{what}: caches of {tuple(shape)} and {tuple(t.shape)}")
-    _check_here(what, *caches)
-    addresses = (ctypes.c_ulonglong * len(caches))(*[t.data_ptr() for t in caches])
-    return caches, addresses, first.element_size()
+    addresses = _tensors.addresses(caches, here) if _tensors else None
+    if addresses is None:
+        for t in caches:
+            _check(t, "a cache", first.dtype)
+            if t.get_device() != here:
+                raise KernelError(f"{what}: a cache on {t.device}, the current device is cuda:{here}")
+            if t.shape != first.shape:
+                raise KernelError(f"{what}: caches of {tuple(first.shape)} and {tuple(t.shape)}")
+        addresses = np.array([t.data_ptr() for t in caches], dtype=np.uint64).tobytes()
+    bits = 0
+    for i in range(0, len(addresses), 8):            # only the lowest four bits are of interest
+        bits |= addresses[i]
+    return first, len(caches), addresses, bits
 
 
-def _unit(row_bytes: int, addresses) -> int:
+def _unit(row_bytes: int, bits: int) -> int:
     """The largest of 16, 8, 4, 2 and 1 bytes that rows and addresses are multiples of."""
-    low = row_bytes | 16
-    for a in addresses:
-        low |= a
+    low = row_bytes | bits | 16
     return low & -low
 
 
@@ -2608,33 +2681,29 @@ def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, m
     (``PageAllocator.shrink``).  The pages are the request's own from ``starts`` on.  ``max_rows``, up to 4,096: the most rows of a request; rows
     beyond are left out, and requests without rows or with a negative start have a count of 0.  An entry that table or
     cache do not have does not move, and ``tc_gemm_check`` reports it."""
-    caches, addresses, size = _cache_list(caches, "keep_drafts")
-    shape = caches[0].shape
-    if len(shape) < 3 or caches[0].numel() == 0:
+    _tensor_calls()
+    here, i32 = _current_device(), torch.int32
+    first, n_caches, addresses, bits = _cache_list(caches, "keep_drafts", here)
+    shape, numel = first.shape, first.numel()
+    if len(shape) < 3 or numel == 0:
         raise KernelError(f"keep_drafts: a cache is [pages, .., page, x], not {tuple(shape)}")
-    _check_ints(starts, "starts", None)
-    R = starts.shape[0]
-    _check_ints(parents, "parents", None)
-    T = parents.shape[0]
-    _check_ints(cu_rows, "cu_rows", R + 1)
-    _check_ints(block_table, "block_table", R, table=True)
-    _check_ints(tokens, "tokens", T)
-    _check_ints(chosen, "chosen", T)
-    _check_here("keep_drafts", block_table, cu_rows, starts, parents, tokens, chosen)
+    _fits(starts, "starts", i32, here, None)
+    _fits(parents, "parents", i32, here, None)
+    R, T = starts.shape[0], parents.shape[0]
+    _fits(cu_rows, "cu_rows", i32, here, R + 1)
+    _fits(block_table, "block_table", i32, here, R, None)
+    _fits(tokens, "tokens", i32, here, T)
+    _fits(chosen, "chosen", i32, here, T)
     if not 0 <= max_rows <= DRAFT_MOST:
         raise KernelError(f"keep_drafts: up to {DRAFT_MOST} rows a request, not {max_rows}")
-    device = starts.device
-    counts = torch.empty(R, dtype=torch.int32, device=device)
-    path = torch.empty((2, R, max_rows), dtype=torch.int32, device=device)
-    pages, page_size, outer = shape[0], shape[-2], caches[0].numel() // (shape[0] * shape[-2] * shape[-1])
-    piece = _unit(shape[-1] * size, addresses)
-    _COUNTER.value += (len(caches) - 1) // 64
-    _ok(_fn("drafts", "rg_keep_drafts")(
-        _at(addresses), c_int(len(caches)), c_int(pages), c_int(outer), c_int(page_size), c_int(shape[-1] * size // piece), c_int(piece),
-        _ptr(block_table), c_int(block_table.shape[1]), _ptr(cu_rows), _ptr(starts), _ptr(parents), _ptr(tokens), _ptr(chosen), c_int(R), c_int(T),
-        c_int(max_rows), _ptr(counts), _ptr(path), c_void_p(path.data_ptr() + 4 * R * max_rows), c_int(num_sms(device)),
-        _ptr(_tc_error_flag(device)), _stream()), "keep_drafts")
-    return counts, path[0], path[1]
+    counts, path, fresh = _new(i32, here, R), _new(i32, here, R, max_rows), _new(i32, here, R, max_rows)
+    row_bytes = shape[-1] * first.element_size()
+    piece = _unit(row_bytes, bits)
+    _COUNTER.value += (n_caches - 1) // 64
+    _ok(_launch("drafts", "rg_keep_drafts", "piiiiiipipppppiiipppip", addresses, n_caches, shape[0],
+                numel // (shape[0] * shape[-2] * shape[-1]), shape[-2], row_bytes // piece, piece, block_table, block_table.shape[1], cu_rows, starts, parents, tokens, chosen, R, T, max_rows, counts, path, fresh,
+                num_sms(starts.device), _tc_error_flag(starts.device)), "keep_drafts")
+    return counts, path, fresh
 
 
 def copy_pages(caches, copies) -> None:
@@ -2643,26 +2712,26 @@ def copy_pages(caches, copies) -> None:
     ``held`` entries of page ``from`` (-1: all of it) to page ``to``; what lies behind them there is left alone.  A page may be
     copied several times; one that is written is written once and read by no copy, so that their order does not matter (a copy of a
     page to itself is none).  The copies are arguments of the launch: a captured graph repeats these."""
-    caches, addresses, size = _cache_list(caches, "copy_pages")
-    copies = np.asarray(copies) if len(copies) else np.empty((0, 3), np.int32)
-    if copies.ndim != 2 or copies.shape[1] != 3 or copies.dtype.kind not in "iu" or (
-            copies.dtype != np.int32 and np.abs(copies.astype(np.float64)).max() >= 1 << 31):
-        raise KernelError(f"copy_pages: copies are whole numbers [n, 3] of 32 bits, not {copies.dtype} {copies.shape}")
-    copies = np.ascontiguousarray(copies, dtype=np.int32)
-    shape, numel = caches[0].shape, caches[0].numel()
+    _tensor_calls()
+    first, n_caches, addresses, bits = _cache_list(caches, "copy_pages", _current_device())
+    if not (type(copies) is np.ndarray and copies.dtype == np.int32 and copies.ndim == 2 and copies.shape[1] == 3 and copies.flags.c_contiguous):
+        copies = np.asarray(copies) if len(copies) else np.empty((0, 3), np.int32)
+        if copies.ndim != 2 or copies.shape[1] != 3 or copies.dtype.kind not in "iu" or (copies.size and max(
+                abs(int(copies.max())), abs(int(copies.min()))) >= 1 << 31):
+            raise KernelError(f"copy_pages: copies are whole numbers [n, 3] of 32 bits, not {copies.dtype} {copies.shape}")
+        copies = np.ascontiguousarray(copies, dtype=np.int32)
+    shape, numel, n, size = first.shape, first.numel(), len(copies), first.element_size()
     if len(shape) < 1:
         raise KernelError("copy_pages: a cache is [pages, ..]")
-    if len(copies) == 0:
+    if n == 0:
         return
     pages = shape[0]
     if numel == 0:
         raise KernelError(f"copy_pages: caches of {tuple(shape)} have no pages to copy")
     page_size, entry = (shape[-2], shape[-1] * size) if len(shape) >= 3 else (1, numel // pages * size)
-    outer = numel * size // (pages * page_size * entry)
-    _COUNTER.value += -(-len(copies) // 256) * -(-len(caches) // 64) - 1
-    code = _fn("page_copy", "rg_copy_pages")(_at(addresses), c_int(len(caches)), c_int(pages), c_int(outer), c_int(page_size), c_longlong(entry),
-                                             c_int(_unit(entry, addresses)), c_void_p(copies.ctypes.data), c_int(len(copies)),
-                                             c_int(num_sms(caches[0].device)), _stream())
+    _COUNTER.value += -(-n // 256) * -(-n_caches // 64) - 1
+    code = _launch("page_copy", "rg_copy_pages", "piiiiiipii", addresses, n_caches, pages, numel * size // (pages * page_size * entry), page_size,
+                   entry, _unit(entry, bits), copies.ctypes.data, n, num_sms(first.device))
     if code in (10002, 10003):
         raise KernelError("copy_pages: " + ("pages and numbers of entries are those of the caches" if code == 10002
                                             else "a page that is written is written once and read by no copy"))
