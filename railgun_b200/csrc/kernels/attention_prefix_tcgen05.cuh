@@ -29,10 +29,11 @@
 #define PT_BN 64                   // entries of a softmax pass
 #define PT_STAGE 128               // entries of a K or V stage
 #define PT_THREADS 384             // warps 0-3, 4-7: softmax of side 0, 1; 8, 10: TMA of K (and Q), of V; 9, 11: MMA issue of side 0, 1
+#define PT_BARRIERS 384            // bytes
 __host__ __device__ constexpr int pt_k_stages(int pieces) { return pieces == 1 ? 5 : 3; }
 __host__ __device__ constexpr int pt_v_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 __host__ __device__ constexpr int pt_smem(int pieces) {
-    return (2 + pt_k_stages(pieces) + pt_v_stages(pieces)) * PT_SIDE * 128 * pieces + 256 + 1024;
+    return (2 + pt_k_stages(pieces) + pt_v_stages(pieces)) * PT_SIDE * 128 * pieces + PT_BARRIERS + 1024;
 }
 
 __device__ __forceinline__ void store8(float* p, const uint32_t (&v)[32], int i) {      // 32 bytes: a whole sector of the row
@@ -51,9 +52,12 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     constexpr uint32_t PIECE = PT_STAGE * 128, TILE = PIECE * PIECES, SUB = PT_BN * 128;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t sQ = base, sK0 = sQ + 2 * TILE, sV0 = sK0 + NK * TILE, bars = sV0 + NV * TILE;
-    const uint32_t q_full = bars, k_full0 = bars + 8, k_empty0 = k_full0 + 8 * NK, v_full0 = k_empty0 + 8 * NK, v_empty0 = v_full0 + 8 * NV,
+    // A stage is full on the barrier of the side whose tile it holds (side 0's, where the tile is both sides').  A wait goes by the parity of
+    // a phase, so that who waits has to have seen all phases before: of barriers that both sides' tiles came through in turn, a side would
+    // see every second one, and take its tile for loaded while the other side's before it was still on its way.
+    const uint32_t q_full = bars, k_full0 = bars + 8, k_empty0 = k_full0 + 16 * NK, v_full0 = k_empty0 + 8 * NK, v_empty0 = v_full0 + 16 * NV,
                    s_full0 = v_empty0 + 8 * NV, p_full0 = s_full0 + 32, p_free0 = p_full0 + 32;    // per side and half stage
-    static_assert(8 + 16 * (NK + NV) + 32 + 64 <= 256, "the barriers have 256 bytes");
+    static_assert(8 + 24 * (NK + NV) + 32 + 64 <= PT_BARRIERS, "the barriers' place");
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -83,8 +87,10 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const uint32_t users = two_parts || n_kt1 == 0 ? 1 : 2;
         abort_flag = 0;
         mbar_init(q_full, 1);
-        for (int s = 0; s < NK; ++s) { mbar_init(k_full0 + 8 * s, 1); mbar_init(k_empty0 + 8 * s, users); }
-        for (int s = 0; s < NV; ++s) { mbar_init(v_full0 + 8 * s, 1); mbar_init(v_empty0 + 8 * s, users); }
+        for (int s = 0; s < 2 * NK; ++s) mbar_init(k_full0 + 8 * s, 1);
+        for (int s = 0; s < 2 * NV; ++s) mbar_init(v_full0 + 8 * s, 1);
+        for (int s = 0; s < NK; ++s) mbar_init(k_empty0 + 8 * s, users);
+        for (int s = 0; s < NV; ++s) mbar_init(v_empty0 + 8 * s, users);
         for (int b = 0; b < 4; ++b) { mbar_init(s_full0 + 8 * b, 1); mbar_init(p_full0 + 8 * b, PT_SIDE); mbar_init(p_free0 + 8 * b, 1); }
         fence_barrier_init();
     }
@@ -127,7 +133,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             const int page = page_next, e = first_of(s) + J * PT_STAGE + box * box_rows, in_page = e & (a.page_size - 1);
             page_next = page_of(b + 1);
             const int st = b % n, u = b / n;
-            const uint32_t full = (kv ? v_full0 : k_full0) + 8 * st, empty = (kv ? v_empty0 : k_empty0) + 8 * st;
+            const uint32_t full = (kv ? v_full0 : k_full0) + 8 * (st + n * s), empty = (kv ? v_empty0 : k_empty0) + 8 * st;
             if (u > 0) ok = mbar_wait_all(empty, (u & 1) ^ 1, err, 51 + kv, &abort_flag);
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(full, TILE);
@@ -145,12 +151,15 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         constexpr uint32_t idesc_s = make_idesc(PT_SIDE, PT_BN, false), idesc_o = make_idesc(PT_SIDE, D, true);
         const bool issuer = elect_one();
         const uint64_t qd = desc_k_major(sQ + (two_parts ? 0 : s) * TILE);
-        // where this side's K and V tiles are in their rings: stage and phase, `step` stages of the stream from one to the next
-        int ki = two_parts ? s : 0, vi = ki, k_phase = 0, v_phase = 0;
+        // where this side's K and V tiles are in their rings, `step` stages of the stream from one to the next
+        const uint32_t k_full = k_full0 + (two_parts ? 8 * NK * s : 0), v_full = v_full0 + (two_parts ? 8 * NV * s : 0);
+        int ki = two_parts ? s : 0, vi = ki;
+        uint32_t k_phase = 0, v_phase = 0;                            // a bit a stage: the phase that this side waits for
         auto step = [&](int J) -> int { return two_parts && (s || J < n_st1) ? 2 : 1; };   // from tile J to tile J + 1
-        auto ahead = [&](int& i, int& phase, int by, int n) {
+        auto ahead = [&](int& i, uint32_t& phase, int by, int n) {    // from a stage that has been waited for
+            phase ^= 1u << i;
             i += by;
-            if (i >= n) { i -= n; phase ^= 1; }
+            if (i >= n) i -= n;
         };
         auto issue_s = [&](int half, bool last) {                     // the next pass's scores: K is there
             if (issuer) {
@@ -167,12 +176,12 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         };
         bool ok = n_kt > 0;
         if (ok) ok = mbar_wait_all(q_full, 0, err, 53, &abort_flag);
-        if (ok) ok = mbar_wait_all(k_full0 + 8 * ki, 0, err, 54, &abort_flag);
+        if (ok) ok = mbar_wait_all(k_full + 8 * ki, 0, err, 54, &abort_flag);
         if (ok) { tc_fence_after(); issue_s(0, n_kt == 1); }
         if (ok && n_kt > 1) issue_s(1, true);                         // the same stage
         const int tail = end_of(s) - first_of(s) - (n_kt - 1) * PT_BN;    // entries of the last pass
         for (int J = 0; J < n_st && ok; ++J) {
-            ok = mbar_wait_all(v_full0 + 8 * vi, v_phase, err, 55, &abort_flag);
+            ok = mbar_wait_all(v_full + 8 * vi, v_phase >> vi & 1, err, 55, &abort_flag);
             if (J + 1 < n_st) ahead(ki, k_phase, step(J), NK);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -190,7 +199,7 @@ prefix_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
                     __syncwarp();
                 }
                 const bool next = j + 2 < n_kt;
-                if (half == 0 && next) ok = mbar_wait_all(k_full0 + 8 * ki, k_phase, err, 54, &abort_flag);
+                if (half == 0 && next) ok = mbar_wait_all(k_full + 8 * ki, k_phase >> ki & 1, err, 54, &abort_flag);
                 if (ok) ok = mbar_wait_all(p_full0 + 16 * s + 8 * half, J & 1, err, 56, &abort_flag);
                 if (!ok) break;
                 tc_fence_after();
