@@ -25,15 +25,37 @@
 #define TT_BN 64                   // entries of a softmax pass
 #define TT_STAGE 128               // entries of a K or V stage: a tile
 #define TT_THREADS 384             // warps 0-3, 4-7: softmax of side 0, 1; 8, 10: TMA of K, of V; 9, 11: MMA issue (and TMA of Q) of side 0, 1
+#define TT_BARRIERS 384            // bytes
 __host__ __device__ constexpr int tt_k_stages(int pieces) { return pieces == 1 ? 5 : 3; }
 __host__ __device__ constexpr int tt_v_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 __host__ __device__ constexpr int tt_smem(int pieces) {
-    return (2 + tt_k_stages(pieces) + tt_v_stages(pieces)) * TT_SIDE * 128 * pieces + 256 + 1024;
+    return (2 + tt_k_stages(pieces) + tt_v_stages(pieces)) * TT_SIDE * 128 * pieces + TT_BARRIERS + 1024;
 }
 
 __device__ __forceinline__ void tt_store8(float* p, const uint32_t (&v)[32], int i) {      // 32 bytes: a whole sector of the row
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]),
                  "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7]) : "memory");
+}
+
+// mbar_wait_all for three barriers at once.
+__device__ __forceinline__ bool wait_all_of(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2, int* err, int code,
+                                            volatile int* abort_flag) {
+    for (uint32_t i = 0; i < RG_SPIN_LIMIT; ++i) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p, q, r;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+                     "and.pred p, p, q;\n\t"
+                     "and.pred p, p, r;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(b0), "r"(p0), "r"(b1), "r"(p1), "r"(b2), "r"(p2) : "memory");
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if ((i & 1023u) == 1023u && __any_sync(0xffffffffu, *abort_flag)) return false;
+    }
+    atomicCAS(err, 0, code);
+    *abort_flag = 1;
+    return false;
 }
 
 // Which of the 64 entries from e on row t sees (n of them are there; n >= 1): those before start, and the nodes that its mask has.
@@ -62,9 +84,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     constexpr uint32_t PIECE = TT_STAGE * 128, TILE = PIECE * PIECES, SUB = TT_BN * 128;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t sQ = base, sK0 = sQ + 2 * TILE, sV0 = sK0 + NK * TILE, bars = sV0 + NV * TILE;
-    const uint32_t q_full0 = bars, k_full0 = bars + 16, k_empty0 = k_full0 + 8 * NK, v_full0 = k_empty0 + 8 * NK, v_empty0 = v_full0 + 8 * NV,
+    // A stage is full on the barrier of the side whose tile it holds (side 0's, where the tile is both sides').  A wait goes by the parity of
+    // a phase, so that who waits has to have seen all phases before: of barriers that both sides' tiles came through in turn, a side would
+    // see every second one, and take its tile for loaded while the other side's before it was still on its way.
+    const uint32_t q_full0 = bars, k_full0 = bars + 16, k_empty0 = k_full0 + 16 * NK, v_full0 = k_empty0 + 8 * NK, v_empty0 = v_full0 + 16 * NV,
                    s_full0 = v_empty0 + 8 * NV, p_full0 = s_full0 + 32, p_free0 = p_full0 + 32;    // per side and half stage
-    static_assert(16 + 16 * (NK + NV) + 96 <= 256, "the barriers have 256 bytes");
+    static_assert(16 + 24 * (NK + NV) + 96 <= TT_BARRIERS, "the barriers' place");
     __shared__ uint32_t tmem_base_slot;
     __shared__ int abort_flag;
     __shared__ TreeStart st;
@@ -76,8 +101,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         abort_flag = 0;
         mbar_init(q_full0, 1);
         mbar_init(q_full0 + 8, 1);
-        for (int s = 0; s < NK; ++s) { mbar_init(k_full0 + 8 * s, 1); mbar_init(k_empty0 + 8 * s, users); }
-        for (int s = 0; s < NV; ++s) { mbar_init(v_full0 + 8 * s, 1); mbar_init(v_empty0 + 8 * s, users); }
+        for (int s = 0; s < 2 * NK; ++s) mbar_init(k_full0 + 8 * s, 1);
+        for (int s = 0; s < 2 * NV; ++s) mbar_init(v_full0 + 8 * s, 1);
+        for (int s = 0; s < NK; ++s) mbar_init(k_empty0 + 8 * s, users);
+        for (int s = 0; s < NV; ++s) mbar_init(v_empty0 + 8 * s, users);
         for (int b = 0; b < 4; ++b) { mbar_init(s_full0 + 8 * b, 1); mbar_init(p_full0 + 8 * b, TT_SIDE); mbar_init(p_free0 + 8 * b, 1); }
         fence_barrier_init();
     }
@@ -115,9 +142,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             w.next(a, --left > 0);
             return row;
         };
+        auto side_of = [&](int b) -> int { return !both && b < 2 * n_t1 ? b & 1 : 0; };
         auto look_up = [&](int b) -> int {                            // of stage b, one after the other
             if (b >= n_stages) return 0;
-            return !both && b < 2 * n_t1 && (b & 1) ? row_of(w1, left1) : row_of(w0, left0);
+            return side_of(b) ? row_of(w1, left1) : row_of(w0, left0);
         };
         int row_next = look_up(0);
         bool ok = true;
@@ -125,7 +153,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             const int row = row_next;
             row_next = look_up(b + 1);
             const int stage = b % n, u = b / n;
-            const uint32_t full = (kv ? v_full0 : k_full0) + 8 * stage, empty = (kv ? v_empty0 : k_empty0) + 8 * stage;
+            const uint32_t full = (kv ? v_full0 : k_full0) + 8 * (stage + n * side_of(b)), empty = (kv ? v_empty0 : k_empty0) + 8 * stage;
             if (u > 0) ok = mbar_wait_all(empty, (u & 1) ^ 1, err, 71 + kv, &abort_flag);
             if (!ok) break;
             if (lane == 0) mbar_expect_tx(full, TILE);
@@ -140,13 +168,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const bool issuer = elect_one();
         const uint32_t q_full = q_full0 + 8 * s, s_full = s_full0 + 16 * s, p_full = p_full0 + 16 * s, p_free = p_free0 + 16 * s;
         const uint64_t qd = desc_k_major(sQ + s * TILE);
-        // where this side's K and V tiles are in their rings: stage and phase, `step` stages of the stream from one to the next
-        int ki = both ? 0 : s, vi = ki, k_phase = 0, v_phase = 0, kt = 0, vt = 0;      // kt, vt: which tile of this side that is
-        auto ahead = [&](int& i, int& phase, int& t, int n) {
+        // where this side's K and V tiles are in their rings, which of its tiles that is, and a bit a stage: the phase it waits for
+        const uint32_t k_full = k_full0 + (both ? 0 : 8 * NK * s), v_full = v_full0 + (both ? 0 : 8 * NV * s);
+        int ki = both ? 0 : s, vi = ki, kt = 0, vt = 0;
+        uint32_t k_phase = 0, v_phase = 0;
+        auto ahead = [&](int& i, int& t, int n) {
             i += !both && (s || t < n_t1) ? 2 : 1;
             ++t;
-            if (i >= n) { i -= n; phase ^= 1; }
+            if (i >= n) i -= n;
         };
+        auto k_seen = [&]() { k_phase ^= 1u << ki; };
+        auto v_seen = [&]() { v_phase ^= 1u << vi; };
         int p_phase[2] = {0, 0}, q_phase = 0;
         TreeWalk w;
         if (n_t) w.at(a, st.r[both ? 0 : s], st.in[both ? 0 : s]);
@@ -169,31 +201,43 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             const int e0 = w.tile * TT_STAGE, e1 = min(w.x.entries, e0 + nt * TT_STAGE), n_kt = (e1 - e0 + TT_BN - 1) / TT_BN;
             if (row >= w.x.rows) {                                    // no queries on this side: give the tiles back
                 for (int J = 0; J < nt && ok; ++J) {
-                    ok = mbar_wait_all(k_full0 + 8 * ki, k_phase, err, 73, &abort_flag);
+                    ok = mbar_wait_all(k_full + 8 * ki, k_phase >> ki & 1, err, 73, &abort_flag);
                     if (ok && lane == 0) mbar_arrive(k_empty0 + 8 * ki);
-                    if (ok) ok = mbar_wait_all(v_full0 + 8 * vi, v_phase, err, 73, &abort_flag);
+                    if (ok) ok = mbar_wait_all(v_full + 8 * vi, v_phase >> vi & 1, err, 73, &abort_flag);
                     if (ok && lane == 0) mbar_arrive(v_empty0 + 8 * vi);
-                    ahead(ki, k_phase, kt, NK);
-                    ahead(vi, v_phase, vt, NV);
+                    k_seen();
+                    v_seen();
+                    ahead(ki, kt, NK);
+                    ahead(vi, vt, NV);
                 }
             } else {
                 // The last item's scores have all been read: its queries may go.
                 if (lane == 0) mbar_expect_tx(q_full, (uint32_t)(PIECES * 128 * group * tile_rows));
                 __syncwarp();
                 if (lane < PIECES) tma_load_3d(sQ + s * TILE + lane * PIECE, &q_map, q_full, 64 * lane, w.kvh() * group, w.x.row0 + row);
-                ok = mbar_wait_all(q_full, q_phase, err, 74, &abort_flag);
+                ok = wait_all_of(q_full, q_phase, k_full + 8 * ki, k_phase >> ki & 1, q_full, q_phase, err, 74, &abort_flag);
                 q_phase ^= 1;
-                if (ok) ok = mbar_wait_all(k_full0 + 8 * ki, k_phase, err, 75, &abort_flag);
+                k_seen();
                 if (ok) { tc_fence_after(); issue_s(0, n_kt == 1); }
                 if (ok && n_kt > 1) issue_s(1, true);                 // the same stage
                 const int tail = e1 - e0 - (n_kt - 1) * TT_BN;        // entries of the last pass
                 for (int J = 0; J < nt && ok; ++J) {
-                    ok = mbar_wait_all(v_full0 + 8 * vi, v_phase, err, 76, &abort_flag);
-                    ahead(ki, k_phase, kt, NK);
+                    ahead(ki, kt, NK);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int j = 2 * J + half;
                         if (!ok || j >= n_kt) break;
+                        const bool next = j + 2 < n_kt;
+                        // this pass's weights, and once a tile V and the next tile's K: asked for together
+                        const uint32_t p_bar = p_full + 8 * half;
+                        if (half) ok = mbar_wait_all(p_bar, p_phase[1], err, 77, &abort_flag);
+                        else {
+                            ok = wait_all_of(p_bar, p_phase[0], v_full + 8 * vi, v_phase >> vi & 1, next ? k_full + 8 * ki : p_bar,
+                                             next ? k_phase >> ki & 1 : p_phase[0], err, 76, &abort_flag);
+                            v_seen();
+                            if (next) k_seen();
+                        }
+                        if (!ok) break;
                         if (j == n_kt - 1 && tail < TT_BN) {
                             // rows of V behind the end may be anything: their weights are 0, and 0 times an infinity is no number
                             // (both sides may write the same zeros)
@@ -205,10 +249,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the product reads them
                             __syncwarp();
                         }
-                        const bool next = j + 2 < n_kt;
-                        if (half == 0 && next) ok = mbar_wait_all(k_full0 + 8 * ki, k_phase, err, 75, &abort_flag);
-                        if (ok) ok = mbar_wait_all(p_full + 8 * half, p_phase[half], err, 77, &abort_flag);
-                        if (!ok) break;
                         p_phase[half] ^= 1;
                         tc_fence_after();
                         if (issuer) {
@@ -224,7 +264,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                         // product that reads them
                         if (next) issue_s(half, half == 1 || j + 2 == n_kt - 1);
                     }
-                    ahead(vi, v_phase, vt, NV);
+                    ahead(vi, vt, NV);
                 }
             }
             done += nt;
@@ -245,6 +285,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             const int e0 = w.tile * TT_STAGE, e1 = min(w.x.entries, e0 + nt * TT_STAGE), n_kt = row_first < w.x.rows ? (e1 - e0 + TT_BN - 1) / TT_BN : 0;
             const int row = row_first + i / group, t = w.x.row0 + row;
             const bool query = i < tile_rows * group && row < w.x.rows;
+            const int plain = min(e1 - e0, max(0, w.x.start - e0)) / TT_BN;      // passes that everybody sees all of
             float m_ref = -INFINITY, l_run = 0.f;                     // reference maximum (log2 domain), row sum
             const bool idle = !__any_sync(0xffffffffu, query);        // a warp without queries only keeps the barriers going
             for (int j = 0; j < n_kt && ok; ++j) {
@@ -255,7 +296,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                 s_phase ^= 1 << half;
                 tc_fence_after();
                 if (idle) { mbar_arrive(p_full + 8 * half); o_phase ^= 1 << half; continue; }   // its lanes of P are scores: lanes have no say in one another
-                const bool edge = n < TT_BN || e + TT_BN > w.x.start;
+                const bool edge = j >= plain;
                 uint64_t seen = ~0ull;
                 if (edge) seen = query ? tree_seen(a, t, w.x.start, e, n) : 0ull;
                 uint32_t pk[TT_BN / 2];
