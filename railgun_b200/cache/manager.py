@@ -88,6 +88,7 @@ def _lib():
         lib.rg_cache_set_chunk.argtypes = [c_void_p, c_int, c_int]
         for name in ("add_request", "release", "has", "num_computed", "slot"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong]
+        lib.rg_cache_fork.argtypes = [c_void_p, c_longlong, c_longlong, c_void_p]
         for name in ("reserve", "commit", "shrink"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong, c_int]
         lib.rg_cache_can_reserve.argtypes = [c_void_p, c_longlong, c_int, c_int]
@@ -236,10 +237,21 @@ class PageAllocator:
         """The request keeps its entries 0 .. new_len - 1 only (``ops.evict_entries``): the pages behind them go back, and
         its position becomes ``new_len``.  As with ``commit``, the caller says what is there: up to what the pages that it has
         hold, entries behind the last commit that were written since among them.  Groups with windows or chunks, which go by
-        position, refuse."""
+        position, refuse, and so does a page that other requests hold as well (``fork``) and that the next token would be written to."""
         code = self._lib.rg_cache_shrink(self._h, req_id, int(new_len))
         if code:
             self._raise(code, f"shrink({req_id}, {new_len})")
+
+    def fork(self, parent: int, child: int) -> list:
+        """A new request ``child`` that goes on from where ``parent`` is (what it has committed): it shares the pages that are full, and for
+        each group's page that is full in part it has one of its own.  Returns, group by group, what is to be copied before either goes on,
+        as ``ops.copy_pages`` takes it: int32 [0 or 1, 3], (from, to, tokens held).  All groups or none.  The child's record is the parent's
+        (``set_request`` gives it a seed of its own).  From then on neither can go back (``commit``, ``shrink``) to write into a page that both hold."""
+        copies = np.empty((len(self.page_sizes), 3), dtype=np.int32)
+        slot = self._lib.rg_cache_fork(self._h, parent, child, copies.ctypes.data)
+        if slot < 0:
+            self._raise(slot, f"fork({parent}, {child})")
+        return [copies[g:g + 1] if copies[g, 0] >= 0 else copies[:0] for g in range(len(copies))]
 
     def release(self, req_id: int) -> None:
         code = self._lib.rg_cache_release(self._h, req_id)
@@ -330,7 +342,7 @@ class PageAllocator:
         return self._lib.rg_cache_num_requests(self._h)
 
     def check(self) -> None:
-        """Raise unless every page and slot is free exactly once or held exactly once."""
+        """Raise unless every page is free exactly once or held as often as it is counted, and every slot free or held exactly once."""
         code = self._lib.rg_cache_check(self._h)
         if code:
             self._raise(code, "check")
@@ -411,6 +423,27 @@ class CacheManager:
         for cid, need in self.state_needs.items():
             self.state[cid] = torch.zeros((self.max_requests, *need.shape), dtype=getattr(torch, need.dtype),
                                           device=device)
+
+    def fork(self, parent: int, child: int) -> None:
+        """``alloc.fork`` with what there is to copy: the pages that are full in part, in all layers of a group at once, and the states of
+        fixed size, on the current stream."""
+        from .. import ops
+        copies = self.alloc.fork(parent, child)
+        try:
+            for g, some in zip(self.groups, copies):
+                if len(some):
+                    # entries that stand for several tokens, or whose number is no page's axis, are copied by whole pages
+                    shape = g.need.shape_of_page(g.page_size)
+                    if g.need.tokens_per_entry > 1 or len(shape) < 2 or shape[-2] != g.page_size:
+                        some = np.array([[some[0, 0], some[0, 1], -1]], dtype=np.int32)
+                    ops.copy_pages([self.kv[cid] for cid in g.cache_ids], some)
+            slots = [(self.alloc.slot(parent), self.alloc.slot(child), -1)]
+            for state in self.state.values():
+                if state.numel():
+                    ops.copy_pages(state.flatten(1) if state.dim() > 1 else state, slots)
+        except BaseException:
+            self.alloc.release(child)
+            raise
 
     def page_size_of(self, cache_id) -> int:
         return self.groups[self.group_of[cache_id]].page_size

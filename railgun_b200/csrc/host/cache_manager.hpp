@@ -17,10 +17,13 @@
 // Policy as in the reference's BlockAllocator
 // (crates/vllm-paged-attention/src/allocator.rs:57-86): FIFO free list
 // (pop front, push back) so that reuse order is deterministic, a reference
-// count per page, and a double free is an error.  The reference shares one
+// count per page, and a double free is an error.  Requests that were forked
+// from one another share the pages that were full then; nobody goes back to
+// write into a page that more than one request holds.  The reference shares one
 // pool between all layers (crates/vllm-paged-attention/src/block.rs:49-59);
 // here a page id addresses one page in every layer of its group.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include <deque>
 #include <unordered_map>
@@ -178,13 +181,66 @@ public:
         return CACHE_OK;
     }
 
+    // A new request that goes on from where `parent` is: it shares the pages that the parent's tokens fill, and gets one of its own
+    // for each page that they fill in part, whose entries the caller copies: copies[3 g] = {from, to, tokens held} for group g, or
+    // {-1, -1, 0} where there is nothing to copy.  Pages that the parent has reserved behind its position stay the parent's.  All groups
+    // or none.  The record is the parent's but for the request's id.  Returns the slot or a negative status.
+    int fork(int64_t parent, int64_t child, int* copies) {
+        auto it = reqs_.find(parent);
+        if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;
+        if (reqs_.count(child)) return CACHE_DUPLICATE;
+        if (free_slots_.empty()) return CACHE_OUT_OF_SLOTS;
+        const int n = records_[it->second.slot].num_computed;
+        auto part_of = [&](size_t g) -> int {                        // the page that the tokens fill in part, -1: none
+            const std::vector<int>& t = it->second.tables[g];
+            const size_t full = (size_t)(n / groups_[g].page_size);
+            return n % groups_[g].page_size && full < t.size() ? t[full] : -1;
+        };
+        for (size_t g = 0; g < groups_.size(); ++g)
+            if (part_of(g) >= 0 && groups_[g].free_list.empty()) return CACHE_OUT_OF_PAGES;
+        CacheRequest r;
+        r.tables.resize(groups_.size());
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            const std::vector<int>& t = it->second.tables[g];
+            const size_t full = std::min(t.size(), (size_t)(n / groups_[g].page_size));
+            r.tables[g].assign(t.begin(), t.begin() + (long)full);
+            r.tables[g].reserve(full + 1);
+        }
+        r.slot = free_slots_.front();
+        records_[r.slot] = records_[it->second.slot];
+        records_[r.slot].request_id = child;
+        auto made = reqs_.emplace(child, std::move(r));               // the last thing that may throw
+        it = reqs_.find(parent);
+        free_slots_.pop_front();
+        CacheRequest& c = made.first->second;
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            CacheGroup& G = groups_[g];
+            for (int p : c.tables[g])
+                if (p >= 0) ++G.refcount[p];
+            const int from = part_of(g);
+            int* copy = copies + 3 * g;
+            copy[0] = copy[1] = -1;
+            copy[2] = 0;
+            if (n % G.page_size == 0 || (size_t)(n / G.page_size) >= it->second.tables[g].size()) continue;
+            int to = -1;                                              // a page that a window has passed is nobody's
+            if (from >= 0) {
+                to = G.free_list.front();
+                G.free_list.pop_front();
+                G.refcount[to] = 1;
+                copy[0] = from; copy[1] = to; copy[2] = n % G.page_size;
+            }
+            c.tables[g].push_back(to);
+        }
+        return c.slot;
+    }
+
     // Tokens [0, new_len) are now in the cache; windowed groups give back what every later query has passed.
     int commit(int64_t id, int new_len) {
         auto it = reqs_.find(id);
         if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;
         CacheRequest& r = it->second;
         for (size_t g = 0; g < groups_.size(); ++g)
-            if (new_len > (int)r.tables[g].size() * groups_[g].page_size) return CACHE_BAD_ARGUMENT;
+            if (new_len > (int)r.tables[g].size() * groups_[g].page_size || shared_at(r, g, new_len)) return CACHE_BAD_ARGUMENT;
         records_[r.slot].num_computed = new_len;
         for (size_t g = 0; g < groups_.size(); ++g) {
             CacheGroup& G = groups_[g];
@@ -213,6 +269,8 @@ public:
         for (size_t g = 0; g < groups_.size(); ++g)
             if (new_len < 0 || groups_[g].window > 0 || groups_[g].chunk > 0 || new_len > (int)r.tables[g].size() * groups_[g].page_size)
                 return CACHE_BAD_ARGUMENT;
+        for (size_t g = 0; g < groups_.size(); ++g)
+            if (new_len % groups_[g].page_size && shared_at(r, g, new_len)) return CACHE_BAD_ARGUMENT;
         for (size_t g = 0; g < groups_.size(); ++g) {
             const size_t keep = (size_t)(new_len + groups_[g].page_size - 1) / groups_[g].page_size;
             while (r.tables[g].size() > keep) {
@@ -247,23 +305,23 @@ public:
         return it == reqs_.end() ? nullptr : &it->second;
     }
 
-    // Every page is free exactly once or held exactly once; every slot likewise.
+    // Every page is free exactly once or held as often as its count says; every slot is free or held exactly once.
     int check() const {
         for (size_t g = 0; g < groups_.size(); ++g) {
             const CacheGroup& G = groups_[g];
-            std::vector<int> seen(G.num_pages, 0);
+            std::vector<int> free(G.num_pages, 0), held(G.num_pages, 0);
             for (int p : G.free_list) {
-                if (p < 0 || p >= G.num_pages || seen[p]++) return CACHE_CORRUPT;
+                if (p < 0 || p >= G.num_pages || free[p]++) return CACHE_CORRUPT;
                 if (G.refcount[p] != 0) return CACHE_CORRUPT;
             }
             for (const auto& kv : reqs_)
                 for (int p : kv.second.tables[g]) {
                     if (p < 0) continue;
-                    if (p >= G.num_pages || seen[p]++) return CACHE_CORRUPT;
-                    if (G.refcount[p] != 1) return CACHE_CORRUPT;
+                    if (p >= G.num_pages || free[p]) return CACHE_CORRUPT;
+                    ++held[p];
                 }
             for (int p = 0; p < G.num_pages; ++p)
-                if (seen[p] != 1) return CACHE_CORRUPT;
+                if (held[p] != G.refcount[p] || (!held[p] && !free[p])) return CACHE_CORRUPT;
         }
         std::vector<int> slot_seen(max_slots_, 0);
         for (int s : free_slots_)
@@ -280,6 +338,11 @@ public:
     }
 
 private:
+    // Does the page that entry e would be written to belong to other requests as well?
+    bool shared_at(const CacheRequest& r, size_t g, int e) const {
+        const size_t i = (size_t)(e / groups_[g].page_size);
+        return i < r.tables[g].size() && r.tables[g][i] >= 0 && groups_[g].refcount[r.tables[g][i]] > 1;
+    }
     int free_page(CacheGroup& G, int p) {
         if (p < 0 || p >= G.num_pages || G.refcount[p] <= 0) return CACHE_CORRUPT;   // double free
         if (--G.refcount[p] == 0) G.free_list.push_back(p);

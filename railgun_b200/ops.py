@@ -90,6 +90,14 @@ def _launch(lib_name: str, fn_name: str, kinds: str, *args) -> int:
     return _tensors.call(*address, *args, stream)
 
 
+def _here() -> int:
+    """The current device, where a launch goes and all its tensors lie."""
+    try:
+        return _current_device()
+    except RuntimeError as e:
+        raise KernelError(f"there is no CUDA device (and no CPU path): {e}") from None
+
+
 def _fits(t, name: str, dtype, here: int, *sizes) -> None:
     """A contiguous tensor of this type on the current device, of these sizes (None: any)."""
     if _tensors and _tensors.fits(t, dtype, here, *sizes):
@@ -2569,7 +2577,7 @@ def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, starts: torch.Tenso
     ``positions`` [T] int32, starts + how many ancestors there are, for rotations.  ``max_rows``, up to 4,096: the most rows of a
     request; rows beyond, rows of requests with a negative start and rows of no request get zeros."""
     _tensor_calls()
-    here, i32 = _current_device(), torch.int32
+    here, i32 = _here(), torch.int32
     _fits(parents, "parents", i32, here, None)
     _fits(starts, "starts", i32, here, None)
     T, R = parents.shape[0], starts.shape[0]
@@ -2593,7 +2601,7 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     negative start and rows of no request are left as they were.  A page that the cache does not have is reported by
     ``tc_gemm_check``, and the result is invalid.  All sums are 32-bit and have one order."""
     _tensor_calls()
-    here, i32, dtype = _current_device(), torch.int32, q.dtype
+    here, i32, dtype = _here(), torch.int32, q.dtype
     code = _dtype_code(q)
     if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
         raise KernelError(f"tree_attention: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
@@ -2682,7 +2690,7 @@ def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, m
     beyond are left out, and requests without rows or with a negative start have a count of 0.  An entry that table or
     cache do not have does not move, and ``tc_gemm_check`` reports it."""
     _tensor_calls()
-    here, i32 = _current_device(), torch.int32
+    here, i32 = _here(), torch.int32
     first, n_caches, addresses, bits = _cache_list(caches, "keep_drafts", here)
     shape, numel = first.shape, first.numel()
     if len(shape) < 3 or numel == 0:
@@ -2713,7 +2721,7 @@ def copy_pages(caches, copies) -> None:
     copied several times; one that is written is written once and read by no copy, so that their order does not matter (a copy of a
     page to itself is none).  The copies are arguments of the launch: a captured graph repeats these."""
     _tensor_calls()
-    first, n_caches, addresses, bits = _cache_list(caches, "copy_pages", _current_device())
+    first, n_caches, addresses, bits = _cache_list(caches, "copy_pages", _here())
     if not (type(copies) is np.ndarray and copies.dtype == np.int32 and copies.ndim == 2 and copies.shape[1] == 3 and copies.flags.c_contiguous):
         copies = np.asarray(copies) if len(copies) else np.empty((0, 3), np.int32)
         if copies.ndim != 2 or copies.shape[1] != 3 or copies.dtype.kind not in "iu" or (copies.size and max(

@@ -180,3 +180,136 @@ def test_shrink_gives_the_pages_behind_back():
     b.reserve(1, 8)
     with pytest.raises(CacheError):
         b.shrink(1, 4)                                 # a window goes by position
+
+
+def test_a_fork_shares_full_pages_and_copies_the_one_that_is_being_filled():
+    a = PageAllocator([4, 8], [10, 6], [0, 0], 4)
+    a.add_request(1)
+    a.reserve(1, 18)                                    # pages behind the position stay the parent's
+    a.commit(1, 10)
+    a.set_request(1, prompt_len=7, temperature=0.5, seed=9)
+    copies = a.fork(1, 2)
+    parent, child = a.block_table(1, 0).tolist(), a.block_table(2, 0).tolist()
+    assert child[:2] == parent[:2] and len(child) == 3 and child[2] not in parent
+    assert [c.tolist() for c in copies] == [[[parent[2], child[2], 2]], [[a.block_table(1, 1)[1], a.block_table(2, 1)[1], 2]]]
+    assert all(c.dtype == np.int32 for c in copies)
+    assert a.num_computed(2) == 10 and a.record(2)["request_id"] == 2 and a.record(2)["prompt_len"] == 7 and a.record(2)["seed"] == 9
+    assert a.free_pages(0) == 10 - 5 - 1 and a.free_pages(1) == 6 - 3 - 1
+    a.check()
+    # a fork of the fork where the pages are full: nothing to copy
+    a.reserve(2, 16)
+    a.commit(2, 16)
+    assert [c.tolist() for c in a.fork(2, 3)] == [[], []]
+    assert a.block_table(3, 0).tolist() == a.block_table(2, 0).tolist()
+    a.check()
+    # nobody writes into what is shared
+    with pytest.raises(CacheError):
+        a.commit(1, 7)
+    with pytest.raises(CacheError):
+        a.shrink(3, 13)
+    with pytest.raises(CacheError):
+        a.commit(3, 12)                                 # the page from 12 on is shared
+    with pytest.raises(CacheError):
+        a.shrink(3, 12)                                 # and in the other group it would be in the middle of one
+    a.shrink(3, 8)
+    a.reserve(3, 9)
+    assert a.block_table(3, 0)[2] not in a.block_table(2, 0).tolist()
+    a.check()
+    a.commit(1, 11)                                     # its own page
+    a.commit(1, 10)
+    before = a.free_pages(0)
+    a.release(1)
+    assert a.free_pages(0) == before + 3                # two of five pages are others' as well
+    a.check()
+    a.release(2)
+    a.release(3)
+    assert a.free_pages(0) == 10 and a.free_pages(1) == 6 and a.free_slots() == 4
+    a.check()
+
+
+def test_a_fork_takes_all_or_nothing():
+    a = PageAllocator([4, 8], [3, 3], [0, 0], 2)
+    a.add_request(1)
+    a.reserve(1, 10)
+    a.commit(1, 10)                                     # all pages of the first group
+    with pytest.raises(OutOfPages):
+        a.fork(1, 2)
+    assert not a.has(2) and a.free_pages(1) == 1 and a.free_slots() == 1
+    a.check()
+    a.shrink(1, 8)
+    a.fork(1, 2)
+    with pytest.raises(CacheError):
+        a.fork(1, 3)                                    # no slot
+    with pytest.raises(CacheError):
+        a.fork(1, 2)                                    # there is one
+    with pytest.raises(CacheError):
+        a.fork(7, 8)
+    a.check()
+    empty = PageAllocator([4], [2], [0], 2)
+    empty.add_request(1)
+    assert [c.tolist() for c in empty.fork(1, 2)] == [[]] and empty.block_table(2).tolist() == []
+    empty.check()
+
+
+def test_forks_with_windows_and_chunks():
+    """Pages that a window has passed are nobody's; shared ones go back when the last request has passed them."""
+    a = PageAllocator([4, 4], [12, 12], [6, 0], 3, chunks=[0, 8])
+    a.add_request(1)
+    a.reserve(1, 14)
+    a.commit(1, 14)
+    free = [a.free_pages(g) for g in range(2)]
+    copies = a.fork(1, 2)
+    for g in range(2):
+        parent, child = a.block_table(1, g).tolist(), a.block_table(2, g).tolist()
+        assert parent[:3] == child[:3] and copies[g].tolist() == [[parent[3], child[3], 2]] and a.free_pages(g) == free[g] - 1
+    a.check()
+    a.reserve(1, 30)
+    a.commit(1, 30)
+    a.check()
+    held = [p for g in range(2) for p in a.block_table(2, g).tolist() if p >= 0]
+    assert held and a.num_computed(2) == 14
+    a.release(1)
+    a.check()
+    a.reserve(2, 30)
+    a.commit(2, 30)
+    a.check()
+    a.release(2)
+    assert [a.free_pages(g) for g in range(2)] == [12, 12]
+    a.check()
+
+
+def test_random_forks_keep_the_books():
+    rng = np.random.default_rng(4)
+    pages = [40, 25]
+    a = PageAllocator([3, 5], pages, [0, 7], 9)
+    live = {}
+    for step in range(3000):
+        kind = rng.integers(5)
+        if kind == 0 and len(live) < 9:
+            a.add_request(step)
+            live[step] = 0
+        elif kind == 1 and live:
+            parent = int(rng.choice(list(live)))
+            try:
+                a.fork(parent, step)
+                live[step] = live[parent]
+            except CacheError:
+                assert not a.has(step)
+        elif kind in (2, 3) and live:
+            rid = int(rng.choice(list(live)))
+            n = live[rid] + int(rng.integers(1, 9))
+            try:
+                a.reserve(rid, n)
+                a.commit(rid, n)
+                live[rid] = n
+            except OutOfPages:
+                pass
+        elif live:
+            rid = int(rng.choice(list(live)))
+            a.release(rid)
+            del live[rid]
+        a.check()
+    for rid in live:
+        a.release(rid)
+    a.check()
+    assert [a.free_pages(g) for g in range(2)] == pages
