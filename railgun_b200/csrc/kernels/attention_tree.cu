@@ -1,6 +1,7 @@
 // Attention of trees of drafted tokens over the paged cache and over one another.  attention_tree.cuh says what is computed and
 // how it is cut.
 #include "attention_tree.cuh"
+#include "attention_tree_rows.cuh"
 #include "attention_tree_tcgen05.cuh"
 #include "mma.cuh"
 
@@ -24,41 +25,41 @@ template <> struct Quad<bf16> {
 __host__ __device__ inline int tg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
 __host__ __device__ inline int tg_stages(int d) { return d <= 128 ? 2 : 1; }   // tiles of K and V in shared memory: the next one is on its way
 
-__device__ __forceinline__ bool node_seen(const TreeArgs& a, int row, int node) {
-    return (node >> 5) < a.words && (a.masks[(size_t)row * a.words + (node >> 5)] >> (node & 31) & 1);
-}
-// Where entry e of request r is in the cache (its key of kv head kvh); a page that the cache does not have is reported, and read
-// as its first one.
-__device__ __forceinline__ long long entry_at(const TreeArgs& a, int r, int kvh, int e) {
-    int page = a.block_table[(size_t)r * a.max_blocks + e / a.page_size];
-    if ((unsigned)page >= (unsigned)a.pages) { atomicCAS(a.err, 0, RG_BAD_PAGE); page = 0; }
-    return (((long long)page * 2 * a.nkv + kvh) * a.page_size + e % a.page_size) * a.d;
-}
-
 // ---------------------------------------------------------------------------------------------------
 // Any head size up to 256, any page size, 32-bit or bfloat16 storage, all arithmetic in 32-bit.
 // Per tile of 64 entries: 2 queries x 4 entries of scores a thread, then a column of the output for all 16 queries a thread;
 // DP = 32 or 64: as many threads share the columns, and TG_THREADS / DP groups of them share the tile's entries.
+// WHOLE: an item to a cluster, whose blocks share its tiles, join through each other's shared memory and leave the output.
 // ---------------------------------------------------------------------------------------------------
-template <typename A, int DP, bool VEC>
-__global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs a) {
+template <typename A, int DP, bool VEC, bool WHOLE>
+__global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs a, A* __restrict__ out, int out_ld, int q_blocks) {
     extern __shared__ __align__(16) float smem[];
     constexpr int GROUPS = TG_THREADS / DP, COLS = DP == 128 ? 2 : 1;
     __shared__ TreeStart st;
     __shared__ long long row_at[2][TG_K];                           // where the rows of a tile are in the cache, -1 behind its end
     pdl_wait();
     pdl_trigger();
-    tree_plan<TG_THREADS>(a, blockIdx.x, 1, 0, st);
-    if (st.r[0] < 0) return;
+    TreeWalk w, ahead;                                              // this tile, and the one whose rows are looked up
+    int n_tiles, C = 1, rank = 0;
+    if constexpr (WHOLE) {
+        C = cg::this_cluster().num_blocks();
+        rank = cg::this_cluster().block_rank();
+        if (!tree_item(a, blockIdx.x / C, q_blocks, w)) return;      // all blocks of the cluster
+        const int per = (w.x.tiles + C - 1) / C;
+        w.tile = min(w.x.tiles, rank * per);
+        n_tiles = min(w.x.tiles, w.tile + per) - w.tile;
+    } else {
+        tree_plan<TG_THREADS>(a, blockIdx.x, 1, 0, st);
+        if (st.r[0] < 0) return;
+        n_tiles = (int)min(st.per, st.total - (long long)blockIdx.x * st.per);
+        w.at(a, st.r[0], st.in[0]);
+    }
     const int d = a.d, ld = tg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = tg_stages(d);
     float* qs = smem;                                               // [16][ld]
     float* kv0 = qs + TG_Q * ld;                                    // [stages][K [64][ld], V [64][ld]]
     float* ps = kv0 + stages * 2 * TG_K * ld;                       // [16][TG_LD]
     float* al = ps + TG_Q * TG_LD;                                  // [16]
     const size_t to_values = (size_t)a.nkv * a.page_size * d;
-    const int n_tiles = (int)min(st.per, st.total - (long long)blockIdx.x * st.per);
-    TreeWalk w, ahead;                                              // this tile, and the one whose rows are looked up
-    w.at(a, st.r[0], st.in[0]);
     ahead = w;
     int looked = 0;
     auto look_up = [&](int slot) {                                  // of the next tile that has not been; the whole block
@@ -102,29 +103,32 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     const int col = tid % DP, part = tid / DP;                      // output: column(s) col (+ 128), entries part + GROUPS j
     float m[2], l[2];
     float acc[COLS][TG_Q];
-    int q0 = 0, nq = 0;
+    int q0 = 0, nq = 0, parts = 0, done = 0;                        // parts of the item, 0: it began before this stretch
+    auto begin = [&]() {                                            // an item
+        q0 = w.block() * TG_Q;
+        nq = min(TG_Q, w.x.rows * group - q0);
+        if constexpr (!WHOLE) parts = w.tile == 0 ? w.parts(done, st.per) : 0;
+        for (int j = tid; j < TG_Q * ld; j += TG_THREADS) {         // nobody reads the last item's any more
+            const int row = j / ld, c = j - row * ld, qi = q0 + row;
+            float v = 0.f;
+            if (row < nq && c < d)
+                v = to_f32(((const A*)a.q)[(size_t)(w.x.row0 + qi / group) * a.q_stride + (w.kvh() * group + qi % group) * d + c]) * a.scale_log2;
+            qs[j] = v;
+        }
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+            for (int j = 0; j < TG_Q; ++j) acc[c][j] = 0.f;
+    };
     look_up(0);
     look_up(1);
     __syncthreads();
-    if (stages == 2) request(0, kv0);
+    if (stages == 2 && n_tiles > 0) request(0, kv0);
+    if (WHOLE) begin();
     for (int step = 0; step < n_tiles; ++step) {
-        if (step == 0 || w.tile == 0) {                                // an item begins
-            q0 = w.block() * TG_Q;
-            nq = min(TG_Q, w.x.rows * group - q0);
-            for (int j = tid; j < TG_Q * ld; j += TG_THREADS) {     // nobody reads the last item's any more
-                const int row = j / ld, c = j - row * ld, qi = q0 + row;
-                float v = 0.f;
-                if (row < nq && c < d)
-                    v = to_f32(((const A*)a.q)[(size_t)(w.x.row0 + qi / group) * a.q_stride + (w.kvh() * group + qi % group) * d + c]) * a.scale_log2;
-                qs[j] = v;
-            }
-            m[0] = m[1] = -INFINITY;
-            l[0] = l[1] = 0.f;
-#pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int j = 0; j < TG_Q; ++j) acc[c][j] = 0.f;
-        }
+        if (!WHOLE && (step == 0 || w.tile == 0)) { done = step; begin(); }
         const int slot = step & 1, e0 = w.tile * TG_K, n = min(TG_K, w.x.entries - e0);
         float* ks = kv0 + (stages == 2 ? slot * 2 * TG_K * ld : 0);
         const float* vs = ks + TG_K * ld;
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
                 }
             }
         }
-        if (step + 1 == n_tiles || w.last_tile()) {                    // the item, or the stretch, ends: leave the part
+        if (!WHOLE && (step + 1 == n_tiles || w.last_tile())) {        // the item, or the stretch, ends: leave the part
             float sums[2] = {l[0], l[1]};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -231,154 +235,226 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (2 * qa + i < nq) {
-                        a.part_ml[(place + 2 * qa + i) * 2] = m[i];
-                        a.part_ml[(place + 2 * qa + i) * 2 + 1] = sums[i];
+                        *reinterpret_cast<float2*>(a.part_ml + (place + 2 * qa + i) * 2) = make_float2(m[i], sums[i]);
+                        const int qi = q0 + 2 * qa + i;
+                        if (parts) a.parts[(size_t)(w.x.row0 + qi / group) * a.nh + w.kvh() * group + qi % group] = make_int2((int)place + 2 * qa + i, parts);
                     }
             __syncthreads();                                        // the queries, and what went through the tile, are read
         }
-        w.next(a, step + 1 < n_tiles);
+        if constexpr (WHOLE) ++w.tile;
+        else w.next(a, step + 1 < n_tiles);
+    }
+    if constexpr (WHOLE) {
+        __shared__ float fin_ml[TG_Q][2], row_ml[TG_Q][2];          // this block's M and L; the query's M and 1 / L
+        cg::cluster_group cluster = cg::this_cluster();
+        float* fin = kv0;                                           // [16][d]
+        rgmma::cp_async_wait<0>();                                  // (where there was no tile, none was waited for)
+        __syncthreads();                                            // the last tile is read
+        if constexpr (GROUPS > 1) {                                 // the groups' sums, added in their order, behind what is left
+            float* sums = kv0 + TG_Q * d;
+#pragma unroll
+            for (int i = 0; i < TG_Q; ++i) sums[i * TG_THREADS + tid] = acc[0][i];
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int i = 0; i < TG_Q; ++i)
+                    for (int g = 1; g < GROUPS; ++g) acc[0][i] += sums[i * TG_THREADS + g * DP + col];
+            }
+        }
+        if (part == 0) {
+#pragma unroll
+            for (int i = 0; i < TG_Q; ++i)
+                if (i < nq)
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c)
+                        if (col + DP * c < d) fin[i * d + col + DP * c] = acc[c][i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+            if (ka == 0) { fin_ml[2 * qa + i][0] = m[i]; fin_ml[2 * qa + i][1] = l[i]; }
+        }
+        cluster.sync();                                             // every block's result is in place
+        if (tid < nq) join_cluster_ml(cluster, &fin_ml[0][0], tid, row_ml[tid][0], row_ml[tid][1]);
+        __syncthreads();
+        const int h0 = w.kvh() * group;
+        // a warp has whole queries, so that it can work out again what is no number
+        for (int i = rank * (TG_THREADS / 32) + (tid >> 5); i < nq; i += C * (TG_THREADS / 32)) {
+            const int t = w.x.row0 + (q0 + i) / group, h = h0 + (q0 + i) % group;
+            A* to = out + (size_t)t * out_ld + (size_t)h * d;
+            bool odd = false;
+            for (int c = tid & 31; c < d; c += 32) {
+                float sum = 0.f;
+                for (int k = 0; k < C; ++k)
+                    sum += exp2f(cluster.map_shared_rank(&fin_ml[0][0], k)[i * 2] - row_ml[i][0]) * cluster.map_shared_rank(fin, k)[i * d + c];
+                sum *= row_ml[i][1];
+                odd |= !isfinite(sum);
+                to[c] = from_f32<A>(sum);
+            }
+            if (__any_sync(0xffffffffu, odd)) row_by_formula<A>(a, w.x, w.r, t, h, to, 0, d);
+        }
+        cluster.sync();                                             // nobody leaves while its results are being read
     }
 }
 
 // ---------------------------------------------------------------------------------------------------
 // Joining the parts of a row and head.
 // ---------------------------------------------------------------------------------------------------
-#define JOIN_THREADS 128
+#define JOIN_THREADS 256
 
-// Row t's request (-1: none that has it among its rows).  Whole warps, all lanes for the same row: a lane looks at every 32nd.
-__device__ __forceinline__ int request_of(const TreeArgs& a, int t) {
-    const int lane = threadIdx.x & 31;
-    unsigned hit = 0;
-    int r0 = 0;
-#pragma unroll 1
-    for (; !hit && r0 < a.R; r0 += 32) {
-        const int r = min(r0 + lane, a.R - 1), first = a.cu_rows[r], next = a.cu_rows[r + 1];
-        hit = __ballot_sync(0xffffffffu, r0 + lane < a.R && first >= 0 && t >= first && t < next);
-    }
-    return hit ? r0 - 32 + __ffs(hit) - 1 : -1;
-}
-
-// Row t, head h as the formula has it, by one warp, from the cache: entry by entry, and an entry that is not seen is not read into a
-// sum.  For rows whose output is no number or infinite: 0, the weight of an entry that is not seen, times such a value is no number.
-template <typename A>
-__device__ __noinline__ void row_by_formula(const TreeArgs& a, const TreeRequest& x, int r, int t, int h, A* to) {
-    const int lane = threadIdx.x & 31, d = a.d, group = a.nh / a.nkv, kvh = h / group;
-    const A* q = (const A*)a.q + (size_t)t * a.q_stride + (size_t)h * d;
-    const A* kv = (const A*)a.kv;
-    const size_t to_values = (size_t)a.nkv * a.page_size * d;
-    float M = -INFINITY, L = 0.f, acc[8] = {};                      // columns lane + 32 k
-    for (int e0 = 0; e0 < x.entries; e0 += 32) {
-        const int e = e0 + lane;
-        const bool seen = e < x.entries && (e < x.start || node_seen(a, t, e - x.start));
-        const long long at = seen ? entry_at(a, r, kvh, e) : 0;
-        float s = -INFINITY;
-        if (seen) {
-            s = 0.f;
-            for (int c = 0; c < d; ++c) s += to_f32(q[c]) * a.scale_log2 * to_f32(kv[at + c]);
-        }
-        const float mn = fmaxf(M, warp_max(s)), ms = mn == -INFINITY ? 0.f : mn, f = exp2f(M - ms), p = exp2f(s - ms);
-        L = L * f + warp_sum(p);
-        M = mn;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] *= f;
-        for (unsigned left = __ballot_sync(0xffffffffu, seen); left; left &= left - 1) {
-            const int j = __ffs(left) - 1;
-            const float pj = __shfl_sync(0xffffffffu, p, j);
-            const long long vj = __shfl_sync(0xffffffffu, at, j) + (long long)to_values;
-            if (pj == 0.f) continue;                                // a score of -infinity, or far below the others
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (lane + 32 * k < d) acc[k] += pj * to_f32(kv[vj + lane + 32 * k]);
-        }
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (lane + 32 * k < d) to[lane + 32 * k] = from_f32<A>(acc[k] * inv);
-}
-
-// One warp joins row t and head h, parts in their order; 4 columns a lane.
-template <typename A>
+// A thread has four columns of a row and head: PS threads share their parts where there are few rows, and a thread has ITEMS of them where
+// there are many, so that the blocks are resident at once (a block is there for two trips to memory, where the parts are and the parts
+// themselves: 16 nodes of 64 requests, 2,056 blocks of one quad a thread, 16 us; 14 with two, 17 with four).
+template <typename A, int PS, int ITEMS>
 __global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeArgs a, A* __restrict__ out, int out_ld) {
+    constexpr int COLS = JOIN_THREADS / PS;                         // threads of a share
+    __shared__ float4 s_acc[PS > 1 ? JOIN_THREADS : 1];
+    __shared__ float2 s_ml[PS > 1 ? JOIN_THREADS : 1];
     pdl_wait();
     pdl_trigger();
-    const long long i = (long long)blockIdx.x * (JOIN_THREADS / 32) + (threadIdx.x >> 5);
-    const int t = (int)(i / a.nh), h = (int)(i % a.nh), lane = threadIdx.x & 31;
-    if (t >= a.T) return;
-    const int r = request_of(a, t);
-    if (r < 0) return;
-    const TreeRequest x = tree_request(a, r);
-    if (t - x.row0 >= x.rows) return;                               // more rows than the call says
-    const int d = a.d, group = a.nh / a.nkv, kvh = h / group, qi = (t - x.row0) * group + h % group, block = qi / a.item_queries;
-    const long long per = a.plan[a.R], tile0 = a.plan[r] + ((long long)kvh * x.blocks + block) * x.tiles;
-    const int w0 = (int)(tile0 / per), n = x.tiles ? (int)((tile0 + x.tiles - 1) / per) - w0 + 1 : 0;
-    // the row's place in the first part; the next part's is item_queries further
-    const size_t place = (size_t)x.row0 * a.nh + (size_t)kvh * x.rows * group + qi + (size_t)w0 * a.item_queries;
-    float M = -INFINITY, L = 0.f;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[(place + (size_t)i * a.item_queries) * 2]);
-    M = warp_max(M);
-    if (M == -INFINITY) M = 0.f;
-    for (int i = lane; i < n; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (place + (size_t)i * a.item_queries) * 2);
-        L += ml.y * exp2f(ml.x - M);
+    const unsigned d = a.d, quads = (d + 3) / 4, share = threadIdx.x / COLS, rows = (unsigned)a.T * a.nh;    // row: t x nh + h
+    const size_t next = a.item_queries;
+    const float2* mls = reinterpret_cast<const float2*>(a.part_ml);
+    unsigned row[ITEMS], c[ITEMS];
+    int n[ITEMS], place[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const unsigned item = (blockIdx.x * ITEMS + k) * COLS + threadIdx.x % COLS;
+        row[k] = item / quads;
+        c[k] = 4 * (item - row[k] * quads);
+        const int2 where = row[k] < rows ? a.parts[row[k]] : make_int2(0, -1);
+        // (of rows in no order at all nobody may have said: nothing outside is read)
+        const bool mine = where.y >= 0 && where.x >= 0 && (long long)where.x + ((long long)where.y - 1) * a.item_queries < a.places;
+        place[k] = mine ? where.x : 0;
+        n[k] = mine ? where.y : -1;
     }
-    L = warp_sum(L);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    A* to = out + (size_t)t * out_ld + (size_t)h * d;
-    bool odd = false;
-    for (int c0 = 0; c0 < d; c0 += 128) {
-        const int c = c0 + 4 * lane;
-        float4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            float f = 0.f;
-            if (i0 + lane < n) f = exp2f(a.part_ml[(place + (size_t)(i0 + lane) * a.item_queries) * 2] - M) * inv;
-            const int some = min(32, n - i0);
-#pragma unroll 4
-            for (int i = 0; i < some; ++i) {
-                const float fi = __shfl_sync(0xffffffffu, f, i);
-                const float* from = a.part_o + (place + (size_t)(i0 + i) * a.item_queries) * d + c;
-                float4 y = {0.f, 0.f, 0.f, 0.f};
-                if (d % 4 == 0) { if (c < d) y = *reinterpret_cast<const float4*>(from); }
-                else { if (c < d) y.x = from[0]; if (c + 1 < d) y.y = from[1]; if (c + 2 < d) y.z = from[2]; if (c + 3 < d) y.w = from[3]; }
-                acc.x += fi * y.x; acc.y += fi * y.y; acc.z += fi * y.z; acc.w += fi * y.w;
+    float M[ITEMS], L[ITEMS];
+    float4 acc[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        M[k] = -INFINITY;
+        L[k] = 0.f;
+        acc[k] = {0.f, 0.f, 0.f, 0.f};
+    }
+    constexpr int AHEAD = ITEMS > 1 ? 2 : 4;                        // parts that are asked for together
+    auto some = [&](int k, int i) {                                 // parts i, i + PS, ... of item k
+        float2 ml[AHEAD];
+        float4 y[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            ml[j] = make_float2(-INFINITY, 0.f);
+            y[j] = {0.f, 0.f, 0.f, 0.f};
+            if (i + j * PS < n[k]) {
+                const size_t at = place[k] + (size_t)(i + j * PS) * next;
+                const float* from = a.part_o + at * d + c[k];
+                ml[j] = mls[at];
+                if (d % 4 == 0) y[j] = *reinterpret_cast<const float4*>(from);
+                else { y[j].x = from[0]; if (c[k] + 1 < d) y[j].y = from[1]; if (c[k] + 2 < d) y[j].z = from[2]; if (c[k] + 3 < d) y[j].w = from[3]; }
             }
         }
-        odd |= !(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w));
-        if (c < d) to[c] = from_f32<A>(acc.x);
-        if (c + 1 < d) to[c + 1] = from_f32<A>(acc.y);
-        if (c + 2 < d) to[c + 2] = from_f32<A>(acc.z);
-        if (c + 3 < d) to[c + 3] = from_f32<A>(acc.w);
+        float m = M[k];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) m = fmaxf(m, ml[j].x);
+        const float ms = m == -INFINITY ? 0.f : m, f = exp2f(M[k] - ms);
+        L[k] *= f; acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const float fj = exp2f(ml[j].x - ms);
+            L[k] += fj * ml[j].y;
+            acc[k].x += fj * y[j].x; acc[k].y += fj * y[j].y; acc[k].z += fj * y[j].z; acc[k].w += fj * y[j].w;
+        }
+        M[k] = m;
+    };
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) some(k, (int)share);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        for (int i = (int)share + AHEAD * PS; i < n[k]; i += AHEAD * PS) some(k, i);
+    if constexpr (PS > 1) {                                         // the shares, in their order (one item a thread)
+        s_acc[threadIdx.x] = acc[0];
+        s_ml[threadIdx.x] = make_float2(M[0], L[0]);
+        __syncthreads();
+        if (share == 0) {
+            float m = M[0];
+#pragma unroll
+            for (int k = 1; k < PS; ++k) m = fmaxf(m, s_ml[threadIdx.x + k * COLS].x);
+            const float ms = m == -INFINITY ? 0.f : m;
+            L[0] = 0.f;
+            acc[0] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < PS; ++k) {
+                const float2 ml = s_ml[threadIdx.x + k * COLS];
+                const float4 y = s_acc[threadIdx.x + k * COLS];
+                const float f = exp2f(ml.x - ms);
+                L[0] += f * ml.y;
+                acc[0].x += f * y.x; acc[0].y += f * y.y; acc[0].z += f * y.z; acc[0].w += f * y.w;
+            }
+        }
     }
-    if (__any_sync(0xffffffffu, odd)) row_by_formula<A>(a, x, r, t, h, to);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        bool odd = false;
+        if (n[k] >= 0 && share == 0) {
+            const float inv = L[k] == 0.f ? 0.f : 1.f / L[k];
+            const float4 v = {acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv};
+            odd = !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+            const unsigned t = row[k] / a.nh, h = row[k] - t * a.nh;
+            A* to = out + (size_t)t * out_ld + (size_t)h * d + c[k];
+            if (sizeof(A) == 2 && c[k] + 3 < d && ((uintptr_t)to & 7) == 0) {
+                *reinterpret_cast<uint2*>(to) = make_uint2(rgmma::pack_bf16(v.x, v.y), rgmma::pack_bf16(v.z, v.w));
+            } else {
+                to[0] = from_f32<A>(v.x);
+                if (c[k] + 1 < d) to[1] = from_f32<A>(v.y);
+                if (c[k] + 2 < d) to[2] = from_f32<A>(v.z);
+                if (c[k] + 3 < d) to[3] = from_f32<A>(v.w);
+            }
+        }
+        // Columns that are no numbers: the warp works them out again, from the first such column of a row and head to the last that it has.
+        for (unsigned left = __ballot_sync(0xffffffffu, odd); left;) {
+            const unsigned i = __shfl_sync(0xffffffffu, row[k], __ffs(left) - 1), same = __ballot_sync(0xffffffffu, odd && row[k] == i);
+            const int from = __shfl_sync(0xffffffffu, c[k], __ffs(same) - 1), last = __shfl_sync(0xffffffffu, c[k], 31 - __clz(same));
+            const int t = i / a.nh, h = i % a.nh, r = request_of(a, t);
+            if (r >= 0) row_by_formula<A>(a, tree_request(a, r), r, t, h, out + (size_t)t * out_ld + (size_t)h * d, from, min(a.d, last + 4));
+            left &= ~same;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------
 static size_t tg_smem(int d) { return (size_t)((TG_Q + tg_stages(d) * 2 * TG_K) * tg_row(d) + TG_Q * TG_LD + TG_Q) * sizeof(float); }
 
-static int launch_tree_general(const TreeArgs& a, int dtype, cudaStream_t s) {
+// cluster: not 0, an item to a cluster of so many blocks.
+static int launch_tree_general(const TreeArgs& a, int dtype, void* out, int out_ld, int cluster, int q_blocks, cudaStream_t s) {
     const size_t smem = tg_smem(a.d);
     const bool vec = a.d % 4 == 0 && (((uintptr_t)a.kv) & (dtype == RG_DTYPE_F32 ? 15 : 7)) == 0;
-#define RG_TG(A, DP, VEC) { RG_ALLOW_SMEM((tree_general_kernel<A, DP, VEC>), 160 * 1024) \
-    return rg_launch(tree_general_kernel<A, DP, VEC>, dim3((unsigned)a.workers), dim3(TG_THREADS), smem, s, 1, a); }
+    const long long blocks = cluster ? (long long)a.R * a.nkv * q_blocks * cluster : a.workers;
+    if (blocks > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+#define RG_TG_(A, DP, VEC, W) { RG_ALLOW_SMEM((tree_general_kernel<A, DP, VEC, W>), 160 * 1024) \
+    return rg_launch(tree_general_kernel<A, DP, VEC, W>, dim3((unsigned)blocks), dim3(TG_THREADS), smem, s, cluster, a, (A*)out, out_ld, q_blocks); }
+#define RG_TG(A, DP, VEC) { if (cluster) RG_TG_(A, DP, VEC, true) RG_TG_(A, DP, VEC, false) }
 #define RG_TG_WIDTH(A, VEC) { if (a.d <= 32) RG_TG(A, 32, VEC) if (a.d <= 64) RG_TG(A, 64, VEC) RG_TG(A, 128, VEC) }
     if (dtype == RG_DTYPE_F32) { if (vec) RG_TG_WIDTH(float, true) RG_TG_WIDTH(float, false) }
     if (vec) RG_TG_WIDTH(bf16, true)
     RG_TG_WIDTH(bf16, false)
 #undef RG_TG_WIDTH
 #undef RG_TG
+#undef RG_TG_
 }
 
-// See attention_tree.cuh for the arguments.  Scratch: plan [R + 1] on an 8-byte boundary, part_o [T nh + workers item_queries, d]
-// on one of 32 bytes and part_ml [.., 2] on one of 8.  tensor_cores: 0 tree_general_kernel; 1 tree_tc_kernel, a stretch a side; 2 the same,
-// a stretch for both sides; tile_rows: rows of a side.
+// See attention_tree.cuh for the arguments.  Scratch: part_o [T nh + workers item_queries, d] on a boundary of 32 bytes, part_ml [.., 2] and
+// parts [T, nh] on one of 8.  tensor_cores: 0 tree_general_kernel; 1 tree_tc_kernel, a stretch a side; 2 the same,
+// a stretch for both sides; tile_rows: rows of a side.  cluster: not 0, items of 16 queries to clusters of so many blocks, in one launch and
+// without scratch.
 extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out_ld, const void* kv, int num_pages, int dtype,
                                  const int* block_table, int max_blocks, const int* cu_rows, const int* starts, const int* masks, int words,
                                  int R, int T, int nh, int nkv, int d, int page_size, float scale, int max_rows, int max_context,
-                                 int blocks, int workers, int item_queries, int least, int tile_rows, int tensor_cores, float* part_o, float* part_ml, long long* plan, int* err, void* stream) {
+                                 int blocks, int workers, int item_queries, int least, int tile_rows, int tensor_cores, int cluster, float* part_o, float* part_ml,
+                                 int2* parts, int* err, void* stream) {
     if (T <= 0 || R <= 0 || max_rows <= 0) return 0;
     if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_blocks < 0 || words < 0 || max_context < 0 || out_ld < nh * d ||
-        workers < 1 || item_queries < 1 || least < 1 || ((uintptr_t)part_o & 31) || ((uintptr_t)part_ml & 7) || ((uintptr_t)plan & 7) ||
-        (long long)T * nh > 0x7fffffffll)
+        (!cluster && workers < 1) || item_queries < 1 || least < 1 || ((uintptr_t)part_o & 31) || ((uintptr_t)part_ml & 7) || ((uintptr_t)parts & 7) ||
+        (long long)T * nh + (long long)workers * item_queries > 0x7fffffffll)
         return RG_ERR_UNSUPPORTED;
     TreeArgs a = {};
     a.q = q; a.q_stride = q_stride; a.kv = kv; a.block_table = block_table; a.max_blocks = max_blocks; a.cu_rows = cu_rows; a.starts = starts;
@@ -387,15 +463,28 @@ extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out
     a.max_rows = max_rows;
     a.limit = (int)min((long long)max_context, min(0x7fffff00ll, (long long)max_blocks * page_size));
     a.workers = workers; a.item_queries = item_queries; a.least = least;
-    a.part_o = part_o; a.part_ml = part_ml; a.plan = plan; a.err = err;
+    a.part_o = part_o; a.part_ml = part_ml; a.parts = parts; a.err = err;
+    a.places = T * nh + workers * item_queries;
     a.page_shift = -1;
     for (int b = 0; b < 31; ++b) if (page_size == (1 << b)) a.page_shift = b;
     a.tile = tensor_cores ? TT_STAGE : TG_K;
+    if (cluster) {
+        if (cluster > 8 || tensor_cores || item_queries != TG_Q) return RG_ERR_UNSUPPORTED;
+        const long long q_blocks = ((long long)max_rows * (nh / nkv) + TG_Q - 1) / TG_Q;
+        if (q_blocks * nkv * R * cluster > 0x7fffffffll) return RG_ERR_UNSUPPORTED;
+        if (tree_rows_ok(a, dtype)) return launch_tree_rows(a, (bf16*)out, out_ld, cluster, (int)q_blocks, (cudaStream_t)stream);
+        return launch_tree_general(a, dtype, out, out_ld, cluster, (int)q_blocks, (cudaStream_t)stream);
+    }
     if (tensor_cores ? !tree_tc_ok(a, dtype) : item_queries != TG_Q || workers != blocks) return RG_ERR_UNSUPPORTED;
-    int e = tensor_cores ? launch_tree_tc(a, tile_rows, tensor_cores == 2, blocks, (cudaStream_t)stream) : launch_tree_general(a, dtype, (cudaStream_t)stream);
+    int e = tensor_cores ? launch_tree_tc(a, tile_rows, tensor_cores == 2, blocks, (cudaStream_t)stream) : launch_tree_general(a, dtype, out, out_ld, 0, 0, (cudaStream_t)stream);
     if (e) return e;
-    const long long joins = ((long long)T * nh + JOIN_THREADS / 32 - 1) / (JOIN_THREADS / 32);
-    if (dtype == RG_DTYPE_F32)
-        return rg_launch(tree_join_kernel<float>, dim3((unsigned)joins), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (float*)out, out_ld);
-    return rg_launch(tree_join_kernel<bf16>, dim3((unsigned)joins), dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (bf16*)out, out_ld);
+    const long long threads = (long long)T * nh * ((d + 3) / 4), joins = (threads + JOIN_THREADS - 1) / JOIN_THREADS;
+    if (threads > 0x7fff0000ll) return RG_ERR_UNSUPPORTED;
+#define RG_TJ(A, PS, ITEMS) return rg_launch(tree_join_kernel<A, PS, ITEMS>, dim3((unsigned)((threads * PS + JOIN_THREADS * ITEMS - 1) / (JOIN_THREADS * ITEMS))), \
+                                             dim3(JOIN_THREADS), 0, (cudaStream_t)stream, 1, a, (A*)out, out_ld);
+#define RG_TJ_SHARES(A) { if (joins > 592) RG_TJ(A, 1, 2) if (joins > 148) RG_TJ(A, 1, 1) RG_TJ(A, 4, 1) }
+    if (dtype == RG_DTYPE_F32) RG_TJ_SHARES(float)
+    RG_TJ_SHARES(bf16)
+#undef RG_TJ_SHARES
+#undef RG_TJ
 }

@@ -11,7 +11,9 @@
 // m = max s and l = sum 2^(s - m), s = scale log2(e) q.k, in 32-bit, and a second kernel joins the parts of every row and head:
 //   out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l,   M = max_parts m
 // A part's numbers lie at (first query of the item in all queries) + worker x (queries of an item): parts along the line never
-// meet, and T x nh + workers x (queries of an item) places are enough.
+// meet, and T x nh + workers x (queries of an item) places are enough.  Who finds an item's first part also says where it is and how
+// many there are, so that the kernel that joins takes two trips to memory: with the requests looked up and the line worked out again
+// there, 16 nodes of 64 requests took 25 us to join, X so.
 #pragma once
 #include "common.cuh"
 
@@ -26,7 +28,8 @@ struct TreeArgs {
     const int* masks;            // [T, words]
     float* part_o;               // [places, d]
     float* part_ml;              // [places, 2]
-    long long* plan;             // [R + 1]: tiles of all items before request r's; then `per`
+    int2* parts;                 // [T, nh]: where a row and head's first part is, and how many there are (-1: a row that is left as it was)
+    int places;                  // of parts
     int* err;
     int R, T, max_rows, limit;   // limit: the most entries of a request that are seen
     int q_stride, max_blocks, words, pages;
@@ -80,14 +83,36 @@ struct TreeWalk {
         skip_empty(a);
     }
     __device__ __forceinline__ bool last_tile() const { return tile + 1 == x.tiles; }
+    // In how many parts the item is cut whose first tile is a worker's `done`-th.
+    __device__ __forceinline__ int parts(int done, long long per) const { return (int)((unsigned)(done + x.tiles - 1) / (unsigned)min(per, 0x7fffffffll)) + 1; }
     // The first query of the item among all rows' and heads'.
     __device__ __forceinline__ long long first_query(const TreeArgs& a) const {
         return (long long)x.row0 * a.nh + (long long)kvh() * x.rows * (a.nh / a.nkv) + (long long)block() * a.item_queries;
     }
 };
 
+// Rows that no request has, or that no launch was sized for, have no parts and are left as they were; rows without entries have none and
+// become 0.
+template <int THREADS>
+__device__ __forceinline__ void tree_gaps(const TreeArgs& a) {
+    auto say = [&](int t, int n) {
+        for (int h = 0; h < a.nh; ++h) a.parts[(size_t)t * a.nh + h] = make_int2(0, n);
+    };
+    const int begin = max(0, min(a.cu_rows[0], a.T)), end = max(0, min(a.cu_rows[a.R], a.T));
+    for (size_t i = threadIdx.x; i < (size_t)begin * a.nh; i += THREADS) a.parts[i] = make_int2(0, -1);
+    for (size_t i = (size_t)end * a.nh + threadIdx.x; i < (size_t)a.T * a.nh; i += THREADS) a.parts[i] = make_int2(0, -1);
+    for (int r = threadIdx.x; r < a.R; r += THREADS) {
+        const TreeRequest x = tree_request(a, r);
+        const int next = min(a.cu_rows[r + 1], a.T);
+        if (x.row0 < 0) continue;
+        for (int t = x.row0 + x.rows; t < next; ++t) say(t, -1);
+        if (x.tiles == 0)
+            for (int t = x.row0; t < x.row0 + x.rows; ++t) say(t, 0);
+    }
+}
+
 // The whole block, THREADS threads: tiles of all items, and the request (with the place among its tiles) in which each of `n`
-// (up to 2) workers, `first` and `first` + `apart`, begins (r -1: it has nothing).  Block 0 leaves the plan for the joining kernel.
+// (up to 2) workers, `first` and `first` + `apart`, begins (r -1: it has nothing).  The last block says which rows nobody has.
 struct TreeStart {
     long long total, per;
     long long in[2];
@@ -131,7 +156,6 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, i
         st.r[0] = st.r[1] = -1;
     }
     __syncthreads();
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[a.R] = per;
     const bool once = a.R <= THREADS;                                    // what was found above still stands
     long long sofar = 0;
     for (int r0 = 0; r0 < a.R; r0 += THREADS) {
@@ -143,11 +167,84 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, i
             sofar += some;
         }
         if (r >= a.R) continue;
-        if (blockIdx.x == 0) a.plan[r] = before;
         for (int i = 0; i < n; ++i) {
             const long long at = (first + (long long)i * apart) * per - before;
             if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; }
         }
     }
+    if (blockIdx.x == gridDim.x - 1) tree_gaps<THREADS>(a);
     __syncthreads();
+}
+
+__device__ __forceinline__ bool node_seen(const TreeArgs& a, int row, int node) {
+    return (node >> 5) < a.words && (a.masks[(size_t)row * a.words + (node >> 5)] >> (node & 31) & 1);
+}
+// Where entry e of request r is in the cache (its key of kv head kvh); a page that the cache does not have is reported, and read
+// as its first one.
+__device__ __forceinline__ long long entry_at(const TreeArgs& a, int r, int kvh, int e) {
+    int page = a.block_table[(size_t)r * a.max_blocks + e / a.page_size];
+    if ((unsigned)page >= (unsigned)a.pages) { atomicCAS(a.err, 0, RG_BAD_PAGE); page = 0; }
+    return (((long long)page * 2 * a.nkv + kvh) * a.page_size + e % a.page_size) * a.d;
+}
+
+// Row t's request (-1: none that has it among its rows).  Whole warps, all lanes for the same row: a lane looks at every 32nd.
+__device__ __forceinline__ int request_of(const TreeArgs& a, int t) {
+    const int lane = threadIdx.x & 31;
+    unsigned hit = 0;
+    int r0 = 0;
+#pragma unroll 1
+    for (; !hit && r0 < a.R; r0 += 32) {
+        const int r = min(r0 + lane, a.R - 1), first = a.cu_rows[r], next = a.cu_rows[r + 1];
+        hit = __ballot_sync(0xffffffffu, r0 + lane < a.R && first >= 0 && t >= first && t < next);
+    }
+    return hit ? r0 - 32 + __ffs(hit) - 1 : -1;
+}
+
+// Row t, head h as the formula has it, by one warp, from the cache: entry by entry, and an entry that is not seen is not read into a
+// sum; columns from_col .. to_col - 1 are written.  For rows whose output is no number or infinite: 0, the weight of an entry that is not seen, times such a value is no number.
+template <typename A>
+__device__ __noinline__ void row_by_formula(const TreeArgs& a, const TreeRequest& x, int r, int t, int h, A* to, int from_col, int to_col) {
+    const int lane = threadIdx.x & 31, d = a.d, group = a.nh / a.nkv, kvh = h / group;
+    const A* q = (const A*)a.q + (size_t)t * a.q_stride + (size_t)h * d;
+    const A* kv = (const A*)a.kv;
+    const size_t to_values = (size_t)a.nkv * a.page_size * d;
+    float M = -INFINITY, L = 0.f, acc[8] = {};                      // columns lane + 32 k
+    for (int e0 = 0; e0 < x.entries; e0 += 32) {
+        const int e = e0 + lane;
+        const bool seen = e < x.entries && (e < x.start || node_seen(a, t, e - x.start));
+        const long long at = seen ? entry_at(a, r, kvh, e) : 0;
+        float s = -INFINITY;
+        if (seen) {
+            s = 0.f;
+            for (int c = 0; c < d; ++c) s += to_f32(q[c]) * a.scale_log2 * to_f32(kv[at + c]);
+        }
+        const float mn = fmaxf(M, warp_max(s)), ms = mn == -INFINITY ? 0.f : mn, f = exp2f(M - ms), p = exp2f(s - ms);
+        L = L * f + warp_sum(p);
+        M = mn;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] *= f;
+        for (unsigned left = __ballot_sync(0xffffffffu, seen); left; left &= left - 1) {
+            const int j = __ffs(left) - 1;
+            const float pj = __shfl_sync(0xffffffffu, p, j);
+            const long long vj = __shfl_sync(0xffffffffu, at, j) + (long long)to_values;
+            if (pj == 0.f) continue;                                // a score of -infinity, or far below the others
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (lane + 32 * k < d) acc[k] += pj * to_f32(kv[vj + lane + 32 * k]);
+        }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (lane + 32 * k >= from_col && lane + 32 * k < to_col) to[lane + 32 * k] = from_f32<A>(acc[k] * inv);
+}
+
+// Item number i of a launch with q_blocks blocks of queries for every request and kv head; false: the request has no such queries.
+__device__ __forceinline__ bool tree_item(const TreeArgs& a, unsigned i, int q_blocks, TreeWalk& w) {
+    const unsigned block = i % q_blocks, rk = i / q_blocks, kvh = rk % a.nkv;
+    w.r = rk / a.nkv;
+    w.x = tree_request(a, w.r);
+    w.item = kvh * w.x.blocks + block;
+    w.tile = 0;
+    return block < w.x.blocks;
 }

@@ -403,7 +403,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
 #pragma unroll
                         for (int x = 0; x < 32; x += 8) tt_store8(a.part_o + place * D + c * 32 + x, o, x);
                 }
-                if (query) *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(m_ref, l_run);
+                if (query) {
+                    *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(m_ref, l_run);
+                    if (w.tile == 0) a.parts[(size_t)t * a.nh + w.kvh() * group + i % group] = make_int2((int)place, w.parts(done, st.per));
+                }
                 tc_fence_before();                                    // before the next item's first product
             }
             done += nt;

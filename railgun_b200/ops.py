@@ -2621,7 +2621,14 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     if T == 0 or R == 0 or max_rows == 0:
         return
     G, blocks, tile_rows, tensor_cores, least = nh // nkv, num_sms(q.device), 0, 0, 1
-    if dtype is torch.bfloat16 and d in (64, 128) and G <= 128 and blocks_a_row and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale):
+    maps = dtype is torch.bfloat16 and blocks_a_row > 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
+    cluster = tree_cluster(R * nkv * -(-max_rows * G // 16), max_context, maps and d % 64 == 0, d)
+    if cluster:
+        _ok(_launch("attention_tree", "rg_tree_attention", "pipipiipipppiiiiiiifiiiiiiiiipppp", q, step, out, out_step, kv_cache, pages, code,
+                    block_table, blocks_a_row, cu_rows, starts, masks, words, R, T, nh, nkv, d, page_size, scale, max_rows, max_context, 0, 0, 16, 1,
+                    0, 0, cluster, None, None, None, _tc_error_flag(q.device)), "tree_attention")
+        return
+    if maps and d in (64, 128) and G <= 128:
         # sides of 128 queries, two a block: a stretch of the work each, or one for both where requests may bring more
         tensor_cores = 1 if max_rows <= 128 // G else 2
         tile_rows = min(max_rows, 128 // G)
@@ -2631,13 +2638,23 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
         blocks = workers
     places = T * nh + workers * queries
     before_ml = _floats_before_ml(places, d)
-    before_plan = before_ml + 2 * places
-    scratch = _new(torch.float32, here, before_plan + 2 * (R + 1))
+    before_parts = before_ml + 2 * places
+    scratch = _new(torch.float32, here, before_parts + 2 * T * nh)
     part_o = scratch.data_ptr()
     _COUNTER.value += 1                          # the parts, and the kernel that joins them
-    _ok(_launch("attention_tree", "rg_tree_attention", "pipipiipipppiiiiiiifiiiiiiiipppp", q, step, out, out_step, kv_cache, pages, code,
-                block_table, blocks_a_row, cu_rows, starts, masks, words, R, T, nh, nkv, d, page_size, scale, max_rows, max_context, blocks, workers, queries, least, tile_rows, tensor_cores,
-                part_o, part_o + 4 * before_ml, part_o + 4 * before_plan, _tc_error_flag(q.device)), "tree_attention")
+    _ok(_launch("attention_tree", "rg_tree_attention", "pipipiipipppiiiiiiifiiiiiiiiipppp", q, step, out, out_step, kv_cache, pages, code,
+                block_table, blocks_a_row, cu_rows, starts, masks, words, R, T, nh, nkv, d, page_size, scale, max_rows, max_context, blocks, workers, queries, least, tile_rows, tensor_cores, 0,
+                part_o, part_o + 4 * before_ml, part_o + 4 * before_parts, _tc_error_flag(q.device)), "tree_attention")
+
+
+@functools.lru_cache(maxsize=4096)
+def tree_cluster(blocks: int, longest: int, fast: bool, d: int) -> int:
+    """How many blocks, a cluster, share each of ``blocks`` items of 16 queries on up to ``longest`` entries and leave nothing to be joined; 0: the
+    work is cut into stretches whose parts another kernel joins."""
+    cluster = 1
+    while cluster < 8 and blocks * cluster * 2 <= 256 and longest > 64 * cluster:
+        cluster *= 2
+    return cluster if -(-longest // cluster) <= 400 and blocks * cluster <= 600 else 0
 
 
 @functools.lru_cache(maxsize=None)

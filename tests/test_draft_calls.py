@@ -90,17 +90,17 @@ def test_nothing_to_do_is_no_launch(calls):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_parts_lie_where_their_loads_can_read_them(calls, dtype):
-    """Places for the parts of all queries and for one more item a worker; (m, l) on their boundaries, the plan behind them."""
+    """Places for the parts of all queries and for one more item a worker; (m, l) on their boundaries, where they are behind them."""
     seen = set()
     for (nh, nkv, d, page), T, R, most in itertools.product([(3, 1, 33, 16), (5, 5, 5, 3), (8, 2, 64, 16), (24, 8, 128, 16), (40, 1, 128, 32), (160, 1, 64, 16)],
                                                             (1, 7, 333), (1, 5), (1, 3, 16, 17, 300)):
         name, args, (scratch,) = calls(ops.tree_attention, **{**tree_args(T, R, nh, nkv, d, page, dtype, words=-(-most // 32)), "max_rows": most})
-        blocks, workers, queries, least, tile_rows, tensor_cores, part_o, part_ml, plan, err = args[-10:]
+        blocks, workers, queries, least, tile_rows, tensor_cores, cluster, part_o, part_ml, parts, err = args[-11:]
         G, at = nh // nkv, scratch.data_ptr()
         seen.add(tensor_cores)
-        assert part_o == at and part_ml % 8 == 0 and plan % 8 == 0 and least >= 1
-        assert at + 4 * d * (T * nh + workers * queries) <= part_ml and plan - part_ml >= 8 * (T * nh + workers * queries)
-        assert plan + 8 * (R + 1) <= at + scratch.numel() * 4
+        assert part_o == at and part_ml % 8 == 0 and parts % 8 == 0 and least >= 1
+        assert at + 4 * d * (T * nh + workers * queries) <= part_ml and parts - part_ml >= 8 * (T * nh + workers * queries)
+        assert parts + 8 * T * nh <= at + scratch.numel() * 4
         if tensor_cores:
             assert dtype == torch.bfloat16 and d in (64, 128) and G <= 128
             assert tile_rows * G <= 128 and queries == tile_rows * G * tensor_cores and workers * tensor_cores == 2 * blocks
