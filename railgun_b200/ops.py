@@ -2618,11 +2618,12 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
         raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; pages hold {page_size} entries")
     if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
-    if T == 0 or R == 0 or max_rows == 0:
+    max_rows = min(max_rows, T)
+    if R == 0 or max_rows == 0:
         return
     G, blocks, tile_rows, tensor_cores, least = nh // nkv, num_sms(q.device), 0, 0, 1
     maps = dtype is torch.bfloat16 and blocks_a_row > 0 and _row_maps_ok(q, step, kv_cache, pages, nkv, page_size, scale)
-    cluster = tree_cluster(R * nkv * -(-max_rows * G // 16), max_context, maps and d % 64 == 0, d)
+    cluster = tree_cluster(R, T, nkv, G, d, max_rows, (max_context + 31) & ~31, maps and d % 64 == 0, blocks)
     if cluster:
         _ok(_launch("attention_tree", "rg_tree_attention", "pipipiipipppiiiiiiifiiiiiiiiipppp", q, step, out, out_step, kv_cache, pages, code,
                     block_table, blocks_a_row, cu_rows, starts, masks, words, R, T, nh, nkv, d, page_size, scale, max_rows, max_context, 0, 0, 16, 1,
@@ -2648,13 +2649,38 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
 
 
 @functools.lru_cache(maxsize=4096)
-def tree_cluster(blocks: int, longest: int, fast: bool, d: int) -> int:
-    """How many blocks, a cluster, share each of ``blocks`` items of 16 queries on up to ``longest`` entries and leave nothing to be joined; 0: the
-    work is cut into stretches whose parts another kernel joins."""
-    cluster = 1
-    while cluster < 8 and blocks * cluster * 2 <= 256 and longest > 64 * cluster:
-        cluster *= 2
-    return cluster if -(-longest // cluster) <= 400 and blocks * cluster <= 600 else 0
+def tree_cluster(R: int, T: int, nkv: int, G: int, d: int, max_rows: int, max_context: int, fast: bool, sms: int) -> int:
+    """How many blocks, a cluster, share each item (a request, a kv head, 16 queries) and leave nothing to be joined; 0: the work is
+    cut into stretches whose parts another kernel joins.  The least of estimates in us, fitted to 660 measured calls (1 to 128 requests of 1
+    to 64 nodes behind 16 to 8,192 entries; what is chosen takes 0.3 to 1.4 % more than the best, at most 37 %): a launch, an item's
+    entries, and what more items than are resident at once add.  32 heads on 8 of 128, clusters against stretches: one request of 16
+    nodes on 512 / 8,192 entries 8.8 to 12.7, 22.9 to 20.5; 16 of 4 on 1,024 16.2 to 24.4; 64 of 16 on 1,024 146 to 82; 128 of 4 on 1,024 106
+    to 115.  1.5 us are set against stretches for the host's second launch and scratch.  Blocks are launched for ``max_rows`` rows of every
+    request: where that is over 8 times what T rows can be, the work is cut into
+    stretches, of which none is empty."""
+    items = R * nkv * -(-max_rows * G // 16)
+    if items > 8 * nkv * (T * G // 16 + R):
+        return 0
+    if fast:
+        resident, first, entry = sms * (3 if d == 64 else 1 if d == 256 else 2), 1.2, 0.0085 + d / 64 * 0.001 if d <= 128 else 0.00008 * d
+        base, wave, more, start, extra = 4.8, 1.65, 3.2, 12.2, (0.0, 0.7, 0.7, 1.5)
+    else:
+        resident, first, entry = sms * tree_general_blocks(d), 1.1 + 0.014 * d, 0.022 + 0.00056 * d
+        base, wave, more, start, extra = 6.0, 1.1, 2.8, 8.0 + 0.066 * min(d, 128), (0.0, 0.7, 0.7, 0.7)
+    if fast and d <= 128 and G <= 128:                  # stretches on the tensor cores, of tiles of 128 entries
+        side = 128 // G * (1 if max_rows <= 128 // G else 2)
+        tiles, tile = R * nkv * -(-max_rows // side) * -(-max_context // 128) / (sms * (2 if max_rows <= 128 // G else 1)), 1.0 + d / 128 * 2.2
+    else:
+        tiles, tile = items * -(-max_context // 64) / (sms * tree_general_blocks(d)), 2.4 + 0.028 * d
+    least, best = start + 1.5 + tile * tiles + T * nkv * G / 16384 * 6, 0
+    for i, cluster in enumerate((1, 2, 4, 8)):
+        if cluster > 1 and (max_context <= 32 * cluster or items * cluster > 296):
+            break
+        one, waves = first + entry * max_context / cluster, items * cluster / resident * (1.3 if resident == sms and cluster == 8 else 1)   # (large ones leave gaps)
+        cost = base + extra[i] + (one if waves <= 0.5 else one * 1.3 if waves <= 1 else waves * (wave * one + more) + 2)
+        if cost < least:
+            least, best = cost, cluster
+    return best
 
 
 @functools.lru_cache(maxsize=None)

@@ -89,36 +89,53 @@ def test_nothing_to_do_is_no_launch(calls):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_parts_lie_where_their_loads_can_read_them(calls, dtype):
-    """Places for the parts of all queries and for one more item a worker; (m, l) on their boundaries, where they are behind them."""
+def test_parts_lie_where_their_loads_can_read_them(calls, monkeypatch, dtype):
+    """Work that is cut into stretches: places for the parts of all queries and for one more item a worker; (m, l) on their boundaries, where they are behind them."""
     seen = set()
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: 0)
     for (nh, nkv, d, page), T, R, most in itertools.product([(3, 1, 33, 16), (5, 5, 5, 3), (8, 2, 64, 16), (24, 8, 128, 16), (40, 1, 128, 32), (160, 1, 64, 16)],
                                                             (1, 7, 333), (1, 5), (1, 3, 16, 17, 300)):
         name, args, (scratch,) = calls(ops.tree_attention, **{**tree_args(T, R, nh, nkv, d, page, dtype, words=-(-most // 32)), "max_rows": most})
         blocks, workers, queries, least, tile_rows, tensor_cores, cluster, part_o, part_ml, parts, err = args[-11:]
         G, at = nh // nkv, scratch.data_ptr()
         seen.add(tensor_cores)
+        assert cluster == 0
         assert part_o == at and part_ml % 8 == 0 and parts % 8 == 0 and least >= 1
         assert at + 4 * d * (T * nh + workers * queries) <= part_ml and parts - part_ml >= 8 * (T * nh + workers * queries)
         assert parts + 8 * T * nh <= at + scratch.numel() * 4
         if tensor_cores:
             assert dtype == torch.bfloat16 and d in (64, 128) and G <= 128
             assert tile_rows * G <= 128 and queries == tile_rows * G * tensor_cores and workers * tensor_cores == 2 * blocks
-            assert (tensor_cores == 1) == (most * G <= 128 // G * G)
+            assert (tensor_cores == 1) == (min(most, T) * G <= 128 // G * G)
         else:
             assert queries == 16 and workers == blocks
     assert seen == ({0} if dtype == torch.float32 else {0, 1, 2})
 
 
-def test_cases_that_the_tensor_cores_kernel_cannot_read(calls):
+def test_cases_that_the_tensor_cores_kernel_cannot_read(calls, monkeypatch):
     """Rows of queries on odd addresses, pages that are no powers of two, scales that are not positive: the general kernel's."""
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: 0)
+
     def cores(**more):
-        return calls(ops.tree_attention, **{**tree_args(), **more})[1][-5]
+        return calls(ops.tree_attention, **{**tree_args(), **more})[1][-6]
     assert cores() == 1
     wide = torch.zeros(6, 8 * 64 + 9, dtype=torch.bfloat16)
     for bad in (dict(q=wide[:, 1:513]), dict(q=torch.zeros(6, 517, dtype=torch.bfloat16)), dict(kv_cache=torch.zeros(9, 2, 2, 12, 64, dtype=torch.bfloat16)),
                 dict(kv_cache=torch.zeros(9, 2, 2, 4, 64, dtype=torch.bfloat16)), dict(scale=-0.1), dict(scale=0.0), dict(block_table=ints(2, 0))):
         assert cores(**bad) == 0
+
+
+def test_calls_whose_items_are_whole(calls):
+    """Few nodes on short contexts: one launch, no scratch; many, or long contexts, are cut into stretches."""
+    name, args, made = calls(ops.tree_attention, **tree_args())
+    assert args[-11:-5] == [0, 0, 16, 1, 0, 0] and args[-5] in (1, 2, 4, 8) and args[-4:] == [None] * 4 and not made
+    for fast, d, G, nkv in itertools.product((True, False), (64, 128, 192, 256), (1, 4, 7, 200), (1, 8)):
+        one = [ops.tree_cluster(1, 1, nkv, G, d, 1, n, fast, 148) for n in (1, 32, 60, 300, 600)]
+        assert one[0] == one[1] == 1 and set(one) <= {0, 1, 2, 4, 8}
+        assert d > 128 or not fast or ops.tree_cluster(64, 64 * 64, 8, 8, d, 64, 8192, fast, 148) == 0
+        assert ops.tree_cluster(64, 64, 8, 8, d, 64, 100, fast, 148) == 0        # room for 64 times the rows that there are
+        for rows, context in ((0, 0), (1, 0), (1 << 30, 1 << 30)):
+            ops.tree_cluster(1, 1, nkv, G, d, rows, context, fast, 148)
 
 
 # ---- layout and what is kept ----------------------------------------------------------------------------------------------

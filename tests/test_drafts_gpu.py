@@ -188,6 +188,43 @@ def test_tree_attention(nh, nkv, d, page, scene, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [0, 1, 2, 4, 8])
+@pytest.mark.parametrize("scene", SCENES)
+@pytest.mark.parametrize("nh,nkv,d,page", [(3, 1, 32, 8), (8, 2, 128, 32), (24, 8, 64, 16), (20, 1, 16, 7), (8, 1, 192, 16), (2, 1, 256, 16), (40, 1, 64, 128)])
+def test_each_way_to_split_the_work(monkeypatch, nh, nkv, d, page, scene, cluster, dtype):
+    """Stretches and clusters, whichever the sizes would have chosen."""
+    from railgun_b200 import ops
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    run_tree(*SCENES[scene], nh, nkv, d, page, dtype, nh + d + len(scene))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [0, 1, 2, 8])
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (8, 2, 80, 16)])
+def test_pages_that_are_not_there(monkeypatch, nh, nkv, d, page, cluster, dtype):
+    """Reported, and read nowhere; entries behind a request's last one may be on any page, and the next call is right again."""
+    from railgun_b200 import ops
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    q, out, args, sizes = run_tree([5, 20, 3], [100, 40, 0], nh, nkv, d, page, dtype, 3)
+    ops.tc_gemm_check()
+    want, table = out.clone(), args[1]
+    behind = table.clone()
+    behind[0, 7:], behind[1, 4:], behind[2, 1:] = -5, 1 << 30, 999999   # 105, 60 and 3 entries
+    ops.tree_attention(q, out, args[0], behind, *args[2:], **sizes)
+    ops.tc_gemm_check()
+    assert torch.equal(out, want)
+    for page_id in (-1, args[0].shape[0], 2 ** 31 - 1):
+        bad = table.clone()
+        bad[1, 2] = page_id
+        ops.tree_attention(q, out, args[0], bad, *args[2:], **sizes)
+        with pytest.raises(ops.KernelError, match="page"):
+            ops.tc_gemm_check()
+    ops.tree_attention(q, out, *args, **sizes)
+    ops.tc_gemm_check()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("share", [0.0, 0.03, 0.5])
 def test_masks_that_are_no_trees(share, dtype):
     """Any nodes may be seen, or none: rows without context then give 0."""
@@ -218,11 +255,14 @@ def test_many_requests(dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("cluster", [None, 0, 2])
 @pytest.mark.parametrize("counts,starts", [([6, 5], [70, 9]), ([40, 33], [500, 0])])
-def test_what_is_not_seen_has_no_say(counts, starts, bad, dtype):
+def test_what_is_not_seen_has_no_say(monkeypatch, counts, starts, cluster, bad, dtype):
     """A node whose key and value are no numbers: rows that see it show it, the others are what they were to their last bit but one
     rounding."""
     from railgun_b200 import ops
+    if cluster is not None:
+        monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
     nh, nkv, d, page, scale = 8, 2, 64, 16, 0.125
     g = torch.Generator(device=DEV).manual_seed(1)
     lens = [n + s for n, s in zip(counts, starts)]
