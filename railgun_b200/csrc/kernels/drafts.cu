@@ -24,51 +24,66 @@ __device__ __forceinline__ int draft_rows(const DraftRows& d, int r, int& row0, 
 
 // ---------------------------------------------------------------------------------------------------
 // Which nodes a node sees (itself and its ancestors, bit j of a row's mask for node j), and its position, start + how many
-// ancestors it has.  A thread walks up from its node: parents come before their children, so the words of a mask are met from the
-// last to the first and each is written once.  A block has a request; the last block writes zeros for rows of no request.
+// ancestors it has.  Nodes go in groups of 32, a word of a mask each.  A warp has a group: five steps, in each of which a node
+// takes over what the node sees that its line has been followed to, find the whole line inside the group and the first ancestor
+// before it.  Then a thread goes up from its node, a group at a time: a word for each that the line touches, zeros for the others, every
+// word written once.  A block has up to 256 rows of a request and looks at the groups up to its last; the last blocks write zeros for
+// rows of no request.  One ancestor at a time instead took 4.8 us for 64 trees of up to 256 nodes, 62 for 12 chains of up to 343.
 // ---------------------------------------------------------------------------------------------------
 #define LAYOUT_THREADS 256
 __global__ void __launch_bounds__(LAYOUT_THREADS) draft_tree_kernel(const DraftRows dr, const int* __restrict__ parents, int* __restrict__ masks,
                                                                     int words, int* __restrict__ positions) {
-    extern __shared__ int up[];
+    extern __shared__ int2 line[];                                    // of a node: what it sees of its group, the first ancestor before that
     pdl_wait();
     pdl_trigger();
-    const int r = blockIdx.x;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+    auto nothing = [&](long long t) {
+        for (int w = 0; w < words; ++w) masks[t * words + w] = 0;
+        positions[t] = 0;
+    };
+    const long long mine = (long long)blockIdx.y * LAYOUT_THREADS + tid, every = (long long)gridDim.y * LAYOUT_THREADS;
     if (r == dr.R) {
         const int first = dr.R ? max(0, min(dr.cu_rows[0], dr.T)) : 0, end = dr.R ? max(0, min(dr.cu_rows[dr.R], dr.T)) : 0;
-        for (int t = threadIdx.x; t < dr.T; t += LAYOUT_THREADS) {
-            if (t >= first && t < end) { t += (end - 1 - t) / LAYOUT_THREADS * LAYOUT_THREADS; continue; }
-            for (int w = 0; w < words; ++w) masks[(size_t)t * words + w] = 0;
-            positions[t] = 0;
-        }
+        for (long long t = mine; t < first; t += every) nothing(t);
+        for (long long t = end + mine; t < dr.T; t += every) nothing(t);
         return;
     }
     int row0, start;
-    const int n = draft_rows(dr, r, row0, start);
-    for (int i = threadIdx.x; i < n; i += LAYOUT_THREADS) up[i] = parents[row0 + i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += LAYOUT_THREADS) {
-        int* mask = masks + (size_t)(row0 + i) * words;
-        int word = words - 1, node = i, depth = 0;
-        unsigned bits = 0;
-        for (;;) {
-            while (word > node >> 5) { mask[word--] = (int)bits; bits = 0; }
-            bits |= 1u << (node & 31);
-            const int parent = up[node];
-            if (parent < 0 || parent >= node) break;                  // a root, or no parent that comes before it
-            node = parent;
-            ++depth;
+    const int n = draft_rows(dr, r, row0, start), last = min(n, ((int)blockIdx.y + 1) * LAYOUT_THREADS);
+    if ((int)blockIdx.y * LAYOUT_THREADS < n) {
+        for (int i0 = tid - lane; i0 < last; i0 += LAYOUT_THREADS) {
+            const int i = i0 + lane;
+            int before = i < n ? parents[row0 + i] : -1, to = lane;
+            if (before >= i) before = -1;                             // no parent that comes before it: a root
+            if (before >= i0) to = before - i0;
+            unsigned bits = 1u << lane;
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                bits |= __shfl_sync(0xffffffffu, bits, to);
+                to = __shfl_sync(0xffffffffu, to, to);
+            }
+            before = __shfl_sync(0xffffffffu, before, to);            // the line's first node in the group has its parent before it, or none
+            line[i] = make_int2((int)bits, before);
         }
-        for (; word >= 0; --word) { mask[word] = (int)bits; bits = 0; }
-        positions[row0 + i] = start + depth;
+    }
+    __syncthreads();
+    if (mine < n) {
+        int* mask = masks + (size_t)(row0 + mine) * words;
+        int word = words - 1, node = (int)mine, depth = -1;
+        while (node >= 0) {
+            const int2 at = line[node];
+            for (; word > node >> 5; --word) mask[word] = 0;
+            mask[word--] = at.x;
+            depth += __popc(at.x);
+            node = at.y;
+        }
+        for (; word >= 0; --word) mask[word] = 0;
+        positions[row0 + mine] = start + depth;
     }
     // rows beyond what the call says see nothing
     const long long all = min((long long)dr.cu_rows[r + 1], (long long)dr.T);
     if (row0 >= 0)
-        for (long long t = row0 + n + threadIdx.x; t < all; t += LAYOUT_THREADS) {
-            for (int w = 0; w < words; ++w) masks[t * words + w] = 0;
-            positions[t] = 0;
-        }
+        for (long long t = row0 + n + mine; t < all; t += every) nothing(t);
 }
 
 extern "C" int rg_draft_tree(const int* parents, const int* cu_rows, const int* starts, int R, int T, int max_rows, int* masks, int words,
@@ -76,8 +91,9 @@ extern "C" int rg_draft_tree(const int* parents, const int* cu_rows, const int* 
     if (T <= 0) return 0;
     if (R < 0 || max_rows < 0 || max_rows > DRAFT_MOST || words != (max_rows + 31) / 32) return RG_ERR_UNSUPPORTED;
     const DraftRows dr = {cu_rows, starts, R, T, max_rows};
-    return rg_launch(draft_tree_kernel, dim3((unsigned)R + 1), dim3(LAYOUT_THREADS), (size_t)max_rows * sizeof(int), (cudaStream_t)stream, 1, dr,
-                     parents, masks, words, positions);
+    const int groups = (max_rows + LAYOUT_THREADS - 1) / LAYOUT_THREADS;
+    return rg_launch(draft_tree_kernel, dim3((unsigned)R + 1, (unsigned)(groups ? groups : 1)), dim3(LAYOUT_THREADS), (size_t)words * 32 * sizeof(int2),
+                     (cudaStream_t)stream, 1, dr, parents, masks, words, positions);
 }
 
 // ---------------------------------------------------------------------------------------------------

@@ -2710,8 +2710,8 @@ def _cache_list(caches, what: str, here: int) -> tuple:
                 raise KernelError(f"{what}: caches of {tuple(first.shape)} and {tuple(t.shape)}")
         addresses = np.array([t.data_ptr() for t in caches], dtype=np.uint64).tobytes()
     bits = 0
-    for i in range(0, len(addresses), 8):            # only the lowest four bits are of interest
-        bits |= addresses[i]
+    for low in set(addresses[::8]):                  # only the lowest four bits are of interest
+        bits |= low
     return first, len(caches), addresses, bits
 
 
