@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
         tree_plan<TG_THREADS>(a, blockIdx.x, 1, 0, st);
         if (st.r[0] < 0) return;
         n_tiles = (int)min(st.per, st.total - (long long)blockIdx.x * st.per);
-        w.at(a, st.r[0], st.in[0]);
+        w.at(st, 0);
     }
     const int d = a.d, ld = tg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = tg_stages(d);
     float* qs = smem;                                               // [16][ld]

@@ -56,6 +56,14 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
 }
 __device__ __forceinline__ long long tree_tiles(const TreeArgs& a, const TreeRequest& x) { return (long long)x.tiles * x.blocks * a.nkv; }
 
+// Tiles of all items, and where (up to two) workers begin: a request, -1: nowhere, and a place among its tiles.
+struct TreeStart {
+    long long total, per;
+    long long in[2];
+    int r[2];
+    TreeRequest x[2];
+};
+
 // Where a worker is on the line: an item and a tile of it.
 struct TreeWalk {
     TreeRequest x;
@@ -65,12 +73,13 @@ struct TreeWalk {
     __device__ __forceinline__ void skip_empty(const TreeArgs& a) {      // to a request that has tiles (one is known to come)
         while (x.tiles == 0 || x.blocks == 0) x = tree_request(a, ++r);
     }
-    // At place `in` of request r's tiles.
-    __device__ __forceinline__ void at(const TreeArgs& a, int r_, long long in) {
-        r = r_;
-        x = tree_request(a, r);
-        item = (int)(in / x.tiles);
-        tile = (int)(in % x.tiles);
+    // Where worker i of `st` begins.
+    __device__ __forceinline__ void at(const TreeStart& st, int i) {
+        r = st.r[i];
+        x = st.x[i];
+        const long long in = st.in[i];
+        item = in >> 32 ? (int)(in / x.tiles) : (int)((unsigned)in / (unsigned)x.tiles);
+        tile = (int)(in - (long long)item * x.tiles);
     }
     // One tile on; `more`: there is one.
     __device__ __forceinline__ void next(const TreeArgs& a, bool more) {
@@ -113,11 +122,6 @@ __device__ __forceinline__ void tree_gaps(const TreeArgs& a) {
 
 // The whole block, THREADS threads: tiles of all items, and the request (with the place among its tiles) in which each of `n`
 // (up to 2) workers, `first` and `first` + `apart`, begins (r -1: it has nothing).  The last block says which rows nobody has.
-struct TreeStart {
-    long long total, per;
-    long long in[2];
-    int r[2];
-};
 template <int THREADS>
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, int apart, TreeStart& st) {
     __shared__ long long sums[THREADS / 32 + 1];
@@ -142,34 +146,36 @@ __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, i
         return before + x - v;
     };
     long long total = 0, mine = 0, before = 0;
+    TreeRequest x;
+    if (threadIdx.x < 2) st.r[threadIdx.x] = -1;
     for (int r0 = 0; r0 < a.R; r0 += THREADS) {
         const int r = r0 + threadIdx.x;
         long long some;
-        mine = r < a.R ? tree_tiles(a, tree_request(a, r)) : 0;
+        if (r < a.R) x = tree_request(a, r);
+        mine = r < a.R ? tree_tiles(a, x) : 0;
         before = total + scan(mine, some);
         total += some;
     }
-    const long long per = max((long long)a.least, (total + a.workers - 1) / a.workers);
+    const long long per = max((long long)a.least, total >> 31 ? (total + a.workers - 1) / a.workers : (long long)((unsigned)total + a.workers - 1u) / a.workers);
     if (threadIdx.x == 0) {
         st.total = total;
         st.per = per;
-        st.r[0] = st.r[1] = -1;
     }
-    __syncthreads();
     const bool once = a.R <= THREADS;                                    // what was found above still stands
     long long sofar = 0;
     for (int r0 = 0; r0 < a.R; r0 += THREADS) {
         const int r = r0 + threadIdx.x;
         if (!once) {
             long long some;
-            mine = r < a.R ? tree_tiles(a, tree_request(a, r)) : 0;
+            if (r < a.R) x = tree_request(a, r);
+            mine = r < a.R ? tree_tiles(a, x) : 0;
             before = sofar + scan(mine, some);
             sofar += some;
         }
         if (r >= a.R) continue;
         for (int i = 0; i < n; ++i) {
             const long long at = (first + (long long)i * apart) * per - before;
-            if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; }
+            if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; st.x[i] = x; }
         }
     }
     if (blockIdx.x == gridDim.x - 1) tree_gaps<THREADS>(a);

@@ -108,16 +108,23 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         for (int b = 0; b < 4; ++b) { mbar_init(s_full0 + 8 * b, 1); mbar_init(p_full0 + 8 * b, TT_SIDE); mbar_init(p_free0 + 8 * b, 1); }
         fence_barrier_init();
     }
+    if (threadIdx.x == 32) {
+        tma_prefetch_map(&q_map);
+        tma_prefetch_map(&kv_map);
+    }
     pdl_wait();                                                       // tables, lengths and queries may come from the kernel before
     pdl_trigger();
     // side s's worker: the second sides' stretches come behind all first sides', so that little work is one stretch an SM
     auto worker_of = [&](int s) -> int { return blockIdx.x + (both ? 0 : s * (int)gridDim.x); };
+    if (warp == 11) tmem_alloc(&tmem_base_slot, 512u);                // (all kernels before are over: nobody who has some waits for this block)
     tree_plan<TT_THREADS>(a, blockIdx.x, both ? 1 : 2, gridDim.x, st);
-    if (st.r[0] < 0) return;                                          // nothing for side 0: nothing at all
-    if (warp == 9) tmem_alloc(&tmem_base_slot, 512u);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (st.r[0] < 0) {                                                // nothing for side 0: nothing at all
+        if (warp == 11) tmem_free(tmem_base_slot, 512u);
+        return;
+    }
     auto tiles_of = [&](int s) -> int { return (int)max(0ll, min(st.per, st.total - (long long)worker_of(s) * st.per)); };
     const int n_t0 = tiles_of(0), n_t1 = both ? 0 : tiles_of(1);      // n_t1: of its own stretch
     // A stage of the stream belongs to both sides, or in turn to either while side 1 has some
@@ -130,8 +137,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const int box_rows = min(a.page_size, TT_STAGE), boxes = TT_STAGE / box_rows, box = lane % boxes, piece = lane / boxes;
         const bool mine = piece < PIECES;
         TreeWalk w0, w1;
-        w0.at(a, st.r[0], st.in[0]);
-        if (n_t1) w1.at(a, st.r[1], st.in[1]);
+        w0.at(st, 0);
+        if (n_t1) w1.at(st, 1);
         int left0 = n_t0, left1 = n_t1;
         const int kv = warp == 10 ? 1 : 0, n = kv ? NV : NK;
         auto row_of = [&](TreeWalk& w, int& left) -> int {            // the cache's row of this lane's box; one tile on
@@ -181,7 +188,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         auto v_seen = [&]() { v_phase ^= 1u << vi; };
         int p_phase[2] = {0, 0}, q_phase = 0;
         TreeWalk w;
-        if (n_t) w.at(a, st.r[both ? 0 : s], st.in[both ? 0 : s]);
+        if (n_t) w.at(st, both ? 0 : s);
         auto issue_s = [&](int half, bool last) {                     // K is there
             if (issuer) {
                 const uint64_t kd = desc_k_major(sK0 + ki * TILE + half * SUB);
@@ -278,7 +285,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const uint32_t s_full = s_full0 + 16 * s, p_full = p_full0 + 16 * s, p_free = p_free0 + 16 * s;
         int s_phase = 0, o_phase = 0;                                 // bit `half`: of the next scores, of the next product
         TreeWalk w;
-        if (n_t) w.at(a, st.r[both ? 0 : s], st.in[both ? 0 : s]);
+        if (n_t) w.at(st, both ? 0 : s);
         bool ok = true;
         for (int done = 0; done < n_t && ok;) {                       // a part of an item
             const int nt = min(n_t - done, w.x.tiles - w.tile), row_first = (w.block() * (both ? 2 : 1) + (both ? s : 0)) * tile_rows;
@@ -420,7 +427,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
         __syncthreads();
     }
-    if (warp == 9) {
+    if (warp == 11) {
         tc_fence_after();
         tmem_free(tmem, 512u);
     }
