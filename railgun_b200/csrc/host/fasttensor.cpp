@@ -25,6 +25,20 @@ static bool of_type(const at::Tensor& t, PyObject* dtype) {
 }
 static bool on_device(const at::Tensor& t, int64_t device) { return t.is_cuda() && t.get_device() == device; }
 
+// One tensor of fits and fits_all: its sizes are a[0] .. a[n - 1].  -1: an error is set.
+static int fits_one(PyObject* tensor, PyObject* dtype, long device, PyObject* const* a, Py_ssize_t n) {
+    if (!THPVariable_Check(tensor)) return 0;
+    const at::Tensor& t = THPVariable_Unpack(tensor);
+    if (!on_device(t, device) || !of_type(t, dtype) || t.layout() != at::kStrided || t.dim() != n) return 0;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (a[i] == Py_None) continue;
+        const long long want = PyLong_AsLongLong(a[i]);
+        if (want == -1 && PyErr_Occurred()) return -1;
+        if (t.size(i) != want) return 0;
+    }
+    return t.is_contiguous();
+}
+
 // fits(tensor, dtype or None, device, sizes..): a contiguous tensor of this type on this CUDA device, of as many dimensions and these
 // sizes (None: any)?
 static PyObject* ft_fits(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -35,16 +49,31 @@ static PyObject* ft_fits(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const long device = PyLong_AsLong(a[2]);
     if (device == -1 && PyErr_Occurred()) return nullptr;
-    if (!THPVariable_Check(a[0])) Py_RETURN_FALSE;
-    const at::Tensor& t = THPVariable_Unpack(a[0]);
-    if (!on_device(t, device) || !of_type(t, a[1]) || t.layout() != at::kStrided || t.dim() != n - 3) Py_RETURN_FALSE;
-    for (Py_ssize_t i = 3; i < n; ++i) {
-        if (a[i] == Py_None) continue;
-        const long long want = PyLong_AsLongLong(a[i]);
-        if (want == -1 && PyErr_Occurred()) return nullptr;
-        if (t.size(i - 3) != want) Py_RETURN_FALSE;
+    const int fits = fits_one(a[0], a[1], device, a + 3, n - 3);
+    if (fits < 0) return nullptr;
+    return PyBool_FromLong(fits);
+    END_HANDLE_TH_ERRORS
+}
+
+// fits_all(device, tensor, dtype, sizes.., tensor, dtype, sizes.., ..): the same of several tensors.
+static PyObject* ft_fits_all(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n < 1) {
+        PyErr_SetString(PyExc_TypeError, "fits_all: a device, and a tensor, a type and sizes for each");
+        return nullptr;
     }
-    return PyBool_FromLong(t.is_contiguous());
+    const long device = PyLong_AsLong(a[0]);
+    if (device == -1 && PyErr_Occurred()) return nullptr;
+    for (Py_ssize_t i = 1; i < n;) {
+        if (i + 1 >= n || !THPVariable_Check(a[i])) Py_RETURN_FALSE;
+        Py_ssize_t end = i + 2;
+        while (end < n && (a[end] == Py_None || (PyIndex_Check(a[end]) && !THPVariable_Check(a[end])))) ++end;
+        const int fits = fits_one(a[i], a[i + 1], device, a + i + 2, end - i - 2);
+        if (fits < 0) return nullptr;
+        if (!fits) Py_RETURN_FALSE;
+        i = end;
+    }
+    Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }
 
@@ -187,6 +216,7 @@ static PyObject* ft_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
 static PyMethodDef methods[] = {
     {"call", (PyCFunction)(void (*)(void))ft_call, METH_FASTCALL, "call(address, kinds, *arguments) -> int"},
     {"fits", (PyCFunction)(void (*)(void))ft_fits, METH_FASTCALL, "is it a contiguous tensor of this type on this device, of these sizes (None: any)?"},
+    {"fits_all", (PyCFunction)(void (*)(void))ft_fits_all, METH_FASTCALL, "are they all contiguous tensors of their types on this device, of their sizes?"},
     {"rows", (PyCFunction)(void (*)(void))ft_rows, METH_FASTCALL, "a matrix's rows and how far they are apart; None if it does not fit"},
     {"addresses", (PyCFunction)(void (*)(void))ft_addresses, METH_FASTCALL, "where tensors of one kind are, as bytes; None if they are not of one kind"},
     {"empty", (PyCFunction)(void (*)(void))ft_empty, METH_FASTCALL, "a new tensor of this type, on this device, of these sizes"},

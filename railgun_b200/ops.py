@@ -109,6 +109,15 @@ def _fits(t, name: str, dtype, here: int, *sizes) -> None:
         raise KernelError(f"{name} is {tuple(t.shape)}, expected [{', '.join('any' if n is None else str(n) for n in sizes)}]")
 
 
+def _all_fit(here: int, names: tuple, *given) -> None:
+    """``_fits`` of several tensors: of each itself, its type and its sizes."""
+    if _tensors and _tensors.fits_all(here, *given):
+        return
+    starts = [i - 1 for i, x in enumerate(given) if isinstance(x, torch.dtype)]
+    for name, a, b in zip(names, starts, starts[1:] + [len(given)]):
+        _fits(given[a], name, given[a + 1], here, *given[a + 2:b])
+
+
 def _rows_fit(t, name: str, dtype, here: int, columns: int) -> tuple:
     """(rows, elements from one to the next) of a matrix on the current device with unit column stride and at least so many columns."""
     got = _tensors.rows(t, dtype, here, columns) if _tensors else None
@@ -2578,8 +2587,7 @@ def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, starts: torch.Tenso
     request; rows beyond, rows of requests with a negative start and rows of no request get zeros."""
     _tensor_calls()
     here, i32 = _here(), torch.int32
-    _fits(parents, "parents", i32, here, None)
-    _fits(starts, "starts", i32, here, None)
+    _all_fit(here, ("parents", "starts"), parents, i32, None, starts, i32, None)
     T, R = parents.shape[0], starts.shape[0]
     _fits(cu_rows, "cu_rows", i32, here, R + 1)
     if not 0 <= max_rows <= DRAFT_MOST:
@@ -2606,12 +2614,10 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     if nkv < 1 or nh < 1 or nh % nkv or not 1 <= d <= 256:
         raise KernelError(f"tree_attention: {nh} query heads on {nkv} of size {d} (a multiple of the kv heads; sizes 1 to 256)")
     T, step = _rows_fit(q, "q", dtype, here, nh * d)
-    _fits(kv_cache, "kv_cache", dtype, here, None, 2, nkv, None, d)
     _fits(starts, "starts", i32, here, None)
     R = starts.shape[0]
-    _fits(cu_rows, "cu_rows", i32, here, R + 1)
-    _fits(block_table, "block_table", i32, here, R, None)
-    _fits(masks, "masks", i32, here, T, None)
+    _all_fit(here, ("kv_cache", "cu_rows", "block_table", "masks"), kv_cache, dtype, None, 2, nkv, None, d, cu_rows, i32, R + 1,
+             block_table, i32, R, None, masks, i32, T, None)
     out_rows, out_step = _rows_fit(out, "out", dtype, here, nh * d)
     (pages, _, _, page_size, _), blocks_a_row, words = kv_cache.shape, block_table.shape[1], masks.shape[1]
     if out_rows != T or out.shape[1] != nh * d or page_size < 1:
@@ -2738,13 +2744,9 @@ def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, m
     shape, numel = first.shape, first.numel()
     if len(shape) < 3 or numel == 0:
         raise KernelError(f"keep_drafts: a cache is [pages, .., page, x], not {tuple(shape)}")
-    _fits(starts, "starts", i32, here, None)
-    _fits(parents, "parents", i32, here, None)
+    _all_fit(here, ("starts", "parents"), starts, i32, None, parents, i32, None)
     R, T = starts.shape[0], parents.shape[0]
-    _fits(cu_rows, "cu_rows", i32, here, R + 1)
-    _fits(block_table, "block_table", i32, here, R, None)
-    _fits(tokens, "tokens", i32, here, T)
-    _fits(chosen, "chosen", i32, here, T)
+    _all_fit(here, ("cu_rows", "block_table", "tokens", "chosen"), cu_rows, i32, R + 1, block_table, i32, R, None, tokens, i32, T, chosen, i32, T)
     if not 0 <= max_rows <= DRAFT_MOST:
         raise KernelError(f"keep_drafts: up to {DRAFT_MOST} rows a request, not {max_rows}")
     counts, path, fresh = _new(i32, here, R), _new(i32, here, R, max_rows), _new(i32, here, R, max_rows)

@@ -199,6 +199,43 @@ def test_each_way_to_split_the_work(monkeypatch, nh, nkv, d, page, scene, cluste
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [None, 0, 1, 2, 8])
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (3, 1, 33, 16), (4, 2, 128, 4)])
+def test_calls_at_the_limits(monkeypatch, nh, nkv, d, page, cluster, dtype):
+    """Scales of any sign, operands on any address, room for more rows than there can be, and calls that say that nothing is seen."""
+    from railgun_b200 import ops
+    if cluster is not None:
+        monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    counts, starts = [5, 20], [100, 0]
+    q, out, args, sizes = run_tree(counts, starts, nh, nkv, d, page, dtype, 17)
+    T, scale = q.shape[0], args[-1]
+    wide = torch.zeros(T * (nh * d + 3) + 1, dtype=dtype, device=DEV)
+    odd = wide[1:].view(T, nh * d + 3)
+    odd[:, :nh * d] = q
+    to = torch.full((T * (nh * d + 1) + 1,), 7.0, dtype=dtype, device=DEV)[1:].view(T, nh * d + 1)
+    mine = to[:, :nh * d]
+    seen = torch.zeros(5, 105, dtype=torch.bool, device=DEV)
+    seen[:, :100] = True
+    seen[:, 100:] = (args[4][1:6, :1] >> torch.arange(5, device=DEV)) & 1 == 1
+    cache = args[0]
+    K, V = [cache[args[1][0, :-(-105 // page)].long()][:, j].double().permute(1, 0, 2, 3).reshape(nkv, -1, d)[:, :105] for j in (0, 1)]
+    for s in (scale, -scale, 0.0):
+        ops.tree_attention(odd, mine, *args[:-1], s, **{**sizes, "max_rows": 1 << 30})
+        assert (to[:, nh * d] == 7).all() and (mine[0] == 7).all() and (mine[-2:] == 7).all()
+        p = attend(q[1:6].view(5, nh, d), K, V, seen, s)
+        want = (p @ V).view(nkv, 5, nh // nkv, d).permute(1, 0, 2, 3).reshape(5, nh * d)
+        # weights that are off by w of themselves, and their rounding and the output's in bfloat16
+        w = max(weight_error(q[1 + i].view(nh, d), K, 105, abs(s), dtype) for i in range(5)) + 218 * U + (2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+        off = w * V.abs().max() + (2.0 ** -8 if dtype == torch.bfloat16 else U) * (want.abs() + w * V.abs().max())
+        assert ((mine[1:6].double() - want).abs() <= off).all()
+    ops.tree_attention(q, out, *args, max_rows=20, max_context=0)
+    assert not out[1:26].any() and (out[0] == 7).all() and (out[26:] == 7).all()
+    ops.tree_attention(q, out, cache, args[1][:, :0].contiguous(), *args[2:], **sizes)           # a table without columns
+    assert not out[1:26].any()
+    ops.tc_gemm_check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("cluster", [0, 1, 2, 8])
 @pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (8, 2, 80, 16)])
 def test_pages_that_are_not_there(monkeypatch, nh, nkv, d, page, cluster, dtype):

@@ -52,10 +52,14 @@ def test_what_does_not_fit(tensors):
     x = torch.zeros(3, 4, dtype=torch.int32)
     for t in (x, None, 5, "text", np.zeros(3)):
         assert tensors.fits(t, torch.int32, 0, 3, 4) is False and tensors.rows(t, torch.int32, 0, 1) is None
+        assert tensors.fits_all(0, t, torch.int32, 3, 4) is False
         assert tensors.addresses([t], 0) is None and tensors.addresses(t, 0) is None
     assert tensors.addresses([], 0) is None
+    assert tensors.fits_all(0) is True and tensors.fits_all(0, x) is False and tensors.fits_all(0, 5, torch.int32) is False
     with pytest.raises(TypeError):
         tensors.fits(x)
+    with pytest.raises(TypeError):
+        tensors.fits_all()
     with pytest.raises(TypeError):
         tensors.empty("int32", 0, 3)
 
@@ -97,3 +101,14 @@ def test_without_the_module_calls_are_the_same(monkeypatch):
     monkeypatch.setattr(ops, "_tensors", False)
     for a, b in zip(with_it, run()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_several_at_once(tensors):
+    x, y = torch.zeros(3, 4, dtype=torch.int32, device="cuda"), torch.zeros(5, device="cuda")
+    f32, i32 = torch.float32, torch.int32
+    assert tensors.fits_all(0, x, i32, 3, 4, y, f32, None, x, i32, np.int64(3), None)
+    for bad in ((x, i32, 3, 4, y, f32, 4), (x, i32, 3, y, f32, 5), (x, i32, 3, 4, y, i32, 5), (x, i32, 3, 4, y[::2], f32, None), (x, i32, 3, 4, y.cpu(), f32, 5),
+                (x, i32, 3, 4, None, f32, 5), (x, i32, 3, 4, y)):
+        assert tensors.fits_all(0, *bad) is False
+    assert tensors.fits_all(1, x, i32, 3, 4) is False
