@@ -30,6 +30,9 @@ __host__ __device__ inline int tg_stages(int d) { return d <= 128 ? 2 : 1; }   /
 // Per tile of 64 entries: 2 queries x 4 entries of scores a thread, then a column of the output for all 16 queries a thread;
 // DP = 32 or 64: as many threads share the columns, and TG_THREADS / DP groups of them share the tile's entries.
 // WHOLE: an item to a cluster, whose blocks share its tiles, join through each other's shared memory and leave the output.
+// What bounds it is shared memory: 96 bytes a thread for 32 products of scores, 272, most of them the same for a warp, for 64 of the output: in
+// 32-bit, 16 heads on 4 of 128, one request of 16 nodes on 1,000 entries takes 26 us, 8 on 4,000 390, 10.7 TFLOP/s.  Smallest calls are the launch and
+// the same three trips as above: two requests of 7 nodes on 61 entries, 3 heads on 1 of 32, 9.3 us in one launch, 12 in two.
 // ---------------------------------------------------------------------------------------------------
 template <typename A, int DP, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs a, A* __restrict__ out, int out_ld, int q_blocks) {
@@ -305,7 +308,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
 
 // A thread has four columns of a row and head: PS threads share their parts where there are few rows, and a thread has ITEMS of them where
 // there are many, so that the blocks are resident at once (a block is there for two trips to memory, where the parts are and the parts
-// themselves: 16 nodes of 64 requests, 2,056 blocks of one quad a thread, 16 us; 14 with two, 17 with four).
+// themselves: 16 nodes of 64 requests, 2,056 blocks of one quad a thread, 16 us; 13 with two, 17 with four).
 template <typename A, int PS, int ITEMS>
 __global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeArgs a, A* __restrict__ out, int out_ld) {
     constexpr int COLS = JOIN_THREADS / PS;                         // threads of a share

@@ -2,7 +2,8 @@
 //
 // A cache is [pages, outer, page, inner bytes]: of a copy (from, to, held) the first `held` of the page's entries are copied, which
 // are one run of held x inner bytes for each of `outer`.  Nothing but the bytes themselves goes to memory or comes from it: where the
-// caches are, and the copies, are arguments of the kernel.
+// caches are, and the copies, are arguments of the kernel.  256 pages of 28 layers (24 heads on 8 of 128, 499 MB there and back) take
+// 77 us, 98 % of what a plain copy reaches; 8 pages of 9 entries in 16 layers 2.1, the launch and a trip each way.
 #include "common.cuh"
 #include <cstdlib>
 
