@@ -455,7 +455,7 @@ extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out
                                  int blocks, int workers, int item_queries, int least, int tile_rows, int tensor_cores, int cluster, float* part_o, float* part_ml,
                                  int2* parts, int* err, void* stream) {
     if (T <= 0 || R <= 0 || max_rows <= 0) return 0;
-    if (d < 1 || d > 256 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_blocks < 0 || words < 0 || max_context < 0 || out_ld < nh * d ||
+    if (d < 1 || d > 256 || num_pages < 1 || nkv < 1 || nh < nkv || nh % nkv || page_size < 1 || max_blocks < 0 || words < 0 || max_context < 0 || out_ld < nh * d ||
         (!cluster && workers < 1) || item_queries < 1 || least < 1 || ((uintptr_t)part_o & 31) || ((uintptr_t)part_ml & 7) || ((uintptr_t)parts & 7) ||
         (long long)T * nh + (long long)workers * item_queries > 0x7fffffffll)
         return RG_ERR_UNSUPPORTED;

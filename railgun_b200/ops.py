@@ -2620,8 +2620,8 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
              block_table, i32, R, None, masks, i32, T, None)
     out_rows, out_step = _rows_fit(out, "out", dtype, here, nh * d)
     (pages, _, _, page_size, _), blocks_a_row, words = kv_cache.shape, block_table.shape[1], masks.shape[1]
-    if out_rows != T or out.shape[1] != nh * d or page_size < 1:
-        raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; pages hold {page_size} entries")
+    if out_rows != T or out.shape[1] != nh * d or page_size < 1 or pages < 1:
+        raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; {pages} pages hold {page_size} entries each")
     if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
     max_rows = min(max_rows, T)

@@ -77,7 +77,7 @@ def test_what_tree_attention_refuses(calls):
                 dict(masks=torch.zeros(6, 1, dtype=torch.int64)), dict(masks=ints(6)), dict(masks=ints(6, 2)[:, :1]), dict(out=a["out"][:5]),
                 dict(out=torch.zeros(6, 8 * 64 + 8, dtype=torch.bfloat16)), dict(out=a["out"].float()), dict(q=a["q"][:, :500]), dict(q=a["q"].half()),
                 dict(kv_cache=a["kv_cache"].float()), dict(kv_cache=a["kv_cache"][:, :1]), dict(kv_cache=a["kv_cache"][0]),
-                dict(kv_cache=torch.zeros(9, 2, 2, 0, 64, dtype=torch.bfloat16)), dict(nh=7), dict(nkv=0), dict(d=0), dict(d=257), dict(nkv=3),
+                dict(kv_cache=torch.zeros(9, 2, 2, 0, 64, dtype=torch.bfloat16)), dict(kv_cache=torch.zeros(0, 2, 2, 16, 64, dtype=torch.bfloat16)), dict(nh=7), dict(nkv=0), dict(d=0), dict(d=257), dict(nkv=3),
                 dict(max_rows=-1), dict(max_context=-1), dict(max_rows=1 << 31), dict(max_context=1 << 32)):
         with pytest.raises(ops.KernelError):
             ops.tree_attention(**{**a, **bad})
