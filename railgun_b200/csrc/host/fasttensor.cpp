@@ -8,6 +8,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/Functions.h>
+#include <algorithm>
+#include <vector>
 
 #if !defined(__linux__) || !(defined(__x86_64__) || defined(__aarch64__))
 #error "the calling conventions relied on are those of 64-bit Linux on x86 and ARM"
@@ -98,7 +100,7 @@ static PyObject* ft_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // addresses(list or tuple of tensors, device): where they are, as 64-bit numbers in a bytes object, if they are contiguous tensors of one shape and
-// type on this CUDA device; None if not.
+// type on this CUDA device, no two in one place; None if not.
 static PyObject* ft_addresses(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 2) {
@@ -127,6 +129,12 @@ static PyObject* ft_addresses(PyObject*, PyObject* const* a, Py_ssize_t n) {
             Py_DECREF(out);
             Py_RETURN_NONE;
         }
+    }
+    std::vector<u64> places(to, to + m);
+    std::sort(places.begin(), places.end());
+    if (std::adjacent_find(places.begin(), places.end()) != places.end()) {
+        Py_DECREF(out);
+        Py_RETURN_NONE;
     }
     return out;
     END_HANDLE_TH_ERRORS

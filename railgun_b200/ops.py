@@ -2714,7 +2714,10 @@ def _cache_list(caches, what: str, here: int) -> tuple:
                 raise KernelError(f"{what}: a cache on {t.device}, the current device is cuda:{here}")
             if t.shape != first.shape:
                 raise KernelError(f"{what}: caches of {tuple(first.shape)} and {tuple(t.shape)}")
-        addresses = np.array([t.data_ptr() for t in caches], dtype=np.uint64).tobytes()
+        places = [t.data_ptr() for t in caches]
+        if len(set(places)) < len(places) and first.numel():
+            raise KernelError(f"{what}: a cache twice (its entries would move twice)")
+        addresses = np.array(places, dtype=np.uint64).tobytes()
     bits = 0
     for low in set(addresses[::8]):                  # only the lowest four bits are of interest
         bits |= low

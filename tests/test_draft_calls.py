@@ -149,7 +149,7 @@ def test_what_draft_tree_refuses(calls):
 
 
 def keep_args():
-    return dict(caches=[torch.zeros(9, 2, 2, 16, 64)] * 3, block_table=ints(2, 5), cu_rows=ints(3), starts=ints(2), parents=ints(6), tokens=ints(6),
+    return dict(caches=[torch.zeros(9, 2, 2, 16, 64) for _ in range(3)], block_table=ints(2, 5), cu_rows=ints(3), starts=ints(2), parents=ints(6), tokens=ints(6),
                 chosen=ints(6), max_rows=4)
 
 
@@ -158,7 +158,7 @@ def test_what_keep_drafts_refuses(calls):
     assert args[1:7] == [3, 9, 4, 16, 16, 16]                            # caches, pages, outer, page, pieces of a row and their bytes
     assert [tuple(t.shape) for t in made] == [(2,), (2, 4), (2, 4)]
     cache = keep_args()["caches"][0]
-    for bad in (dict(caches=[]), dict(caches=[cache, cache[:8]]), dict(caches=[cache, cache.double()]), dict(caches=cache.transpose(1, 2)),
+    for bad in (dict(caches=[]), dict(caches=[cache, cache.clone(), cache]), dict(caches=[cache, cache[:8]]), dict(caches=[cache, cache.double()]), dict(caches=cache.transpose(1, 2)),
                 dict(caches=torch.zeros(9, 16)), dict(caches=torch.zeros(0, 2, 16, 64)), dict(block_table=ints(3, 5)), dict(cu_rows=ints(2)),
                 dict(tokens=ints(5)), dict(chosen=ints(7)), dict(chosen=torch.zeros(6, dtype=torch.int64)), dict(max_rows=-1), dict(max_rows=ops.DRAFT_MOST + 1)):
         with pytest.raises(ops.KernelError):
@@ -189,6 +189,8 @@ def test_what_copies_are_made_of(calls):
             ops.copy_pages(cache, bad)
     with pytest.raises(ops.KernelError):
         ops.copy_pages([], [(0, 1, 3)])
+    with pytest.raises(ops.KernelError):
+        ops.copy_pages([cache, cache], [(0, 1, 3)])
     with pytest.raises(ops.KernelError):
         ops.copy_pages(torch.zeros(0, 2, 16, 64), [(0, 1, 3)])
 

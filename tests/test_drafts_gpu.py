@@ -507,6 +507,19 @@ def test_a_whole_chain_is_kept():
         assert torch.equal(rows(cache), expected)
 
 
+def test_a_cache_twice_is_refused():
+    """Its entries would move twice, and the second time from where others had moved to."""
+    from railgun_b200 import ops
+    cache = torch.randn(8, 2, 2, 16, 8, device=DEV)
+    before, args = cache.clone(), (i32([[0, 1]]), i32([0, 3]), i32([3]), i32([-1, 0, 0]), i32([1, 2, 3]), i32([3, 1, 1]))
+    for caches in ([cache, cache], [cache, before, cache]):
+        with pytest.raises(ops.KernelError, match="twice"):
+            ops.keep_drafts(caches, *args, max_rows=3)
+        with pytest.raises(ops.KernelError, match="twice"):
+            ops.copy_pages(caches, [(0, 1, -1)])
+    assert torch.equal(cache, before)
+
+
 def test_keep_leaves_out_what_it_should():
     from railgun_b200 import ops
     cache = torch.randn(8, 2, 2, 16, 8, device=DEV)
