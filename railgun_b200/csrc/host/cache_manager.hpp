@@ -207,12 +207,11 @@ public:
             r.tables[g].reserve(full + 1);
         }
         r.slot = free_slots_.front();
-        records_[r.slot] = records_[it->second.slot];
-        records_[r.slot].request_id = child;
-        auto made = reqs_.emplace(child, std::move(r));               // the last thing that may throw
+        CacheRequest& c = reqs_.emplace(child, std::move(r)).first->second;   // the last thing that may throw
         it = reqs_.find(parent);
         free_slots_.pop_front();
-        CacheRequest& c = made.first->second;
+        records_[c.slot] = records_[it->second.slot];
+        records_[c.slot].request_id = child;
         for (size_t g = 0; g < groups_.size(); ++g) {
             CacheGroup& G = groups_[g];
             for (int p : c.tables[g])
@@ -240,7 +239,7 @@ public:
         if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;
         CacheRequest& r = it->second;
         for (size_t g = 0; g < groups_.size(); ++g)
-            if (new_len > (int)r.tables[g].size() * groups_[g].page_size || shared_at(r, g, new_len)) return CACHE_BAD_ARGUMENT;
+            if (new_len > (int)r.tables[g].size() * groups_[g].page_size || shared_from(r, g, new_len)) return CACHE_BAD_ARGUMENT;
         records_[r.slot].num_computed = new_len;
         for (size_t g = 0; g < groups_.size(); ++g) {
             CacheGroup& G = groups_[g];
@@ -338,7 +337,13 @@ public:
     }
 
 private:
-    // Does the page that entry e would be written to belong to other requests as well?
+    // Does any of the pages from entry e on belong to other requests as well?  (None does from a request's position on.)
+    bool shared_from(const CacheRequest& r, size_t g, int e) const {
+        for (size_t i = e < 0 ? 0 : (size_t)(e / groups_[g].page_size); i < r.tables[g].size(); ++i)
+            if (r.tables[g][i] >= 0 && groups_[g].refcount[r.tables[g][i]] > 1) return true;
+        return false;
+    }
+    // Does the page that entry e would be written to?
     bool shared_at(const CacheRequest& r, size_t g, int e) const {
         const size_t i = (size_t)(e / groups_[g].page_size);
         return i < r.tables[g].size() && r.tables[g][i] >= 0 && groups_[g].refcount[r.tables[g][i]] > 1;

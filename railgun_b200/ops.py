@@ -2697,7 +2697,7 @@ def tree_general_blocks(d: int) -> int:
 
 
 def _cache_list(caches, what: str, here: int) -> tuple:
-    """One cache or several of one shape and type on the current device: (the first one, how many, their addresses as 64-bit numbers in
+    """One cache or several different ones of one shape and type on the current device: (the first one, how many, their addresses as 64-bit numbers in
     bytes, the bits of all addresses)."""
     if isinstance(caches, torch.Tensor):
         caches = (caches,)

@@ -278,6 +278,26 @@ def test_forks_with_windows_and_chunks():
     a.check()
 
 
+def test_nobody_goes_back_behind_what_is_shared():
+    """A page of one's own, and one that is shared after it: going back to the first would lead into the second."""
+    a = PageAllocator([4], [12], [6], 3)
+    a.add_request(1)
+    a.reserve(1, 12)
+    a.commit(1, 12)
+    a.fork(1, 2)
+    a.reserve(2, 14)
+    a.commit(2, 14)                                     # has passed the page of entries 4 to 7; 8 to 11 are shared
+    assert a.block_table(2).tolist()[:2] == [-1, -1] and a.block_table(2)[2] == a.block_table(1)[2]
+    for n in (5, 7, 8, 11):
+        with pytest.raises(CacheError):
+            a.commit(1, n)
+    a.commit(1, 12)
+    a.reserve(1, 20)
+    a.commit(1, 17)
+    a.commit(1, 16)                                     # nothing behind is another's
+    a.check()
+
+
 def test_random_forks_keep_the_books():
     rng = np.random.default_rng(4)
     pages = [40, 25]
