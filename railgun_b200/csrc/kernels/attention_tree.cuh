@@ -224,6 +224,10 @@ __device__ __noinline__ void row_by_formula(const TreeArgs& a, const TreeRequest
             s = 0.f;
             for (int c = 0; c < d; ++c) s += to_f32(q[c]) * a.scale_log2 * to_f32(kv[at + c]);
         }
+        if (__any_sync(0xffffffffu, seen && !(s < INFINITY))) {     // a score that is no number, or infinite: so is the whole row
+            L = NAN;
+            break;
+        }
         const float mn = fmaxf(M, warp_max(s)), ms = mn == -INFINITY ? 0.f : mn, f = exp2f(M - ms), p = exp2f(s - ms);
         L = L * f + warp_sum(p);
         M = mn;

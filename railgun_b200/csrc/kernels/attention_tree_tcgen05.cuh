@@ -360,11 +360,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                     return x + y;
                 };
                 auto pass = [&](float ms) -> float { return edge ? exp_pass(std::true_type{}, ms) : exp_pass(std::false_type{}, ms); };
-                bool redo = j == 0;
+                bool redo = j == 0, mine = redo;                      // mine: this query's reference moves; the warp's others keep theirs
                 float row_sum = 0.f;
                 if (!redo) {
                     row_sum = pass(m_ref == -INFINITY ? 0.f : m_ref);
-                    redo = __any_sync(0xffffffffu, query && (!(row_sum <= 256.f) || m_ref == -INFINITY));   // inf and NaN, too
+                    mine = query && (!(row_sum <= 256.f) || m_ref == -INFINITY);   // inf and NaN, too
+                    redo = __any_sync(0xffffffffu, mine);
                 }
                 if (redo) {
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // on raw scores: the scale is positive
@@ -376,7 +377,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                         for (int x = 0; x < 32; ++x)
                             if (seen >> (32 * c + x) & 1) mx4[x & 3] = fmaxf(mx4[x & 3], __uint_as_float(v[x]));
                     }
-                    const float m_new = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2);
+                    const float m_new = mine ? fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2) : m_ref;
                     if (j > 0) {
                         // O must be complete through pass j - 1 (the product of pass j waits for this pass's P)
                         ok = mbar_wait_all(p_free + 8 * (half ^ 1), (o_phase >> (half ^ 1) & 1) ^ 1, err, 79, &abort_flag);

@@ -331,6 +331,27 @@ def test_what_is_not_seen_has_no_say(monkeypatch, counts, starts, cluster, bad, 
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [None, 0, 2])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_queries_that_are_no_numbers(monkeypatch, bad, cluster, dtype):
+    """Their rows and heads are no numbers, quickly, and nobody else's: long contexts, where entry by entry would take its time."""
+    from railgun_b200 import ops
+    if cluster is not None:
+        monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    nh, nkv, d = 8, 2, 64
+    q, out, args, sizes = run_tree([20, 40], [3000, 100], nh, nkv, d, 16, dtype, 23)
+    hurt = q.clone()
+    hurt[3, :d] = bad                                                    # a head of a row
+    hurt[25:41] = bad                                                    # rows of the other request
+    after = torch.full_like(out, 7.0)
+    ops.tree_attention(hurt, after, *args, **sizes)
+    no = torch.zeros(after.shape, dtype=torch.bool, device=DEV)
+    no[3, :d] = True
+    no[25:41] = True
+    assert not torch.isfinite(after[no]).any() and torch.equal(after[~no], out[~no])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_what_a_call_says_is_what_is_seen(dtype):
     """Rows beyond max_rows are left as they were, nodes beyond them and entries beyond max_context are not seen; a request with a
     negative start is left out."""
