@@ -242,6 +242,11 @@ __device__ __noinline__ void row_by_formula(const TreeArgs& a, const TreeRequest
             for (int k = 0; k < 8; ++k)
                 if (lane + 32 * k < d) acc[k] += pj * to_f32(kv[vj + lane + 32 * k]);
         }
+        bool settled = true;                                        // what is no number stays so
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (lane + 32 * k >= from_col && lane + 32 * k < to_col) settled &= acc[k] != acc[k];
+        if (__all_sync(0xffffffffu, settled)) break;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll

@@ -349,6 +349,13 @@ def test_queries_that_are_no_numbers(monkeypatch, bad, cluster, dtype):
     no[3, :d] = True
     no[25:41] = True
     assert not torch.isfinite(after[no]).any() and torch.equal(after[~no], out[~no])
+    # and values: of the first request's first entry and kv head
+    cache, table = args[0].clone(), args[1]
+    cache[table[0, 0].long(), 1, 0, 0] = bad
+    ops.tree_attention(q, after, cache, table, *args[2:], **sizes)
+    no[:] = False
+    no[1:21, :nh // nkv * d] = True
+    assert not torch.isfinite(after[no]).any() and torch.equal(after[~no], out[~no])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
