@@ -9,6 +9,7 @@
 #define TG_Q 16                // queries of an item
 #define TG_K 64                // entries of a tile
 #define TG_LD (TG_K + 4)
+#define TG_BEGIN 0             // places in front of an item's tiles: queries come out of L2 and a part goes there, a tile's time takes longer
 
 template <typename A> struct Quad;                                  // four numbers of a row at once
 template <> struct Quad<float> {
@@ -53,9 +54,9 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
         n_tiles = min(w.x.tiles, w.tile + per) - w.tile;
     } else {
         tree_plan<TG_THREADS>(a, blockIdx.x, 1, 0, st);
-        if (st.r[0] < 0) return;
-        n_tiles = (int)min(st.per, st.total - (long long)blockIdx.x * st.per);
-        w.at(st, 0);
+        n_tiles = st.tiles(0);
+        if (n_tiles == 0) return;
+        w.at(a, st, 0);
     }
     const int d = a.d, ld = tg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = tg_stages(d);
     float* qs = smem;                                               // [16][ld]
@@ -106,11 +107,11 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     const int col = tid % DP, part = tid / DP;                      // output: column(s) col (+ 128), entries part + GROUPS j
     float m[2], l[2];
     float acc[COLS][TG_Q];
-    int q0 = 0, nq = 0, parts = 0, done = 0;                        // parts of the item, 0: it began before this stretch
+    int q0 = 0, nq = 0, parts = 0;                                  // parts of the item, 0: it began before this stretch
     auto begin = [&]() {                                            // an item
         q0 = w.block() * TG_Q;
         nq = min(TG_Q, w.x.rows * group - q0);
-        if constexpr (!WHOLE) parts = w.tile == 0 ? w.parts(done, st.per) : 0;
+        if constexpr (!WHOLE) parts = w.tile == 0 ? w.parts(st.per) : 0;
         for (int j = tid; j < TG_Q * ld; j += TG_THREADS) {         // nobody reads the last item's any more
             const int row = j / ld, c = j - row * ld, qi = q0 + row;
             float v = 0.f;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     if (stages == 2 && n_tiles > 0) request(0, kv0);
     if (WHOLE) begin();
     for (int step = 0; step < n_tiles; ++step) {
-        if (!WHOLE && (step == 0 || w.tile == 0)) { done = step; begin(); }
+        if (!WHOLE && (step == 0 || w.tile == 0)) begin();
         const int slot = step & 1, e0 = w.tile * TG_K, n = min(TG_K, w.x.entries - e0);
         float* ks = kv0 + (stages == 2 ? slot * 2 * TG_K * ld : 0);
         const float* vs = ks + TG_K * ld;
@@ -471,6 +472,7 @@ extern "C" int rg_tree_attention(const void* q, int q_stride, void* out, int out
     a.page_shift = -1;
     for (int b = 0; b < 31; ++b) if (page_size == (1 << b)) a.page_shift = b;
     a.tile = tensor_cores ? TT_STAGE : TG_K;
+    a.begin = tensor_cores ? TT_BEGIN : TG_BEGIN;
     if (cluster) {
         if (cluster > 8 || tensor_cores || item_queries != TG_Q) return RG_ERR_UNSUPPORTED;
         const long long q_blocks = ((long long)max_rows * (nh / nkv) + TG_Q - 1) / TG_Q;

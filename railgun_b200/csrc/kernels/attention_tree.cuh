@@ -6,7 +6,8 @@
 //
 // An item is (request, kv head, block of queries); query i of a request and kv head is row i / group, head i % group.  An item has
 // ceil(entries / tile) tiles.  All items' tiles, one item after the other, are one line that is cut into as many stretches of `per`
-// tiles as there are workers: whatever the requests' lengths, every worker has the same number of tiles to read.  A stretch
+// places as there are workers: whatever the requests' lengths, every worker has the same work.  In front of an item's tiles are `begin`
+// places that hold none, for what an item costs a worker besides (the last one's part left, queries and a first maximum had).  A stretch
 // may end inside an item; what a worker finds for an item, its part, is left as the unnormalised output o = sum 2^(s - m) v with
 // m = max s and l = sum 2^(s - m), s = scale log2(e) q.k, in 32-bit, and a second kernel joins the parts of every row and head:
 //   out = sum_parts 2^(m - M) o / sum_parts 2^(m - M) l,   M = max_parts m
@@ -34,7 +35,8 @@ struct TreeArgs {
     int R, T, max_rows, limit;   // limit: the most entries of a request that are seen
     int q_stride, max_blocks, words, pages;
     int nh, nkv, d, page_size, page_shift;      // page_shift: log2 of the page size, or -1
-    int tile, item_queries, workers, least;     // entries of a tile, queries of an item, workers, least tiles of a stretch
+    int tile, item_queries, workers, least;     // entries of a tile, queries of an item, workers, least places of a stretch
+    int begin;                   // places in front of an item's tiles
     float scale_log2;
 };
 
@@ -51,40 +53,42 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
     x.start = start;
     x.entries = x.rows ? (int)min((long long)a.limit, (long long)start + x.rows) : 0;
     x.tiles = (x.entries + a.tile - 1) / a.tile;
-    x.blocks = (int)(((long long)x.rows * (a.nh / a.nkv) + a.item_queries - 1) / a.item_queries);
+    x.blocks = (int)(((unsigned)x.rows * (unsigned)(a.nh / a.nkv) + a.item_queries - 1u) / (unsigned)a.item_queries);   // (T x nh is below 2^31)
     return x;
 }
-__device__ __forceinline__ long long tree_tiles(const TreeArgs& a, const TreeRequest& x) { return (long long)x.tiles * x.blocks * a.nkv; }
-
-// Tiles of all items, and where (up to two) workers begin: a request, -1: nowhere, and a place among its tiles.
+// Places of a stretch, and of up to two workers: where they begin (a request, -1: nowhere; an item of it; a place of that) and how many
+// tiles lie on the line before that and before their end.
 struct TreeStart {
-    long long total, per;
-    long long in[2];
-    int r[2];
+    long long per, from[2], to[2];
+    int r[2], item[2], in[2];
     TreeRequest x[2];
+    __device__ __forceinline__ int tiles(int i) const { return r[i] < 0 ? 0 : (int)min(0x7fffffffll, to[i] - from[i]); }
 };
 
 // Where a worker is on the line: an item and a tile of it.
 struct TreeWalk {
     TreeRequest x;
     int r, item, tile;           // item: kv head x blocks + block of queries
+    int place;                   // of the tile, in the worker's stretch
     __device__ __forceinline__ int kvh() const { return item / x.blocks; }
     __device__ __forceinline__ int block() const { return item % x.blocks; }
     __device__ __forceinline__ void skip_empty(const TreeArgs& a) {      // to a request that has tiles (one is known to come)
         while (x.tiles == 0 || x.blocks == 0) x = tree_request(a, ++r);
     }
-    // Where worker i of `st` begins.
-    __device__ __forceinline__ void at(const TreeStart& st, int i) {
+    // The first tile of worker i of `st`, which has some.
+    __device__ __forceinline__ void at(const TreeArgs& a, const TreeStart& st, int i) {
         r = st.r[i];
         x = st.x[i];
-        const long long in = st.in[i];
-        item = in >> 32 ? (int)(in / x.tiles) : (int)((unsigned)in / (unsigned)x.tiles);
-        tile = (int)(in - (long long)item * x.tiles);
+        item = st.item[i];
+        place = max(0, a.begin - st.in[i]);
+        tile = max(0, st.in[i] - a.begin);
     }
-    // One tile on; `more`: there is one.
-    __device__ __forceinline__ void next(const TreeArgs& a, bool more) {
-        if (++tile < x.tiles) return;
+    // n tiles on, of which all but the last are this item's; `more`: there is one.
+    __device__ __forceinline__ void next(const TreeArgs& a, bool more, int n = 1) {
+        place += n;
+        if ((tile += n) < x.tiles) return;
         tile = 0;
+        place += a.begin;
         if (++item < x.blocks * a.nkv) return;
         item = 0;
         if (!more) return;
@@ -92,8 +96,10 @@ struct TreeWalk {
         skip_empty(a);
     }
     __device__ __forceinline__ bool last_tile() const { return tile + 1 == x.tiles; }
-    // In how many parts the item is cut whose first tile is a worker's `done`-th.
-    __device__ __forceinline__ int parts(int done, long long per) const { return (int)((unsigned)(done + x.tiles - 1) / (unsigned)min(per, 0x7fffffffll)) + 1; }
+    // In how many parts the item is cut whose first tile this is.
+    __device__ __forceinline__ int parts(long long per) const {
+        return (int)((unsigned)(place + x.tiles - 1) / (unsigned)min(per, 0x7fffffffll)) + 1;
+    }
     // The first query of the item among all rows' and heads'.
     __device__ __forceinline__ long long first_query(const TreeArgs& a) const {
         return (long long)x.row0 * a.nh + (long long)kvh() * x.rows * (a.nh / a.nkv) + (long long)block() * a.item_queries;
@@ -120,62 +126,72 @@ __device__ __forceinline__ void tree_gaps(const TreeArgs& a) {
     }
 }
 
-// The whole block, THREADS threads: tiles of all items, and the request (with the place among its tiles) in which each of `n`
-// (up to 2) workers, `first` and `first` + `apart`, begins (r -1: it has nothing).  The last block says which rows nobody has.
+// The whole block, THREADS threads: where each of `n` (up to 2) workers, `first` and `first` + `apart`, begins and how many tiles it
+// has.  The last block says which rows nobody has.
 template <int THREADS>
 __device__ __forceinline__ void tree_plan(const TreeArgs& a, int first, int n, int apart, TreeStart& st) {
-    __shared__ long long sums[THREADS / 32 + 1];
+    __shared__ long long s_places[THREADS / 32];
+    __shared__ int s_items[THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto scan = [&](long long v, long long& total) -> long long {       // exclusive, over the block
-        long long x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) sums[warp] = x;
-        __syncthreads();
-        long long before = 0;
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += sums[w];
-            total += sums[w];
-        }
-        return before + x - v;
-    };
-    long long total = 0, mine = 0, before = 0;
+    // Loops stay loops here: this code runs once a launch and comes from memory, each 128 bytes of it a trip.
+    long long mine = 0, before = 0, total = 0;                           // places of this thread's request, of the requests before it, of all
+    int items = 0, items_before = 0, items_total = 0;
     TreeRequest x;
-    if (threadIdx.x < 2) st.r[threadIdx.x] = -1;
-    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
-        const int r = r0 + threadIdx.x;
-        long long some;
-        if (r < a.R) x = tree_request(a, r);
-        mine = r < a.R ? tree_tiles(a, x) : 0;
-        before = total + scan(mine, some);
-        total += some;
-    }
-    const long long per = max((long long)a.least, total >> 31 ? (total + a.workers - 1) / a.workers : (long long)((unsigned)total + a.workers - 1u) / a.workers);
-    if (threadIdx.x == 0) {
-        st.total = total;
-        st.per = per;
-    }
-    const bool once = a.R <= THREADS;                                    // what was found above still stands
-    long long sofar = 0;
-    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
-        const int r = r0 + threadIdx.x;
-        if (!once) {
-            long long some;
-            if (r < a.R) x = tree_request(a, r);
-            mine = r < a.R ? tree_tiles(a, x) : 0;
-            before = sofar + scan(mine, some);
-            sofar += some;
+    auto look = [&](int r0) {                                            // at THREADS requests from r0 on; what came before is in the totals
+        const int r = r0 + threadIdx.x, some = a.R - r0;
+        items = 0;
+        mine = 0;
+        if (r < a.R) {
+            x = tree_request(a, r);
+            items = x.tiles ? x.blocks * a.nkv : 0;
+            mine = (long long)items * (x.tiles + a.begin);
         }
-        if (r >= a.R) continue;
-        for (int i = 0; i < n; ++i) {
-            const long long at = (first + (long long)i * apart) * per - before;
-            if (at >= 0 && at < mine) { st.r[i] = r; st.in[i] = at; st.x[i] = x; }
+        long long p = mine;
+        int n = items;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long q = __shfl_up_sync(0xffffffffu, p, o);
+            const int m = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) { p += q; n += m; }
+        }
+        __syncthreads();
+        if (lane == 31) { s_places[warp] = p; s_items[warp] = n; }
+        __syncthreads();
+        before = total + p - mine;
+        items_before = items_total + n - items;
+#pragma unroll 1
+        for (int w = 0; w < THREADS / 32 && 32 * w < some; ++w) {
+            if (w < warp) { before += s_places[w]; items_before += s_items[w]; }
+            total += s_places[w];
+            items_total += s_items[w];
+        }
+    };
+    if (threadIdx.x < 2) st.r[threadIdx.x] = -1;
+    for (int r0 = 0; r0 < a.R; r0 += THREADS) look(r0);
+    const long long all = total;
+    const long long per = max((long long)a.least, all >> 31 ? (all + a.workers - 1) / a.workers : (long long)(((unsigned)all + a.workers - 1u) / a.workers));
+    if (threadIdx.x == 0) st.per = per;
+    if (threadIdx.x < n && (first + (long long)threadIdx.x * apart + 1) * per >= all) st.to[threadIdx.x] = all - (long long)items_total * a.begin;
+    const bool once = a.R <= THREADS;                                    // what was found above still stands
+    if (!once) total = items_total = 0;
+    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
+        if (!once) look(r0);
+        if (mine == 0) continue;
+        const int len = x.tiles + a.begin;
+#pragma unroll 1
+        for (int i = 0; i < 2 * n; ++i) {                                // the places where the workers begin, and where they end
+            const long long place = (first + (long long)(i >> 1) * apart + (i & 1)) * per, at = place - before;
+            if (at < 0 || at >= mine) continue;
+            const int item = at >> 32 ? (int)(at / len) : (int)((unsigned)at / (unsigned)len), in = (int)(at - (long long)item * len);
+            const long long tiles = place - (long long)(items_before + item) * a.begin - min(in, a.begin);
+            if (i & 1) st.to[i >> 1] = tiles;
+            else {
+                st.from[i >> 1] = tiles;
+                st.r[i >> 1] = r0 + threadIdx.x;
+                st.item[i >> 1] = item;
+                st.in[i >> 1] = in;
+                st.x[i >> 1] = x;
+            }
         }
     }
     if (blockIdx.x == gridDim.x - 1) tree_gaps<THREADS>(a);

@@ -34,6 +34,9 @@
 #define TT_STAGE 128               // entries of a K or V stage: a tile
 #define TT_THREADS 384             // warps 0-3, 4-7: softmax of side 0, 1; 8, 10: TMA of K, of V; 9, 11: MMA issue (and TMA of Q) of side 0, 1
 #define TT_BARRIERS 384            // bytes
+// Places in front of an item's tiles.  With 0, 2 and 3 of them: 4 requests of 64 nodes on 8,192 entries 59.0, 55.1 and 54.5 us, 64 of 16 behind up to
+// 4,096 147.9, 146.2 and 148.1, 128 of 16 behind up to 500 74.4, 72.1 and 72.8, 128 nodes on 65,536 145.1, 141.8 and 141.8.
+#define TT_BEGIN 2
 __host__ __device__ constexpr int tt_k_stages(int pieces) { return pieces == 1 ? 5 : 3; }
 __host__ __device__ constexpr int tt_v_stages(int pieces) { return pieces == 1 ? 4 : 2; }
 __host__ __device__ constexpr int tt_smem(int pieces) {
@@ -129,14 +132,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (st.r[0] < 0) {                                                // nothing for side 0: nothing at all
+    const int n_t0 = st.tiles(0), n_t1 = both ? 0 : st.tiles(1);      // n_t1: of its own stretch
+    if (n_t0 + n_t1 == 0) {
         if (warp == 11) tmem_free(tmem_base_slot, 512u);
         return;
     }
-    auto tiles_of = [&](int s) -> int { return (int)max(0ll, min(st.per, st.total - (long long)worker_of(s) * st.per)); };
-    const int n_t0 = tiles_of(0), n_t1 = both ? 0 : tiles_of(1);      // n_t1: of its own stretch
-    // A stage of the stream belongs to both sides, or in turn to either while side 1 has some
-    const int n_stages = n_t0 + n_t1;
+    // A stage of the stream belongs to both sides, or in turn to either while both have some, then to who has more
+    const int n_stages = n_t0 + n_t1, n_turns = min(n_t0, n_t1);
+    auto stages_on = [&](int s, int t) -> int {                       // from side s's tile t to its next
+        return both || t >= n_turns ? 1 : t + 1 < n_turns ? 2 : 2 - s;
+    };
     // side s: scores and weights in columns [256 s, 256 s + 128), O in [256 s + 128, 256 s + 128 + D)
     const uint32_t tmem = tmem_base_slot;
 
@@ -145,8 +150,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const int box_rows = min(a.page_size, TT_STAGE), boxes = TT_STAGE / box_rows, box = lane % boxes, piece = lane / boxes;
         const bool mine = piece < PIECES;
         TreeWalk w0, w1;
-        w0.at(st, 0);
-        if (n_t1) w1.at(st, 1);
+        if (n_t0) w0.at(a, st, 0);
+        if (n_t1) w1.at(a, st, 1);
         int left0 = n_t0, left1 = n_t1;
         const int kv = warp == 10 ? 1 : 0, n = kv ? NV : NK;
         auto row_of = [&](TreeWalk& w, int& left) -> int {            // the cache's row of this lane's box; one tile on
@@ -157,7 +162,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
             w.next(a, --left > 0);
             return row;
         };
-        auto side_of = [&](int b) -> int { return !both && b < 2 * n_t1 ? b & 1 : 0; };
+        auto side_of = [&](int b) -> int { return b < 2 * n_turns ? b & 1 : n_t1 > n_t0; };
         auto look_up = [&](int b) -> int {                            // of stage b, one after the other
             if (b >= n_stages) return 0;
             return side_of(b) ? row_of(w1, left1) : row_of(w0, left0);
@@ -185,10 +190,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const uint64_t qd = desc_k_major(sQ + s * TILE);
         // where this side's K and V tiles are in their rings, which of its tiles that is, and a bit a stage: the phase it waits for
         const uint32_t k_full = k_full0 + (both ? 0 : 8 * NK * s), v_full = v_full0 + (both ? 0 : 8 * NV * s);
-        int ki = both ? 0 : s, vi = ki, kt = 0, vt = 0;
+        int ki = n_turns ? s : 0, vi = ki, kt = 0, vt = 0;
         uint32_t k_phase = 0, v_phase = 0;
         auto ahead = [&](int& i, int& t, int n) {
-            i += !both && (s || t < n_t1) ? 2 : 1;
+            i += stages_on(s, t);
             ++t;
             if (i >= n) i -= n;
         };
@@ -196,7 +201,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         auto v_seen = [&]() { v_phase ^= 1u << vi; };
         int p_phase[2] = {0, 0}, q_phase = 0;
         TreeWalk w;
-        if (n_t) w.at(st, both ? 0 : s);
+        if (n_t) w.at(a, st, both ? 0 : s);
         auto issue_s = [&](int half, bool last) {                     // K is there
             if (issuer) {
                 const uint64_t kd = desc_k_major(sK0 + ki * TILE + half * SUB);
@@ -283,8 +288,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                 }
             }
             done += nt;
-            w.tile += nt - 1;
-            w.next(a, done < n_t);
+            w.next(a, done < n_t, nt);
         }
     } else if (warp < 8) {
         // ---- softmax and parts: thread = query
@@ -293,7 +297,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
         const uint32_t s_full = s_full0 + 16 * s, p_full = p_full0 + 16 * s, p_free = p_free0 + 16 * s;
         int s_phase = 0, o_phase = 0;                                 // bit `half`: of the next scores, of the next product
         TreeWalk w;
-        if (n_t) w.at(st, both ? 0 : s);
+        if (n_t) w.at(a, st, both ? 0 : s);
         bool ok = true;
         for (int done = 0; done < n_t && ok;) {                       // a part of an item
             const int nt = min(n_t - done, w.x.tiles - w.tile), row_first = (w.block() * (both ? 2 : 1) + (both ? s : 0)) * tile_rows;
@@ -421,13 +425,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant_
                 }
                 if (query) {
                     *reinterpret_cast<float2*>(a.part_ml + place * 2) = make_float2(m_ref, l_run);
-                    if (w.tile == 0) a.parts[(size_t)t * a.nh + w.kvh() * group + i % group] = make_int2((int)place, w.parts(done, st.per));
+                    if (w.tile == 0) a.parts[(size_t)t * a.nh + w.kvh() * group + i % group] = make_int2((int)place, w.parts(st.per));
                 }
                 tc_fence_before();                                    // before the next item's first product
             }
             done += nt;
-            w.tile += nt - 1;
-            w.next(a, done < n_t);
+            w.next(a, done < n_t, nt);
         }
     }
     tc_fence_before();
