@@ -283,8 +283,25 @@ def test_odd_sizes(nh, nkv, d, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_many_requests(dtype):
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 2, 64, 16), (24, 8, 128, 16), (5, 5, 24, 4), (80, 2, 128, 32), (4, 1, 256, 16)])
+@pytest.mark.parametrize("seed", range(4))
+def test_stretches_that_begin_and_end_anywhere(monkeypatch, seed, nh, nkv, d, page, dtype):
+    """Requests of all lengths, so that stretches begin and end in the middle of items, between them, and where there is little or nothing."""
+    from railgun_b200 import ops
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: 0)
+    rng = random.Random(seed)
+    n = rng.choice([1, 3, 17, 60])
+    most, longest = rng.choice([1, 4, 20, 50]), rng.choice([0, 30, 300, 1500])
+    run_tree([rng.randrange(most + 1) for _ in range(n - 1)] + [most], [rng.randrange(longest + 1) for _ in range(n)], nh, nkv, d, page, dtype, seed)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [None, 0])
+def test_many_requests(monkeypatch, cluster, dtype):
     """More requests than a block has threads, most of them short."""
+    from railgun_b200 import ops
+    if cluster is not None:
+        monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
     rng = random.Random(3)
     n = 700
     run_tree([rng.choice([0, 1, 1, 2, 5]) for _ in range(n)], [rng.choice([0, 1, 9, 40]) for _ in range(n)], 4, 2, 64, 16, dtype, 8)
