@@ -9,7 +9,9 @@
 #define TG_Q 16                // queries of an item
 #define TG_K 64                // entries of a tile
 #define TG_LD (TG_K + 4)
-#define TG_BEGIN 0             // places in front of an item's tiles: queries come out of L2 and a part goes there, a tile's time takes longer
+// Places in front of an item's tiles.  In 32-bit, 16 heads on 4, with 0, 1 and 2 of them: 16 requests of 16 nodes behind up to 700 entries
+// (128) 88.5, 83.4 and 89.7 us, 4 of 64 on 2,000 (64) 156.5, 154.5 and 160.5, 64 of 4 behind up to 300 (128) 68.4, 68.8 and 73.7.
+#define TG_BEGIN 1
 
 template <typename A> struct Quad;                                  // four numbers of a row at once
 template <> struct Quad<float> {
