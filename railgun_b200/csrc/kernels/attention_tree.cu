@@ -25,8 +25,18 @@ template <> struct Quad<bf16> {
     }
 };
 
-__host__ __device__ inline int tg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
+__host__ __device__ constexpr int tg_row(int d) { return ((d + 3) & ~3) + 4; }   // floats a row in shared memory
 __host__ __device__ inline int tg_stages(int d) { return d <= 128 ? 2 : 1; }   // tiles of K and V in shared memory: the next one is on its way
+// Floats of a stage: a tile's K and V, and no fewer than the sums that go through it where an item ends and groups of threads share the
+// columns (d up to 64), since the next stage then holds the next item's first tile already.  Heads of 1 to 8 have tiles of fewer.
+#define TG_SUMS (TG_Q * TG_THREADS)
+__host__ __device__ constexpr int tg_stage(int d) {
+    const int tile = 2 * TG_K * tg_row(d);
+    return d <= 64 && tile < TG_SUMS ? TG_SUMS : tile;
+}
+static_assert(tg_stage(1) >= TG_SUMS && tg_stage(8) >= TG_SUMS && tg_stage(9) >= TG_SUMS && tg_stage(64) >= TG_SUMS, "the groups' sums fit a stage");
+static_assert(2 * tg_stage(1) >= TG_SUMS + TG_Q && 2 * tg_stage(32) >= TG_SUMS + TG_Q * 32 && 2 * tg_stage(64) >= TG_SUMS + TG_Q * 64,
+              "and behind a cluster's results both stages");
 
 // ---------------------------------------------------------------------------------------------------
 // Any head size up to 256, any page size, 32-bit or bfloat16 storage, all arithmetic in 32-bit.
@@ -62,8 +72,9 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     }
     const int d = a.d, ld = tg_row(d), group = a.nh / a.nkv, tid = threadIdx.x, stages = tg_stages(d);
     float* qs = smem;                                               // [16][ld]
-    float* kv0 = qs + TG_Q * ld;                                    // [stages][K [64][ld], V [64][ld]]
-    float* ps = kv0 + stages * 2 * TG_K * ld;                       // [16][TG_LD]
+    const int stage = tg_stage(d);
+    float* kv0 = qs + TG_Q * ld;                                    // [stages][K [64][ld], V [64][ld]], `stage` floats each
+    float* ps = kv0 + stages * stage;                               // [16][TG_LD]
     float* al = ps + TG_Q * TG_LD;                                  // [16]
     const size_t to_values = (size_t)a.nkv * a.page_size * d;
     ahead = w;
@@ -136,7 +147,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
     for (int step = 0; step < n_tiles; ++step) {
         if (!WHOLE && (step == 0 || w.tile == 0)) begin();
         const int slot = step & 1, e0 = w.tile * TG_K, n = min(TG_K, w.x.entries - e0);
-        float* ks = kv0 + (stages == 2 ? slot * 2 * TG_K * ld : 0);
+        float* ks = kv0 + (stages == 2 ? slot * stage : 0);
         const float* vs = ks + TG_K * ld;
         if (stages == 1) {
             __syncthreads();                                        // the last tile's values are read
@@ -144,7 +155,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
         }
         rgmma::cp_async_wait<0>();
         __syncthreads();                                            // the tile is there; with two stages the last one is read
-        if (stages == 2 && step + 1 < n_tiles) request(slot ^ 1, kv0 + (slot ^ 1) * 2 * TG_K * ld);
+        if (stages == 2 && step + 1 < n_tiles) request(slot ^ 1, kv0 + (slot ^ 1) * stage);
         float sc[2][4] = {};
 #pragma unroll 4
         for (int c = 0; c < d; c += 4) {
@@ -218,7 +229,7 @@ __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs
                 for (int o = 8; o > 0; o >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], o);
             }
             const size_t place = (size_t)w.first_query(a) + (size_t)blockIdx.x * TG_Q;
-            if constexpr (GROUPS > 1) {                             // the groups' sums, added in their order, through this tile's K and V
+            if constexpr (GROUPS > 1) {                             // the groups' sums, added in their order, through this stage
                 __syncthreads();
 #pragma unroll
                 for (int i = 0; i < TG_Q; ++i) ks[i * TG_THREADS + tid] = acc[0][i];
@@ -428,7 +439,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) tree_join_kernel(const TreeArgs 
 }
 
 // ---------------------------------------------------------------------------------------------------
-static size_t tg_smem(int d) { return (size_t)((TG_Q + tg_stages(d) * 2 * TG_K) * tg_row(d) + TG_Q * TG_LD + TG_Q) * sizeof(float); }
+static size_t tg_smem(int d) { return (size_t)(TG_Q * tg_row(d) + tg_stages(d) * tg_stage(d) + TG_Q * TG_LD + TG_Q) * sizeof(float); }
 
 // cluster: not 0, an item to a cluster of so many blocks.
 static int launch_tree_general(const TreeArgs& a, int dtype, void* out, int out_ld, int cluster, int q_blocks, cudaStream_t s) {

@@ -297,6 +297,20 @@ def test_stretches_that_begin_and_end_anywhere(monkeypatch, seed, nh, nkv, d, pa
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("cluster", [None, 0])
+@pytest.mark.parametrize("nh,nkv,d,page", [(8, 8, 8, 16), (8, 8, 1, 16), (8, 8, 4, 4), (6, 6, 5, 7), (16, 8, 3, 16), (8, 8, 9, 16), (8, 4, 32, 8)])
+def test_small_heads_in_stretches(monkeypatch, nh, nkv, d, page, cluster, dtype):
+    """More items of a tile or two than there are workers, so that stretches go on behind an item's end while the next item's first tile is
+    there: sums of groups of threads that share columns have room of their own."""
+    from railgun_b200 import ops
+    if cluster is not None:
+        monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    rng = random.Random(d)
+    n = 256
+    run_tree([rng.choice([1, 1, 1, 2]) for _ in range(n)], [rng.choice([63, 62, 64, 20, 130]) for _ in range(n)], nh, nkv, d, page, dtype, d)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cluster", [None, 0])
 def test_many_requests(monkeypatch, cluster, dtype):
     """More requests than a block has threads, most of them short."""
     from railgun_b200 import ops
