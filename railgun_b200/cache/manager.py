@@ -432,9 +432,9 @@ class CacheManager:
         try:
             for g, some in zip(self.groups, copies):
                 if len(some):
-                    # entries that stand for several tokens, or whose number is no page's axis, are copied by whole pages
-                    shape = g.need.shape_of_page(g.page_size)
-                    if g.need.tokens_per_entry > 1 or len(shape) < 2 or shape[-2] != g.page_size:
+                    # entries that stand for several tokens, and tokens that are not the last axis but one, are copied by whole pages
+                    shape = g.need.page_shape
+                    if g.need.tokens_per_entry > 1 or (shape is not None and (len(shape) < 2 or shape[-2] != "page")):
                         some = np.array([[some[0, 0], some[0, 1], -1]], dtype=np.int32)
                     ops.copy_pages([self.kv[cid] for cid in g.cache_ids], some)
             slots = [(self.alloc.slot(parent), self.alloc.slot(child), -1)]

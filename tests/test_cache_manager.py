@@ -333,3 +333,31 @@ def test_random_forks_keep_the_books():
         a.release(rid)
     a.check()
     assert [a.free_pages(g) for g in range(2)] == pages
+
+
+@pytest.mark.parametrize("need,page_size,held", [
+    (PagedKVNeed(2, 8), 4, 2),                                           # keys and values
+    (PagedKVNeed(1, 8, page_shape=("page", 8)), 4, 2),
+    (PagedKVNeed(1, 8, page_shape=(3, "page", 8)), 4, 2),
+    (PagedKVNeed(4, 8, page_shape=("page", 4, 8)), 4, -1),               # as many heads as a page has tokens: not the tokens' axis
+    (PagedKVNeed(4, 8, page_shape=(4, 8, "page")), 4, -1),
+    (PagedKVNeed(1, 8, page_shape=("page",)), 4, -1),
+    (PagedKVNeed(1, 8, page_shape=()), 4, -1),
+    (PagedKVNeed(2, 8, page_size=2, tokens_per_entry=2), 4, -1),         # entries of two tokens
+])
+def test_a_fork_copies_tokens_only_along_their_own_axis(monkeypatch, need, page_size, held):
+    """The page that is being filled is copied as far as it is full where its last axis but one is the tokens', whole elsewhere."""
+    import torch
+    from railgun_b200 import ops
+    from railgun_b200.cache.manager import CacheManager
+    copied = []
+    monkeypatch.setattr(ops, "copy_pages", lambda caches, copies: copied.append((caches, np.asarray(copies).tolist())))
+    cache = CacheManager({"a": need, "b": need}, page_size, 40, 3, torch.float32, "cpu")
+    cache.alloc.add_request(1)
+    cache.alloc.reserve(1, 6)
+    cache.alloc.commit(1, 6)
+    cache.fork(1, 2)
+    (caches, copies), = copied
+    assert [c.data_ptr() for c in caches] == [cache.kv["a"].data_ptr(), cache.kv["b"].data_ptr()]
+    assert copies == [[int(cache.alloc.block_table(1)[1]), int(cache.alloc.block_table(2)[1]), held]]
+    cache.alloc.check()
