@@ -89,7 +89,7 @@ def _lib():
         for name in ("add_request", "release", "has", "num_computed", "slot"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong]
         lib.rg_cache_fork.argtypes = [c_void_p, c_longlong, c_longlong, c_void_p]
-        for name in ("reserve", "commit", "shrink"):
+        for name in ("reserve", "commit", "shrink", "shares"):
             getattr(lib, f"rg_cache_{name}").argtypes = [c_void_p, c_longlong, c_int]
         lib.rg_cache_can_reserve.argtypes = [c_void_p, c_longlong, c_int, c_int]
         lib.rg_cache_table.argtypes = [c_void_p, c_longlong, c_int, c_void_p, c_int]
@@ -246,12 +246,23 @@ class PageAllocator:
         """A new request ``child`` that goes on from where ``parent`` is (what it has committed): it shares the pages that are full, and for
         each group's page that is full in part it has one of its own.  Returns, group by group, what is to be copied before either goes on,
         as ``ops.copy_pages`` takes it: int32 [0 or 1, 3], (from, to, tokens held).  All groups or none.  The child's record is the parent's
-        (``set_request`` gives it a seed of its own).  From then on neither can go back (``commit``, ``shrink``) to write into a page that both hold."""
+        (``set_request`` gives it a seed of its own).  From then on neither can go back (``commit``, ``shrink``) to write into a page that both hold.  What moves entries inside
+        of them, ``ops.evict_entries`` above all, would change the other's: ``shares`` says where that may not be done."""
         copies = np.empty((len(self.page_sizes), 3), dtype=np.int32)
         slot = self._lib.rg_cache_fork(self._h, parent, child, copies.ctypes.data)
         if slot < 0:
             self._raise(slot, f"fork({parent}, {child})")
         return [copies[g:g + 1] if copies[g, 0] >= 0 else copies[:0] for g in range(len(copies))]
+
+    def shares(self, req_id: int, end: int | None = None) -> bool:
+        """Do other requests hold any of the pages of entries 0 .. ``end`` - 1 (None: any page of the request) as well?  ``ops.evict_entries``
+        writes into the pages of the entries that stay and must not be called then."""
+        if end is not None and not 0 <= end < 1 << 31:
+            raise CacheError(f"shares({req_id}, {end}): bad argument")
+        code = self._lib.rg_cache_shares(self._h, req_id, -1 if end is None else int(end))
+        if code < 0:
+            self._raise(code, f"shares({req_id}, {end})")
+        return code == 1
 
     def release(self, req_id: int) -> None:
         code = self._lib.rg_cache_release(self._h, req_id)

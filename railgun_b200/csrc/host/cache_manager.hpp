@@ -19,7 +19,8 @@
 // (pop front, push back) so that reuse order is deterministic, a reference
 // count per page, and a double free is an error.  Requests that were forked
 // from one another share the pages that were full then; nobody goes back to
-// write into a page that more than one request holds.  The reference shares one
+// write into a page that more than one request holds, and who would move
+// entries inside of pages asks whether they are shared.  The reference shares one
 // pool between all layers (crates/vllm-paged-attention/src/block.rs:49-59);
 // here a page id addresses one page in every layer of its group.
 #pragma once
@@ -231,6 +232,19 @@ public:
             c.tables[g].push_back(to);
         }
         return c.slot;
+    }
+
+    // Do other requests hold any of the pages of this one's entries [0, end) (end < 0: of all that it has) as well?  1, 0 or a negative status.
+    int shares(int64_t id, int end) const {
+        auto it = reqs_.find(id);
+        if (it == reqs_.end()) return CACHE_UNKNOWN_REQUEST;
+        for (size_t g = 0; g < groups_.size(); ++g) {
+            const std::vector<int>& t = it->second.tables[g];
+            const size_t pages = end < 0 ? t.size() : std::min(t.size(), ((size_t)end + groups_[g].page_size - 1) / groups_[g].page_size);
+            for (size_t i = 0; i < pages; ++i)
+                if (t[i] >= 0 && groups_[g].refcount[t[i]] > 1) return 1;
+        }
+        return 0;
     }
 
     // Tokens [0, new_len) are now in the cache; windowed groups give back what every later query has passed.

@@ -123,8 +123,15 @@ class LongPrompts:
             raise
         return prompt
 
+    def check_own(self, prompt: Prompt) -> None:
+        """Eviction moves entries into those that stay: their pages have to be the prompt's alone."""
+        if self.alloc.shares(prompt.request, min(prompt.entries, self.budget)):
+            raise ValueError(f"request {prompt.request}: entries cannot be evicted from pages that other requests hold, too")
+
     def evict(self, prompts) -> None:
         """Every layer's and kv head's lightest entries above the budget go, and with them the pages behind."""
+        for p in prompts:
+            self.check_own(p)
         table, slots = self.table_of([p.request for p in prompts]), self.ints([p.slot for p in prompts])
         lens, keep = self.ints([p.entries for p in prompts]), self.ints([self.budget] * len(prompts))
         newest = self.ints([p.tokens - 1 for p in prompts])
@@ -203,6 +210,8 @@ class LongPrompts:
         self.check_end(prompt.tokens + max_new_tokens)
         most, out = prompt.entries + max_new_tokens, []
         if self.budget is not None:
+            if most >= self.budget + self.page_size:    # entries will go
+                self.check_own(prompt)
             most = min(most, self.budget + self.page_size)
         if most > self.max_entries:
             raise ValueError(f"{most} entries; there is room for {self.max_entries}")

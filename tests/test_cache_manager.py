@@ -361,3 +361,56 @@ def test_a_fork_copies_tokens_only_along_their_own_axis(monkeypatch, need, page_
     assert [c.data_ptr() for c in caches] == [cache.kv["a"].data_ptr(), cache.kv["b"].data_ptr()]
     assert copies == [[int(cache.alloc.block_table(1)[1]), int(cache.alloc.block_table(2)[1]), held]]
     cache.alloc.check()
+
+
+def test_who_would_move_entries_asks_whether_their_pages_are_shared():
+    a = PageAllocator([4, 8], [12, 8], [0, 0], 3)
+    a.add_request(1)
+    a.reserve(1, 22)
+    a.commit(1, 22)
+    assert not a.shares(1) and not a.shares(1, 0) and not a.shares(1, 22)
+    a.fork(1, 2)
+    for r in (1, 2):                                    # entries 0 to 19 and 0 to 15; the pages behind are each one's own
+        assert a.shares(r) and a.shares(r, 1) and a.shares(r, 1 << 30) and not a.shares(r, 0)
+    with pytest.raises(CacheError):
+        a.shares(7)
+    for end in (-1, 1 << 31):
+        with pytest.raises(CacheError):
+            a.shares(1, end)
+    a.release(1)
+    assert not a.shares(2)
+    windows = PageAllocator([4], [12], [6], 3)          # what a window has passed is nobody's
+    windows.add_request(1)
+    windows.reserve(1, 12)
+    windows.commit(1, 12)
+    windows.fork(1, 2)
+    assert not windows.shares(2, 4) and windows.shares(2, 8)
+    windows.reserve(1, 30)
+    windows.commit(1, 30)
+    assert not windows.shares(1) and not windows.shares(2)
+
+
+def test_prompts_whose_pages_are_shared_are_not_evicted(monkeypatch):
+    """Before any entry moves, and before a prompt goes on that would have to."""
+    import torch
+    from railgun_b200.examples import long_prompts
+    moved = []
+    monkeypatch.setattr(long_prompts.ops, "evict_entries", lambda *a, **k: moved.append(a))
+    lp = object.__new__(long_prompts.LongPrompts)
+    lp.alloc, lp.page_size, lp.budget, lp.max_entries = PageAllocator([4], [40], [0], 4), 4, 8, 100
+    lp.protect_first = lp.protect_last = lp.nkv = lp.d = 1
+    lp.kv = lp.weights = lp.places = [None]
+    lp.device, lp.check_end = torch.device("cpu"), lambda n: None
+    lp.alloc.add_request(1)
+    lp.alloc.reserve(1, 14)
+    lp.alloc.commit(1, 14)
+    prompt = long_prompts.Prompt(1, lp.alloc.slot(1), 14, 14, 0)
+    lp.alloc.fork(1, 2)
+    with pytest.raises(ValueError, match="other requests"):
+        lp.evict([prompt])
+    with pytest.raises(ValueError, match="other requests"):
+        lp.go_on(prompt, 3)
+    assert not moved and lp.alloc.num_computed(1) == prompt.entries == 14
+    lp.alloc.release(2)
+    lp.evict([prompt])
+    assert len(moved) == 1 and lp.alloc.num_computed(1) == prompt.entries == 8
