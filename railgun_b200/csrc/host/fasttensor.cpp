@@ -100,7 +100,7 @@ static PyObject* ft_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // addresses(list or tuple of tensors, device): where they are, as 64-bit numbers in a bytes object, if they are contiguous tensors of one shape and
-// type on this CUDA device, no two in one place; None if not.
+// type on this CUDA device, no two of which share memory; None if not.
 static PyObject* ft_addresses(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     if (n != 2) {
@@ -132,7 +132,8 @@ static PyObject* ft_addresses(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     std::vector<u64> places(to, to + m);
     std::sort(places.begin(), places.end());
-    if (std::adjacent_find(places.begin(), places.end()) != places.end()) {
+    const u64 bytes = std::max<u64>(1, first.nbytes());
+    if (std::adjacent_find(places.begin(), places.end(), [&](u64 x, u64 y) { return y - x < bytes; }) != places.end()) {
         Py_DECREF(out);
         Py_RETURN_NONE;
     }

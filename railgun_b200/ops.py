@@ -2697,7 +2697,7 @@ def tree_general_blocks(d: int) -> int:
 
 
 def _cache_list(caches, what: str, here: int) -> tuple:
-    """One cache or several different ones of one shape and type on the current device: (the first one, how many, their addresses as 64-bit numbers in
+    """One cache or several of one shape and type on the current device, which share no memory: (the first one, how many, their addresses as 64-bit numbers in
     bytes, the bits of all addresses)."""
     if isinstance(caches, torch.Tensor):
         caches = (caches,)
@@ -2715,8 +2715,9 @@ def _cache_list(caches, what: str, here: int) -> tuple:
             if t.shape != first.shape:
                 raise KernelError(f"{what}: caches of {tuple(first.shape)} and {tuple(t.shape)}")
         places = [t.data_ptr() for t in caches]
-        if len(set(places)) < len(places) and first.numel():
-            raise KernelError(f"{what}: a cache twice (its entries would move twice)")
+        order, size = sorted(places), first.numel() * first.element_size()
+        if any(b - a < size for a, b in zip(order, order[1:])):
+            raise KernelError(f"{what}: a cache twice, or caches that share memory (entries would move twice)")
         addresses = np.array(places, dtype=np.uint64).tobytes()
     bits = 0
     for low in set(addresses[::8]):                  # only the lowest four bits are of interest
@@ -2736,7 +2737,7 @@ def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, m
     lowest child whose token is the one chosen behind its parent is confirmed, until there is none.  Returns ``counts`` [R] int32, how many
     nodes are (node 0 is, always), ``path`` [R, max_rows] int32, their numbers, and ``fresh`` [R, max_rows] int32, the tokens chosen
     behind them: the request's next ``counts[r]`` tokens, the last of which begins its next tree; -1 behind them.  In every
-    cache [pages, .., page, x] of ``caches`` (one, or a list of different ones of one shape) the k-th confirmed node's entry moves from starts + its
+    cache [pages, .., page, x] of ``caches`` (one, or a list of several of one shape that share no memory) the k-th confirmed node's entry moves from starts + its
     number to starts + k, so that the request has starts + counts entries and what lies behind may be given back
     (``PageAllocator.shrink``).  The pages are the request's own from ``starts`` on.  ``max_rows``, up to 4,096: the most rows of a request; rows
     beyond are left out, and requests without rows or with a negative start have a count of 0.  An entry that table or
@@ -2763,7 +2764,7 @@ def keep_drafts(caches, block_table, cu_rows, starts, parents, tokens, chosen, m
 
 
 def copy_pages(caches, copies) -> None:
-    """Copies of pages in every cache of ``caches`` (one, or a list of different ones of one shape and type, [pages, .., page, x]; [slots, ..] of fewer than three
+    """Copies of pages in every cache of ``caches`` (one, or a list of several of one shape and type that share no memory, [pages, .., page, x]; [slots, ..] of fewer than three
     dimensions as whole rows).  ``copies`` [n, 3] int32 on the host (what ``PageAllocator.fork`` returns): (from, to, held), the first
     ``held`` entries of page ``from`` (-1: all of it) to page ``to``; what lies behind them there is left alone.  A page may be
     copied several times; one that is written is written once and read by no copy, so that their order does not matter (a copy of a

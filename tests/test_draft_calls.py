@@ -165,6 +165,18 @@ def test_what_keep_drafts_refuses(calls):
             ops.keep_drafts(**{**keep_args(), **bad})
 
 
+def test_caches_that_share_memory_are_refused(calls):
+    """Wherever they begin: entries would move twice.  Caches one behind the other are different ones."""
+    both = torch.zeros(10, 2, 2, 16, 64)
+    for bad in ([both[:9], both[1:]], [both[1:], both[:9]], [both[:5], both[5:], both[4:9]]):
+        with pytest.raises(ops.KernelError, match="share memory"):
+            ops.keep_drafts(**{**keep_args(), "caches": bad})
+        with pytest.raises(ops.KernelError, match="share memory"):
+            ops.copy_pages(bad, [(0, 1, -1)])
+    assert calls(ops.keep_drafts, **{**keep_args(), "caches": [both[5:], both[:5]]})[1][1] == 2
+    assert calls(ops.copy_pages, [both[5:], both[:5]], [(0, 1, -1)])[1][1] == 2
+
+
 @pytest.mark.parametrize("shape,dtype,piece", [((4, 2, 8, 64), torch.bfloat16, 16), ((4, 2, 8, 5), torch.bfloat16, 2), ((4, 2, 8, 6), torch.float32, 8),
                                                ((4, 8, 33), torch.uint8, 1), ((4, 8, 12), torch.uint8, 4)])
 def test_rows_move_in_the_largest_pieces_that_they_are_made_of(calls, shape, dtype, piece):

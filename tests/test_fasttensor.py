@@ -84,6 +84,16 @@ def test_what_fits(tensors):
 
 
 @pytest.mark.gpu
+def test_addresses_of_tensors_that_share_memory(tensors):
+    x = torch.zeros(10, 3, device="cuda:0")
+    for bad in ([x, x], [x[:9], x[1:]], [x[1:], x[:9]], [x[:5], x[5:], x[4:9]]):
+        assert tensors.addresses(bad, 0) is None
+        with pytest.raises(ops.KernelError, match="share memory"):
+            ops.copy_pages(bad, [(0, 1, -1)])
+    assert np.frombuffer(tensors.addresses([x[5:], x[:5]], 0), np.uint64).tolist() == [x[5:].data_ptr(), x.data_ptr()]
+
+
+@pytest.mark.gpu
 def test_without_the_module_calls_are_the_same(monkeypatch):
     """The way through Python alone, which machines without torch's headers take."""
     def run():
