@@ -131,6 +131,14 @@ def _rows_fit(t, name: str, dtype, here: int, columns: int) -> tuple:
     return got
 
 
+def _rows_apart(a, b, a_step: int, b_step: int, rows: int, columns: int) -> bool:
+    """Do two matrices of one type, whose rows are so far apart, share no memory?  One may be columns beside the other's of the same buffer."""
+    at, size = (b.data_ptr() - a.data_ptr()) // a.element_size(), (rows - 1) * a_step + columns
+    if at >= size or -at >= (rows - 1) * b_step + columns:
+        return True
+    return a_step == b_step and columns <= at % a_step <= a_step - columns
+
+
 def _new(dtype, here: int, *sizes) -> torch.Tensor:
     if _tensors:
         return _tensors.empty(dtype, here, *sizes)
@@ -2600,7 +2608,8 @@ def draft_tree(parents: torch.Tensor, cu_rows: torch.Tensor, starts: torch.Tenso
 
 def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: int, nkv: int, d: int, scale: float, max_rows: int,
                    max_context: int) -> None:
-    """Attention of trees of drafted tokens: ``out`` [T, nh * d], row t of ``q`` [T, at least nh * d] (head h at column h * d).  Request r's rows
+    """Attention of trees of drafted tokens: ``out`` [T, nh * d], which shares no memory with ``q``, row t of ``q`` [T, at least nh * d] (head h
+    at column h * d).  Request r's rows
     are ``cu_rows[r]`` .. ``cu_rows[r + 1]`` - 1; its entries, through ``block_table[r]``, are ``starts[r]`` of earlier tokens, which all its
     rows see, and then one for each of its rows (already in the cache), of which a row sees those whose bits ``masks`` [T, words] int32
     has (``draft_tree``; any other choice will do).  A row that sees nothing gives 0; keys and values that a row does not see have no say
@@ -2622,6 +2631,8 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     (pages, _, _, page_size, _), blocks_a_row, words = kv_cache.shape, block_table.shape[1], masks.shape[1]
     if out_rows != T or out.shape[1] != nh * d or page_size < 1 or pages < 1:
         raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; {pages} pages hold {page_size} entries each")
+    if T and not _rows_apart(q, out, step, out_step, T, nh * d):
+        raise KernelError("tree_attention: q and out share memory (a row may be read again after it was written)")
     if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")
     max_rows = min(max_rows, T)

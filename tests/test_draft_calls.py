@@ -83,6 +83,20 @@ def test_what_tree_attention_refuses(calls):
             ops.tree_attention(**{**a, **bad})
 
 
+def test_queries_and_outputs_that_share_memory_are_refused(calls):
+    """A row whose output is no number is worked out again from its queries, which would be written over by then."""
+    n = 8 * 64
+    wide, flat = torch.zeros(7, 3 * n, dtype=torch.bfloat16), torch.zeros(12 * n, dtype=torch.bfloat16)
+    first, last = flat[:6 * n].view(6, n), flat[6 * n:].view(6, n)
+    for q, out in ((first, first), (wide[:6, :n], wide[:6, :n]), (wide[:6, :n], wide[:6, n - 1:2 * n - 1]), (wide[:6, n:2 * n], wide[:6, 1:n + 1]),
+                   (wide[:6, :n], wide[1:, :n]), (wide[1:, :n], wide[:6, :n]), (flat.view(6, 2 * n), last), (first, flat[6 * n - 1:12 * n - 1].view(6, n))):
+        with pytest.raises(ops.KernelError, match="share memory"):
+            ops.tree_attention(**{**tree_args(), "q": q, "out": out})
+    for q, out in ((first, last), (last, first), (wide[:6, :n], wide[:6, n:2 * n]), (wide[:6, 2 * n:], wide[:6, :n]), (wide[:6, n:2 * n], wide[1:, :n]),
+                   (wide[:6], wide[:6, n:2 * n])):                       # of the last, only the first columns are read
+        calls(ops.tree_attention, **{**tree_args(), "q": q, "out": out})
+
+
 def test_nothing_to_do_is_no_launch(calls):
     for none in (tree_args(T=0), tree_args(R=0), {**tree_args(), "max_rows": 0}):
         ops.tree_attention(**none)
