@@ -128,6 +128,10 @@ def _rows_fit(t, name: str, dtype, here: int, columns: int) -> tuple:
         if t.shape[1] < columns:
             raise KernelError(f"{name} has {t.shape[1]} columns, {columns} are needed")
         got = t.shape[0], t.stride(0)
+    if got[1] >= 1 << 31:                        # launchers take 32 bits
+        if got[0] > 1:
+            raise KernelError(f"{name}: rows {got[1]} elements apart (up to 2^31 - 1)")
+        got = got[0], t.shape[1]                 # one row is apart from nothing
     return got
 
 

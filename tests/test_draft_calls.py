@@ -97,6 +97,21 @@ def test_queries_and_outputs_that_share_memory_are_refused(calls):
         calls(ops.tree_attention, **{**tree_args(), "q": q, "out": out})
 
 
+@pytest.mark.parametrize("step", [(1 << 31) - 8, 1 << 31, (1 << 32) + 512])
+def test_rows_that_are_far_apart(calls, monkeypatch, step):
+    """Launchers take distances of 32 bits: none is cut to them."""
+    def rows(n):
+        return torch.empty_strided((n, 512), (step, 1), dtype=torch.bfloat16, device="meta")
+    for n in (0, 1):
+        got = ops._rows_fit(rows(n), "q", torch.bfloat16, -1, 512)
+        assert got[0] == n and 512 <= got[1] < 1 << 31
+    if step < 1 << 31:
+        assert ops._rows_fit(rows(2), "q", torch.bfloat16, -1, 512) == (2, step)
+    else:
+        with pytest.raises(ops.KernelError, match="apart"):
+            ops._rows_fit(rows(2), "q", torch.bfloat16, -1, 512)
+
+
 def test_nothing_to_do_is_no_launch(calls):
     for none in (tree_args(T=0), tree_args(R=0), {**tree_args(), "max_rows": 0}):
         ops.tree_attention(**none)
