@@ -139,6 +139,10 @@ class Drafts:
         or more, and adds them to it."""
         if len({t.request for t in texts}) != len(texts):
             raise ValueError("a text stands once in a step")
+        if len(trees) != len(texts):
+            raise ValueError(f"{len(trees)} trees; a step has a tree for each text, {len(texts)} of them")
+        if not texts:
+            return []
         counts, starts = [len(tokens) for _, tokens in trees], [len(t.tokens) - 1 for t in texts]
         for (parents, tokens), text, start in zip(trees, texts, starts):
             depths = []

@@ -414,3 +414,23 @@ def test_prompts_whose_pages_are_shared_are_not_evicted(monkeypatch):
     lp.alloc.release(2)
     lp.evict([prompt])
     assert len(moved) == 1 and lp.alloc.num_computed(1) == prompt.entries == 8
+
+
+def test_a_step_of_drafts_has_a_tree_for_each_text():
+    """More trees than texts, or fewer: nothing is reserved, nothing is run."""
+    from railgun_b200.engine.request import SamplingParams
+    from railgun_b200.examples import drafts
+    d = object.__new__(drafts.Drafts)
+    d.alloc = PageAllocator([4], [40], [0], 4)
+    texts = []
+    for r in (1, 2):
+        d.alloc.add_request(r)
+        d.alloc.reserve(r, 5)
+        d.alloc.commit(r, 5)
+        texts.append(drafts.Text(r, [1, 2, 3, 4, 5, 6], 5, SamplingParams()))
+    free, tree = d.alloc.free_pages(), ([-1], [6])
+    for bad in ([], [tree], [tree] * 3):
+        with pytest.raises(ValueError, match="a tree for each text"):
+            d.step(texts, bad)
+    assert d.step([], []) == []
+    assert d.alloc.free_pages() == free and [t.checked for t in texts] == [0, 0]
