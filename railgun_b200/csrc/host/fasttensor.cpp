@@ -99,6 +99,31 @@ static PyObject* ft_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// apart(matrix, matrix, columns): do two matrices of one type and as many rows, of which so many columns are used, share no memory?  The one may
+// be columns beside the other's in a buffer.
+static PyObject* ft_apart(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 3 || !THPVariable_Check(a[0]) || !THPVariable_Check(a[1]) || !PyLong_Check(a[2])) {
+        PyErr_SetString(PyExc_TypeError, "apart: two matrices and columns");
+        return nullptr;
+    }
+    const at::Tensor &x = THPVariable_Unpack(a[0]), &y = THPVariable_Unpack(a[1]);
+    const long long columns = PyLong_AsLongLong(a[2]);
+    if (columns == -1 && PyErr_Occurred()) return nullptr;
+    if (x.dim() != 2 || y.dim() != 2 || x.size(0) != y.size(0) || x.scalar_type() != y.scalar_type()) {
+        PyErr_SetString(PyExc_TypeError, "apart: matrices of one type and as many rows");
+        return nullptr;
+    }
+    if (x.size(0) == 0 || columns <= 0) Py_RETURN_TRUE;
+    const long long at = ((long long)y.data_ptr() - (long long)x.data_ptr()) / (long long)x.element_size(), before = x.size(0) - 1;
+    if (at >= before * x.stride(0) + columns || -at >= before * y.stride(0) + columns) Py_RETURN_TRUE;
+    const long long step = x.stride(0);
+    if (step < 1 || step != y.stride(0)) Py_RETURN_FALSE;
+    const long long beside = (at % step + step) % step;
+    return PyBool_FromLong(columns <= beside && beside <= step - columns);
+    END_HANDLE_TH_ERRORS
+}
+
 // addresses(list or tuple of tensors, device): where they are, as 64-bit numbers in a bytes object, if they are contiguous tensors of one shape and
 // type on this CUDA device, no two of which share memory; None if not.
 static PyObject* ft_addresses(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -227,6 +252,7 @@ static PyMethodDef methods[] = {
     {"fits", (PyCFunction)(void (*)(void))ft_fits, METH_FASTCALL, "is it a contiguous tensor of this type on this device, of these sizes (None: any)?"},
     {"fits_all", (PyCFunction)(void (*)(void))ft_fits_all, METH_FASTCALL, "are they all contiguous tensors of their types on this device, of their sizes?"},
     {"rows", (PyCFunction)(void (*)(void))ft_rows, METH_FASTCALL, "a matrix's rows and how far they are apart; None if it does not fit"},
+    {"apart", (PyCFunction)(void (*)(void))ft_apart, METH_FASTCALL, "do two matrices, of which so many columns are used, share no memory?"},
     {"addresses", (PyCFunction)(void (*)(void))ft_addresses, METH_FASTCALL, "where tensors of one kind are, as bytes; None if they are not of one kind"},
     {"empty", (PyCFunction)(void (*)(void))ft_empty, METH_FASTCALL, "a new tensor of this type, on this device, of these sizes"},
     {nullptr, nullptr, 0, nullptr}};

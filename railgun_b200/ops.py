@@ -135,12 +135,16 @@ def _rows_fit(t, name: str, dtype, here: int, columns: int) -> tuple:
     return got
 
 
-def _rows_apart(a, b, a_step: int, b_step: int, rows: int, columns: int) -> bool:
-    """Do two matrices of one type, whose rows are so far apart, share no memory?  One may be columns beside the other's of the same buffer."""
-    at, size = (b.data_ptr() - a.data_ptr()) // a.element_size(), (rows - 1) * a_step + columns
-    if at >= size or -at >= (rows - 1) * b_step + columns:
+def _rows_apart(a, b, columns: int) -> bool:
+    """Do two matrices of one type and as many rows, of which so many columns are used, share no memory?  One may be columns beside the
+    other's of the same buffer."""
+    if _tensors:
+        return _tensors.apart(a, b, columns)
+    rows, step, other = a.shape[0] - 1, a.stride(0), b.stride(0)
+    at = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if rows < 0 or at >= rows * step + columns or -at >= rows * other + columns:
         return True
-    return a_step == b_step and columns <= at % a_step <= a_step - columns
+    return step == other and columns <= at % step <= step - columns
 
 
 def _new(dtype, here: int, *sizes) -> torch.Tensor:
@@ -2635,7 +2639,7 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     (pages, _, _, page_size, _), blocks_a_row, words = kv_cache.shape, block_table.shape[1], masks.shape[1]
     if out_rows != T or out.shape[1] != nh * d or page_size < 1 or pages < 1:
         raise KernelError(f"tree_attention: out is {tuple(out.shape)}, expected [{T}, {nh * d}]; {pages} pages hold {page_size} entries each")
-    if T and not _rows_apart(q, out, step, out_step, T, nh * d):
+    if not _rows_apart(q, out, nh * d):
         raise KernelError("tree_attention: q and out share memory (a row may be read again after it was written)")
     if min(max_rows, max_context) < 0 or max(max_rows, max_context) >= 1 << 31:
         raise KernelError("tree_attention: max_rows and max_context are counts below 2^31")

@@ -64,6 +64,28 @@ def test_what_does_not_fit(tensors):
         tensors.empty("int32", 0, 3)
 
 
+def test_matrices_that_share_memory(tensors, monkeypatch):
+    """The module and the way through Python against marks in memory."""
+    flat = torch.zeros(400, dtype=torch.int16)
+    for rows in (0, 1, 2, 5):
+        for xs, ys in ((10, 10), (10, 7), (30, 30), (4, 4)):
+            for columns in (1, 3, 4):
+                for xo, yo in ((0, 0), (0, 3), (3, 0), (0, 4), (4, 0), (0, 26), (0, 10), (0, 33), (12, 60), (60, 12), (20, 30), (0, 200), (200, 0), (7, 40)):
+                    x, y = (flat.as_strided((rows, 4), (step, 1), o) for step, o in ((xs, xo), (ys, yo)))
+                    flat.zero_()
+                    x[:, :columns] = 1
+                    want = not y[:, :columns].any().item()
+                    got = []
+                    for module in (tensors, False):
+                        monkeypatch.setattr(ops, "_tensors", module)
+                        got.append(ops._rows_apart(x, y, columns))
+                    assert got[0] is got[1] and (want or not got[0])        # never apart where they are not
+                    assert got[0] == want or (xs != ys)                      # rows at different distances may be refused
+    for bad in ((flat, flat, 3), (x, y.float(), 3), (x, y[1:], 3), (x, y), (x, y, 1.0), (x, None, 3)):
+        with pytest.raises(TypeError):
+            tensors.apart(*bad)
+
+
 @pytest.mark.gpu
 def test_what_fits(tensors):
     x = torch.zeros(3, 4, 5, dtype=torch.int32, device="cuda:0")
