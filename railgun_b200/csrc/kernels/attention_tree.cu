@@ -45,7 +45,7 @@ static_assert(2 * tg_stage(1) >= TG_SUMS + TG_Q && 2 * tg_stage(32) >= TG_SUMS +
 // WHOLE: an item to a cluster, whose blocks share its tiles, join through each other's shared memory and leave the output.
 // What bounds it is shared memory: 96 bytes a thread for 32 products of scores, 272, most of them the same for a warp, for 64 of the output: in
 // 32-bit, 16 heads on 4 of 128, one request of 16 nodes on 1,000 entries takes 26 us, 8 on 4,000 390, 10.7 TFLOP/s.  Smallest calls are the launch and
-// the same three trips as above: two requests of 7 nodes on 61 entries, 3 heads on 1 of 32, 9.3 us in one launch, 12 in two.
+// three trips to memory, for the request, the table and the entries: two requests of 7 nodes on 61 entries, 3 heads on 1 of 32, 9.3 us in one launch, 12 in two.
 // ---------------------------------------------------------------------------------------------------
 template <typename A, int DP, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(TG_THREADS) tree_general_kernel(const TreeArgs a, A* __restrict__ out, int out_ld, int q_blocks) {

@@ -17,8 +17,9 @@
 // What bounds it, 32 heads on 8 of 128.  Few queries: the cache.  64 requests of 16 nodes behind up to 4,096 entries, 817 MB, take 134 us and 13 to
 // join, 93 % of what a copy reaches; called on and on, the power limit takes the clock to 1.5 GHz and a call to 163 to 177.  Many: 128 nodes of
 // one request on 65,536 entries take 132 us and 10 to join, 137 GFLOP, 83 us at the rate of a large product.  A pass of both sides takes
-// 2,090 cycles there.  Its products are 1,300 (N 64 is bound by what it fetches from shared memory), its exponentials 1,080 by themselves and
-// 1,180 beside products; the sides fall into step, and the waits between one and the other are covered by neither.  Slower, in us for these
+// 2,090 cycles there.  Alone its products take 1,300 (N 64 is bound by what it fetches from shared memory) and its exponentials 1,080, or 1,180
+// where nothing but products runs beside them.  In the kernel a softmax warp spends 1,300 of the 2,090 on exponentials, 200 on storing weights and
+// the rest on its loop and on waiting for the next scores: the sides fall into step, and neither covers the other's waits.  Slower, in us for these
 // two, 149 and 148 then: an issuing warp for a side's even and one for its odd passes 153 and 155, the next scores loaded beside the store of
 // the weights 154 and 158, passes of 128 entries and one issuing warp for both sides 161 and 171, two threads a query 167 and 152.
 //

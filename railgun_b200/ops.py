@@ -2624,7 +2624,7 @@ def tree_attention(q, out, kv_cache, block_table, cu_rows, starts, masks, nh: in
     in it, whatever they are, and a score of -infinity is a weight of 0.  ``max_rows``, ``max_context``: the most rows of a request, and
     the most entries (earlier and its own) that are seen; scratch is sized by rows.  Rows beyond ``max_rows``, rows of requests with a
     negative start and rows of no request are left as they were.  A page that the cache does not have is reported by
-    ``tc_gemm_check``, and the result is invalid.  All sums are 32-bit and have one order."""
+    ``tc_gemm_check`` (behind a replayed graph after ``mark_tc_unchecked``), and the result is invalid.  All sums are 32-bit and have one order."""
     _tensor_calls()
     here, i32, dtype = _here(), torch.int32, q.dtype
     code = _dtype_code(q)
@@ -3200,7 +3200,8 @@ def probe_sm100(device="cuda:0") -> dict:
 
 def tc_gemm_check(device=None) -> None:
     """Raise if a wait inside a tcgen05 product gave up since the last check, or an operator over trees of drafted tokens met a page
-    that its cache does not have (synchronises; free when no such kernel ran since)."""
+    that its cache does not have (synchronises; free when no such kernel was launched since; a replayed graph counts as none
+    unless ``mark_tc_unchecked`` says so)."""
     global _tc_unchecked
     if not _tc_unchecked:
         return

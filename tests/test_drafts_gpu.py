@@ -479,6 +479,30 @@ def test_trees_in_a_captured_graph(dtype):
             assert (s["out"][cu[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("cluster", [0, 2])
+def test_a_replayed_graph_reports_pages_that_are_not_there(monkeypatch, cluster):
+    """Once who replays it has said so: a replay is no call that could be seen from here."""
+    from railgun_b200 import ops
+    monkeypatch.setattr(ops, "tree_cluster", lambda *a: cluster)
+    q, out, args, sizes = run_tree([5, 20], [100, 40], 8, 2, 64, 16, torch.bfloat16, 3)
+    ops.tc_gemm_check()
+    want, table = out.clone(), args[1].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.tree_attention(q, out, *args, **sizes)
+    ops.tc_gemm_check()
+    args[1][1, 2] = -1
+    graph.replay()
+    ops.mark_tc_unchecked()
+    with pytest.raises(ops.KernelError, match="page"):
+        ops.tc_gemm_check()
+    args[1].copy_(table)
+    graph.replay()
+    ops.mark_tc_unchecked()
+    ops.tc_gemm_check()
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_pages_beyond_two_to_the_31_elements(dtype):
     from railgun_b200 import ops
